@@ -46,6 +46,13 @@ EXPORTED = (
     "bl_ipc_close",
     "bl_paged_prefill",
     "bl_rms_norm",
+    "bl_paged_append_fp8",
+    "bl_paged_gather_fp8",
+    "bl_paged_decode_fp8_workspace_bytes",
+    "bl_paged_decode_fp8",
+    "bl_paged_prefill_fp8_workspace_bytes",
+    "bl_paged_prefill_fp8",
+    "bl_copy_blocks",
     "bl_last_error",
     "bl_abi_version",
     "bl_decode_path",
@@ -221,6 +228,110 @@ class RmsNormArgs(Structure):
     ]
 
 
+class Fp8Layer(Structure):
+    _fields_ = [("kv", PagedLayer), ("k_scale", c_void_p), ("v_scale", c_void_p)]
+
+
+class AppendFp8Args(Structure):
+    _fields_ = [
+        ("layer", Fp8Layer),
+        ("k_new", c_void_p),
+        ("v_new", c_void_p),
+        ("new_stride_b", c_int64),
+        ("new_stride_h", c_int64),
+        ("new_stride_t", c_int64),
+        ("v_stride_b", c_int64),
+        ("v_stride_h", c_int64),
+        ("v_stride_t", c_int64),
+        ("start_pos", c_void_p),
+        ("new_offsets", c_void_p),
+        ("batch", c_int64),
+        ("max_new_tokens", c_int64),
+        ("err", c_void_p),
+    ]
+
+
+class GatherFp8Args(Structure):
+    _fields_ = [
+        ("layer", Fp8Layer),
+        ("seq_lens", c_void_p),
+        ("batch", c_int64),
+        ("k_out", c_void_p),
+        ("v_out", c_void_p),
+        ("out_stride_b", c_int64),
+        ("out_stride_h", c_int64),
+        ("out_stride_t", c_int64),
+        ("max_len", c_int64),
+        ("zero_fill", c_int32),
+        ("err", c_void_p),
+    ]
+
+
+class DecodeFp8Args(Structure):
+    _fields_ = [
+        ("layer", Fp8Layer),
+        ("q", c_void_p),
+        ("q_stride_b", c_int64),
+        ("q_stride_h", c_int64),
+        ("out", c_void_p),
+        ("out_stride_b", c_int64),
+        ("out_stride_h", c_int64),
+        ("seq_lens", c_void_p),
+        ("batch", c_int64),
+        ("num_q_heads", c_int64),
+        ("scale", c_float),
+        ("plan_ready", c_int32),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+        ("max_seq_len", c_int64),
+        ("err", c_void_p),
+    ]
+
+
+class PrefillFp8Args(Structure):
+    _fields_ = [
+        ("layer", Fp8Layer),
+        ("q", c_void_p),
+        ("q_stride_b", c_int64),
+        ("q_stride_t", c_int64),
+        ("q_stride_h", c_int64),
+        ("out", c_void_p),
+        ("out_stride_b", c_int64),
+        ("out_stride_t", c_int64),
+        ("out_stride_h", c_int64),
+        ("q_offsets", c_void_p),
+        ("seq_lens", c_void_p),
+        ("batch", c_int64),
+        ("num_q_heads", c_int64),
+        ("max_q_len", c_int64),
+        ("scale", c_float),
+        ("pad0", c_int32),
+        ("max_seq_len", c_int64),
+        ("total_blocks", c_int64),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+        ("err", c_void_p),
+    ]
+
+
+class CopyBlocksArgs(Structure):
+    _fields_ = [
+        ("k_pool", c_void_p),
+        ("v_pool", c_void_p),
+        ("k_scale", c_void_p),
+        ("v_scale", c_void_p),
+        ("num_layers", c_int64),
+        ("num_blocks", c_int64),
+        ("num_kv_heads", c_int64),
+        ("block_size", c_int64),
+        ("head_dim", c_int64),
+        ("elem_bytes", c_int64),
+        ("src", c_void_p),
+        ("dst", c_void_p),
+        ("count", c_int64),
+    ]
+
+
 STRUCTS = {
     "bl_paged_layer": PagedLayer,
     "bl_qk_prep_args": QkPrepArgs,
@@ -231,6 +342,12 @@ STRUCTS = {
     "bl_ipc_handle": IpcHandle,
     "bl_prefill_args": PrefillArgs,
     "bl_rms_norm_args": RmsNormArgs,
+    "bl_fp8_layer": Fp8Layer,
+    "bl_append_fp8_args": AppendFp8Args,
+    "bl_gather_fp8_args": GatherFp8Args,
+    "bl_decode_fp8_args": DecodeFp8Args,
+    "bl_prefill_fp8_args": PrefillFp8Args,
+    "bl_copy_blocks_args": CopyBlocksArgs,
 }
 
 _lib: ctypes.CDLL | None = None
@@ -274,6 +391,20 @@ def load() -> ctypes.CDLL:
     lib.bl_paged_prefill.restype = c_int
     lib.bl_rms_norm.argtypes = [POINTER(RmsNormArgs), c_void_p]
     lib.bl_rms_norm.restype = c_int
+    lib.bl_paged_append_fp8.argtypes = [POINTER(AppendFp8Args), c_void_p]
+    lib.bl_paged_append_fp8.restype = c_int
+    lib.bl_paged_gather_fp8.argtypes = [POINTER(GatherFp8Args), c_void_p]
+    lib.bl_paged_gather_fp8.restype = c_int
+    lib.bl_paged_decode_fp8_workspace_bytes.argtypes = [c_int64] * 4
+    lib.bl_paged_decode_fp8_workspace_bytes.restype = c_size_t
+    lib.bl_paged_decode_fp8.argtypes = [POINTER(DecodeFp8Args), c_void_p]
+    lib.bl_paged_decode_fp8.restype = c_int
+    lib.bl_paged_prefill_fp8_workspace_bytes.argtypes = [c_int32] + [c_int64] * 7
+    lib.bl_paged_prefill_fp8_workspace_bytes.restype = c_size_t
+    lib.bl_paged_prefill_fp8.argtypes = [POINTER(PrefillFp8Args), c_void_p]
+    lib.bl_paged_prefill_fp8.restype = c_int
+    lib.bl_copy_blocks.argtypes = [POINTER(CopyBlocksArgs), c_void_p]
+    lib.bl_copy_blocks.restype = c_int
     lib.bl_last_error.argtypes = []
     lib.bl_last_error.restype = c_char_p
     lib.bl_abi_version.argtypes = []

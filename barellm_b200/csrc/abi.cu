@@ -88,6 +88,27 @@ bool make_tmap_2d_16bit(CUtensorMap* map, const void* base, uint64_t row_elems, 
   return true;
 }
 
+bool make_tmap_rows_8bit(CUtensorMap* map, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t box_x,
+                         uint32_t box_y) {
+  auto fn = get_encode_fn();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled is unavailable from the driver");
+    return false;
+  }
+  cuuint64_t dims[2] = {row_bytes, rows};
+  cuuint64_t strides[1] = {row_bytes};
+  cuuint32_t box[2] = {box_x, box_y};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, box_x == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled (8-bit rows) failed with CUresult %d", (int)r);
+    return false;
+  }
+  return true;
+}
+
 // Paged pools viewed page by page: x = 64 elements (one 128-byte half of a
 // 256-byte token row), y = 8 token rows (256 B apart), z = the row's two
 // halves (128 B apart), w = groups of 8 rows (2 KB apart).  A box of

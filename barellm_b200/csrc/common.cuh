@@ -513,6 +513,11 @@ __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sy
 bool make_tmap_2d_16bit(CUtensorMap* map, const void* base, uint64_t row_elems, uint64_t rows,
                         uint32_t box_x, uint32_t box_y, bool bf16);
 
+// 2-D tiled tensor map over `rows` rows of `row_bytes` bytes (8-bit codes), box
+// box_x x box_y, swizzled over box_x bytes (64 or 128).
+bool make_tmap_rows_8bit(CUtensorMap* map, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t box_x,
+                         uint32_t box_y);
+
 // Cached tensor map over a K or V pool viewed as `rows` rows of 128 16-bit
 // elements, box 64 x 16, 128-byte swizzle (one 16-token page half per box).
 bool get_pool_tmap(const void* pool, uint64_t rows, int dtype, CUtensorMap* out);

@@ -1,0 +1,574 @@
+// Chunked-prefill attention over an 8-bit paged cache.  Query i of row b (C_b
+// queries, total length L_b) sees keys 0 .. L_b - C_b + i, as in prefill.cu;
+// K and V are code * scale (fp8.cuh).  Reference counterpart: the prefill SDPA of
+// src/barellm/attention/backend.py:52-61 over a dense read of the cache.
+//
+// Two ways, chosen by shape (use_tc below):
+//   expand + prefill_tc_kernel  16-bit q, head_dim 128.  The rows' pages are
+//       dequantised once into a 16-bit paged scratch (exact in bf16: a code has
+//       four significant bits), which the tcgen05 kernel of prefill_tc.cu then
+//       reads.  The expansion moves 1 + 2 bytes per cached element once; a
+//       CTA of the attention kernel reads the 2-byte form, and every 128 query
+//       tokens times group re-read it (mostly from L2), so dequantising in that
+//       kernel would repeat the conversion for every query tile.  Block sizes
+//       other than 16 become 16-token pages on the way, and a query group
+//       that the kernel is not built for (3, 5, 16, ...) becomes several KV heads
+//       with the same contents and a group of 8, 4, 2 or 1.
+//   fp8_prefill_simt_kernel     any element type, head_dim <= 256, block size
+//       and group: 64 queries x 64 keys a tile in fp32, pages dequantised
+//       into shared memory.
+#include <cstring>
+#include <mutex>
+
+#include "fp8.cuh"
+#include "prefill_tc.cuh"
+
+namespace bl {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kPage = 16;  // tokens of a scratch page
+constexpr int kTCDim = 128;
+
+inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+// How a call's scratch looks: 16-token pages of `heads` KV heads, each cached
+// head repeated `dup` times.
+struct Scratch {
+  int64_t width, pages, heads, dup;
+  size_t table, k, v, total;
+};
+
+bool use_tc(int32_t dtype, int64_t d) { return (dtype == BL_BF16 || dtype == BL_F16) && d == kTCDim; }
+
+// False when the scratch would not fit the tcgen05 kernel's 32-bit row coordinates.
+bool plan_scratch(int64_t batch, int64_t hq, int64_t hkv, int64_t bs, int64_t max_seq_len, int64_t total_blocks,
+                  Scratch* w) {
+  const int64_t g = hq / hkv;
+  int64_t gt = 8;
+  while (g % gt) gt /= 2;
+  w->dup = g / gt;
+  w->heads = hkv * w->dup;
+  w->width = (max_seq_len + kPage - 1) / kPage;
+  // every row ends in at most one partial page; more than batch * width cannot be in use
+  const double bound = (double)total_blocks * (double)bs / kPage + (double)batch + 1;
+  w->pages = (int64_t)std::min(bound, (double)batch * (double)w->width);
+  if ((double)w->pages * w->heads * kPage > (double)(INT32_MAX - 64) || w->heads > 65535) return false;
+  size_t off = align256((size_t)batch * w->width * sizeof(int32_t));
+  const size_t half = align256((size_t)w->pages * w->heads * kPage * kTCDim * 2);
+  w->table = 0;
+  w->k = off;
+  w->v = off + half;
+  w->total = off + 2 * half;
+  return true;
+}
+
+struct ExpandArgs {
+  const uint8_t* k_pool;
+  const uint8_t* v_pool;
+  const float* k_scale;
+  const float* v_scale;
+  void* k_out;
+  void* v_out;
+  int32_t* table;  // [batch][width]
+  int64_t num_blocks, layer, width, pages, bt_stride, bt_width;
+  const int32_t* block_tables;
+  const int32_t* row_ids;
+  const int32_t* seq_lens;
+  const int32_t* q_offsets;
+  int64_t max_q, o_sb, o_st, o_sh;
+  void* out;
+  int32_t hkv, bs, dup, hq;
+  int32_t* err;
+};
+
+constexpr int kExpandPages = 4;  // pages of a CTA
+constexpr int kExpandThreads = 256;  // one page of one head: 16 tokens x 16 eight-code vectors
+
+// grid: (ceil(width / kExpandPages), hkv, batch)
+template <typename T>
+__global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(const ExpandArgs a) {
+  const int tid = threadIdx.x, h = blockIdx.y;
+  const int64_t b = blockIdx.z;
+  const int64_t len = max((int64_t)a.seq_lens[b], (int64_t)0);
+  if (blockIdx.x == 0 && h == 0) {
+    // queries that see no key at all (more queries than tokens): zeros
+    int64_t qo = 0, nq = a.max_q;
+    if (a.q_offsets) {
+      qo = a.q_offsets[b];
+      nq = (int64_t)a.q_offsets[b + 1] - qo;
+    }
+    for (int64_t i = 0; i < nq - len; ++i)
+      for (int e = tid; e < a.hq * kTCDim; e += kExpandThreads)
+        reinterpret_cast<T*>(a.out)[b * a.o_sb + (qo + i) * a.o_st + (int64_t)(e / kTCDim) * a.o_sh + e % kTCDim] =
+            from_f32<T>(0.f);
+    if (tid == 0 && len > a.width * kPage) raise_dev(a.err, BL_DEVERR_WORKSPACE);  // longer than max_seq_len
+  }
+  const int64_t j0 = (int64_t)blockIdx.x * kExpandPages;
+  if (j0 * kPage >= len) return;
+
+  // first scratch page of the row: the pages of the rows before it
+  __shared__ int64_t s_sum[kExpandThreads / 32];
+  int64_t base = 0;
+  for (int64_t r = tid; r < b; r += kExpandThreads)
+    base += (min(max((int64_t)a.seq_lens[r], (int64_t)0), a.width * kPage) + kPage - 1) / kPage;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o);
+  if ((tid & 31) == 0) s_sum[tid >> 5] = base;
+  __syncthreads();
+  base = 0;
+#pragma unroll
+  for (int w = 0; w < kExpandThreads / 32; ++w) base += s_sum[w];
+
+  const int64_t row = a.row_ids ? (int64_t)a.row_ids[b] : b;
+  const int tok = tid >> 4, v = tid & 15;
+  uint2 kc[kExpandPages], vc[kExpandPages];
+  float ks[kExpandPages], vs[kExpandPages];
+  bool ok[kExpandPages];
+#pragma unroll
+  for (int p = 0; p < kExpandPages; ++p) {
+    const int64_t j = j0 + p, t = j * kPage + tok;
+    ok[p] = false;
+    if (j >= a.width || j * kPage >= len) continue;
+    const bool fits = base + j < a.pages;
+    if (h == 0 && tid == 0) {
+      a.table[b * a.width + j] = fits ? (int32_t)(base + j) : -1;
+      if (!fits) raise_dev(a.err, BL_DEVERR_WORKSPACE);
+    }
+    if (!fits || t >= len) continue;
+    const int64_t lb = t / a.bs;
+    if (lb >= a.bt_width) {
+      raise_dev(a.err, BL_DEVERR_TABLE);
+      continue;
+    }
+    int64_t phys = a.block_tables[row * a.bt_stride + lb];
+    if (phys < 0 || phys >= a.num_blocks) {
+      raise_dev(a.err, BL_DEVERR_BLOCK_ID);
+      continue;
+    }
+    const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + h;
+    const int64_t src = (slot * a.bs + (t - lb * a.bs)) * kTCDim + v * 8;
+    kc[p] = *reinterpret_cast<const uint2*>(a.k_pool + src);
+    vc[p] = *reinterpret_cast<const uint2*>(a.v_pool + src);
+    ks[p] = a.k_scale[slot];
+    vs[p] = a.v_scale[slot];
+    ok[p] = true;
+  }
+#pragma unroll
+  for (int p = 0; p < kExpandPages; ++p) {
+    const int64_t j = j0 + p;
+    if (j >= a.width || base + j >= a.pages || j * kPage >= len) continue;
+    // a token whose block cannot be read, and the slots behind the length, become zeros
+    union {
+      T t[8];
+      uint4 u;
+    } ko, vo;
+    ko.u = vo.u = make_uint4(0, 0, 0, 0);
+    if (ok[p]) {
+      const uint32_t kw[2] = {kc[p].x, kc[p].y}, vw[2] = {vc[p].x, vc[p].y};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float2 a0 = e4m3x2_to_float2((uint16_t)kw[i]), a1 = e4m3x2_to_float2((uint16_t)(kw[i] >> 16));
+        const float2 b0 = e4m3x2_to_float2((uint16_t)vw[i]), b1 = e4m3x2_to_float2((uint16_t)(vw[i] >> 16));
+        ko.t[4 * i] = dequant_to<T>(a0.x * ks[p]), ko.t[4 * i + 1] = dequant_to<T>(a0.y * ks[p]);
+        ko.t[4 * i + 2] = dequant_to<T>(a1.x * ks[p]), ko.t[4 * i + 3] = dequant_to<T>(a1.y * ks[p]);
+        vo.t[4 * i] = dequant_to<T>(b0.x * vs[p]), vo.t[4 * i + 1] = dequant_to<T>(b0.y * vs[p]);
+        vo.t[4 * i + 2] = dequant_to<T>(b1.x * vs[p]), vo.t[4 * i + 3] = dequant_to<T>(b1.y * vs[p]);
+      }
+    }
+    for (int r = 0; r < a.dup; ++r) {
+      const int64_t dst = ((((base + j) * a.hkv + h) * a.dup + r) * kPage + tok) * kTCDim + v * 8;
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.k_out) + dst) = ko.u;
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.v_out) + dst) = vo.u;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// SIMT kernel
+// ---------------------------------------------------------------------------
+constexpr int kBQ = 64, kBK = 64;
+constexpr int kSimtThreads = 256;  // 16 x 16: a thread owns 4 queries x (4 keys | 4 dims of every 64)
+constexpr int kPStride = kBK + 4;
+
+struct SimtArgs {
+  const void* q;
+  int64_t q_sb, q_st, q_sh;
+  void* out;
+  int64_t o_sb, o_st, o_sh;
+  const int32_t* q_offsets;
+  const int32_t* seq_lens;
+  const uint8_t* k_pool;
+  const uint8_t* v_pool;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* block_tables;
+  int64_t bt_stride, bt_width;
+  const int32_t* row_ids;
+  int64_t num_blocks, layer, max_q;
+  int32_t hkv, g, bs, d, stride;  // stride: floats between rows of a shared tile
+  float scale_log2;
+  int32_t* err;
+};
+
+struct SimtShared {
+  int64_t row[kBK];  // byte offset of the token's codes, -1: none
+  float ks[kBK], vs[kBK];
+};
+
+// Rows of a shared tile start an odd number of 16-byte units apart, so 16
+// threads reading 16 rows' float4 touch every bank once.
+int tile_stride(int d) {
+  int s = (d + 3) / 4 * 4 + 4;
+  if ((s / 4) % 2 == 0) s += 4;
+  return s;
+}
+size_t simt_smem(int d) {
+  return sizeof(SimtShared) + sizeof(float) * ((size_t)(kBQ + kBK) * tile_stride(d) + kBQ * kPStride);
+}
+
+// grid: (ceil(max_q / kBQ), hq, batch).  NC = ceil(head_dim / 64).
+template <typename T, int NC>
+__global__ void __launch_bounds__(kSimtThreads) fp8_prefill_simt_kernel(const SimtArgs a) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  SimtShared* sh = reinterpret_cast<SimtShared*>(smem_raw);
+  float* qs = reinterpret_cast<float*>(smem_raw + sizeof(SimtShared));
+  float* kv = qs + kBQ * a.stride;
+  float* ps = kv + kBK * a.stride;
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const int64_t b = blockIdx.z;
+  const int hq = blockIdx.y, h = hq / a.g;
+  int64_t qo = 0, nq = a.max_q;
+  if (a.q_offsets) {
+    qo = a.q_offsets[b];
+    nq = (int64_t)a.q_offsets[b + 1] - qo;
+  }
+  const int64_t q0 = ((int64_t)gridDim.x - 1 - blockIdx.x) * kBQ;  // the tiles with most keys first
+  if (q0 >= nq) return;
+  const int64_t len = a.seq_lens[b], prefix = len - nq;
+  const int64_t kend = prefix + min(q0 + kBQ, nq);
+  const int64_t row = a.row_ids ? (int64_t)a.row_ids[b] : b;
+  const int d4 = (a.d + 3) / 4;
+
+  const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_sb + (int64_t)hq * a.q_sh;
+  for (int e = tid; e < kBQ * 4 * d4; e += kSimtThreads) {
+    const int r = e / (4 * d4), d = e - r * 4 * d4;
+    qs[r * a.stride + d] =
+        (q0 + r < nq && d < a.d) ? to_f32<T>(qp[(qo + q0 + r) * a.q_st + d]) * a.scale_log2 : 0.f;
+  }
+  float m[4], l[4], o[4][NC][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) o[i][c][0] = o[i][c][1] = o[i][c][2] = o[i][c][3] = 0.f;
+  }
+
+  auto load_tile = [&](const uint8_t* pool, const float* sc) {
+    const bool words = (a.d & 3) == 0;
+    for (int e = tid; e < kBK * d4; e += kSimtThreads) {
+      const int t = e / d4, c = e - t * d4;
+      const int64_t r = sh->row[t];
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r >= 0) {
+        const float s = sc[t];
+        if (words) {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(pool + r + 4 * c);
+          const float2 lo = e4m3x2_to_float2((uint16_t)w), hi = e4m3x2_to_float2((uint16_t)(w >> 16));
+          x = make_float4(lo.x * s, lo.y * s, hi.x * s, hi.y * s);
+        } else {
+          const uint8_t* p = pool + r + 4 * c;
+          const int n = a.d - 4 * c;
+          x.x = e4m3_to_float(p[0]) * s;
+          if (n > 1) x.y = e4m3_to_float(p[1]) * s;
+          if (n > 2) x.z = e4m3_to_float(p[2]) * s;
+          if (n > 3) x.w = e4m3_to_float(p[3]) * s;
+        }
+      }
+      *reinterpret_cast<float4*>(kv + t * a.stride + 4 * c) = x;
+    }
+  };
+
+  for (int64_t k0 = 0; k0 < kend; k0 += kBK) {
+    __syncthreads();  // the previous tile (and ps) is no longer read; qs is complete
+    if (tid < kBK) {
+      const int64_t t = k0 + tid;
+      int64_t r = -1;
+      if (t < kend) {
+        const int64_t lb = t / a.bs;
+        if (lb >= a.bt_width) {
+          raise_dev(a.err, BL_DEVERR_TABLE);
+        } else {
+          const int64_t phys = a.block_tables[row * a.bt_stride + lb];
+          if (phys < 0 || phys >= a.num_blocks) {
+            raise_dev(a.err, BL_DEVERR_BLOCK_ID);
+          } else {
+            const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + h;
+            r = (slot * a.bs + (t - lb * a.bs)) * a.d;
+            sh->ks[tid] = a.k_scale[slot];
+            sh->vs[tid] = a.v_scale[slot];
+          }
+        }
+      }
+      sh->row[tid] = r;
+    }
+    __syncthreads();
+    load_tile(a.k_pool, sh->ks);
+    __syncthreads();
+    float s[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    for (int d = 0; d < d4; ++d) {
+      float4 qv[4], kx[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(qs + (ty * 4 + i) * a.stride + 4 * d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) kx[j] = *reinterpret_cast<const float4*>(kv + (tx + 16 * j) * a.stride + 4 * d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          s[i][j] = fmaf(qv[i].x, kx[j].x, fmaf(qv[i].y, kx[j].y, fmaf(qv[i].z, kx[j].z, fmaf(qv[i].w, kx[j].w, s[i][j]))));
+    }
+    bool live[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) live[j] = sh->row[tx + 16 * j] >= 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t last = prefix + q0 + ty * 4 + i - k0;  // last key of the tile that the query sees
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!live[j] || tx + 16 * j > last) s[i][j] = -INFINITY;
+        mx = fmaxf(mx, s[i][j]);
+      }
+#pragma unroll
+      for (int of = 1; of < 16; of <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, of));
+      const float mn = fmaxf(m[i], mx);
+      const float al = mn == m[i] ? 1.f : fast_exp2(m[i] - mn);
+      const float u = mn == -INFINITY ? 0.f : mn;
+      m[i] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p = fast_exp2(s[i][j] - u);
+        sum += p;
+        ps[(ty * 4 + i) * kPStride + tx + 16 * j] = p;
+      }
+      l[i] = l[i] * al + sum;  // this thread's keys; the 16 threads' sums are joined at the end
+#pragma unroll
+      for (int c = 0; c < NC; ++c) o[i][c][0] *= al, o[i][c][1] *= al, o[i][c][2] *= al, o[i][c][3] *= al;
+    }
+    __syncthreads();
+    load_tile(a.v_pool, sh->vs);
+    __syncthreads();
+    for (int k = 0; k < kBK; k += 4) {
+      float4 p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const float4*>(ps + (ty * 4 + i) * kPStride + k);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int col = tx * 4 + 64 * c;
+        if (col < 4 * d4) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float4 x = *reinterpret_cast<const float4*>(kv + (k + w) * a.stride + col);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float pw = w == 0 ? p[i].x : w == 1 ? p[i].y : w == 2 ? p[i].z : p[i].w;
+              o[i][c][0] = fmaf(pw, x.x, o[i][c][0]);
+              o[i][c][1] = fmaf(pw, x.y, o[i][c][1]);
+              o[i][c][2] = fmaf(pw, x.z, o[i][c][2]);
+              o[i][c][3] = fmaf(pw, x.w, o[i][c][3]);
+            }
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float sum = l[i];
+#pragma unroll
+    for (int of = 1; of < 16; of <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, of);
+    const int64_t r = q0 + ty * 4 + i;
+    if (r >= nq) continue;
+    T* op = reinterpret_cast<T*>(a.out) + b * a.o_sb + (qo + r) * a.o_st + (int64_t)hq * a.o_sh;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = tx * 4 + 64 * c + e;
+        if (d < a.d) op[d] = from_f32<T>(sum == 0.f ? 0.f : o[i][c][e] / sum);
+      }
+  }
+}
+
+template <typename T, int NC>
+int launch_simt_nc(const SimtArgs& k, dim3 grid, cudaStream_t s) {
+  if (cudaFuncSetAttribute(fp8_prefill_simt_kernel<T, NC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)simt_smem(64 * NC)) != cudaSuccess) {
+    set_error("fp8_prefill_simt_kernel: %s", cudaGetErrorString(cudaGetLastError()));
+    return BL_ERR_LAUNCH;
+  }
+  fp8_prefill_simt_kernel<T, NC><<<grid, kSimtThreads, simt_smem(k.d), s>>>(k);
+  BL_CHECK_LAUNCH("fp8_prefill_simt_kernel");
+  return BL_OK;
+}
+
+template <typename T>
+int launch_simt(const bl_prefill_fp8_args& a, cudaStream_t s) {
+  const bl_paged_layer& kv = a.layer.kv;
+  SimtArgs k;
+  k.q = a.q;
+  k.q_sb = a.q_stride_b, k.q_st = a.q_stride_t, k.q_sh = a.q_stride_h;
+  k.out = a.out;
+  k.o_sb = a.out_stride_b, k.o_st = a.out_stride_t, k.o_sh = a.out_stride_h;
+  k.q_offsets = a.q_offsets;
+  k.seq_lens = a.seq_lens;
+  k.k_pool = (const uint8_t*)kv.k_pool;
+  k.v_pool = (const uint8_t*)kv.v_pool;
+  k.k_scale = a.layer.k_scale;
+  k.v_scale = a.layer.v_scale;
+  k.block_tables = kv.block_tables;
+  k.bt_stride = kv.bt_stride;
+  k.bt_width = kv.bt_width;
+  k.row_ids = kv.row_ids;
+  k.num_blocks = kv.num_blocks;
+  k.layer = kv.layer;
+  k.max_q = a.max_q_len;
+  k.hkv = (int32_t)kv.num_kv_heads;
+  k.g = (int32_t)(a.num_q_heads / kv.num_kv_heads);
+  k.bs = (int32_t)kv.block_size;
+  k.d = (int32_t)kv.head_dim;
+  k.stride = tile_stride(k.d);
+  k.scale_log2 = a.scale * kLog2e;
+  k.err = a.err;
+  dim3 grid((unsigned)((a.max_q_len + kBQ - 1) / kBQ), (unsigned)a.num_q_heads, (unsigned)a.batch);
+  switch ((k.d + 63) / 64) {
+    case 1: return launch_simt_nc<T, 1>(k, grid, s);
+    case 2: return launch_simt_nc<T, 2>(k, grid, s);
+    case 3: return launch_simt_nc<T, 3>(k, grid, s);
+    default: return launch_simt_nc<T, 4>(k, grid, s);
+  }
+}
+
+template <typename T>
+int launch_tc(const bl_prefill_fp8_args& a, const Scratch& w, cudaStream_t s) {
+  const bl_paged_layer& kv = a.layer.kv;
+  char* ws = (char*)a.workspace;
+  ExpandArgs e;
+  e.k_pool = (const uint8_t*)kv.k_pool;
+  e.v_pool = (const uint8_t*)kv.v_pool;
+  e.k_scale = a.layer.k_scale;
+  e.v_scale = a.layer.v_scale;
+  e.k_out = ws + w.k;
+  e.v_out = ws + w.v;
+  e.table = (int32_t*)(ws + w.table);
+  e.num_blocks = kv.num_blocks;
+  e.layer = kv.layer;
+  e.width = w.width;
+  e.pages = w.pages;
+  e.bt_stride = kv.bt_stride;
+  e.bt_width = kv.bt_width;
+  e.block_tables = kv.block_tables;
+  e.row_ids = kv.row_ids;
+  e.seq_lens = a.seq_lens;
+  e.q_offsets = a.q_offsets;
+  e.max_q = a.max_q_len;
+  e.out = a.out;
+  e.o_sb = a.out_stride_b, e.o_st = a.out_stride_t, e.o_sh = a.out_stride_h;
+  e.hkv = (int32_t)kv.num_kv_heads;
+  e.bs = (int32_t)kv.block_size;
+  e.dup = (int32_t)w.dup;
+  e.hq = (int32_t)a.num_q_heads;
+  e.err = a.err;
+  dim3 grid((unsigned)((w.width + kExpandPages - 1) / kExpandPages), (unsigned)e.hkv, (unsigned)a.batch);
+  fp8_expand_kernel<T><<<grid, kExpandThreads, 0, s>>>(e);
+  BL_CHECK_LAUNCH("fp8_expand_kernel");
+
+  bl_prefill_args p;
+  memset(&p, 0, sizeof(p));
+  p.kv.k_pool = e.k_out;
+  p.kv.v_pool = e.v_out;
+  p.kv.num_layers = 1;
+  p.kv.num_blocks = w.pages;
+  p.kv.num_kv_heads = w.heads;
+  p.kv.block_size = kPage;
+  p.kv.head_dim = kTCDim;
+  p.kv.dtype = kv.dtype;
+  p.kv.layer = 0;
+  p.kv.block_tables = e.table;
+  p.kv.bt_stride = w.width;
+  p.kv.bt_width = w.width;
+  p.kv.row_ids = nullptr;
+  p.q = a.q;
+  p.q_stride_b = a.q_stride_b, p.q_stride_t = a.q_stride_t, p.q_stride_h = a.q_stride_h;
+  p.out = a.out;
+  p.out_stride_b = a.out_stride_b, p.out_stride_t = a.out_stride_t, p.out_stride_h = a.out_stride_h;
+  p.q_offsets = a.q_offsets;
+  p.seq_lens = a.seq_lens;
+  p.batch = a.batch;
+  p.num_q_heads = a.num_q_heads;
+  p.max_q_len = a.max_q_len;
+  p.scale = a.scale;
+  p.err = a.err;
+  return prefill_tc_launch(p, s);
+}
+
+// Strides and pointers that the tcgen05 kernel reads pairs of elements through.
+bool tc_alignment(const bl_prefill_fp8_args& a) {
+  return ((uintptr_t)a.q & 3) == 0 && ((uintptr_t)a.out & 3) == 0 && a.q_stride_b % 2 == 0 && a.q_stride_t % 2 == 0 &&
+         a.q_stride_h % 2 == 0 && a.out_stride_b % 2 == 0 && a.out_stride_t % 2 == 0 && a.out_stride_h % 2 == 0;
+}
+
+}  // namespace
+}  // namespace bl
+
+using namespace bl;
+
+extern "C" size_t bl_paged_prefill_fp8_workspace_bytes(int32_t dtype, int64_t batch, int64_t num_q_heads,
+                                                       int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                                       int64_t max_seq_len, int64_t total_blocks) {
+  if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || block_size <= 0 ||
+      max_seq_len <= 0 || total_blocks <= 0 || !use_tc(dtype, head_dim))
+    return 0;
+  Scratch w;
+  return plan_scratch(batch, num_q_heads, num_kv_heads, block_size, max_seq_len, total_blocks, &w) ? w.total : 0;
+}
+
+extern "C" int bl_paged_prefill_fp8(const bl_prefill_fp8_args* args, void* stream) {
+  const char* who = "bl_paged_prefill_fp8";
+  BL_CHECK_ARG(args != nullptr, "%s: args is null", who);
+  const bl_prefill_fp8_args& a = *args;
+  const int rc = check_fp8_layer(a.layer, who);
+  if (rc) return rc;
+  const bl_paged_layer& kv = a.layer.kv;
+  BL_CHECK_ARG(a.q && a.out && a.seq_lens, "%s: null q/out/seq_lens", who);
+  BL_CHECK_ARG(a.batch > 0 && a.batch <= 65535, "%s: batch must be in [1, 65535]", who);
+  BL_CHECK_ARG(a.num_q_heads > 0 && a.num_q_heads <= 65535 && a.num_q_heads % kv.num_kv_heads == 0,
+               "num_heads must divide evenly by num_kv_heads");
+  BL_CHECK_ARG(a.max_q_len > 0 && a.max_q_len <= INT32_MAX, "K/V sequence length must be greater than zero");
+  BL_CHECK_ARG(a.max_seq_len > 0 && a.max_seq_len <= INT32_MAX, "%s: max_seq_len must be in [1, 2^31)", who);
+  BL_CHECK_ARG(a.total_blocks > 0, "%s: total_blocks must be positive", who);
+  const int es = elem_size(kv.dtype);
+  BL_CHECK_ARG(((uintptr_t)a.q % es) == 0 && ((uintptr_t)a.out % es) == 0,
+               "%s: q/out must be aligned to their element type", who);
+  cudaStream_t s = (cudaStream_t)stream;
+  Scratch w;
+  if (use_tc(kv.dtype, kv.head_dim) && tc_alignment(a) &&
+      plan_scratch(a.batch, a.num_q_heads, kv.num_kv_heads, kv.block_size, a.max_seq_len, a.total_blocks, &w)) {
+    if (!a.workspace || a.workspace_bytes < w.total) {
+      set_error("%s: workspace too small (%zu < %zu bytes)", who, a.workspace ? a.workspace_bytes : (size_t)0, w.total);
+      return BL_ERR_CAPACITY;
+    }
+    BL_CHECK_ARG(((uintptr_t)a.workspace & 255) == 0, "%s: workspace must be 256-byte aligned", who);
+    return kv.dtype == BL_BF16 ? launch_tc<__nv_bfloat16>(a, w, s) : launch_tc<__half>(a, w, s);
+  }
+  switch (kv.dtype) {
+    case BL_F32: return launch_simt<float>(a, s);
+    case BL_F16: return launch_simt<__half>(a, s);
+    default: return launch_simt<__nv_bfloat16>(a, s);
+  }
+}

@@ -46,6 +46,7 @@
 // Every mbarrier wait is bounded; on a time-out the CTA records
 // BL_DEVERR_TIMEOUT, drains what it issued and frees its TMEM.
 // Roofline: tensor.  Algorithmic flops per request: 4 * Hq * D * (C*P + C(C+1)/2).
+#include <atomic>
 #include <type_traits>
 
 #include "prefill_tc.cuh"
@@ -554,14 +555,18 @@ size_t smem_bytes() { return 1024 + kSmemData + sizeof(Shared); }
 
 template <bool BF16>
 int launch(const bl_prefill_args& a, cudaStream_t s) {
-  static bool attr_done = false;
-  if (!attr_done) {
+  // the attribute belongs to one device's copy of the kernel: set once per device
+  static std::atomic<bool> attr_done[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const bool known = dev >= 0 && dev < 64 && attr_done[dev].load();
+  if (!known) {
     if (cudaFuncSetAttribute(prefill_tc_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)smem_bytes()) != cudaSuccess) {
       set_error("prefill: cudaFuncSetAttribute failed");
       return BL_ERR_LAUNCH;
     }
-    attr_done = true;
+    if (dev >= 0 && dev < 64) attr_done[dev].store(true);
   }
   Args k;
   k.q = a.q;

@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 import math
 
+import numpy as np
 import torch
 
 from . import _native as nat
@@ -669,6 +670,357 @@ def rms_norm(
                         0 if xo2 is None else xo2.stride(0), o2.stride(0), float(eps), DTYPE_CODE[x.dtype])
     _raise_rc(nat.load().bl_rms_norm(a, _stream(x.device)))
     return out if residual is None else (x_out, out)
+
+
+# ---------------------------------------------------------------------------
+# 8-bit paged cache: e4m3 codes with one power-of-two scale per (layer, block,
+# KV head); a stored value is code * scale (format: include/barellm_b200.h)
+# ---------------------------------------------------------------------------
+FP8_DTYPE = torch.float8_e4m3fn
+
+
+def _call(fn, args, device: torch.device) -> None:
+    """Launches on ``device``'s current stream, whichever device is current."""
+    if _dev_index(device) == torch.cuda.current_device():
+        _raise_rc(fn(args, _stream(device)))
+        return
+    with torch.cuda.device(device):
+        _raise_rc(fn(args, _stream(device)))
+
+
+def _vector_i32(t: torch.Tensor, device: torch.device, n: int, name: str) -> torch.Tensor:
+    _int32_on(t, device, name)
+    _check(t.ndim == 1 and t.shape[0] == n and (n == 1 or t.stride(0) == 1), f"{name} must be a contiguous [{n}] tensor")
+    return t
+
+
+def _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, dtype, batch) -> nat.Fp8Layer:
+    """Checks an 8-bit pool, its scales and its block tables, and describes them."""
+    _require_cuda(key_cache, "key_cache")
+    ks = key_cache.shape
+    dev = key_cache.device
+    _check(key_cache.ndim == 5, "K/V pool must have shape [L, P, H, S, D]")
+    _check(value_cache.shape == ks, "K/V pools must have identical shape")
+    _check(key_cache.dtype is FP8_DTYPE and value_cache.dtype is FP8_DTYPE, "8-bit K/V pools must be float8_e4m3fn")
+    _check(value_cache.device == dev, "K/V device must match")
+    _check(key_cache.is_contiguous() and value_cache.is_contiguous(), "K/V pools must be contiguous")
+    for t, name in ((key_scale, "key_scale"), (value_scale, "value_scale")):
+        _check(t.shape == ks[:3] and t.dtype is torch.float32 and t.device == dev and t.is_contiguous(),
+               f"{name} must be a contiguous float32 [L, P, H] tensor on the pool's device")
+    _check(dtype in DTYPE_CODE, f"unsupported dtype {dtype}")
+    if not 0 <= layer < ks[0]:
+        raise IndexError(f"Invalid layer index: {layer}")
+    _int32_on(block_tables, dev, "block_tables")
+    _check(block_tables.ndim == 2 and block_tables.shape[1] > 0 and (block_tables.shape[1] == 1 or block_tables.stride(1) == 1),
+           "block_tables must be [rows, width] with unit inner stride")
+    if row_ids is not None:
+        _vector_i32(row_ids, dev, batch, "row_ids")
+    else:
+        _check(block_tables.shape[0] >= batch, "block_tables must have a row for every request")
+    # a one-row table may carry any outer stride; the kernels want at least the width
+    pl = nat.PagedLayer(key_cache.data_ptr(), value_cache.data_ptr(), ks[0], ks[1], ks[2], ks[3], ks[4], DTYPE_CODE[dtype],
+                        layer, block_tables.data_ptr(),
+                        block_tables.stride(0) if block_tables.shape[0] > 1 else block_tables.shape[1],
+                        block_tables.shape[1], _ptr(row_ids))
+    return nat.Fp8Layer(pl, key_scale.data_ptr(), value_scale.data_ptr())
+
+
+def _softmax_scale(scale: float | None, d: int) -> float:
+    s = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    _check(0.0 < s < math.inf, "scale must be positive and finite")
+    return s
+
+
+def _err_word(err: torch.Tensor | None, device: torch.device) -> int | None:
+    if err is None:
+        return None
+    _check(err.dtype is torch.int32 and err.device == device and err.numel() >= 1, f"err must be an int32 tensor on {device}")
+    return err.data_ptr()
+
+
+def _scratch(ws: torch.Tensor | None, nbytes: int, device: torch.device) -> torch.Tensor:
+    """The caller's workspace, or a fresh one from torch's allocator (so calls
+    on several streams, and several captured graphs, never share scratch)."""
+    if ws is None:
+        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+    _check(ws.device == device and ws.is_contiguous(), f"ws must be a contiguous tensor on {device}")
+    return ws
+
+
+def paged_append_fp8(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scale: torch.Tensor,
+    value_scale: torch.Tensor,
+    layer: int,
+    block_tables: torch.Tensor,
+    start_pos: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    *,
+    row_ids: torch.Tensor | None = None,
+    new_offsets: torch.Tensor | None = None,
+    max_new_tokens: int | None = None,
+    err: torch.Tensor | None = None,
+) -> None:
+    """Quantises new K/V tokens into their 8-bit pool slots.
+
+    The 8-bit form of :func:`paged_append` (same arguments, plus the scale
+    tables ``[L, P, Hkv]``).  A block that receives tokens gets the scale
+    ``max(its old scale if it holds tokens before start_pos, the smallest
+    power of two that brings the new tokens' largest finite magnitude to at most
+    448)``, per KV head, K and V apart; the codes it already holds are rounded
+    to a raised scale.  Infinities saturate, NaN stays NaN, slots behind the
+    new tokens keep their bytes.  A block may receive tokens from one row of a
+    call only.
+    """
+    batch = start_pos.shape[0]
+    fl = _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, key.dtype, batch)
+    dev = key_cache.device
+    _check(key.ndim == 4 and value.ndim == 4, "K/V must have shape [B, H, T, D]")
+    _check(key.shape == value.shape, "K/V must have identical shape")
+    _check(key.shape[1] == key_cache.shape[2], "KV-head count cannot change")
+    _check(key.shape[2] > 0, "K/V sequence length must be greater than zero")
+    _check(key.shape[3] == key_cache.shape[4], "Head dimension cannot change")
+    _check(key.dtype == value.dtype, "K/V dtype must match")
+    _check(key.device == dev and value.device == dev, "K/V device cannot change")
+    _check((key.stride(3) == 1 and value.stride(3) == 1) or key.shape[3] == 1, "K/V head_dim must be contiguous")
+    _vector_i32(start_pos, dev, batch, "start_pos")
+    packed = new_offsets is not None
+    if packed:
+        _vector_i32(new_offsets, dev, batch + 1, "new_offsets")
+        _check(key.shape[0] == 1, "packed K/V need [1, H, T, D] and [B+1] offsets")
+        _check(max_new_tokens is not None and max_new_tokens > 0, "packed append needs max_new_tokens")
+    else:
+        _check(key.shape[0] == batch, "batch size must match number of caches")
+    ks, vs = key.stride(), value.stride()
+    a = nat.AppendFp8Args(fl, key.data_ptr(), value.data_ptr(), 0 if packed else ks[0], ks[1], ks[2],
+                          0 if packed else vs[0], vs[1], vs[2], start_pos.data_ptr(), _ptr(new_offsets), batch,
+                          int(max_new_tokens) if packed else key.shape[2], _err_word(err, dev))
+    _call(nat.load().bl_paged_append_fp8, a, dev)
+
+
+def paged_gather_fp8(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scale: torch.Tensor,
+    value_scale: torch.Tensor,
+    layer: int,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    max_len: int,
+    *,
+    dtype: torch.dtype,
+    row_ids: torch.Tensor | None = None,
+    out: tuple[torch.Tensor, torch.Tensor] | None = None,
+    zero_fill: bool = True,
+    err: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Dense ``[B, Hkv, max_len, D]`` copy of the cached tokens' values
+    (code * scale) in ``dtype``, zero padded: the 8-bit form of
+    :func:`paged_gather`.  Values saturate at the type's largest finite value.
+    """
+    batch = seq_lens.shape[0]
+    fl = _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, dtype, batch)
+    dev = key_cache.device
+    _vector_i32(seq_lens, dev, batch, "seq_lens")
+    _check(max_len > 0, "KV cache is empty")
+    shape = (batch, key_cache.shape[2], max_len, key_cache.shape[4])
+    if out is None:
+        k_out = torch.empty(shape, dtype=dtype, device=dev)
+        v_out = torch.empty_like(k_out)
+    else:
+        k_out, v_out = out
+        for t in out:
+            _check(t.shape == shape and t.dtype is dtype and t.device == dev, "gather output must be [B, H, max_len, D] of dtype")
+        _check(k_out.stride() == v_out.stride() and (k_out.stride(3) == 1 or shape[3] == 1),
+               "gather outputs need identical strides, D contiguous")
+    a = nat.GatherFp8Args(fl, seq_lens.data_ptr(), batch, k_out.data_ptr(), v_out.data_ptr(), k_out.stride(0),
+                          k_out.stride(1), k_out.stride(2), max_len, 1 if zero_fill else 0, _err_word(err, dev))
+    _call(nat.load().bl_paged_gather_fp8, a, dev)
+    return k_out, v_out
+
+
+def decode_fp8_workspace_bytes(batch: int, num_q_heads: int, head_dim: int, max_seq_len: int) -> int:
+    return int(nat.load().bl_paged_decode_fp8_workspace_bytes(batch, num_q_heads, head_dim, max_seq_len))
+
+
+def paged_decode_fp8(
+    q: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scale: torch.Tensor,
+    value_scale: torch.Tensor,
+    layer: int,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    max_seq_len: int,
+    *,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+    row_ids: torch.Tensor | None = None,
+    ws: torch.Tensor | None = None,
+    plan_ready: bool = False,
+    err: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """One-token GQA attention over an 8-bit paged cache; returns ``[B, Hq, D]``.
+
+    The 8-bit form of :func:`paged_decode`.  ``seq_lens`` are post-append
+    lengths; a row of length 0 gets zeros.  ``max_seq_len`` is a host-side
+    upper bound on them.  ``ws``: at least :func:`decode_fp8_workspace_bytes`;
+    by default every call takes its own from torch's allocator.  With
+    ``plan_ready`` the (required) ``ws`` still holds the plan of an earlier call
+    with the same ``seq_lens``, ``max_seq_len`` and q shape, as a step's later
+    layers have it.
+    """
+    _require_cuda(q, "q")
+    if q.ndim == 4:
+        _check(q.shape[2] == 1, "decode takes one query token per request")
+        q3 = q[:, :, 0, :]
+    else:
+        q3 = q
+    _check(q3.ndim == 3, "q must be [B, Hq, D] or [B, Hq, 1, D]")
+    batch, hq, d = q3.shape
+    fl = _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, q3.dtype, batch)
+    dev = key_cache.device
+    _check(q3.device == dev, "q must be on the K/V pool's device")
+    _check(d == key_cache.shape[4], "Head dimension cannot change")
+    _check(q3.stride(2) == 1 or d == 1, "q head_dim must be contiguous")
+    _check(hq > 0 and hq % key_cache.shape[2] == 0, "num_heads must divide evenly by num_kv_heads")
+    _vector_i32(seq_lens, dev, batch, "seq_lens")
+    _check(max_seq_len > 0, "KV cache is empty")
+    if out is None:
+        out = torch.empty((batch, hq, d), dtype=q3.dtype, device=dev)
+        out3 = out
+    else:
+        out3 = out[:, :, 0, :] if out.ndim == 4 else out
+        _check(out3.shape == q3.shape and (out3.stride(2) == 1 or d == 1) and out3.dtype is q3.dtype and out3.device == dev,
+               "decode output must be [B, Hq, D] like q, D contiguous")
+    _check(ws is not None or not plan_ready, "plan_ready needs the workspace that holds the plan")
+    ws = _scratch(ws, decode_fp8_workspace_bytes(batch, hq, d, max_seq_len), dev)
+    a = nat.DecodeFp8Args(fl, q3.data_ptr(), q3.stride(0), q3.stride(1), out3.data_ptr(), out3.stride(0), out3.stride(1),
+                          seq_lens.data_ptr(), batch, hq, _softmax_scale(scale, d), 1 if plan_ready else 0, ws.data_ptr(),
+                          ws.numel() * ws.element_size(), max_seq_len, _err_word(err, dev))
+    _call(nat.load().bl_paged_decode_fp8, a, dev)
+    return out
+
+
+def paged_prefill_fp8(
+    q: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scale: torch.Tensor,
+    value_scale: torch.Tensor,
+    layer: int,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    max_seq_len: int,
+    *,
+    total_blocks: int | None = None,
+    q_offsets: torch.Tensor | None = None,
+    max_q_len: int | None = None,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+    row_ids: torch.Tensor | None = None,
+    ws: torch.Tensor | None = None,
+    err: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Causal attention of new queries over an 8-bit cached prefix plus
+    themselves: the 8-bit form of :func:`paged_prefill` (same query layouts and
+    result layout).  Queries that see no key (a row with more queries than
+    tokens) get zeros.
+
+    ``max_seq_len`` and ``total_blocks`` are host-side upper bounds on
+    ``seq_lens`` and on the rows' blocks together (default: ``max_seq_len`` for
+    every row); they size the scratch into which the tensor-core path expands
+    the rows' pages.
+    """
+    _require_cuda(q, "q")
+    _check(q.ndim == 4, "q must be [B, Hq, T, D]")
+    b0, hq, t, d = q.shape
+    batch = seq_lens.shape[0]
+    fl = _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, q.dtype, batch)
+    dev = key_cache.device
+    hkv, bs = key_cache.shape[2], key_cache.shape[3]
+    _check(q.device == dev, "q must be on the K/V pool's device")
+    _check(d == key_cache.shape[4], "Head dimension cannot change")
+    _check(t > 0, "K/V sequence length must be greater than zero")
+    _check(q.stride(3) == 1 or d == 1, "q head_dim must be contiguous")
+    _check(hq > 0 and hq % hkv == 0, "num_heads must divide evenly by num_kv_heads")
+    _vector_i32(seq_lens, dev, batch, "seq_lens")
+    _check(max_seq_len > 0, "KV cache is empty")
+    packed = q_offsets is not None
+    if packed:
+        _vector_i32(q_offsets, dev, batch + 1, "q_offsets")
+        _check(b0 == 1, "packed queries need [1, Hq, T, D] and [B+1] offsets")
+        _check(max_q_len is not None and max_q_len > 0, "packed prefill needs max_q_len")
+        mq = int(max_q_len)
+    else:
+        _check(b0 == batch, "batch size must match number of caches")
+        mq = t
+    if total_blocks is None:
+        total_blocks = batch * -(-max_seq_len // bs)
+    _check(total_blocks > 0, "total_blocks must be positive")
+    if out is None:
+        out = torch.empty((b0, t, hq, d), dtype=q.dtype, device=dev).transpose(1, 2)
+    _check(out.shape == q.shape and (out.stride(3) == 1 or d == 1) and out.dtype is q.dtype and out.device == dev,
+           "prefill output must match q's shape, D contiguous")
+    lib = nat.load()
+    nbytes = int(lib.bl_paged_prefill_fp8_workspace_bytes(DTYPE_CODE[q.dtype], batch, hq, hkv, d, bs, max_seq_len, total_blocks))
+    ws = _scratch(ws, nbytes, dev)
+    qs, os_ = q.stride(), out.stride()
+    a = nat.PrefillFp8Args(fl, q.data_ptr(), 0 if packed else qs[0], qs[2], qs[1], out.data_ptr(), 0 if packed else os_[0],
+                           os_[2], os_[1], _ptr(q_offsets), seq_lens.data_ptr(), batch, hq, mq, _softmax_scale(scale, d), 0,
+                           max_seq_len, total_blocks, ws.data_ptr(), ws.numel() * ws.element_size(), _err_word(err, dev))
+    _call(lib.bl_paged_prefill_fp8, a, dev)
+    return out
+
+
+def _block_ids(ids, name: str, num_blocks: int) -> np.ndarray:
+    a = np.asarray(ids)
+    if a.size == 0:
+        return np.zeros(0, dtype=np.int32)
+    _check(a.ndim == 1 and a.dtype.kind in "iu", f"{name} must be a sequence of block ids")
+    _check(int(a.min()) >= 0 and int(a.max()) < num_blocks, f"{name} holds a block id outside the pool")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
+def copy_blocks(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    src,
+    dst,
+    *,
+    key_scale: torch.Tensor | None = None,
+    value_scale: torch.Tensor | None = None,
+) -> None:
+    """Copies whole blocks inside a pool, every layer, K and V:
+    ``pool[:, dst[i]] = pool[:, src[i]]`` (and the scales of an 8-bit pool).
+
+    ``src`` / ``dst`` are host sequences of block ids (as ``BlockPool`` hands
+    them out).  A block that would be written twice, or both read and written,
+    raises ``ValueError`` before anything is copied."""
+    _require_cuda(key_cache, "key_cache")
+    _check(key_cache.ndim == 5, "K/V pool must have shape [L, P, H, S, D]")
+    _check(key_cache.shape == value_cache.shape, "K/V pools must have identical shape")
+    _check(key_cache.dtype == value_cache.dtype, "K/V dtype must match")
+    _check(key_cache.device == value_cache.device, "K/V device must match")
+    _check(key_cache.is_contiguous() and value_cache.is_contiguous(), "K/V pools must be contiguous")
+    _check(key_cache.dtype in DTYPE_CODE or key_cache.dtype is FP8_DTYPE, f"unsupported dtype {key_cache.dtype}")
+    _check((key_cache.dtype is FP8_DTYPE) == (key_scale is not None) == (value_scale is not None),
+           "8-bit pools, and only they, are copied with their scales")
+    l, p, h, s, d = key_cache.shape
+    for t, name in ((key_scale, "key_scale"), (value_scale, "value_scale")):
+        _check(t is None or (t.shape == (l, p, h) and t.dtype is torch.float32 and t.device == key_cache.device
+                             and t.is_contiguous()),
+               f"{name} must be a contiguous float32 [L, P, H] tensor on the pool's device")
+    sa, da = _block_ids(src, "src", p), _block_ids(dst, "dst", p)
+    _check(sa.size == da.size, "src and dst must have the same length")
+    if sa.size == 0:
+        return
+    a = nat.CopyBlocksArgs(key_cache.data_ptr(), value_cache.data_ptr(), _ptr(key_scale), _ptr(value_scale), l, p, h, s, d,
+                           key_cache.element_size(), sa.ctypes.data, da.ctypes.data, sa.size)
+    _call(nat.load().bl_copy_blocks, a, key_cache.device)
 
 
 def decode_path(dtype: torch.dtype, head_dim: int, block_size: int, num_q_heads: int, num_kv_heads: int) -> int:

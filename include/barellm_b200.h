@@ -379,6 +379,157 @@ typedef struct bl_rms_norm_args {
 BL_API int bl_rms_norm(const bl_rms_norm_args* args, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* 8-bit paged cache.                                                        */
+/*                                                                          */
+/* The pools hold e4m3 codes (1 byte) in the layout above; k_scale and       */
+/* v_scale hold one fp32 scale for each (layer, block, KV head):             */
+/* [num_layers, num_blocks, num_kv_heads].  A stored value is code * scale.  */
+/* kv.dtype is the element type of the caller's K, V, q and output tensors.  */
+/* Pools must be 16-byte aligned; head_dim <= 256.                           */
+/* A scale is a power of two, 2^k with k in [-100, 119]: the smallest with   */
+/* max |x| <= 448 * 2^k over the block's finite values.  Infinities are      */
+/* stored as +-448 codes, NaN stays NaN.                                     */
+/* The reference keeps its cache in the model's element type only; each      */
+/* entry point below is the 8-bit form of the one that it names.             */
+typedef struct bl_fp8_layer {
+  bl_paged_layer kv;
+  float* k_scale;
+  float* v_scale;
+} bl_fp8_layer;
+
+/* Quantising append (bl_paged_append).  A block that receives tokens gets    */
+/* the scale max(old scale if it holds tokens before start_pos, the scale    */
+/* the new tokens need); where that raises the scale, the codes it holds are */
+/* rounded to the new one.  Slots behind the new tokens are left as they     */
+/* were.  A block may receive tokens from one row of a call only: two rows   */
+/* that share a block which both append to are not supported.                */
+typedef struct bl_append_fp8_args {
+  bl_fp8_layer layer;
+  const void* k_new;
+  const void* v_new;
+  int64_t new_stride_b;
+  int64_t new_stride_h;
+  int64_t new_stride_t;
+  int64_t v_stride_b;
+  int64_t v_stride_h;
+  int64_t v_stride_t;
+  const int32_t* start_pos;   /* [batch], device */
+  const int32_t* new_offsets; /* [batch+1], device, or NULL */
+  int64_t batch;
+  int64_t max_new_tokens;
+  int32_t* err;               /* device int32 or NULL */
+} bl_append_fp8_args;
+
+BL_API int bl_paged_append_fp8(const bl_append_fp8_args* args, void* stream);
+
+/* Dequantising dense read (bl_paged_gather): code * scale in kv.dtype,       */
+/* saturating at the type's largest finite value.                            */
+typedef struct bl_gather_fp8_args {
+  bl_fp8_layer layer;
+  const int32_t* seq_lens; /* [batch], device */
+  int64_t batch;
+  void* k_out;
+  void* v_out;
+  int64_t out_stride_b;
+  int64_t out_stride_h;
+  int64_t out_stride_t;
+  int64_t max_len;
+  int32_t zero_fill;
+  int32_t* err;
+} bl_gather_fp8_args;
+
+BL_API int bl_paged_gather_fp8(const bl_gather_fp8_args* args, void* stream);
+
+/* Decode attention over the 8-bit pages (bl_paged_decode), one query token  */
+/* per request.  A row of length 0 gets zeros.  Rows are split into fixed    */
+/* 512-token chunks, as there: a row's result does not depend on the batch.  */
+/* plan_ready: the workspace holds the plan that an earlier call with the    */
+/* same seq_lens, batch, num_q_heads, head_dim and max_seq_len left there.   */
+typedef struct bl_decode_fp8_args {
+  bl_fp8_layer layer;
+  const void* q;
+  int64_t q_stride_b;
+  int64_t q_stride_h;
+  void* out;
+  int64_t out_stride_b;
+  int64_t out_stride_h;
+  const int32_t* seq_lens; /* [batch], device */
+  int64_t batch;
+  int64_t num_q_heads;
+  float scale;
+  int32_t plan_ready;
+  void* workspace; /* device scratch, >= bl_paged_decode_fp8_workspace_bytes, 256-byte aligned */
+  size_t workspace_bytes;
+  int64_t max_seq_len; /* host upper bound on seq_lens[] */
+  int32_t* err;
+} bl_decode_fp8_args;
+
+BL_API size_t bl_paged_decode_fp8_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t head_dim,
+                                                  int64_t max_seq_len);
+BL_API int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream);
+
+/* Chunked-prefill attention over the 8-bit pages (bl_paged_prefill): query i */
+/* of a row with C queries sees keys 0 .. seq_len - C + i.  Queries of a row  */
+/* that see no key get zeros.                                                */
+/* max_seq_len and total_blocks are host upper bounds on seq_lens[] and on   */
+/* the sum over the rows of ceil(seq_len / block_size); they size the        */
+/* workspace (0 bytes where the call needs none).                            */
+typedef struct bl_prefill_fp8_args {
+  bl_fp8_layer layer;
+  const void* q;
+  int64_t q_stride_b;
+  int64_t q_stride_t;
+  int64_t q_stride_h;
+  void* out;
+  int64_t out_stride_b;
+  int64_t out_stride_t;
+  int64_t out_stride_h;
+  const int32_t* q_offsets; /* [batch+1], device, or NULL */
+  const int32_t* seq_lens;  /* [batch], device: prefix + C_b */
+  int64_t batch;
+  int64_t num_q_heads;
+  int64_t max_q_len;
+  float scale;
+  int32_t pad0;
+  int64_t max_seq_len;
+  int64_t total_blocks;
+  void* workspace; /* device scratch, >= bl_paged_prefill_fp8_workspace_bytes, 256-byte aligned */
+  size_t workspace_bytes;
+  int32_t* err;
+} bl_prefill_fp8_args;
+
+BL_API size_t bl_paged_prefill_fp8_workspace_bytes(int32_t dtype, int64_t batch, int64_t num_q_heads,
+                                                   int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                                   int64_t max_seq_len, int64_t total_blocks);
+BL_API int bl_paged_prefill_fp8(const bl_prefill_fp8_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Page copies: pool[l, dst[i]] = pool[l, src[i]] for every layer l, K and V */
+/* (and their scales when given), any element type.  What forking a request  */
+/* or moving its pages needs; no counterpart in the reference.               */
+/* src and dst are HOST arrays: the ids travel in the kernels' parameters.   */
+/* Ids outside the pool, a block that is written twice, and a block that is  */
+/* both read and written are refused, so the order of the copies does not    */
+/* matter.  count 0 does nothing.                                            */
+typedef struct bl_copy_blocks_args {
+  void* k_pool;
+  void* v_pool;
+  float* k_scale; /* [num_layers, num_blocks, num_kv_heads] or NULL (both) */
+  float* v_scale;
+  int64_t num_layers;
+  int64_t num_blocks;
+  int64_t num_kv_heads;
+  int64_t block_size;
+  int64_t head_dim;
+  int64_t elem_bytes;
+  const int32_t* src;
+  const int32_t* dst;
+  int64_t count;
+} bl_copy_blocks_args;
+
+BL_API int bl_copy_blocks(const bl_copy_blocks_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Misc.                                                                     */
 BL_API const char* bl_last_error(void);
 BL_API int bl_abi_version(void);

@@ -1,0 +1,356 @@
+"""Decode and chunked prefill over 8-bit pages against float64 attention on the
+stored values; the bounds follow from the kernels' arithmetic
+(fp8_helpers.attention_bound)."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from barellm_b200 import _native as nat
+from barellm_b200 import ops
+from fp8_helpers import Pool, assert_within, attention_bound, filled, i32
+from oracle import fp8_oracle as f8
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def check_decode(out, q, pool, table, lens, layer, scale=None):
+    eps = 2.0 ** -11 if q.dtype is not F32 else 0.0  # P in fp16 on the tensor cores
+    qn, got = q.double().cpu().numpy(), out.double().cpu().numpy()
+    for b, n in enumerate(lens):
+        k, v = (f8.read(c, s, layer, table[b], n) for c, s in zip(pool.codes, pool.scales))
+        want, spread, reach, flat = f8.attention(qn[b][:, None], k, v, scale)
+        assert_within(got[b][:, None], want, attention_bound(want, spread, reach, flat, qn[b][:, None], q.dtype, eps, n))
+
+
+SHAPES = [  # hq, hkv, bs, d
+    (16, 8, 16, 128), (32, 8, 16, 128), (8, 8, 16, 128), (16, 1, 16, 128), (12, 4, 16, 128), (20, 2, 32, 128), (8, 2, 48, 128),
+    (16, 8, 16, 64), (9, 1, 16, 64), (8, 2, 16, 256), (11, 1, 32, 256), (12, 4, 8, 128), (4, 2, 16, 80), (6, 3, 5, 3), (2, 1, 1, 256),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("hq,hkv,bs,d", SHAPES)
+def test_decode(cuda, native_lib, dtype, hq, hkv, bs, d):
+    lens = [1, 0, 15, 16, 17, 31, 33, 511, 512, 513, 1100]
+    pool, table, bt = filled(cuda, lens, hkv, bs, d, dtype, seed=hq * 7 + d)
+    q = torch.randn(len(lens), hq, d, generator=torch.Generator().manual_seed(d)).to(dtype).to(cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = ops.paged_decode_fp8(q, *pool.args, 1, bt, i32(lens, cuda), 1100, err=err)
+    assert int(err) == 0
+    assert bool((out[1] == 0).all())
+    check_decode(out, q, pool, table, lens, 1)
+
+
+@pytest.mark.parametrize("max_len", [5, 512])
+def test_decode_short_rows_and_no_rows(cuda, native_lib, max_len):
+    """Calls whose rows all fit one chunk have no join kernel; empty rows are zeros there too."""
+    lens = [0, 5, 1, 0, max_len]
+    pool, table, bt = filled(cuda, lens, 8, 16, 128, BF16)
+    q = torch.randn(5, 16, 128, device=cuda).to(BF16)
+    out = torch.full((5, 16, 128), 9.0, dtype=BF16, device=cuda)
+    ops.paged_decode_fp8(q, *pool.args, 1, bt, i32(lens, cuda), max_len, out=out)
+    check_decode(out, q, pool, table, lens, 1)
+    out.fill_(9.0)
+    ops.paged_decode_fp8(q, *pool.args, 1, bt, i32([0] * 5, cuda), max_len, out=out)
+    assert bool((out == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_decode_long_row(cuda, native_lib, dtype):
+    lens = [20000, 3]
+    pool, table, bt = filled(cuda, lens, 2, 16, 128, dtype, layers=1, layer=0)
+    q = torch.randn(2, 8, 128, device=cuda).to(dtype)
+    out = ops.paged_decode_fp8(q, *pool.args, 0, bt, i32(lens, cuda), 20000)
+    check_decode(out, q, pool, table, lens, 0)
+
+
+@pytest.mark.parametrize("spread", [4.0, 12.0])
+def test_decode_scales_far_apart(cuda, native_lib, spread):
+    """Blocks whose V scales differ by many binades: the running reference moves up, and small blocks are added apart."""
+    rs = np.random.RandomState(int(spread))
+    n, h, d = 700, 2, 128
+    pool = Pool(cuda, 1, 50, h, 16, d)
+    table = pool.table([n])
+    bt = torch.from_numpy(table).to(cuda)
+    size = np.exp2(np.repeat(rs.uniform(-spread, spread, (h, 44)), 16, axis=1)[:, :n, None])
+    k = rs.randn(1, h, n, d).astype(np.float32)
+    v = (rs.randn(h, n, d) * size).astype(np.float32)[None]
+    v[0, 0, 96:112] = 0.0  # a block of zeros has the smallest scale there is
+    ops.paged_append_fp8(*pool.args, 0, bt, i32([0], cuda), torch.from_numpy(k).to(cuda), torch.from_numpy(v).to(cuda))
+    pool.download()
+    for dtype in (BF16, F16, F32):
+        q = (3 * torch.randn(1, 8, d, generator=torch.Generator().manual_seed(1))).to(dtype).to(cuda)
+        check_decode(ops.paged_decode_fp8(q, *pool.args, 0, bt, i32([n], cuda), n), q, pool, table, [n], 0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("factor", [0.0, 2.0 ** -40, 30.0])
+def test_decode_q_magnitudes(cuda, native_lib, dtype, factor):
+    """q of any magnitude (bf16 reaches far past fp16), sharp softmaxes, a head of zeros."""
+    pool, table, bt = filled(cuda, [600], 2, 16, 128, dtype)
+    q = torch.randn(1, 4, 128, generator=torch.Generator().manual_seed(2))
+    q[0, 1] *= 2.0 ** 10
+    q[0, 2] = 0
+    q[0, 3, ::3] *= 2.0 ** -9
+    q = (q * factor).to(dtype).to(cuda)
+    check_decode(ops.paged_decode_fp8(q, *pool.args, 1, bt, i32([600], cuda), 600), q, pool, table, [600], 1)
+    scale = 0.7
+    out = ops.paged_decode_fp8(q, *pool.args, 1, bt, i32([600], cuda), 600, scale=scale)
+    check_decode(out, q, pool, table, [600], 1, scale)
+
+
+def test_decode_nan_in_the_cache_reaches_its_head_only(cuda, native_lib):
+    pool, table, bt = filled(cuda, [40, 40], 2, 16, 128, BF16)
+    x = torch.randn(2, 2, 1, 128, device=cuda).to(BF16)
+    x[0, 1, 0, 7] = float("nan")
+    for which in (0, 1):  # K, then V
+        p, t, b = filled(cuda, [40, 40], 2, 16, 128, BF16)
+        kv = [torch.randn_like(x), torch.randn_like(x)]
+        kv[which] = x
+        ops.paged_append_fp8(*p.args, 1, b, i32([39, 39], cuda), *kv)
+        q = torch.randn(2, 4, 128, device=cuda).to(BF16)
+        nan = torch.isnan(ops.paged_decode_fp8(q, *p.args, 1, b, i32([40, 40], cuda), 40))
+        want = torch.zeros_like(nan)
+        if which == 0:
+            want[0, 2:] = True
+        else:
+            want[0, 2:, 7] = True
+        assert torch.equal(nan, want)
+
+
+def test_decode_layouts_plan_reuse_and_batch_invariance(cuda, native_lib):
+    lens = [900, 1, 513, 40, 2000, 16]
+    pool, table, bt = filled(cuda, lens, 8, 16, 128, BF16)
+    q = torch.randn(6, 32, 128, device=cuda).to(BF16)
+    seq = i32(lens, cuda)
+    base = ops.paged_decode_fp8(q, *pool.args, 1, bt, seq, 2000)
+    # every row alone, bit for bit
+    for b in range(6):
+        alone = ops.paged_decode_fp8(q[b:b + 1], *pool.args, 1, bt[b:b + 1], seq[b:b + 1], lens[b])
+        assert torch.equal(alone[0], base[b])
+    # row indirection
+    rows = i32([4, 0, 2], cuda)
+    assert torch.equal(ops.paged_decode_fp8(q[[4, 0, 2]], *pool.args, 1, bt, seq[[4, 0, 2]], 2000, row_ids=rows), base[[4, 0, 2]])
+    # [B, Hq, 1, D] views, strided and misaligned q and out
+    wide = torch.zeros(6, 32, 3, 131, dtype=BF16, device=cuda)
+    wide[:, :, 1, 1:129] = q
+    out = torch.zeros(6, 40, 1, 130, dtype=BF16, device=cuda)
+    ops.paged_decode_fp8(wide[:, :, 1:2, 1:129], *pool.args, 1, bt, seq, 2000, out=out[:, 4:36, :, 1:129])
+    assert torch.equal(out[:, 4:36, 0, 1:129], base)
+    out[:, 4:36, :, 1:129] = 0
+    assert not bool(out.any())
+    # the plan of one layer serves the next
+    ws = torch.empty(ops.decode_fp8_workspace_bytes(6, 32, 128, 2000), dtype=torch.uint8, device=cuda)
+    assert torch.equal(ops.paged_decode_fp8(q, *pool.args, 1, bt, seq, 2000, ws=ws), base)
+    assert torch.equal(ops.paged_decode_fp8(q, *pool.args, 1, bt, seq, 2000, ws=ws, plan_ready=True), base)
+
+
+def test_decode_reports_what_it_cannot_do(cuda, native_lib):
+    pool, table, bt = filled(cuda, [40, 600], 2, 16, 128, BF16)
+    q = torch.randn(2, 4, 128, device=cuda).to(BF16)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+
+    def word(**kw):
+        err.zero_()
+        a = dict(bt=bt, seq=i32([40, 600], cuda), n=600, ws=None, plan_ready=False) | kw
+        ops.paged_decode_fp8(q, *pool.args, 1, a["bt"], a["seq"], a["n"], ws=a["ws"], plan_ready=a["plan_ready"], err=err)
+        return int(err)
+
+    assert word() == 0
+    bad = bt.clone()
+    bad[1, 3] = 1 << 20
+    assert word(bt=bad) == nat.BL_DEVERR_BLOCK_ID
+    assert word(bt=bt[:, :20].contiguous()) & nat.BL_DEVERR_TABLE
+    assert word(n=100) & nat.BL_DEVERR_WORKSPACE  # a row longer than max_seq_len
+    blank = torch.zeros(ops.decode_fp8_workspace_bytes(2, 4, 128, 600), dtype=torch.uint8, device=cuda)
+    assert word(ws=blank, plan_ready=True) == nat.BL_DEVERR_WORKSPACE
+
+
+def prefill_case(device, prefixes, chunks, hq, hkv, bs, d, dtype, seed=0):
+    lens = [p + c for p, c in zip(prefixes, chunks)]
+    pool, table, bt = filled(device, lens, hkv, bs, d, dtype, seed=seed)
+    n = sum(chunks)
+    q = torch.randn(n, hq, d, generator=torch.Generator().manual_seed(seed)).to(dtype).to(device).unsqueeze(0).transpose(1, 2)
+    off = i32(np.concatenate([[0], np.cumsum(chunks)]), device)
+    return pool, table, bt, lens, q, off
+
+
+def check_prefill(out, q, pool, table, lens, chunks, layer, scale=None, tc=True):
+    eps = torch.finfo(q.dtype).eps / 2 if tc else 0.0  # P in the element type on the tensor cores
+    got, qn, at = out.double().cpu().numpy()[0], q.double().cpu().numpy()[0], 0
+    for b, (n, c) in enumerate(zip(lens, chunks)):
+        k, v = (f8.read(x, s, layer, table[b], n) for x, s in zip(pool.codes, pool.scales))
+        want, spread, reach, flat = f8.attention(qn[:, at:at + c], k, v, scale)
+        bound = attention_bound(want, spread, reach, flat, qn[:, at:at + c], q.dtype, eps, n)
+        assert_within(got[:, at:at + c], want, bound)
+        at += c
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("hq,hkv,bs,d", SHAPES)
+def test_prefill(cuda, native_lib, dtype, hq, hkv, bs, d):
+    prefixes, chunks = [0, 0, 5, 130, 16, 700], [1, 33, 1, 70, 200, 40]
+    pool, table, bt, lens, q, off = prefill_case(cuda, prefixes, chunks, hq, hkv, bs, d, dtype, seed=hq + d)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    total = sum(-(-n // bs) for n in lens)
+    out = ops.paged_prefill_fp8(q, *pool.args, 1, bt, i32(lens, cuda), max(lens), total_blocks=total, q_offsets=off,
+                                max_q_len=max(chunks), err=err)
+    assert int(err) == 0
+    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32 and d == 128)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64), (F32, 128)])
+def test_prefill_queries_that_see_no_key(cuda, native_lib, dtype, d):
+    """More queries than tokens: the first ones see nothing and get zeros; an empty row gets zeros throughout."""
+    chunks, lens = [40, 7, 300, 5], [13, 0, 2, 5]
+    pool, table, bt = filled(cuda, lens, 2, 16, d, dtype)
+    q = torch.randn(1, 8, sum(chunks), d, device=cuda).to(dtype)
+    off = i32(np.concatenate([[0], np.cumsum(chunks)]), cuda)
+    out = torch.full_like(q, 5.0)
+    ops.paged_prefill_fp8(q, *pool.args, 1, bt, i32(lens, cuda), 13, q_offsets=off, max_q_len=300, out=out)
+    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32 and d == 128)
+    assert bool((out[0, :, :27] == 0).all()) and bool((out[0, :, 40:47] == 0).all())
+
+
+def test_prefill_rectangular_strided_and_bounds(cuda, native_lib):
+    lens, t = [50, 300, 33], 33
+    pool, table, bt = filled(cuda, lens, 8, 16, 128, BF16)
+    q = torch.randn(3, 16, t, 128, device=cuda).to(BF16)
+    seq = i32(lens, cuda)
+    base = ops.paged_prefill_fp8(q, *pool.args, 1, bt, seq, 300)
+    assert base.shape == q.shape and base.transpose(1, 2).is_contiguous()
+    packed = torch.cat(list(q), dim=1).unsqueeze(0)
+    check_prefill(torch.cat(list(base), dim=1).unsqueeze(0), packed, pool, table, lens, [t] * 3, 1)
+    # a larger bound, its own workspace and row indirection change nothing
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device=cuda)
+    assert torch.equal(ops.paged_prefill_fp8(q[[2, 0]], *pool.args, 1, bt, seq[[2, 0]], 1000, row_ids=i32([2, 0], cuda), ws=ws), base[[2, 0]])
+    # odd strides take the kernel that reads single elements
+    wide = torch.zeros(3, 16, t, 131, dtype=BF16, device=cuda)
+    wide[..., 1:129] = q
+    out = torch.zeros(3, 16, t, 131, dtype=BF16, device=cuda)
+    ops.paged_prefill_fp8(wide[..., 1:129], *pool.args, 1, bt, seq, 300, out=out[..., 2:130])
+    check_prefill(torch.cat(list(out[..., 2:130]), dim=1).unsqueeze(0), packed, pool, table, lens, [t] * 3, 1)
+    assert not bool(out[..., :2].any()) and not bool(out[..., 130:].any())
+    with pytest.raises(ValueError, match="workspace"):
+        ops.paged_prefill_fp8(q, *pool.args, 1, bt, seq, 300, ws=ws[:1024])
+
+
+def test_prefill_reports_what_it_cannot_do(cuda, native_lib):
+    for dtype in (BF16, F32):
+        pool, table, bt = filled(cuda, [40, 600], 2, 16, 128, dtype)
+        q = torch.randn(2, 4, 8, 128, device=cuda).to(dtype)
+        err = torch.zeros(1, dtype=torch.int32, device=cuda)
+
+        def word(table, n, **kw):
+            err.zero_()
+            ops.paged_prefill_fp8(q, *pool.args, 1, table, i32([40, 600], cuda), n, err=err, **kw)
+            return int(err)
+
+        assert word(bt, 600) == 0
+        bad = bt.clone()
+        bad[1, 3] = -7
+        assert word(bad, 600) & nat.BL_DEVERR_BLOCK_ID
+        assert word(bt[:, :20].contiguous(), 600) & nat.BL_DEVERR_TABLE
+        if dtype is BF16:  # the bounds size the expanded pages
+            assert word(bt, 100) & nat.BL_DEVERR_WORKSPACE
+            assert word(bt, 600, total_blocks=5) & nat.BL_DEVERR_WORKSPACE
+
+
+def test_refusals(cuda, native_lib):
+    pool, table, bt = filled(cuda, [40, 20], 2, 16, 128, BF16)
+    q = torch.randn(2, 4, 128, device=cuda).to(BF16)
+    seq = i32([40, 20], cuda)
+    k = torch.randn(2, 2, 1, 128, device=cuda).to(BF16)
+    kc, vc, ks, vs = pool.args
+
+    def bad(fn, exc=ValueError):
+        with pytest.raises(exc):
+            fn()
+
+    dec = lambda **kw: ops.paged_decode_fp8(kw.pop("q", q), kw.pop("kc", kc), vc, kw.pop("ks", ks), vs, kw.pop("layer", 1),
+                                            kw.pop("bt", bt), kw.pop("seq", seq), kw.pop("n", 40), **kw)
+    dec()
+    bad(lambda: dec(q=q.cpu()), RuntimeError)
+    bad(lambda: dec(kc=kc.view(torch.uint8)))
+    bad(lambda: dec(ks=ks.double()))
+    bad(lambda: dec(ks=ks[:, :, :1]))
+    bad(lambda: dec(layer=2), IndexError)
+    bad(lambda: dec(bt=bt.long()))
+    bad(lambda: dec(bt=bt[:1]))
+    bad(lambda: dec(seq=seq[:1]))
+    bad(lambda: dec(seq=seq.long()))
+    bad(lambda: dec(q=q[:, :3]))
+    bad(lambda: dec(q=q[..., ::2]))
+    bad(lambda: dec(q=q.double()))
+    bad(lambda: dec(n=0))
+    bad(lambda: dec(scale=0.0))
+    bad(lambda: dec(scale=float("nan")))
+    bad(lambda: dec(plan_ready=True))
+    bad(lambda: dec(out=torch.empty(2, 4, 128, device=cuda)))
+    bad(lambda: dec(row_ids=i32([0], cuda)))
+    bad(lambda: dec(err=torch.zeros(1, device=cuda)))
+    app = lambda key, value, start=i32([0, 0], cuda), **kw: ops.paged_append_fp8(*pool.args, 1, bt, start, key, value, **kw)
+    bad(lambda: app(k, k[:1]))
+    bad(lambda: app(k.float(), k))
+    bad(lambda: app(k[:, :1], k[:, :1]))
+    bad(lambda: app(k[:, :, :0], k[:, :, :0]))
+    bad(lambda: app(k, k, start=i32([0], cuda)))
+    bad(lambda: app(k[:1], k[:1], new_offsets=i32([0, 1, 1], cuda)))
+    pre = lambda **kw: ops.paged_prefill_fp8(kw.pop("q", q.unsqueeze(2)), *pool.args, 1, bt, seq, kw.pop("n", 40), **kw)
+    pre()
+    bad(lambda: pre(n=0))
+    bad(lambda: pre(total_blocks=0))
+    bad(lambda: pre(q=q))
+    bad(lambda: pre(scale=-1.0))
+    bad(lambda: ops.paged_gather_fp8(*pool.args, 1, bt, seq, 0, dtype=BF16))
+    bad(lambda: ops.paged_gather_fp8(*pool.args, 1, bt, seq, 4, dtype=torch.float64))
+
+
+def test_graphs_streams_and_concurrent_calls(cuda, native_lib):
+    """A serving step captured twice (two graphs, own scratch each), replayed together on two streams with new inputs."""
+    lens = [700, 30, 1500]
+    steps = []
+    for seed in (1, 2):
+        pool, table, bt = filled(cuda, [n + 8 for n in lens], 8, 16, 128, BF16, seed=seed)
+        g = torch.Generator(device=cuda).manual_seed(seed)
+        mk = lambda *s: torch.randn(*s, generator=g, device=cuda).to(BF16)
+        steps.append(dict(pool=pool, bt=bt, k=mk(3, 8, 1, 128), v=mk(3, 8, 1, 128), q=mk(3, 16, 128), q2=mk(3, 16, 4, 128),
+                          start=i32(lens, cuda), seq=i32([n + 1 for n in lens], cuda)))
+
+    for s in steps:
+        s["pair"] = s["pool"].free[:2]  # blocks in no row's table
+
+    def run(s):
+        ops.paged_append_fp8(*s["pool"].args, 1, s["bt"], s["start"], s["k"], s["v"])
+        a = ops.paged_decode_fp8(s["q"], *s["pool"].args, 1, s["bt"], s["seq"], 1600)
+        b = ops.paged_prefill_fp8(s["q2"], *s["pool"].args, 1, s["bt"], s["seq"], 1600)
+        c = ops.paged_gather_fp8(*s["pool"].args, 1, s["bt"], s["seq"], 1501, dtype=BF16)
+        ops.copy_blocks(*s["pool"].args[:2], [s["pair"][0]], [s["pair"][1]], key_scale=s["pool"].args[2], value_scale=s["pool"].args[3])
+        return a, b, *c
+
+    graphs = []
+    for s in steps:
+        run(s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = run(s)
+        graphs.append((graph, outs))
+    streams = [torch.cuda.Stream() for _ in steps]
+    for rep in range(3):
+        for s in steps:
+            for name in ("k", "v", "q", "q2"):
+                s[name].copy_(torch.randn_like(s[name]))
+        torch.cuda.synchronize()
+        for (graph, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        got = [[o.clone() for o in outs] for _, outs in graphs]
+        for s, g in zip(steps, got):
+            for x, y in zip(run(s), g):
+                assert torch.equal(x, y)
