@@ -50,8 +50,17 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t v) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
   return r;
 }
-__device__ __forceinline__ uint32_t e4m3lo_to_f16x2(uint32_t v) { return e4m3x2_to_f16x2((uint16_t)v); }
-__device__ __forceinline__ uint32_t e4m3hi_to_f16x2(uint32_t v) { return e4m3x2_to_f16x2((uint16_t)(v >> 16)); }
+// the low and the high half of a word of four codes
+__device__ __forceinline__ uint32_t e4m3lo_to_f16x2(uint32_t v) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3hi_to_f16x2(uint32_t v) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(v));
+  return r;
+}
 __device__ __forceinline__ float2 e4m3x2_to_float2(uint16_t v) { return unpack2<__half>(e4m3x2_to_f16x2(v)); }
 __device__ __forceinline__ float e4m3_to_float(uint8_t v) { return e4m3x2_to_float2(v).x; }
 

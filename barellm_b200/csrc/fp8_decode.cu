@@ -5,7 +5,10 @@
 // SDPAAttentionBackend.attend, src/barellm/attention/backend.py:34-61.
 //
 // Kernels
-//   decode_plan_kernel     (decode.cu) splits rows into 512-token chunks.
+//   fp8_decode_plan_kernel one CTA.  Splits rows into 512-token chunks and lists
+//                          the units, full chunks first, then partial ones by
+//                          decreasing size.  A unit's record holds all that the
+//                          attention kernel's producer needs to start on it.
 //   fp8_decode_tc_kernel   bf16 / fp16 q, head_dim 64, 128 or 256, block_size a
 //                          multiple of 16.  Persistent CTAs walk (chunk, KV head,
 //                          8 query heads) items.  One producer warp streams 32
@@ -23,22 +26,31 @@
 // down to 2^-16 of the head's largest and loses at most 2^-25 of that below.
 // k_scale multiplies the score in fp32.  P (<= 2^8, see below) is rounded to
 // fp16, 2^-12 relative.  V's scales are applied to the fp32 sums.
+#include <cstddef>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
-#include "decode_plan.cuh"
 #include "fp8.cuh"
 
 namespace bl {
 namespace {
 
-constexpr int kChunk = kDecodeChunkTokens;
+constexpr int kChunk = 512;  // tokens; fixed, so that a row's result does not depend on the batch
+constexpr int kChunkTiles = kChunk / 16;
+constexpr int32_t kPlanMagic = 0x38504c46;
 constexpr float kLog2e = 1.4426950408889634f;
 
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
+// One chunk of a row, as the plan records it.
+struct alignas(16) Unit {
+  int32_t row, chunk, len, part;  // len: the row's length, at most what its table covers; part: slot of its partial
+  int32_t table_row, pad[3];
+};
+
 struct WsLayout {
-  size_t hdr, row_base, exec, lse, o, total;
+  size_t hdr, row_base, units, lse, o, total;
   int64_t max_units;
 };
 
@@ -48,13 +60,112 @@ WsLayout ws_layout(int64_t batch, int64_t hq, int64_t d, int64_t max_seq_len) {
   size_t off = 0;
   w.hdr = off;      off += align256(4 * sizeof(int32_t));
   w.row_base = off; off += align256((batch + 1) * sizeof(int32_t));
-  w.exec = off;     off += align256(w.max_units * sizeof(int2));
+  w.units = off;    off += align256(w.max_units * sizeof(Unit));
   // a row of one chunk leaves no partial
   const int64_t parts = max_seq_len > kChunk ? w.max_units : 0;
   w.lse = off;      off += align256(parts * hq * sizeof(float));
   w.o = off;        off += align256(parts * hq * d * sizeof(float));
   w.total = off;
   return w;
+}
+
+// ---------------------------------------------------------------------------
+// plan
+// ---------------------------------------------------------------------------
+constexpr int kPlanThreads = 1024;
+
+struct PlanArgs {
+  const int32_t* seq_lens;
+  const int32_t* row_ids;
+  int32_t batch, max_units;
+  int64_t cap;        // tokens a table row covers
+  int32_t* hdr;       // [0] units, [1] magic, [2] batch, [3] max_units
+  int32_t* row_base;  // [batch + 1]
+  Unit* units;        // [max_units]
+  int32_t* err;
+};
+
+// Exclusive sums of v over the CTA's 32 warps; total over all.  s: 32 ints.
+__device__ __forceinline__ int cta_exclusive(int v, int* s, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) s[warp] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    const int t = s[w];
+    if (w < warp) before += t;
+    total += t;
+  }
+  __syncthreads();
+  return before + x - v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) fp8_decode_plan_kernel(const PlanArgs a) {
+  pdl_trigger();  // the attention kernel may launch; it waits for this grid to complete
+  __shared__ int s_sum[kPlanThreads / 32];
+  __shared__ int s_count[kChunkTiles], s_next[kChunkTiles];  // partial chunks by size in tiles, minus one
+  const int tid = threadIdx.x;
+  if (tid < kChunkTiles) s_count[tid] = 0;
+  __syncthreads();
+  auto put = [&](int pos, int row, int chunk, int len, int base, int table_row) {
+    if (pos >= a.max_units) return;
+    int4* u = reinterpret_cast<int4*>(a.units + pos);
+    u[0] = make_int4(row, chunk, len, base + chunk);
+    u[1] = make_int4(table_row, 0, 0, 0);
+  };
+  auto length = [&](int b) {
+    const int64_t len = a.seq_lens[b];
+    return (int)min(max(len, (int64_t)0), a.cap);
+  };
+  int all = 0, full = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    const int len = b < a.batch ? length(b) : 0;
+    if (b < a.batch && a.seq_lens[b] > a.cap) raise_dev(a.err, BL_DEVERR_TABLE);
+    const int nfull = len / kChunk, nall = (int)(((int64_t)len + kChunk - 1) / kChunk);
+    int tot_all, tot_full;
+    const int my_all = all + cta_exclusive(nall, s_sum, tot_all);
+    const int my_full = full + cta_exclusive(nfull, s_sum, tot_full);
+    if (b < a.batch) {
+      a.row_base[b] = my_all;
+      const int table_row = a.row_ids ? a.row_ids[b] : b;
+      for (int c = 0; c < nfull; ++c) put(my_full + c, b, c, len, my_all, table_row);
+      if (nall > nfull) atomicAdd(&s_count[(len - nfull * kChunk + 15) / 16 - 1], 1);
+    }
+    all += tot_all;
+    full += tot_full;
+  }
+  __syncthreads();
+  if (tid < kChunkTiles) {
+    int pos = full;  // partial chunks follow the full ones, the largest first
+    for (int s = tid + 1; s < kChunkTiles; ++s) pos += s_count[s];
+    s_next[tid] = pos;
+  }
+  if (tid == 0) {
+    if (all > a.max_units) raise_dev(a.err, BL_DEVERR_WORKSPACE);  // a row is longer than max_seq_len
+    a.row_base[a.batch] = all;
+    a.hdr[0] = min(all, a.max_units);
+    a.hdr[1] = kPlanMagic;
+    a.hdr[2] = a.batch;
+    a.hdr[3] = a.max_units;
+  }
+  __syncthreads();
+  // (the order among chunks of one size is left to the atomics: it changes no result)
+  for (int b = tid; b < a.batch; b += kPlanThreads) {
+    const int len = length(b), nfull = len / kChunk, rest = len - nfull * kChunk;
+    if (rest > 0)
+      put(atomicAdd(&s_next[(rest + 15) / 16 - 1], 1), b, nfull, len, a.row_base[b], a.row_ids ? a.row_ids[b] : b);
+  }
+  // complete only after the kernel before it has (the step's append)
+  pdl_wait();
 }
 
 struct Args {
@@ -72,11 +183,11 @@ struct Args {
   const int32_t* seq_lens;
   int64_t num_blocks, layer;
   int32_t batch, hq, hkv, g, head_tiles, bs, d;
-  int32_t q_vec;  // q rows can be read four elements at a time
+  int32_t q_vec, o_vec;  // q / out rows can be read / written four 16-bit elements at a time
   float scale_log2;
   const int32_t* hdr;
   const int32_t* row_base;
-  const int2* exec;
+  const Unit* units;
   float* ws_lse;
   float* ws_o;
   int32_t max_units, has_parts;
@@ -85,37 +196,41 @@ struct Args {
 
 // One item: a chunk of a row, a KV head and up to eight of its query heads.
 struct Item {
-  int b, chunk, h, hq0, heads;
-  int len, t0, t1;  // the chunk's tokens are [t0, t1), t1 <= len
-  int nch;          // chunks of the row
+  int b, h, hq0, heads;
+  int t0, t1;     // the chunk's tokens are [t0, t1)
+  int nch, part;  // chunks of the row, slot of this one's partial
+  int table_row;
 };
 
-// False when the plan names a unit outside the batch or the row's length.
-__device__ __forceinline__ bool get_item(const Args& a, int64_t item, Item& it) {
-  const int per_unit = a.hkv * a.head_tiles;
-  const int u = (int)(item / per_unit);
-  const int r = (int)(item - (int64_t)u * per_unit);
+__device__ __forceinline__ Unit load_unit(const Args& a, int64_t item) {
+  const int4* p = reinterpret_cast<const int4*>(a.units + item / (a.hkv * a.head_tiles));
+  const int4 x = p[0], y = p[1];
+  Unit u;
+  u.row = x.x, u.chunk = x.y, u.len = x.z, u.part = x.w, u.table_row = y.x;
+  return u;
+}
+
+// False when the plan names a unit outside the batch or the table.
+__device__ __forceinline__ bool make_item(const Args& a, int64_t item, const Unit& u, Item& it) {
+  const int r = (int)(item % (a.hkv * a.head_tiles));
   it.h = r / a.head_tiles;
   const int ht = r - it.h * a.head_tiles;
   it.hq0 = it.h * a.g + ht * 8;
   it.heads = min(8, a.g - ht * 8);
-  const int2 bc = a.exec[u];
-  it.b = bc.x;
-  it.chunk = bc.y;
-  if (bc.x < 0 || bc.x >= a.batch || bc.y < 0) return false;
-  const int64_t cap = a.bt_width * a.bs;
-  it.len = (int)min((int64_t)a.seq_lens[bc.x], cap);
-  const int64_t t0 = (int64_t)bc.y * kChunk;
-  if (t0 >= it.len) return false;
-  it.t0 = (int)t0;
-  it.t1 = (int)min(t0 + kChunk, (int64_t)it.len);
-  it.nch = (int)(((int64_t)it.len + kChunk - 1) / kChunk);
-  return true;
+  it.b = u.row;
+  it.table_row = u.table_row;
+  it.part = u.part;
+  it.t0 = u.chunk * kChunk;
+  it.t1 = min(it.t0 + kChunk, u.len);
+  it.nch = (u.len + kChunk - 1) / kChunk;
+  const bool ok = u.row >= 0 && u.row < a.batch && u.chunk >= 0 && it.t0 < u.len && u.len <= a.bt_width * a.bs;
+  if (!ok) it.t0 = it.t1 = it.heads = 0;  // no steps, no outputs
+  return ok;
 }
 
 __device__ __forceinline__ int plan_units(const Args& a) {
   const int units = a.hdr[0];
-  if (a.hdr[1] != kDecodePlanMagic || a.hdr[2] != a.batch || units < 0 || units > a.max_units) {
+  if (a.hdr[1] != kPlanMagic || a.hdr[2] != a.batch || a.hdr[3] != a.max_units || units < 0 || units > a.max_units) {
     if (threadIdx.x == 0 && blockIdx.x == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
     return 0;
   }
@@ -134,23 +249,10 @@ __device__ __forceinline__ void zero_empty_rows(const Args& a, int nthreads) {
   }
 }
 
-// One element of an item's result: the output for a row of one chunk, else the
-// chunk's partial (o, log2-sum-exp) for the reduce kernel.
-template <typename T>
-__device__ __forceinline__ void store_result(const Args& a, const Item& it, int hd, int d, float M, float L, float O) {
-  const int hq = it.hq0 + hd;
-  const float val = L == 0.f ? 0.f : O / L;  // a NaN sum stays NaN
-  if (it.nch <= 1) {
-    reinterpret_cast<T*>(a.out)[(int64_t)it.b * a.o_sb + (int64_t)hq * a.o_sh + d] = from_f32<T>(val);
-    return;
-  }
-  const int64_t slot = (int64_t)a.row_base[it.b] + it.chunk;
-  if (!a.has_parts || slot < 0 || slot >= a.max_units) {  // longer than max_seq_len allows
-    if (d == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
-    return;
-  }
-  a.ws_o[(slot * a.hq + hq) * a.d + d] = val;
-  if (d == 0) a.ws_lse[slot * a.hq + hq] = L == 0.f ? -INFINITY : M + __log2f(L);
+// Whether the item's partial has a place in the workspace (it has none where a
+// row is longer than max_seq_len).
+__device__ __forceinline__ bool has_part(const Args& a, const Item& it) {
+  return a.has_parts && it.part >= 0 && it.part < a.max_units;
 }
 
 // ---------------------------------------------------------------------------
@@ -168,16 +270,30 @@ struct Cfg {
   static constexpr int kHalves = D / kRow;
   static constexpr int kTile = 16 * D;            // K (or V) codes of one tile
   static constexpr int kSlot = 4 * kTile;         // K and V of two tiles
-  static constexpr int kStages = D == 256 ? 4 : 8;
+  static constexpr int kDepth = D == 64 ? 4 : 2;  // ring slots of a consumer warp
   static constexpr int kBox = 16 * kRow;
+  static constexpr int kKS = D / 16;              // 16-dim steps of the score product
+  static constexpr int kLaneDims = kRow / 8;      // output dims a lane owns per half
+  static constexpr int kWords = kLaneDims / 4;    // V words a lane reads per token and half
+  static constexpr int kVecs = D / 16;            // float4s of sums a lane holds (two heads)
+};
+
+// What the planner warp hands to the consumers, an item at a time.
+template <int D>
+struct alignas(16) ItemSlot {
+  float2 f[4];                      // score factors of heads 2t and 2t + 1
+  int32_t y[kTiles];                // pool row of each tile
+  float ks[kTiles], vs[kTiles];     // its scales
+  Item it;
 };
 
 template <int D>
-struct TCShared {
-  uint64_t full[Cfg<D>::kStages];
-  uint64_t empty[Cfg<D>::kStages];
-  float scales[Cfg<D>::kStages][4];  // k_scale of the two tiles, v_scale of the two tiles
-  float ml[kNW][8][2];
+struct alignas(16) TCShared {  // the query fragments and the merge buffer behind it are read 16 bytes at a time
+  ItemSlot<D> items[2];
+  float2 ml[kNW][8];  // maximum and sum of each class and head
+  uint64_t full[kNW][Cfg<D>::kDepth];
+  uint64_t item_full[2], item_empty[2];
+  uint64_t comb_full, comb_free;
   int abort;
 };
 
@@ -187,24 +303,154 @@ __device__ __forceinline__ int swizzled(int r, int c) {
   return r * ROW + ((ROW == 128 ? (c ^ (r & 7)) : (c ^ ((r >> 1) & 3))) << 4);
 }
 
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float4 lds128f(uint32_t addr) {
+  const uint4 v = lds128(addr);
+  return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+__device__ __forceinline__ void sts128f(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+
+// D += A(16x16) * B(16x8) in fp16 with fp32 sums.  Not volatile: a pure function
+// of its registers, so the compiler may interleave independent products.
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Waits unless the CTA gave up; a wait that runs out makes it give up.
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, int* abort, int32_t* err) {
+  if (*(volatile int*)abort) return false;
+  if (mbar_wait(bar, parity)) return true;
+  raise_dev(err, BL_DEVERR_TIMEOUT);
+  *(volatile int*)abort = 1;
+  return false;
+}
+
+// An item on its way to the ring: lane i holds tile i of the chunk.  begin()
+// issues the loads that the plan's record leads to, finish() those behind the
+// block id; a whole item lies between them, so neither is waited for.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreadsTC) fp8_decode_tc_kernel(const Args a, const __grid_constant__ CUtensorMap kmap,
-                                                                   const __grid_constant__ CUtensorMap vmap) {
+struct Pending {
+  Item it;
+  bool valid;
+  int tok, lb;
+  int32_t phys, y;
+  float ks, vs;
+  uint2 q[Cfg<D>::kKS];  // dims 16 k + 4 t + {0..3} of head g, as stored
+
+  __device__ __forceinline__ void begin(const Args& a, int64_t item, const Unit& u, int lane) {
+    valid = make_item(a, item, u, it);
+    tok = it.t0 + 16 * lane;
+    lb = tok / a.bs;
+    phys = 0;
+    if (tok < it.t1) phys = a.block_tables[(int64_t)it.table_row * a.bt_stride + lb];
+    const int g_row = lane >> 2, t4 = lane & 3;
+    const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(valid ? it.b : 0) * a.q_sb +
+                  (int64_t)(it.hq0 + (g_row < it.heads ? g_row : 0)) * a.q_sh + 4 * t4;
+#pragma unroll
+    for (int k = 0; k < Cfg<D>::kKS; ++k) {
+      if (a.q_vec) {
+        q[k] = *reinterpret_cast<const uint2*>(qp + k * 16);
+      } else {
+        const T* p = qp + k * 16;
+        q[k] = make_uint2(pack2<T>(to_f32<T>(p[0]), to_f32<T>(p[1])), pack2<T>(to_f32<T>(p[2]), to_f32<T>(p[3])));
+      }
+    }
+  }
+
+  __device__ __forceinline__ void finish(const Args& a) {
+    y = 0;
+    ks = vs = 1.f;
+    if (tok < it.t1) {
+      int64_t p = phys;
+      if (p < 0 || p >= a.num_blocks) {
+        raise_dev(a.err, BL_DEVERR_BLOCK_ID);
+        p = 0;
+      }
+      const int64_t slot = (a.layer * a.num_blocks + p) * a.hkv + it.h;
+      ks = a.k_scale[slot];
+      vs = a.v_scale[slot];
+      y = (int32_t)(slot * a.bs + (tok - lb * a.bs));
+    }
+  }
+
+  // The query heads as fp16 B fragments and score factors, for this lane.
+  // Position k of a 16-dim step stands for dim 16 ks + 4 t + {0, 1} (k = 2t,
+  // 2t+1) and + {2, 3} (k = 2t+8, 2t+9): the order in which a lane finds the K
+  // codes of one 32-bit word.
+  // Lanes of heads that the item does not have store nothing: `qs` has room for
+  // min(g, 8) heads, lane by lane.
+  __device__ __forceinline__ void stage(const Args& a, int lane, ItemSlot<D>& out, uint2* qs) const {
+    const int t4 = lane & 3, room = 4 * min(a.g, 8);
+    float amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < Cfg<D>::kKS; ++k) {
+      const float2 x = unpack2<T>(q[k].x), y2 = unpack2<T>(q[k].y);
+      amax = fmaxf(fmaxf(amax, fmaxf(finite_abs(x.x), finite_abs(x.y))), fmaxf(finite_abs(y2.x), finite_abs(y2.y)));
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    int e = (int)(__float_as_uint(amax) >> 23) - 127;
+    e = amax > 0.f ? min(max(e, -126), 126) : 0;
+    const float down = exp2_int(-e);
+#pragma unroll
+    for (int k = 0; k < Cfg<D>::kKS; ++k) {
+      const float2 x = unpack2<T>(q[k].x), y2 = unpack2<T>(q[k].y);
+      const uint2 v = make_uint2(pack2<__half>(x.x * down, x.y * down), pack2<__half>(y2.x * down, y2.y * down));
+      if (lane < room) qs[k * room + lane] = v;
+    }
+    const float f = exp2_int(e) * a.scale_log2;
+    const float f0 = __shfl_sync(0xffffffffu, f, 8 * t4);
+    const float f1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
+    if (lane < 4) out.f[lane] = make_float2(f0, f1);
+    out.y[lane] = y;
+    out.ks[lane] = ks;
+    // a step with one tile repeats its V scale for the missing one (no effect: its codes are masked)
+    const float before = __shfl_up_sync(0xffffffffu, vs, 1);
+    out.vs[lane] = tok < it.t1 ? vs : before;
+    if (lane == 0) out.it = it;
+  }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
+    fp8_decode_tc_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using C = Cfg<D>;
+  static_assert(sizeof(TCShared<D>) % 16 == 0 && C::kDepth * C::kSlot % 1024 == 0 && C::kKS * 4 * sizeof(uint2) % 16 == 0 &&
+                    offsetof(ItemSlot<D>, ks) % 8 == 0 && offsetof(ItemSlot<D>, vs) % 8 == 0,
+                "vector accesses to shared memory");
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* slots =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* comb_o = reinterpret_cast<float*>(slots + C::kStages * C::kSlot);  // [kNW][min(g, 8)][D]
-  const int gmax = min(a.g, 8);
-  TCShared<D>* sh = reinterpret_cast<TCShared<D>*>(comb_o + kNW * gmax * D);
+  TCShared<D>* sh = reinterpret_cast<TCShared<D>*>(slots + kNW * C::kDepth * C::kSlot);
+  const int room = 4 * min(a.g, 8);                              // lanes of the heads an item can have
+  uint2* qs = reinterpret_cast<uint2*>(sh + 1);                  // [2][kKS][room] fragments
+  float* comb = reinterpret_cast<float*>(qs + 2 * C::kKS * room);  // [kNW - 1][kVecs][8 * head pairs] float4
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&sh->full[s], 1);
-      mbar_init(&sh->empty[s], 1);
+    for (int s = 0; s < kNW * C::kDepth; ++s) mbar_init(&sh->full[0][0] + s, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sh->item_full[s], 1);
+      mbar_init(&sh->item_empty[s], kNW);
     }
+    mbar_init(&sh->comb_full, kNW - 1);
+    mbar_init(&sh->comb_free, 1);
     sh->abort = 0;
     fence_mbar_init();
   }
@@ -214,136 +460,125 @@ __global__ void __launch_bounds__(kThreadsTC) fp8_decode_tc_kernel(const Args a,
   const int64_t items = (int64_t)plan_units(a) * a.hkv * a.head_tiles;
 
   if (warp == kNW) {
-    // ------------------------------ producer ------------------------------
-    if (lane == 0) {
-      prefetch_tensormap(&kmap);
-      prefetch_tensormap(&vmap);
+    // ------------------------------ planner ------------------------------
+    // Describes item by item to the consumers, one item ahead of them; the loads
+    // behind the item after that one are in flight meanwhile.
+    int n_item = 0;
+    int64_t item = blockIdx.x;
+    Pending<T, D> cur, nxt;
+    Unit unit = {};
+    if (item < items) {
+      cur.begin(a, item, load_unit(a, item), lane);
+      if (item + gridDim.x < items) unit = load_unit(a, item + gridDim.x);
+      cur.finish(a);
     }
-    const uint64_t policy = policy_evict_first();
-    int issued = 0;  // steps issued so far == ring index of the next
-    bool ok = true;
-    for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      Item it;
-      if (!get_item(a, item, it)) {
-        if (lane == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
-        continue;
+    for (; item < items; ++n_item) {
+      if (!cur.valid && lane == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
+      item += gridDim.x;
+      if (item < items) {
+        nxt.begin(a, item, unit, lane);
+        if (item + gridDim.x < items) unit = load_unit(a, item + gridDim.x);
       }
-      // lane i holds tile i of the chunk: its pool row and its scales
-      const int tok = it.t0 + 16 * lane;
-      int32_t y = 0;
-      float ks = 1.f, vs = 1.f;
-      if (tok < it.t1) {
-        const int64_t row = a.row_ids ? (int64_t)a.row_ids[it.b] : (int64_t)it.b;
-        const int lb = tok / a.bs;
-        int64_t phys = a.block_tables[row * a.bt_stride + lb];
-        if (phys < 0 || phys >= a.num_blocks) {
-          raise_dev(a.err, BL_DEVERR_BLOCK_ID);
-          phys = 0;
-        }
-        const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + it.h;
-        ks = a.k_scale[slot];
-        vs = a.v_scale[slot];
-        y = (int32_t)(slot * a.bs + (tok - lb * a.bs));
-      }
-      const int ntiles = (it.t1 - it.t0 + 15) / 16;
-      for (int t = 0; t < ntiles; t += 2) {
-        const int slot = issued % C::kStages;
-        if (!__all_sync(0xffffffffu, mbar_wait(&sh->empty[slot], ((issued / C::kStages) & 1) ^ 1))) {
-          raise_dev(a.err, BL_DEVERR_TIMEOUT);
-          sh->abort = 1;
-          ok = false;
-          break;
-        }
-        const int x = lane - t;  // this lane's tile of the step: 0 or 1
-        const int n = min(2, ntiles - t);
-        if (x >= 0 && x < 2) {
-          // a step with one tile repeats its V scale for the missing one (no effect: its codes are masked)
-          sh->scales[slot][x] = ks;
-          sh->scales[slot][2 + x] = vs;
-        }
-        const float vs0 = __shfl_sync(0xffffffffu, vs, t);
-        __syncwarp();
-        if (lane == 0) {
-          if (n == 1) sh->scales[slot][3] = vs0;
-          mbar_arrive_expect_tx(&sh->full[slot], n * 2 * C::kTile);
-        }
-        __syncwarp();
-        if (x >= 0 && x < n) {
-          unsigned char* kd = slots + slot * C::kSlot + x * C::kTile;
-          unsigned char* vd = kd + 2 * C::kTile;
-#pragma unroll
-          for (int hf = 0; hf < C::kHalves; ++hf) {
-            tma_load_2d_hint(kd + hf * C::kBox, &kmap, &sh->full[slot], hf * 128, y, policy);
-            tma_load_2d_hint(vd + hf * C::kBox, &vmap, &sh->full[slot], hf * 128, y, policy);
-          }
-        }
-        ++issued;
-      }
-    }
-    // Drain: every issued copy lands before the CTA can exit.
-    __syncwarp();
-    if (lane == 0) {
-      for (int s = 0; s < C::kStages && s < issued; ++s) {
-        const int last = s + ((issued - 1 - s) / C::kStages) * C::kStages;
-        if (!mbar_wait(&sh->full[s], (last / C::kStages) & 1)) raise_dev(a.err, BL_DEVERR_TIMEOUT);
-      }
+      const int k = n_item & 1;
+      if (!__all_sync(0xffffffffu, wait_or_abort(&sh->item_empty[k], ((n_item >> 1) & 1) ^ 1, &sh->abort, a.err))) break;
+      cur.stage(a, lane, sh->items[k], qs + k * C::kKS * room);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->item_full[k]);
+      if (item < items) nxt.finish(a);
+      cur = nxt;
     }
     return;
   }
 
   // ------------------------------ consumers ------------------------------
+  if (lane == 0) {
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&vmap);
+  }
   zero_empty_rows<T>(a, kNW * 32);
-  constexpr int kKS = D / 16;                // 16-dim steps of the score product
-  constexpr int kLaneDims = C::kRow / 8;     // output dims a lane owns per half
-  constexpr int kWords = kLaneDims / 4;      // V words a lane reads per token and half
+  constexpr int kKS = C::kKS, kLaneDims = C::kLaneDims, kWords = C::kWords, kDepth = C::kDepth;
   const int g_row = lane >> 2;  // mma group: token (scores), query head (q, P), dim block (output)
   const int t4 = lane & 3;
-  int base = 0;  // ring index of the item's first step
+  unsigned char* ring = slots + warp * kDepth * C::kSlot;
+  const int k_row = (lane & 7) + (lane & 8);  // this lane's ldmatrix row of a K tile
+  const uint32_t v_off = (uint32_t)((g_row * kLaneDims) & 15);
+  // merge buffer: the lanes that hold heads, (head pairs) x 8 of them, side by side
+  const int pairs = (min(a.g, 8) + 1) / 2;
+  const uint32_t comb_a = smem_u32(comb) + 16 * (g_row * pairs + t4);
+  const uint32_t comb_vec = 16 * 8 * pairs;  // bytes between a lane's float4s
+  const uint64_t policy = policy_evict_first();
+  const int my_items = items > blockIdx.x ? (int)((items - blockIdx.x + gridDim.x - 1) / gridDim.x) : 0;
 
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    Item it;
-    if (!get_item(a, item, it)) continue;  // flagged by the producer
-    const int nsteps = (it.t1 - it.t0 + kStepTokens - 1) / kStepTokens;
-
-    // q as fp16 B fragments.  Position k of a 16-dim step stands for dim
-    // 16 ks + 4 t + {0, 1} (k = 2t, 2t+1) and + {2, 3} (k = 2t+8, 2t+9): the order
-    // in which a lane finds the K codes of one 32-bit word.
-    uint32_t qf[kKS][2];
-    float f0, f1;  // scale * log2(e) * the head's power of two, heads 2 t4 and 2 t4 + 1
-    {
-      const bool valid = g_row < it.heads;
-      const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)it.b * a.q_sb +
-                    (int64_t)(it.hq0 + (valid ? g_row : 0)) * a.q_sh;
-      float qv[kKS][4];
-      float amax = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < kKS; ++ks) {
-        const T* p = qp + ks * 16 + 4 * t4;
-        if (a.q_vec) {
-          const uint2 w = *reinterpret_cast<const uint2*>(p);
-          const float2 x = unpack2<T>(w.x), y = unpack2<T>(w.y);
-          qv[ks][0] = x.x, qv[ks][1] = x.y, qv[ks][2] = y.x, qv[ks][3] = y.y;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) qv[ks][e] = to_f32<T>(p[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) amax = fmaxf(amax, finite_abs(qv[ks][e]));
+  // A warp issues its own copies into a ring of its own: kDepth steps of 32
+  // tokens.  One producer warp for the CTA had to pass every step through two
+  // barriers and could not keep HBM busy (measured: its loop took ~850 cycles a
+  // step, 2.7 TB/s from one CTA per SM whatever the ring's size).  The issue
+  // cursor (item, step) runs ahead of the steps consumed, into the next item
+  // once the planner has described it.
+  int issued = 0, taken = 0;       // steps
+  int at_item = -1, at_step = 0, at_steps = 0;
+  int at_tiles = 0;
+  // Issues the next step if there is one; `may_wait` false: only if its item is
+  // described already.  n_item: the item being consumed.
+  auto issue = [&](int n_item, bool may_wait) -> bool {
+    while (at_step >= at_steps) {
+      const int next = at_item + 1;
+      if (next >= my_items || next > n_item + 1) return false;
+      const int k = next & 1;
+      if (!may_wait) {
+        if (!__all_sync(0xffffffffu, mbar_try_wait(&sh->item_full[k], (next >> 1) & 1))) return false;
+      } else if (!__all_sync(0xffffffffu, wait_or_abort(&sh->item_full[k], (next >> 1) & 1, &sh->abort, a.err))) {
+        return false;
       }
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      int e = (int)(__float_as_uint(amax) >> 23) - 127;
-      e = amax > 0.f ? min(max(e, -126), 126) : 0;
-      const float down = valid ? exp2_int(-e) : 0.f;
-#pragma unroll
-      for (int ks = 0; ks < kKS; ++ks) {
-        qf[ks][0] = pack2<__half>(valid ? qv[ks][0] * down : 0.f, valid ? qv[ks][1] * down : 0.f);
-        qf[ks][1] = pack2<__half>(valid ? qv[ks][2] * down : 0.f, valid ? qv[ks][3] * down : 0.f);
-      }
-      const float f = exp2_int(e) * a.scale_log2;
-      f0 = __shfl_sync(0xffffffffu, f, 8 * t4);
-      f1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
+      at_item = next;
+      const Item& it = sh->items[k].it;
+      at_tiles = (it.t1 - it.t0 + 15) / 16;
+      at_steps = (at_tiles + 1) / 2;
+      at_step = (warp + next) & (kNW - 1);
     }
+    const int slot = issued % kDepth;
+    if (lane == 0) {
+      const ItemSlot<D>& is = sh->items[at_item & 1];
+      const int n = min(2, at_tiles - 2 * at_step);
+      uint64_t* bar = &sh->full[warp][slot];
+      fence_proxy_async_smem();  // the warp's reads of the slot come before the copies into it
+      mbar_arrive_expect_tx(bar, n * 2 * C::kTile);
+      unsigned char* kd = ring + slot * C::kSlot;
+      unsigned char* vd = kd + 2 * C::kTile;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (x < n) {
+          const int32_t y = is.y[2 * at_step + x];
+#pragma unroll
+          for (int hf = 0; hf < C::kHalves; ++hf) {
+            tma_load_2d_hint(kd + x * C::kTile + hf * C::kBox, &kmap, bar, hf * 128, y, policy);
+            tma_load_2d_hint(vd + x * C::kTile + hf * C::kBox, &vmap, bar, hf * 128, y, policy);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    at_step += kNW;
+    ++issued;
+    return true;
+  };
+  bool ok = true;
+
+  for (int n_item = 0; n_item < my_items && ok; ++n_item) {
+    // all waits are per warp and bounded; a CTA that gave up leaves them at once
+    const int slot_i = n_item & 1;
+    ok = __all_sync(0xffffffffu, wait_or_abort(&sh->item_full[slot_i], (n_item >> 1) & 1, &sh->abort, a.err));
+    if (!ok) break;
+    while (issued - taken < kDepth && issue(n_item, false)) {
+    }
+    const Item it = sh->items[slot_i].it;
+    const float2 fs = sh->items[slot_i].f[t4];
+    uint2 qf[kKS];
+#pragma unroll
+    for (int ks = 0; ks < kKS; ++ks)
+      qf[ks] = g_row < it.heads ? lds64(smem_u32(qs + (slot_i * kKS + ks) * room + lane)) : make_uint2(0u, 0u);
+    const float f0 = fs.x, f1 = fs.y;
+    const int nsteps = (it.t1 - it.t0 + kStepTokens - 1) / kStepTokens;
 
     // Running softmax state of this warp, per query head (column).  m follows
     // the maximum lazily: it moves only when a score passes it by 8 (log2
@@ -358,54 +593,108 @@ __global__ void __launch_bounds__(kThreadsTC) fp8_decode_tc_kernel(const Args a,
 #pragma unroll
       for (int j = 0; j < 2 * kWords; ++j) o[hf][j][0] = o[hf][j][1] = o[hf][j][2] = o[hf][j][3] = 0.f;
 
-    for (int i = warp; i < nsteps; i += kNW) {
-      const int gi = base + i;
-      const int slot = gi % C::kStages;
-      if (*(volatile int*)&sh->abort) break;
-      if (!mbar_wait(&sh->full[slot], (gi / C::kStages) & 1)) {
-        raise_dev(a.err, BL_DEVERR_TIMEOUT);
-        *(volatile int*)&sh->abort = 1;
-        break;
-      }
-      __syncwarp();
-      const float4 sc = *reinterpret_cast<const float4*>(sh->scales[slot]);
-      const uint32_t kb = smem_u32(slots + slot * C::kSlot);
-      const unsigned char* vb = slots + slot * C::kSlot + 2 * C::kTile;
+    // The item's steps are dealt to the warps by class (step mod kNW); which warp
+    // has which class turns from item to item, so that the warp of class 0, which
+    // joins the others' sums below, is not always the same.  A class's sums do not
+    // depend on its warp, so a row's result does not depend on what ran before it.
+    const int cls = (warp + n_item) & (kNW - 1);
+    for (int i = cls; i < nsteps; i += kNW) {
+      if (issued == taken) ok = issue(n_item, true);
+      const int slot = taken % kDepth;
+      ok = ok && __all_sync(0xffffffffu,
+                            wait_or_abort(&sh->full[warp][slot], (taken / kDepth) & 1, &sh->abort, a.err));
+      if (!ok) break;
+      const float2 ks2 = *reinterpret_cast<const float2*>(&sh->items[slot_i].ks[2 * i]);
+      const float2 vs2 = *reinterpret_cast<const float2*>(&sh->items[slot_i].vs[2 * i]);
+      const float4 sc = make_float4(ks2.x, ks2.y, vs2.x, vs2.y);
+      const uint32_t kb = smem_u32(ring + slot * C::kSlot);
+      const uint32_t vb = kb + 2 * C::kTile;
 
-      // S^T[token][head] = K[token] . q[head]
+      // S^T[token][head] = K[token] . q[head], codes times normalised q.  Two chains of
+      // sums per tile, joined at the end: the products of a chain wait for one another.
       float s[2][4];
+      {
+        float z[2][2][4];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) z[x][0][e] = z[x][1][e] = 0.f;
+#pragma unroll
+        for (int hf = 0; hf < C::kHalves; ++hf) {
+          uint32_t r[2][C::kRow / 32][4];
+#pragma unroll
+          for (int c = 0; c < C::kRow / 32; ++c)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              ldmatrix_x4(kb + x * C::kTile + hf * C::kBox + swizzled<C::kRow>(k_row, 2 * c + (lane >> 4)), r[x][c][0],
+                          r[x][c][1], r[x][c][2], r[x][c][3]);
+#pragma unroll
+          for (int c = 0; c < C::kRow / 32; ++c)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int ks = hf * (C::kRow / 16) + 2 * c;
+              mma_f16(z[x][0], e4m3lo_to_f16x2(r[x][c][0]), e4m3lo_to_f16x2(r[x][c][1]), e4m3hi_to_f16x2(r[x][c][0]),
+                      e4m3hi_to_f16x2(r[x][c][1]), qf[ks].x, qf[ks].y);
+              mma_f16(z[x][1], e4m3lo_to_f16x2(r[x][c][2]), e4m3lo_to_f16x2(r[x][c][3]), e4m3hi_to_f16x2(r[x][c][2]),
+                      e4m3hi_to_f16x2(r[x][c][3]), qf[ks + 1].x, qf[ks + 1].y);
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[x][e] = z[x][0][e] + z[x][1][e];
+      }
+      const int nvalid = it.t1 - (it.t0 + i * kStepTokens);  // tokens of the step that exist
+
+      // V's codes into registers; then the slot takes the next copies, ahead of the
+      // softmax below.  A lane takes the kLaneDims consecutive dims
+      // g_row * kLaneDims of tokens 2t, 2t+1, 2t+8, 2t+9.
+      uint32_t w[2][C::kHalves][4][kWords];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int hf = 0; hf < C::kHalves; ++hf)
 #pragma unroll
-          for (int c = 0; c < C::kRow / 16; c += 2) {
-            uint32_t r0, r1, r2, r3;
-            const int r = (lane & 7) + (lane & 8);
-            ldmatrix_x4(kb + x * C::kTile + hf * C::kBox + swizzled<C::kRow>(r, c + (lane >> 4)), r0, r1, r2, r3);
-            const int ks = hf * (C::kRow / 16) + c;
-            mma_16816<__half>(s[x][0], s[x][1], s[x][2], s[x][3], e4m3lo_to_f16x2(r0), e4m3lo_to_f16x2(r1),
-                              e4m3hi_to_f16x2(r0), e4m3hi_to_f16x2(r1), qf[ks][0], qf[ks][1]);
-            mma_16816<__half>(s[x][0], s[x][1], s[x][2], s[x][3], e4m3lo_to_f16x2(r2), e4m3lo_to_f16x2(r3),
-                              e4m3hi_to_f16x2(r2), e4m3hi_to_f16x2(r3), qf[ks + 1][0], qf[ks + 1][1]);
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t addr = vb + x * C::kTile + hf * C::kBox + v_off +
+                                  swizzled<C::kRow>(2 * t4 + (k & 1) + 8 * (k >> 1), (g_row * kLaneDims) >> 4);
+            if constexpr (kWords == 4) {
+              const uint4 v = lds128(addr);
+              w[x][hf][k][0] = v.x, w[x][hf][k][1] = v.y, w[x][hf][k][2] = v.z, w[x][hf][k][3] = v.w;
+            } else {
+              const uint2 v = lds64(addr);
+              w[x][hf][k][0] = v.x, w[x][hf][k][1] = v.y;
+            }
           }
+      ++taken;
+      __syncwarp();
+      while (issued - taken < kDepth && issue(n_item, false)) {
       }
-      const int nvalid = it.t1 - (it.t0 + i * kStepTokens);  // tokens of the step that exist
+      if (nvalid < kStepTokens) {
+        // slots past the length hold stale codes (possibly NaN): 0 * NaN is NaN
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float ks = x ? sc.y : sc.x;
-        s[x][0] *= f0 * ks, s[x][1] *= f1 * ks, s[x][2] *= f0 * ks, s[x][3] *= f1 * ks;
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int hf = 0; hf < C::kHalves; ++hf)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int j = 0; j < kWords; ++j)
+                w[x][hf][k][j] = 16 * x + 2 * t4 + (k & 1) + 8 * (k >> 1) < nvalid ? w[x][hf][k][j] : 0u;
       }
+
+      float c00 = f0 * sc.x, c01 = f1 * sc.x, c10 = f0 * sc.y, c11 = f1 * sc.y;  // log2 units
       if (nvalid < kStepTokens) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           if (16 * x + g_row >= nvalid) s[x][0] = s[x][1] = -INFINITY;
           if (16 * x + g_row + 8 >= nvalid) s[x][2] = s[x][3] = -INFINITY;
         }
+        // (a factor that underflowed would make NaN of the mask)
+        c00 = fmaxf(c00, 1.2e-38f), c01 = fmaxf(c01, 1.2e-38f), c10 = fmaxf(c10, 1.2e-38f), c11 = fmaxf(c11, 1.2e-38f);
       }
-      float mx0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
-      float mx1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
+      float mx0 = fmaxf(fmaxf(s[0][0], s[0][2]) * c00, fmaxf(s[1][0], s[1][2]) * c10);
+      float mx1 = fmaxf(fmaxf(s[0][1], s[0][3]) * c01, fmaxf(s[1][1], s[1][3]) * c11);
       if (__any_sync(0xffffffffu, mx0 > m0 + 8.f || mx1 > m1 + 8.f)) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
@@ -425,132 +714,187 @@ __global__ void __launch_bounds__(kThreadsTC) fp8_decode_tc_kernel(const Args a,
             o[hf][j][1] *= al1, o[hf][j][3] *= al1;
           }
       }
-      const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
+      const float u0 = m0 == -INFINITY ? 0.f : -m0, u1 = m1 == -INFINITY ? 0.f : -m1;
       // exponentials and row sums
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        s[x][0] = fast_exp2(s[x][0] - u0), s[x][2] = fast_exp2(s[x][2] - u0);
-        s[x][1] = fast_exp2(s[x][1] - u1), s[x][3] = fast_exp2(s[x][3] - u1);
-        l0 += s[x][0] + s[x][2];
-        l1 += s[x][1] + s[x][3];
-      }
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float vs = x ? sc.w : sc.z;
-        // A much larger scale becomes the reference (the sums shrink by a
-        // power of two); a much smaller one is added through its own sums.
-        if (vs > vref * 16.f) {
-          const float r = vref * pow2_inverse(vs);
-          vref = vs;
-          vinv = pow2_inverse(vs);
-#pragma unroll
-          for (int hf = 0; hf < C::kHalves; ++hf)
-#pragma unroll
-            for (int j = 0; j < 2 * kWords; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[hf][j][e] *= r;
-        }
-        const float ratio = vs * vinv;
-        const bool fold = ratio >= 0.015625f;
-        const float pr = fold ? ratio : 1.f;
+      s[0][0] = fast_exp2(fmaf(s[0][0], c00, u0)), s[0][2] = fast_exp2(fmaf(s[0][2], c00, u0));
+      s[0][1] = fast_exp2(fmaf(s[0][1], c01, u1)), s[0][3] = fast_exp2(fmaf(s[0][3], c01, u1));
+      s[1][0] = fast_exp2(fmaf(s[1][0], c10, u0)), s[1][2] = fast_exp2(fmaf(s[1][2], c10, u0));
+      s[1][1] = fast_exp2(fmaf(s[1][1], c11, u1)), s[1][3] = fast_exp2(fmaf(s[1][3], c11, u1));
+      l0 += (s[0][0] + s[0][2]) + (s[1][0] + s[1][2]);
+      l1 += (s[0][1] + s[0][3]) + (s[1][1] + s[1][3]);
+
+      // O^T[dim][head] += V^T[dim][token] P^T[token][head] of tile x.  Two tokens' bytes
+      // are paired, so a converted pair is one A register (row = dim, two
+      // consecutive tokens).  APART: the tile's sums are made on their own and
+      // added times `ratio`.
+      auto pv = [&](int x, float ratio, auto apart) {
+        constexpr bool kApart = decltype(apart)::value;
         // P^T (tokens x heads) -> B fragment (k = token, n = head)
-        const uint32_t pb0 = movmatrix_trans(pack2<__half>(s[x][0] * pr, s[x][1] * pr));
-        const uint32_t pb1 = movmatrix_trans(pack2<__half>(s[x][2] * pr, s[x][3] * pr));
-        // O^T[dim][head] += V^T[dim][token] P^T[token][head].  A lane reads the
-        // 16 (kLaneDims) consecutive dims g_row * kLaneDims of tokens 2t, 2t+1,
-        // 2t+8, 2t+9 and pairs two tokens' bytes, so a converted pair is one A
-        // register (row = dim, two consecutive tokens).
-        const int r0 = 2 * t4;
-        const int left = nvalid - 16 * x;
+        const uint32_t pb0 = movmatrix_trans(pack2<__half>(s[x][0], s[x][1]));
+        const uint32_t pb1 = movmatrix_trans(pack2<__half>(s[x][2], s[x][3]));
 #pragma unroll
         for (int hf = 0; hf < C::kHalves; ++hf) {
-          const unsigned char* box = vb + x * C::kTile + hf * C::kBox;
-          uint32_t w[4][kWords];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int r = r0 + (k & 1) + 8 * (k >> 1);
-            const unsigned char* p =
-                box + swizzled<C::kRow>(r, (g_row * kLaneDims) >> 4) + ((g_row * kLaneDims) & 15);
-            if constexpr (kWords == 4) {
-              const uint4 v = *reinterpret_cast<const uint4*>(p);
-              w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
-            } else {
-              const uint2 v = *reinterpret_cast<const uint2*>(p);
-              w[k][0] = v.x, w[k][1] = v.y;
-            }
-            // slots past the length hold stale codes (possibly NaN): 0 * NaN is NaN
-            if (left < 16 && r >= left) {
-#pragma unroll
-              for (int j = 0; j < kWords; ++j) w[k][j] = 0u;
-            }
-          }
 #pragma unroll
           for (int j = 0; j < kWords; ++j) {
-            const uint32_t lo01 = __byte_perm(w[0][j], w[1][j], 0x5140), lo23 = __byte_perm(w[0][j], w[1][j], 0x7362);
-            const uint32_t hi01 = __byte_perm(w[2][j], w[3][j], 0x5140), hi23 = __byte_perm(w[2][j], w[3][j], 0x7362);
+            const uint32_t(&v)[4][kWords] = w[x][hf];
+            const uint32_t lo01 = __byte_perm(v[0][j], v[1][j], 0x5140), lo23 = __byte_perm(v[0][j], v[1][j], 0x7362);
+            const uint32_t hi01 = __byte_perm(v[2][j], v[3][j], 0x5140), hi23 = __byte_perm(v[2][j], v[3][j], 0x7362);
             float(&d0)[4] = o[hf][2 * j];
             float(&d1)[4] = o[hf][2 * j + 1];
-            if (fold) {
-              mma_16816<__half>(d0[0], d0[1], d0[2], d0[3], e4m3lo_to_f16x2(lo01), e4m3hi_to_f16x2(lo01),
-                                e4m3lo_to_f16x2(hi01), e4m3hi_to_f16x2(hi01), pb0, pb1);
-              mma_16816<__half>(d1[0], d1[1], d1[2], d1[3], e4m3lo_to_f16x2(lo23), e4m3hi_to_f16x2(lo23),
-                                e4m3lo_to_f16x2(hi23), e4m3hi_to_f16x2(hi23), pb0, pb1);
+            if constexpr (!kApart) {
+              mma_f16(d0, e4m3lo_to_f16x2(lo01), e4m3hi_to_f16x2(lo01), e4m3lo_to_f16x2(hi01), e4m3hi_to_f16x2(hi01), pb0,
+                      pb1);
+              mma_f16(d1, e4m3lo_to_f16x2(lo23), e4m3hi_to_f16x2(lo23), e4m3lo_to_f16x2(hi23), e4m3hi_to_f16x2(hi23), pb0,
+                      pb1);
             } else {
               float z0[4] = {0.f, 0.f, 0.f, 0.f}, z1[4] = {0.f, 0.f, 0.f, 0.f};
-              mma_16816<__half>(z0[0], z0[1], z0[2], z0[3], e4m3lo_to_f16x2(lo01), e4m3hi_to_f16x2(lo01),
-                                e4m3lo_to_f16x2(hi01), e4m3hi_to_f16x2(hi01), pb0, pb1);
-              mma_16816<__half>(z1[0], z1[1], z1[2], z1[3], e4m3lo_to_f16x2(lo23), e4m3hi_to_f16x2(lo23),
-                                e4m3lo_to_f16x2(hi23), e4m3hi_to_f16x2(hi23), pb0, pb1);
+              mma_f16(z0, e4m3lo_to_f16x2(lo01), e4m3hi_to_f16x2(lo01), e4m3lo_to_f16x2(hi01), e4m3hi_to_f16x2(hi01), pb0,
+                      pb1);
+              mma_f16(z1, e4m3lo_to_f16x2(lo23), e4m3hi_to_f16x2(lo23), e4m3lo_to_f16x2(hi23), e4m3hi_to_f16x2(hi23), pb0,
+                      pb1);
 #pragma unroll
               for (int e = 0; e < 4; ++e) d0[e] += ratio * z0[e], d1[e] += ratio * z1[e];
             }
           }
         }
+      };
+      // A much larger V scale becomes the reference (the sums shrink by a power
+      // of two); a much smaller one is added apart.
+      const float vmax = fmaxf(sc.z, sc.w);
+      if (vmax > vref * 16.f) {
+        const float r = vref * pow2_inverse(vmax);
+        vref = vmax;
+        vinv = pow2_inverse(vmax);
+#pragma unroll
+        for (int hf = 0; hf < C::kHalves; ++hf)
+#pragma unroll
+          for (int j = 0; j < 2 * kWords; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[hf][j][e] *= r;
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->empty[slot]);
+      const float r0 = sc.z * vinv, r1 = sc.w * vinv;
+      if (fminf(r0, r1) >= 0.015625f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0][e] *= r0, s[1][e] *= r1;
+        pv(0, 1.f, std::false_type());
+        pv(1, 1.f, std::false_type());
+      } else {
+        pv(0, r0, std::true_type());
+        pv(1, r1, std::true_type());
+      }
     }
-    base += nsteps;
+    __syncwarp();
+    if (!ok) break;
+    if (lane == 0) mbar_arrive(&sh->item_empty[slot_i]);
 
-    // ---- merge the warps ----
+    // ---- merge the warps: the one with class 0 joins the others' sums to its own ----
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, off);
       l1 += __shfl_xor_sync(0xffffffffu, l1, off);
     }
     const int h0 = 2 * t4, h1 = 2 * t4 + 1;
-    if (g_row == 0) {
-      sh->ml[warp][h0][0] = m0, sh->ml[warp][h0][1] = l0;
-      sh->ml[warp][h1][0] = m1, sh->ml[warp][h1][1] = l1;
-    }
-    float* cw = comb_o + warp * gmax * D;
-#pragma unroll
-    for (int hf = 0; hf < C::kHalves; ++hf)
-#pragma unroll
-      for (int j = 0; j < 2 * kWords; ++j) {
-        const int d0 = hf * 128 + g_row * kLaneDims + 2 * j;
-        if (h0 < it.heads) *reinterpret_cast<float2*>(cw + h0 * D + d0) = make_float2(o[hf][j][0] * vref, o[hf][j][2] * vref);
-        if (h1 < it.heads) *reinterpret_cast<float2*>(cw + h1 * D + d0) = make_float2(o[hf][j][1] * vref, o[hf][j][3] * vref);
+    const bool holds = h0 < it.heads;
+    // the previous item's sums have been read (every warp waits here, so no phase is skipped)
+    ok = __all_sync(0xffffffffu, wait_or_abort(&sh->comb_free, (n_item & 1) ^ 1, &sh->abort, a.err));
+    if (!ok) break;
+    if (cls != 0) {
+      const int w = cls - 1;
+      if (g_row == 0) {
+        sh->ml[w][h0] = make_float2(m0, l0);
+        sh->ml[w][h1] = make_float2(m1, l1);
       }
-    named_barrier_sync(1, kNW * 32);
-    for (int e = threadIdx.x; e < it.heads * D; e += kNW * 32) {
-      const int hd = e / D;
-      const int d = e - hd * D;
-      float M = -INFINITY;
+      if (holds) {
+        const uint32_t dst = comb_a + w * C::kVecs * comb_vec;
 #pragma unroll
-      for (int w = 0; w < kNW; ++w) M = fmaxf(M, sh->ml[w][hd][0]);
-      float L = 0.f, O = 0.f;
+        for (int hf = 0; hf < C::kHalves; ++hf)
 #pragma unroll
-      for (int w = 0; w < kNW; ++w) {
-        const float mw = sh->ml[w][hd][0];
-        const float f = mw == -INFINITY ? 0.f : (mw == M ? 1.f : fast_exp2(mw - M));
-        L += f * sh->ml[w][hd][1];
-        O += f * comb_o[(w * gmax + hd) * D + d];
+          for (int j = 0; j < 2 * kWords; ++j) {
+            const float(&x)[4] = o[hf][j];
+            sts128f(dst + (hf * 2 * kWords + j) * comb_vec, x[0] * vref, x[1] * vref, x[2] * vref, x[3] * vref);
+          }
       }
-      store_result<T>(a, it, hd, d, M, L, O);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->comb_full);
+      continue;
     }
-    named_barrier_sync(1, kNW * 32);
+    ok = __all_sync(0xffffffffu, wait_or_abort(&sh->comb_full, n_item & 1, &sh->abort, a.err));
+    if (!ok) break;
+    if (holds) {
+      float M0 = m0, M1 = m1;
+      float2 ml0[kNW - 1], ml1[kNW - 1];
+#pragma unroll
+      for (int w = 0; w < kNW - 1; ++w) {
+        ml0[w] = sh->ml[w][h0], ml1[w] = sh->ml[w][h1];
+        M0 = fmaxf(M0, ml0[w].x), M1 = fmaxf(M1, ml1[w].x);
+      }
+      auto weight = [](float m, float M) { return m == -INFINITY ? 0.f : (m == M ? 1.f : fast_exp2(m - M)); };
+      const float s0 = weight(m0, M0), s1 = weight(m1, M1);
+      float L0 = s0 * l0, L1 = s1 * l1;
+      const float r0 = s0 * vref, r1 = s1 * vref;
+#pragma unroll
+      for (int hf = 0; hf < C::kHalves; ++hf)
+#pragma unroll
+        for (int j = 0; j < 2 * kWords; ++j) {
+          float(&x)[4] = o[hf][j];
+          x[0] *= r0, x[2] *= r0, x[1] *= r1, x[3] *= r1;
+        }
+#pragma unroll
+      for (int w = 0; w < kNW - 1; ++w) {
+        const float w0 = weight(ml0[w].x, M0), w1 = weight(ml1[w].x, M1);
+        L0 += w0 * ml0[w].y, L1 += w1 * ml1[w].y;
+        const uint32_t src = comb_a + w * C::kVecs * comb_vec;
+#pragma unroll
+        for (int hf = 0; hf < C::kHalves; ++hf)
+#pragma unroll
+          for (int j = 0; j < 2 * kWords; ++j) {
+            const float4 y = lds128f(src + (hf * 2 * kWords + j) * comb_vec);
+            float(&x)[4] = o[hf][j];
+            x[0] += w0 * y.x, x[1] += w1 * y.y, x[2] += w0 * y.z, x[3] += w1 * y.w;
+          }
+      }
+      // sum 0: no token (nothing seen); a NaN sum stays NaN
+      const float i0 = L0 == 0.f ? 0.f : 1.f / L0, i1 = L1 == 0.f ? 0.f : 1.f / L1;
+      const bool parts = it.nch > 1;
+      if (parts && !has_part(a, it)) {
+        raise_dev(a.err, BL_DEVERR_WORKSPACE);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (c == 1 && h1 >= it.heads) break;
+          const int hq = it.hq0 + (c ? h1 : h0);
+          const float inv = c ? i1 : i0;
+          T* dst = reinterpret_cast<T*>(a.out) + (int64_t)it.b * a.o_sb + (int64_t)hq * a.o_sh;
+          float* part = a.ws_o + ((int64_t)it.part * a.hq + hq) * D;
+          if (parts && g_row == 0)
+            a.ws_lse[(int64_t)it.part * a.hq + hq] = c ? (L1 == 0.f ? -INFINITY : M1 + __log2f(L1))
+                                                       : (L0 == 0.f ? -INFINITY : M0 + __log2f(L0));
+#pragma unroll
+          for (int hf = 0; hf < C::kHalves; ++hf)
+#pragma unroll
+            for (int j = 0; j < 2 * kWords; j += 2) {
+              const int d = hf * 128 + g_row * kLaneDims + 2 * j;
+              const float v0 = o[hf][j][c] * inv, v1 = o[hf][j][2 + c] * inv;
+              const float v2 = o[hf][j + 1][c] * inv, v3 = o[hf][j + 1][2 + c] * inv;
+              if (parts) {
+                *reinterpret_cast<float4*>(part + d) = make_float4(v0, v1, v2, v3);
+              } else if (a.o_vec) {
+                *reinterpret_cast<uint2*>(dst + d) = make_uint2(pack2<T>(v0, v1), pack2<T>(v2, v3));
+              } else {
+                dst[d] = from_f32<T>(v0), dst[d + 1] = from_f32<T>(v1);
+                dst[d + 2] = from_f32<T>(v2), dst[d + 3] = from_f32<T>(v3);
+              }
+            }
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh->comb_free);
   }
+  // Drain: every copy this warp issued lands before the CTA can exit (some are
+  // left only where the CTA gave up).
+  for (; taken < issued; ++taken)
+    if (!mbar_wait(&sh->full[warp][taken % kDepth], (taken / kDepth) & 1)) raise_dev(a.err, BL_DEVERR_TIMEOUT);
 }
 
 // ---------------------------------------------------------------------------
@@ -607,7 +951,7 @@ __global__ void __launch_bounds__(kSimtThreads) fp8_decode_simt_kernel(const Arg
 
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     Item it;
-    if (!get_item(a, item, it)) {
+    if (!make_item(a, item, load_unit(a, item), it)) {
       if (tid == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
       continue;
     }
@@ -621,7 +965,7 @@ __global__ void __launch_bounds__(kSimtThreads) fp8_decode_simt_kernel(const Arg
     float acc[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[k] = 0.f;
-    const int64_t row = a.row_ids ? (int64_t)a.row_ids[it.b] : (int64_t)it.b;
+    const int64_t row = it.table_row;
     for (int t0 = it.t0; t0 < it.t1; t0 += kSimtTokens) {
       __syncthreads();  // the previous tile is no longer read; qs is complete
       if (tid < kSimtTokens) {
@@ -689,7 +1033,16 @@ __global__ void __launch_bounds__(kSimtThreads) fp8_decode_simt_kernel(const Arg
       for (int k = 0; k < 8; ++k) {
         const int h = vh0 + k * vstep;
         if (h >= it.heads) break;
-        store_result<T>(a, it, h, vd, sh->m[h], sh->l[h], acc[k]);
+        const int hq = it.hq0 + h;
+        const float L = sh->l[h], val = L == 0.f ? 0.f : acc[k] / L;  // a NaN sum stays NaN
+        if (it.nch <= 1) {
+          reinterpret_cast<T*>(a.out)[(int64_t)it.b * a.o_sb + (int64_t)hq * a.o_sh + vd] = from_f32<T>(val);
+        } else if (!has_part(a, it)) {
+          if (vd == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
+        } else {
+          a.ws_o[((int64_t)it.part * a.hq + hq) * a.d + vd] = val;
+          if (vd == 0) a.ws_lse[(int64_t)it.part * a.hq + hq] = L == 0.f ? -INFINITY : sh->m[h] + __log2f(L);
+        }
       }
     }
   }
@@ -703,28 +1056,32 @@ size_t simt_smem(int d) { return sizeof(SimtShared) + sizeof(float) * (8 * (size
 constexpr int kReduceThreads = 128;
 constexpr int kReduceTile = 512;  // chunks whose weights are in shared memory at a time
 
-// grid: (batch, hq)
+// grid: (batch, hq).  Warp w sums every fourth chunk, a lane four consecutive
+// dims at a time; the warps' sums are joined in shared memory.
 template <typename T>
 __global__ void __launch_bounds__(kReduceThreads) fp8_decode_reduce_kernel(const Args a) {
   pdl_wait();  // the partials are complete and visible
-  const int b = blockIdx.x, hq = blockIdx.y, tid = threadIdx.x;
+  constexpr int kWarps = kReduceThreads / 32;
+  const int b = blockIdx.x, hq = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t len = min((int64_t)a.seq_lens[b], a.bt_width * a.bs);
   if (len <= kChunk) return;
   const int nch = (int)((len + kChunk - 1) / kChunk);
   const int64_t base = a.row_base[b];
   if (base < 0 || base + nch > a.max_units) return;  // flagged by the plan or the attention kernel
   __shared__ float s_w[kReduceTile];
-  __shared__ float s_red[kReduceThreads / 32];
+  __shared__ float s_red[kWarps];
+  __shared__ float s_num[kWarps][256];
   float M = -INFINITY;
   for (int c = tid; c < nch; c += kReduceThreads) M = fmaxf(M, a.ws_lse[(base + c) * a.hq + hq]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  if ((tid & 31) == 0) s_red[tid >> 5] = M;
+  if (lane == 0) s_red[warp] = M;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kReduceThreads / 32; ++w) M = fmaxf(M, s_red[w]);
-  float num[2] = {0.f, 0.f}, den = 0.f;  // head_dim <= 2 * kReduceThreads
+  for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_red[w]);
+  float num[2][4] = {}, den = 0.f;
   const int64_t cstride = (int64_t)a.hq * a.d;
+  const bool vec = (a.d & 3) == 0;
   for (int c0 = 0; c0 < nch; c0 += kReduceTile) {
     const int n = min(kReduceTile, nch - c0);
     __syncthreads();
@@ -736,19 +1093,33 @@ __global__ void __launch_bounds__(kReduceThreads) fp8_decode_reduce_kernel(const
     const float* po = a.ws_o + ((base + c0) * a.hq + hq) * a.d;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int d = tid + k * kReduceThreads;
+      const int d = 4 * lane + 128 * k;
       if (d >= a.d) break;
+      if (vec) {
 #pragma unroll 8
-      for (int c = 0; c < n; ++c) num[k] += s_w[c] * po[c * cstride + d];
+        for (int c = warp; c < n; c += kWarps) {
+          const float4 x = *reinterpret_cast<const float4*>(po + c * cstride + d);
+          const float f = s_w[c];
+          num[k][0] += f * x.x, num[k][1] += f * x.y, num[k][2] += f * x.z, num[k][3] += f * x.w;
+        }
+      } else {
+        for (int c = warp; c < n; c += kWarps)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < a.d) num[k][e] += s_w[c] * po[c * cstride + d + e];
+      }
     }
     for (int c = 0; c < n; ++c) den += s_w[c];
   }
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int d = tid + k * kReduceThreads;
-    if (d < a.d)
-      reinterpret_cast<T*>(a.out)[(int64_t)b * a.o_sb + (int64_t)hq * a.o_sh + d] =
-          from_f32<T>(den == 0.f ? 0.f : num[k] / den);
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s_num[warp][4 * lane + 128 * k + e] = num[k][e];
+  __syncthreads();
+  T* dst = reinterpret_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)hq * a.o_sh;
+  for (int d = tid; d < a.d; d += kReduceThreads) {
+    const float x = (s_num[0][d] + s_num[1][d]) + (s_num[2][d] + s_num[3][d]);
+    dst[d] = from_f32<T>(den == 0.f ? 0.f : x / den);
   }
 }
 
@@ -771,8 +1142,12 @@ int launch_tc(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
   if (!make_tmap_rows_8bit(&kmap, kv.k_pool, D, rows, C::kRow, 16) ||
       !make_tmap_rows_8bit(&vmap, kv.v_pool, D, rows, C::kRow, 16))
     return BL_ERR_LAUNCH;
-  const size_t fixed = 1024 + (size_t)C::kStages * C::kSlot + sizeof(TCShared<D>);
-  const size_t smem = fixed + (size_t)kNW * std::min(k.g, 8) * D * sizeof(float);
+  const auto smem_for = [](int g) {
+    const size_t heads = std::min(g, 8);
+    return 1024 + (size_t)kNW * C::kDepth * C::kSlot + sizeof(TCShared<D>) + 2 * C::kKS * 4 * heads * sizeof(uint2) +
+           (size_t)(kNW - 1) * C::kVecs * 8 * ((heads + 1) / 2) * sizeof(float4);
+  };
+  const size_t smem = smem_for(k.g);
   const int64_t items = (int64_t)k.max_units * k.hkv * k.head_tiles;
   // resident CTAs per SM, asked once per device and head tile (the attribute is per device too)
   static std::mutex mu;
@@ -785,7 +1160,7 @@ int launch_tc(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
     if (*slot == 0) {
       int o = 0;
       if (cudaFuncSetAttribute(fp8_decode_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)(fixed + (size_t)kNW * 8 * D * sizeof(float))) != cudaSuccess ||
+                               (int)smem_for(8)) != cudaSuccess ||
           cudaOccupancyMaxActiveBlocksPerMultiprocessor(&o, fp8_decode_tc_kernel<T, D>, kThreadsTC, smem) !=
               cudaSuccess) {
         set_error("fp8_decode_tc_kernel: %s", cudaGetErrorString(cudaGetLastError()));
@@ -900,10 +1275,11 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
   k.bs = (int32_t)kv.block_size;
   k.d = (int32_t)kv.head_dim;
   k.q_vec = ((uintptr_t)a.q & 7) == 0 && a.q_stride_b % 4 == 0 && a.q_stride_h % 4 == 0;
+  k.o_vec = ((uintptr_t)a.out & 7) == 0 && a.out_stride_b % 4 == 0 && a.out_stride_h % 4 == 0;
   k.scale_log2 = a.scale * kLog2e;
   k.hdr = (const int32_t*)(ws + w.hdr);
   k.row_base = (const int32_t*)(ws + w.row_base);
-  k.exec = (const int2*)(ws + w.exec);
+  k.units = (const Unit*)(ws + w.units);
   k.ws_lse = (float*)(ws + w.lse);
   k.ws_o = (float*)(ws + w.o);
   k.max_units = (int32_t)w.max_units;
@@ -911,19 +1287,20 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
   k.err = a.err;
 
   if (!a.plan_ready) {
-    DecodePlanArgs p;
+    PlanArgs p;
     p.seq_lens = a.seq_lens;
+    p.row_ids = kv.row_ids;
     p.batch = k.batch;
-    p.bs = 1;  // chunks are counted in tokens
-    p.chunk_blocks = kChunk;
-    p.bt_width = (int32_t)std::min<int64_t>(kv.bt_width * kv.block_size, INT32_MAX);
     p.max_units = k.max_units;
+    p.cap = kv.bt_width * kv.block_size;
     p.hdr = (int32_t*)(ws + w.hdr);
     p.row_base = (int32_t*)(ws + w.row_base);
-    p.exec = (int2*)(ws + w.exec);
+    p.units = (Unit*)(ws + w.units);
     p.err = a.err;
-    rc = launch_decode_plan(p, s);
-    if (rc) return rc;
+    if (launch_pdl(fp8_decode_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p) != cudaSuccess) {
+      set_error("fp8_decode_plan_kernel: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+      return BL_ERR_LAUNCH;
+    }
   }
   switch (kv.dtype) {
     case BL_F32: return launch_all<float>(k, kv, s);
