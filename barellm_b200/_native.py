@@ -8,6 +8,7 @@ There is no fallback: if the shared library is missing the first call raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
@@ -350,6 +351,28 @@ STRUCTS = {
     "bl_copy_blocks_args": CopyBlocksArgs,
 }
 
+_FORMAT = {c_void_p: "P", c_int64: "q", c_int32: "i", c_float: "f", c_size_t: "N"}
+
+
+def _format(cls) -> str:
+    return "".join(_format(t) if issubclass(t, Structure) else _FORMAT[t] for _, t in cls._fields_)
+
+
+def _packer(cls):
+    """``cls``'s fields, nested ones in line, to the bytes of the C structure
+    (native sizes and alignment; a null pointer is 0): a fraction of the cost of
+    filling a ctypes Structure field by field, for calls of a few microseconds."""
+    s = struct.Struct("@" + _format(cls))
+    assert s.size == ctypes.sizeof(cls), cls
+    return s.pack
+
+
+pack_append_fp8_args = _packer(AppendFp8Args)
+pack_gather_fp8_args = _packer(GatherFp8Args)
+pack_decode_fp8_args = _packer(DecodeFp8Args)
+pack_prefill_fp8_args = _packer(PrefillFp8Args)
+pack_copy_blocks_args = _packer(CopyBlocksArgs)
+
 _lib: ctypes.CDLL | None = None
 
 
@@ -391,19 +414,19 @@ def load() -> ctypes.CDLL:
     lib.bl_paged_prefill.restype = c_int
     lib.bl_rms_norm.argtypes = [POINTER(RmsNormArgs), c_void_p]
     lib.bl_rms_norm.restype = c_int
-    lib.bl_paged_append_fp8.argtypes = [POINTER(AppendFp8Args), c_void_p]
+    lib.bl_paged_append_fp8.argtypes = [c_void_p, c_void_p]  # a packed AppendFp8Args, or a reference to one
     lib.bl_paged_append_fp8.restype = c_int
-    lib.bl_paged_gather_fp8.argtypes = [POINTER(GatherFp8Args), c_void_p]
+    lib.bl_paged_gather_fp8.argtypes = [c_void_p, c_void_p]  # a packed GatherFp8Args, or a reference to one
     lib.bl_paged_gather_fp8.restype = c_int
     lib.bl_paged_decode_fp8_workspace_bytes.argtypes = [c_int64] * 4
     lib.bl_paged_decode_fp8_workspace_bytes.restype = c_size_t
-    lib.bl_paged_decode_fp8.argtypes = [POINTER(DecodeFp8Args), c_void_p]
+    lib.bl_paged_decode_fp8.argtypes = [c_void_p, c_void_p]  # a packed DecodeFp8Args, or a reference to one
     lib.bl_paged_decode_fp8.restype = c_int
     lib.bl_paged_prefill_fp8_workspace_bytes.argtypes = [c_int32] + [c_int64] * 7
     lib.bl_paged_prefill_fp8_workspace_bytes.restype = c_size_t
-    lib.bl_paged_prefill_fp8.argtypes = [POINTER(PrefillFp8Args), c_void_p]
+    lib.bl_paged_prefill_fp8.argtypes = [c_void_p, c_void_p]  # a packed PrefillFp8Args, or a reference to one
     lib.bl_paged_prefill_fp8.restype = c_int
-    lib.bl_copy_blocks.argtypes = [POINTER(CopyBlocksArgs), c_void_p]
+    lib.bl_copy_blocks.argtypes = [c_void_p, c_void_p]
     lib.bl_copy_blocks.restype = c_int
     lib.bl_last_error.argtypes = []
     lib.bl_last_error.restype = c_char_p

@@ -118,8 +118,8 @@ extern "C" int bl_copy_blocks(const bl_copy_blocks_args* args, void* stream) {
   for (int64_t at = 0; at < a.count; at += kPairsPerLaunch) {
     const int n = (int)std::min<int64_t>(kPairsPerLaunch, a.count - at);
     for (int i = 0; i < n; ++i) {
-      k.src[i] = a.src[at + i];
-      k.dst[i] = a.dst[at + i];
+      k.src[i] = (int32_t)a.src[at + i];
+      k.dst[i] = (int32_t)a.dst[at + i];
     }
     dim3 grid((unsigned)(n * k.parts), 2, (unsigned)a.num_layers);
     if (vec)

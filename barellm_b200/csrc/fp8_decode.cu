@@ -303,24 +303,6 @@ __device__ __forceinline__ int swizzled(int r, int c) {
   return r * ROW + ((ROW == 128 ? (c ^ (r & 7)) : (c ^ ((r >> 1) & 3))) << 4);
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ float4 lds128f(uint32_t addr) {
-  const uint4 v = lds128(addr);
-  return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
-}
-__device__ __forceinline__ void sts128f(uint32_t addr, float a, float b, float c, float d) {
-  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
-}
-
 // D += A(16x16) * B(16x8) in fp16 with fp32 sums.  Not volatile: a pure function
 // of its registers, so the compiler may interleave independent products.
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -331,13 +313,29 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Waits unless the CTA gave up; a wait that runs out makes it give up.
+// Waits unless the CTA gave up; a wait that runs out (2 s) makes it give up.  A
+// waiting warp sleeps in the barrier unit up to the hint's time, so that it does
+// not take issue slots from the others.
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, int* abort, int32_t* err) {
-  if (*(volatile int*)abort) return false;
-  if (mbar_wait(bar, parity)) return true;
-  raise_dev(err, BL_DEVERR_TIMEOUT);
-  *(volatile int*)abort = 1;
-  return false;
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    if (done) return true;
+    if (*(volatile int*)abort) return false;
+    if (global_timer_ns() - t0 > 2000000000ull) {
+      raise_dev(err, BL_DEVERR_TIMEOUT);
+      *(volatile int*)abort = 1;
+      return false;
+    }
+  }
 }
 
 // An item on its way to the ring: lane i holds tile i of the chunk.  begin()
@@ -434,8 +432,7 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
                     offsetof(ItemSlot<D>, ks) % 8 == 0 && offsetof(ItemSlot<D>, vs) % 8 == 0,
                 "vector accesses to shared memory");
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  unsigned char* slots =
-      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* slots = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   TCShared<D>* sh = reinterpret_cast<TCShared<D>*>(slots + kNW * C::kDepth * C::kSlot);
   const int room = 4 * min(a.g, 8);                              // lanes of the heads an item can have
   uint2* qs = reinterpret_cast<uint2*>(sh + 1);                  // [2][kKS][room] fragments
@@ -504,8 +501,8 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
   const uint32_t v_off = (uint32_t)((g_row * kLaneDims) & 15);
   // merge buffer: the lanes that hold heads, (head pairs) x 8 of them, side by side
   const int pairs = (min(a.g, 8) + 1) / 2;
-  const uint32_t comb_a = smem_u32(comb) + 16 * (g_row * pairs + t4);
-  const uint32_t comb_vec = 16 * 8 * pairs;  // bytes between a lane's float4s
+  float4* const mine = reinterpret_cast<float4*>(comb) + g_row * pairs + t4;
+  const int comb_vec = 8 * pairs;  // float4s between a lane's own
   const uint64_t policy = policy_evict_first();
   const int my_items = items > blockIdx.x ? (int)((items - blockIdx.x + gridDim.x - 1) / gridDim.x) : 0;
 
@@ -519,7 +516,9 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
   int at_item = -1, at_step = 0, at_steps = 0;
   int at_tiles = 0;
   // Issues the next step if there is one; `may_wait` false: only if its item is
-  // described already.  n_item: the item being consumed.
+  // described already.  n_item: the item being consumed; the cursor goes at most
+  // one item further, since the planner describes that one only after this warp
+  // has taken its steps of the item before n_item.
   auto issue = [&](int n_item, bool may_wait) -> bool {
     while (at_step >= at_steps) {
       const int next = at_item + 1;
@@ -569,14 +568,12 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
     const int slot_i = n_item & 1;
     ok = __all_sync(0xffffffffu, wait_or_abort(&sh->item_full[slot_i], (n_item >> 1) & 1, &sh->abort, a.err));
     if (!ok) break;
-    while (issued - taken < kDepth && issue(n_item, false)) {
-    }
     const Item it = sh->items[slot_i].it;
     const float2 fs = sh->items[slot_i].f[t4];
     uint2 qf[kKS];
 #pragma unroll
     for (int ks = 0; ks < kKS; ++ks)
-      qf[ks] = g_row < it.heads ? lds64(smem_u32(qs + (slot_i * kKS + ks) * room + lane)) : make_uint2(0u, 0u);
+      qf[ks] = g_row < it.heads ? qs[(slot_i * kKS + ks) * room + lane] : make_uint2(0u, 0u);
     const float f0 = fs.x, f1 = fs.y;
     const int nsteps = (it.t1 - it.t0 + kStepTokens - 1) / kStepTokens;
 
@@ -599,16 +596,20 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
     // depend on its warp, so a row's result does not depend on what ran before it.
     const int cls = (warp + n_item) & (kNW - 1);
     for (int i = cls; i < nsteps; i += kNW) {
-      if (issued == taken) ok = issue(n_item, true);
+      // The slots freed by earlier steps are filled here, so that copies are in
+      // flight for one step beyond this one.  (More does not help: HBM gives these
+      // scattered 2 KB pages at its best rate with about 96 KB in flight per SM.)
+      while (issued - taken < kDepth && issue(n_item, issued == taken)) {
+      }
       const int slot = taken % kDepth;
-      ok = ok && __all_sync(0xffffffffu,
-                            wait_or_abort(&sh->full[warp][slot], (taken / kDepth) & 1, &sh->abort, a.err));
+      ok = issued > taken && __all_sync(0xffffffffu, wait_or_abort(&sh->full[warp][slot], (taken / kDepth) & 1, &sh->abort,
+                                                                   a.err));
       if (!ok) break;
       const float2 ks2 = *reinterpret_cast<const float2*>(&sh->items[slot_i].ks[2 * i]);
       const float2 vs2 = *reinterpret_cast<const float2*>(&sh->items[slot_i].vs[2 * i]);
       const float4 sc = make_float4(ks2.x, ks2.y, vs2.x, vs2.y);
       const uint32_t kb = smem_u32(ring + slot * C::kSlot);
-      const uint32_t vb = kb + 2 * C::kTile;
+      const unsigned char* vb = ring + slot * C::kSlot + 2 * C::kTile + v_off;
 
       // S^T[token][head] = K[token] . q[head], codes times normalised q.  Two chains of
       // sums per tile, joined at the end: the products of a chain wait for one another.
@@ -645,44 +646,6 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
           for (int e = 0; e < 4; ++e) s[x][e] = z[x][0][e] + z[x][1][e];
       }
       const int nvalid = it.t1 - (it.t0 + i * kStepTokens);  // tokens of the step that exist
-
-      // V's codes into registers; then the slot takes the next copies, ahead of the
-      // softmax below.  A lane takes the kLaneDims consecutive dims
-      // g_row * kLaneDims of tokens 2t, 2t+1, 2t+8, 2t+9.
-      uint32_t w[2][C::kHalves][4][kWords];
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int hf = 0; hf < C::kHalves; ++hf)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t addr = vb + x * C::kTile + hf * C::kBox + v_off +
-                                  swizzled<C::kRow>(2 * t4 + (k & 1) + 8 * (k >> 1), (g_row * kLaneDims) >> 4);
-            if constexpr (kWords == 4) {
-              const uint4 v = lds128(addr);
-              w[x][hf][k][0] = v.x, w[x][hf][k][1] = v.y, w[x][hf][k][2] = v.z, w[x][hf][k][3] = v.w;
-            } else {
-              const uint2 v = lds64(addr);
-              w[x][hf][k][0] = v.x, w[x][hf][k][1] = v.y;
-            }
-          }
-      ++taken;
-      __syncwarp();
-      while (issued - taken < kDepth && issue(n_item, false)) {
-      }
-      if (nvalid < kStepTokens) {
-        // slots past the length hold stale codes (possibly NaN): 0 * NaN is NaN
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int hf = 0; hf < C::kHalves; ++hf)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-              for (int j = 0; j < kWords; ++j)
-                w[x][hf][k][j] = 16 * x + 2 * t4 + (k & 1) + 8 * (k >> 1) < nvalid ? w[x][hf][k][j] : 0u;
-      }
-
       float c00 = f0 * sc.x, c01 = f1 * sc.x, c10 = f0 * sc.y, c11 = f1 * sc.y;  // log2 units
       if (nvalid < kStepTokens) {
 #pragma unroll
@@ -705,14 +668,16 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
         // (-inf) - (-inf) is NaN: a head whose scores are all -inf so far keeps its (zero) sums
         const float al0 = n0 == m0 ? 1.f : fast_exp2(m0 - n0), al1 = n1 == m1 ? 1.f : fast_exp2(m1 - n1);
         m0 = n0, m1 = n1;
-        l0 *= al0, l1 *= al1;
+        if (i != cls) {  // (on a warp's first step there are no sums yet)
+          l0 *= al0, l1 *= al1;
 #pragma unroll
-        for (int hf = 0; hf < C::kHalves; ++hf)
+          for (int hf = 0; hf < C::kHalves; ++hf)
 #pragma unroll
-          for (int j = 0; j < 2 * kWords; ++j) {
-            o[hf][j][0] *= al0, o[hf][j][2] *= al0;
-            o[hf][j][1] *= al1, o[hf][j][3] *= al1;
-          }
+            for (int j = 0; j < 2 * kWords; ++j) {
+              o[hf][j][0] *= al0, o[hf][j][2] *= al0;
+              o[hf][j][1] *= al1, o[hf][j][3] *= al1;
+            }
+        }
       }
       const float u0 = m0 == -INFINITY ? 0.f : -m0, u1 = m1 == -INFINITY ? 0.f : -m1;
       // exponentials and row sums
@@ -723,20 +688,41 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
       l0 += (s[0][0] + s[0][2]) + (s[1][0] + s[1][2]);
       l1 += (s[0][1] + s[0][3]) + (s[1][1] + s[1][3]);
 
-      // O^T[dim][head] += V^T[dim][token] P^T[token][head] of tile x.  Two tokens' bytes
-      // are paired, so a converted pair is one A register (row = dim, two
-      // consecutive tokens).  APART: the tile's sums are made on their own and
-      // added times `ratio`.
+      // O^T[dim][head] += V^T[dim][token] P^T[token][head] of tile x.  A lane takes the
+      // kLaneDims consecutive dims g_row * kLaneDims of tokens 2t, 2t+1, 2t+8, 2t+9 and
+      // pairs two tokens' bytes, so a converted pair is one A register (row =
+      // dim, two consecutive tokens).  APART: the tile's sums are made on their
+      // own and added times `ratio`.
       auto pv = [&](int x, float ratio, auto apart) {
         constexpr bool kApart = decltype(apart)::value;
         // P^T (tokens x heads) -> B fragment (k = token, n = head)
         const uint32_t pb0 = movmatrix_trans(pack2<__half>(s[x][0], s[x][1]));
         const uint32_t pb1 = movmatrix_trans(pack2<__half>(s[x][2], s[x][3]));
+        const int left = nvalid - 16 * x;
 #pragma unroll
         for (int hf = 0; hf < C::kHalves; ++hf) {
+          uint32_t v[4][kWords];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const unsigned char* p = vb + x * C::kTile + hf * C::kBox +
+                                     swizzled<C::kRow>(2 * t4 + (k & 1) + 8 * (k >> 1), (g_row * kLaneDims) >> 4);
+            if constexpr (kWords == 4) {
+              const uint4 u = *reinterpret_cast<const uint4*>(p);
+              v[k][0] = u.x, v[k][1] = u.y, v[k][2] = u.z, v[k][3] = u.w;
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2*>(p);
+              v[k][0] = u.x, v[k][1] = u.y;
+            }
+          }
+          if (left < 16) {
+            // slots past the length hold stale codes (possibly NaN): 0 * NaN is NaN
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int j = 0; j < kWords; ++j) v[k][j] = 2 * t4 + (k & 1) + 8 * (k >> 1) < left ? v[k][j] : 0u;
+          }
 #pragma unroll
           for (int j = 0; j < kWords; ++j) {
-            const uint32_t(&v)[4][kWords] = w[x][hf];
             const uint32_t lo01 = __byte_perm(v[0][j], v[1][j], 0x5140), lo23 = __byte_perm(v[0][j], v[1][j], 0x7362);
             const uint32_t hi01 = __byte_perm(v[2][j], v[3][j], 0x5140), hi23 = __byte_perm(v[2][j], v[3][j], 0x7362);
             float(&d0)[4] = o[hf][2 * j];
@@ -765,12 +751,14 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
         const float r = vref * pow2_inverse(vmax);
         vref = vmax;
         vinv = pow2_inverse(vmax);
+        if (i != cls) {
 #pragma unroll
-        for (int hf = 0; hf < C::kHalves; ++hf)
+          for (int hf = 0; hf < C::kHalves; ++hf)
 #pragma unroll
-          for (int j = 0; j < 2 * kWords; ++j)
+            for (int j = 0; j < 2 * kWords; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[hf][j][e] *= r;
+              for (int e = 0; e < 4; ++e) o[hf][j][e] *= r;
+        }
       }
       const float r0 = sc.z * vinv, r1 = sc.w * vinv;
       if (fminf(r0, r1) >= 0.015625f) {
@@ -782,6 +770,8 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
         pv(0, r0, std::true_type());
         pv(1, r1, std::true_type());
       }
+      ++taken;
+      __syncwarp();
     }
     __syncwarp();
     if (!ok) break;
@@ -805,13 +795,13 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
         sh->ml[w][h1] = make_float2(m1, l1);
       }
       if (holds) {
-        const uint32_t dst = comb_a + w * C::kVecs * comb_vec;
+        float4* dst = mine + w * C::kVecs * comb_vec;
 #pragma unroll
         for (int hf = 0; hf < C::kHalves; ++hf)
 #pragma unroll
           for (int j = 0; j < 2 * kWords; ++j) {
             const float(&x)[4] = o[hf][j];
-            sts128f(dst + (hf * 2 * kWords + j) * comb_vec, x[0] * vref, x[1] * vref, x[2] * vref, x[3] * vref);
+            dst[(hf * 2 * kWords + j) * comb_vec] = make_float4(x[0] * vref, x[1] * vref, x[2] * vref, x[3] * vref);
           }
       }
       __syncwarp();
@@ -843,12 +833,12 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
       for (int w = 0; w < kNW - 1; ++w) {
         const float w0 = weight(ml0[w].x, M0), w1 = weight(ml1[w].x, M1);
         L0 += w0 * ml0[w].y, L1 += w1 * ml1[w].y;
-        const uint32_t src = comb_a + w * C::kVecs * comb_vec;
+        const float4* src = mine + w * C::kVecs * comb_vec;
 #pragma unroll
         for (int hf = 0; hf < C::kHalves; ++hf)
 #pragma unroll
           for (int j = 0; j < 2 * kWords; ++j) {
-            const float4 y = lds128f(src + (hf * 2 * kWords + j) * comb_vec);
+            const float4 y = src[(hf * 2 * kWords + j) * comb_vec];
             float(&x)[4] = o[hf][j];
             x[0] += w0 * y.x, x[1] += w1 * y.y, x[2] += w0 * y.z, x[3] += w1 * y.w;
           }

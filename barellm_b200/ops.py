@@ -10,6 +10,7 @@ or without the built library, every call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import numpy as np
@@ -679,33 +680,37 @@ def rms_norm(
 FP8_DTYPE = torch.float8_e4m3fn
 
 
-def _call(fn, args, device: torch.device) -> None:
-    """Launches on ``device``'s current stream, whichever device is current."""
-    if _dev_index(device) == torch.cuda.current_device():
-        _raise_rc(fn(args, _stream(device)))
-        return
-    with torch.cuda.device(device):
-        _raise_rc(fn(args, _stream(device)))
+_raw_device = getattr(torch._C, "_cuda_getDevice", None)
+_F32, _I32 = torch.float32, torch.int32
 
 
-def _vector_i32(t: torch.Tensor, device: torch.device, n: int, name: str) -> torch.Tensor:
-    _int32_on(t, device, name)
-    _check(t.ndim == 1 and t.shape[0] == n and (n == 1 or t.stride(0) == 1), f"{name} must be a contiguous [{n}] tensor")
-    return t
+def _call(fn, args: bytes, dev: int) -> None:
+    """Launches on device ``dev``'s current stream, whichever device is current."""
+    if (_raw_device() if _raw_device is not None else torch.cuda.current_device()) == dev:
+        rc = fn(args, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _raise_rc(rc)
 
 
-def _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, dtype, batch) -> nat.Fp8Layer:
-    """Checks an 8-bit pool, its scales and its block tables, and describes them."""
+def _vector_i32(t: torch.Tensor, dev: int, n: int, name: str) -> None:
+    if not (t.dtype is _I32 and t.get_device() == dev and t.shape == (n,) and (n == 1 or t.stride(0) == 1)):
+        raise ValueError(f"{name} must be a contiguous int32 [{n}] tensor on cuda:{dev}")
+
+
+def _fp8_layer_checks(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, dtype, batch) -> None:
+    """The 8-bit pool / table checks one at a time, raising the first that fails."""
     _require_cuda(key_cache, "key_cache")
-    ks = key_cache.shape
-    dev = key_cache.device
+    ks, dev = key_cache.shape, key_cache.device
     _check(key_cache.ndim == 5, "K/V pool must have shape [L, P, H, S, D]")
     _check(value_cache.shape == ks, "K/V pools must have identical shape")
     _check(key_cache.dtype is FP8_DTYPE and value_cache.dtype is FP8_DTYPE, "8-bit K/V pools must be float8_e4m3fn")
     _check(value_cache.device == dev, "K/V device must match")
     _check(key_cache.is_contiguous() and value_cache.is_contiguous(), "K/V pools must be contiguous")
     for t, name in ((key_scale, "key_scale"), (value_scale, "value_scale")):
-        _check(t.shape == ks[:3] and t.dtype is torch.float32 and t.device == dev and t.is_contiguous(),
+        _check(t.shape == ks[:3] and t.dtype is _F32 and t.device == dev and t.is_contiguous(),
                f"{name} must be a contiguous float32 [L, P, H] tensor on the pool's device")
     _check(dtype in DTYPE_CODE, f"unsupported dtype {dtype}")
     if not 0 <= layer < ks[0]:
@@ -713,37 +718,61 @@ def _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tabl
     _int32_on(block_tables, dev, "block_tables")
     _check(block_tables.ndim == 2 and block_tables.shape[1] > 0 and (block_tables.shape[1] == 1 or block_tables.stride(1) == 1),
            "block_tables must be [rows, width] with unit inner stride")
+    _check(row_ids is not None or block_tables.shape[0] >= batch, "block_tables must have a row for every request")
+    raise ValueError("block_tables must be [rows, width] with rows at least a row apart")
+
+
+def _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, dtype, batch):
+    """(pool shape, device index, bl_fp8_layer fields) of a checked 8-bit layer.
+
+    Every check in one expression (the common, valid case); on a failure the
+    step-by-step checks raise the specific error."""
+    shape = key_cache.shape
+    dev = key_cache.get_device()
+    ts = block_tables.shape
+    code = DTYPE_CODE.get(dtype)
+    if not (dev >= 0 and len(shape) == 5 and key_cache.dtype is FP8_DTYPE and value_cache.dtype is FP8_DTYPE
+            and value_cache.shape == shape and value_cache.get_device() == dev and key_cache.is_contiguous()
+            and value_cache.is_contiguous() and key_scale.shape == shape[:3] and value_scale.shape == shape[:3]
+            and key_scale.dtype is _F32 and value_scale.dtype is _F32 and key_scale.get_device() == dev
+            and value_scale.get_device() == dev and key_scale.is_contiguous() and value_scale.is_contiguous()
+            and code is not None and 0 <= layer < shape[0] and block_tables.dtype is _I32
+            and block_tables.get_device() == dev and len(ts) == 2 and ts[1] > 0 and (row_ids is not None or ts[0] >= batch)):
+        _fp8_layer_checks(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, dtype, batch)
+    outer, inner = block_tables.stride()
+    if ts[0] == 1 and outer < ts[1]:
+        outer = ts[1]  # a one-row table may carry any outer stride
+    if outer < ts[1] or (inner != 1 and ts[1] > 1):
+        _fp8_layer_checks(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, dtype, batch)
+    rows = 0
     if row_ids is not None:
         _vector_i32(row_ids, dev, batch, "row_ids")
-    else:
-        _check(block_tables.shape[0] >= batch, "block_tables must have a row for every request")
-    # a one-row table may carry any outer stride; the kernels want at least the width
-    pl = nat.PagedLayer(key_cache.data_ptr(), value_cache.data_ptr(), ks[0], ks[1], ks[2], ks[3], ks[4], DTYPE_CODE[dtype],
-                        layer, block_tables.data_ptr(),
-                        block_tables.stride(0) if block_tables.shape[0] > 1 else block_tables.shape[1],
-                        block_tables.shape[1], _ptr(row_ids))
-    return nat.Fp8Layer(pl, key_scale.data_ptr(), value_scale.data_ptr())
+        rows = row_ids.data_ptr()
+    return shape, dev, (key_cache.data_ptr(), value_cache.data_ptr(), *shape, code, layer, block_tables.data_ptr(), outer,
+                        ts[1], rows, key_scale.data_ptr(), value_scale.data_ptr())
 
 
 def _softmax_scale(scale: float | None, d: int) -> float:
-    s = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if scale is None:
+        return 1.0 / math.sqrt(d)
+    s = float(scale)
     _check(0.0 < s < math.inf, "scale must be positive and finite")
     return s
 
 
-def _err_word(err: torch.Tensor | None, device: torch.device) -> int | None:
+def _err_word(err: torch.Tensor | None, dev: int) -> int:
     if err is None:
-        return None
-    _check(err.dtype is torch.int32 and err.device == device and err.numel() >= 1, f"err must be an int32 tensor on {device}")
+        return 0
+    _check(err.dtype is _I32 and err.get_device() == dev and err.numel() >= 1, f"err must be an int32 tensor on cuda:{dev}")
     return err.data_ptr()
 
 
-def _scratch(ws: torch.Tensor | None, nbytes: int, device: torch.device) -> torch.Tensor:
+def _scratch(ws: torch.Tensor | None, nbytes: int, like: torch.Tensor) -> torch.Tensor:
     """The caller's workspace, or a fresh one from torch's allocator (so calls
     on several streams, and several captured graphs, never share scratch)."""
     if ws is None:
-        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
-    _check(ws.device == device and ws.is_contiguous(), f"ws must be a contiguous tensor on {device}")
+        return torch.empty(nbytes or 256, dtype=torch.uint8, device=like.device)
+    _check(ws.device == like.device and ws.is_contiguous(), f"ws must be a contiguous tensor on {like.device}")
     return ws
 
 
@@ -775,28 +804,35 @@ def paged_append_fp8(
     call only.
     """
     batch = start_pos.shape[0]
-    fl = _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, key.dtype, batch)
-    dev = key_cache.device
-    _check(key.ndim == 4 and value.ndim == 4, "K/V must have shape [B, H, T, D]")
-    _check(key.shape == value.shape, "K/V must have identical shape")
-    _check(key.shape[1] == key_cache.shape[2], "KV-head count cannot change")
-    _check(key.shape[2] > 0, "K/V sequence length must be greater than zero")
-    _check(key.shape[3] == key_cache.shape[4], "Head dimension cannot change")
-    _check(key.dtype == value.dtype, "K/V dtype must match")
-    _check(key.device == dev and value.device == dev, "K/V device cannot change")
-    _check((key.stride(3) == 1 and value.stride(3) == 1) or key.shape[3] == 1, "K/V head_dim must be contiguous")
-    _vector_i32(start_pos, dev, batch, "start_pos")
+    shape, dev, fields = _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, key.dtype,
+                                    batch)
+    xs = key.shape
     packed = new_offsets is not None
+    if not (len(xs) == 4 and value.shape == xs and xs[1] == shape[2] and xs[2] > 0 and xs[3] == shape[4]
+            and value.dtype is key.dtype and key.get_device() == dev and value.get_device() == dev
+            and xs[0] == (1 if packed else batch)):
+        _check(key.ndim == 4 and value.ndim == 4, "K/V must have shape [B, H, T, D]")
+        _check(key.shape == value.shape, "K/V must have identical shape")
+        _check(key.shape[1] == key_cache.shape[2], "KV-head count cannot change")
+        _check(key.shape[2] > 0, "K/V sequence length must be greater than zero")
+        _check(key.shape[3] == key_cache.shape[4], "Head dimension cannot change")
+        _check(key.dtype == value.dtype, "K/V dtype must match")
+        _check(key.device == key_cache.device and value.device == key_cache.device, "K/V device cannot change")
+        _check(not packed, "packed K/V need [1, H, T, D] and [B+1] offsets")
+        raise ValueError("batch size must match number of caches")
+    ks, vs = key.stride(), value.stride()
+    _check((ks[3] == 1 and vs[3] == 1) or xs[3] == 1, "K/V head_dim must be contiguous")
+    _vector_i32(start_pos, dev, batch, "start_pos")
     if packed:
         _vector_i32(new_offsets, dev, batch + 1, "new_offsets")
-        _check(key.shape[0] == 1, "packed K/V need [1, H, T, D] and [B+1] offsets")
         _check(max_new_tokens is not None and max_new_tokens > 0, "packed append needs max_new_tokens")
+        # packed rows are addressed by new_offsets alone
+        a = nat.pack_append_fp8_args(*fields, key.data_ptr(), value.data_ptr(), 0, ks[1], ks[2], 0, vs[1], vs[2],
+                                     start_pos.data_ptr(), new_offsets.data_ptr(), batch, int(max_new_tokens),
+                                     _err_word(err, dev))
     else:
-        _check(key.shape[0] == batch, "batch size must match number of caches")
-    ks, vs = key.stride(), value.stride()
-    a = nat.AppendFp8Args(fl, key.data_ptr(), value.data_ptr(), 0 if packed else ks[0], ks[1], ks[2],
-                          0 if packed else vs[0], vs[1], vs[2], start_pos.data_ptr(), _ptr(new_offsets), batch,
-                          int(max_new_tokens) if packed else key.shape[2], _err_word(err, dev))
+        a = nat.pack_append_fp8_args(*fields, key.data_ptr(), value.data_ptr(), *ks[:3], *vs[:3], start_pos.data_ptr(), 0,
+                                     batch, xs[2], _err_word(err, dev))
     _call(nat.load().bl_paged_append_fp8, a, dev)
 
 
@@ -821,26 +857,28 @@ def paged_gather_fp8(
     :func:`paged_gather`.  Values saturate at the type's largest finite value.
     """
     batch = seq_lens.shape[0]
-    fl = _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, dtype, batch)
-    dev = key_cache.device
+    pool, dev, fields = _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, dtype, batch)
     _vector_i32(seq_lens, dev, batch, "seq_lens")
     _check(max_len > 0, "KV cache is empty")
-    shape = (batch, key_cache.shape[2], max_len, key_cache.shape[4])
+    shape = (batch, pool[2], max_len, pool[4])
     if out is None:
-        k_out = torch.empty(shape, dtype=dtype, device=dev)
-        v_out = torch.empty_like(k_out)
+        k_out = torch.empty(shape, dtype=dtype, device=key_cache.device)
+        v_out = torch.empty(shape, dtype=dtype, device=key_cache.device)
+        st = k_out.stride()
     else:
         k_out, v_out = out
         for t in out:
-            _check(t.shape == shape and t.dtype is dtype and t.device == dev, "gather output must be [B, H, max_len, D] of dtype")
-        _check(k_out.stride() == v_out.stride() and (k_out.stride(3) == 1 or shape[3] == 1),
-               "gather outputs need identical strides, D contiguous")
-    a = nat.GatherFp8Args(fl, seq_lens.data_ptr(), batch, k_out.data_ptr(), v_out.data_ptr(), k_out.stride(0),
-                          k_out.stride(1), k_out.stride(2), max_len, 1 if zero_fill else 0, _err_word(err, dev))
+            _check(t.shape == shape and t.dtype is dtype and t.get_device() == dev,
+                   "gather output must be [B, H, max_len, D] of dtype")
+        st = k_out.stride()
+        _check(st == v_out.stride() and (st[3] == 1 or shape[3] == 1), "gather outputs need identical strides, D contiguous")
+    a = nat.pack_gather_fp8_args(*fields, seq_lens.data_ptr(), batch, k_out.data_ptr(), v_out.data_ptr(), st[0], st[1], st[2],
+                                 max_len, 1 if zero_fill else 0, _err_word(err, dev))
     _call(nat.load().bl_paged_gather_fp8, a, dev)
     return k_out, v_out
 
 
+@functools.lru_cache(maxsize=256)
 def decode_fp8_workspace_bytes(batch: int, num_q_heads: int, head_dim: int, max_seq_len: int) -> int:
     return int(nat.load().bl_paged_decode_fp8_workspace_bytes(batch, num_q_heads, head_dim, max_seq_len))
 
@@ -874,35 +912,43 @@ def paged_decode_fp8(
     layers have it.
     """
     _require_cuda(q, "q")
-    if q.ndim == 4:
-        _check(q.shape[2] == 1, "decode takes one query token per request")
-        q3 = q[:, :, 0, :]
-    else:
-        q3 = q
-    _check(q3.ndim == 3, "q must be [B, Hq, D] or [B, Hq, 1, D]")
-    batch, hq, d = q3.shape
-    fl = _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, q3.dtype, batch)
-    dev = key_cache.device
-    _check(q3.device == dev, "q must be on the K/V pool's device")
-    _check(d == key_cache.shape[4], "Head dimension cannot change")
-    _check(q3.stride(2) == 1 or d == 1, "q head_dim must be contiguous")
-    _check(hq > 0 and hq % key_cache.shape[2] == 0, "num_heads must divide evenly by num_kv_heads")
+    qs, qst = q.shape, q.stride()
+    if len(qs) == 4:
+        _check(qs[2] == 1, "decode takes one query token per request")
+        qs, qst = (qs[0], qs[1], qs[3]), (qst[0], qst[1], qst[3])
+    _check(len(qs) == 3, "q must be [B, Hq, D] or [B, Hq, 1, D]")
+    batch, hq, d = qs
+    dtype = q.dtype
+    pool, dev, fields = _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, dtype, batch)
+    _check(q.get_device() == dev, "q must be on the K/V pool's device")
+    _check(d == pool[4], "Head dimension cannot change")
+    _check(qst[2] == 1 or d == 1, "q head_dim must be contiguous")
+    _check(hq > 0 and hq % pool[2] == 0, "num_heads must divide evenly by num_kv_heads")
     _vector_i32(seq_lens, dev, batch, "seq_lens")
     _check(max_seq_len > 0, "KV cache is empty")
     if out is None:
-        out = torch.empty((batch, hq, d), dtype=q3.dtype, device=dev)
-        out3 = out
+        out = torch.empty(qs, dtype=dtype, device=q.device)
+        ost = (hq * d, d)
     else:
-        out3 = out[:, :, 0, :] if out.ndim == 4 else out
-        _check(out3.shape == q3.shape and (out3.stride(2) == 1 or d == 1) and out3.dtype is q3.dtype and out3.device == dev,
+        os_, ost = out.shape, out.stride()
+        if len(os_) == 4 and os_[2] == 1:
+            os_, ost = (os_[0], os_[1], os_[3]), (ost[0], ost[1], ost[3])
+        _check(tuple(os_) == tuple(qs) and (ost[2] == 1 or d == 1) and out.dtype is dtype and out.get_device() == dev,
                "decode output must be [B, Hq, D] like q, D contiguous")
     _check(ws is not None or not plan_ready, "plan_ready needs the workspace that holds the plan")
-    ws = _scratch(ws, decode_fp8_workspace_bytes(batch, hq, d, max_seq_len), dev)
-    a = nat.DecodeFp8Args(fl, q3.data_ptr(), q3.stride(0), q3.stride(1), out3.data_ptr(), out3.stride(0), out3.stride(1),
-                          seq_lens.data_ptr(), batch, hq, _softmax_scale(scale, d), 1 if plan_ready else 0, ws.data_ptr(),
-                          ws.numel() * ws.element_size(), max_seq_len, _err_word(err, dev))
+    ws = _scratch(ws, decode_fp8_workspace_bytes(batch, hq, d, max_seq_len), q)
+    a = nat.pack_decode_fp8_args(*fields, q.data_ptr(), qst[0], qst[1], out.data_ptr(), ost[0], ost[1], seq_lens.data_ptr(),
+                                 batch, hq, _softmax_scale(scale, d), 1 if plan_ready else 0, ws.data_ptr(), ws.nbytes,
+                                 max_seq_len, _err_word(err, dev))
     _call(nat.load().bl_paged_decode_fp8, a, dev)
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def prefill_fp8_workspace_bytes(dtype: torch.dtype, batch: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                                block_size: int, max_seq_len: int, total_blocks: int) -> int:
+    return int(nat.load().bl_paged_prefill_fp8_workspace_bytes(DTYPE_CODE[dtype], batch, num_q_heads, num_kv_heads, head_dim,
+                                                               block_size, max_seq_len, total_blocks))
 
 
 def paged_prefill_fp8(
@@ -936,16 +982,17 @@ def paged_prefill_fp8(
     the rows' pages.
     """
     _require_cuda(q, "q")
-    _check(q.ndim == 4, "q must be [B, Hq, T, D]")
-    b0, hq, t, d = q.shape
+    qs, qst = q.shape, q.stride()
+    _check(len(qs) == 4, "q must be [B, Hq, T, D]")
+    b0, hq, t, d = qs
     batch = seq_lens.shape[0]
-    fl = _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, q.dtype, batch)
-    dev = key_cache.device
-    hkv, bs = key_cache.shape[2], key_cache.shape[3]
-    _check(q.device == dev, "q must be on the K/V pool's device")
-    _check(d == key_cache.shape[4], "Head dimension cannot change")
+    dtype = q.dtype
+    pool, dev, fields = _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tables, row_ids, dtype, batch)
+    hkv, bs = pool[2], pool[3]
+    _check(q.get_device() == dev, "q must be on the K/V pool's device")
+    _check(d == pool[4], "Head dimension cannot change")
     _check(t > 0, "K/V sequence length must be greater than zero")
-    _check(q.stride(3) == 1 or d == 1, "q head_dim must be contiguous")
+    _check(qst[3] == 1 or d == 1, "q head_dim must be contiguous")
     _check(hq > 0 and hq % hkv == 0, "num_heads must divide evenly by num_kv_heads")
     _vector_i32(seq_lens, dev, batch, "seq_lens")
     _check(max_seq_len > 0, "KV cache is empty")
@@ -962,27 +1009,27 @@ def paged_prefill_fp8(
         total_blocks = batch * -(-max_seq_len // bs)
     _check(total_blocks > 0, "total_blocks must be positive")
     if out is None:
-        out = torch.empty((b0, t, hq, d), dtype=q.dtype, device=dev).transpose(1, 2)
-    _check(out.shape == q.shape and (out.stride(3) == 1 or d == 1) and out.dtype is q.dtype and out.device == dev,
+        out = torch.empty((b0, t, hq, d), dtype=dtype, device=q.device).transpose(1, 2)
+    ost = out.stride()
+    _check(out.shape == qs and (ost[3] == 1 or d == 1) and out.dtype is dtype and out.get_device() == dev,
            "prefill output must match q's shape, D contiguous")
-    lib = nat.load()
-    nbytes = int(lib.bl_paged_prefill_fp8_workspace_bytes(DTYPE_CODE[q.dtype], batch, hq, hkv, d, bs, max_seq_len, total_blocks))
-    ws = _scratch(ws, nbytes, dev)
-    qs, os_ = q.stride(), out.stride()
-    a = nat.PrefillFp8Args(fl, q.data_ptr(), 0 if packed else qs[0], qs[2], qs[1], out.data_ptr(), 0 if packed else os_[0],
-                           os_[2], os_[1], _ptr(q_offsets), seq_lens.data_ptr(), batch, hq, mq, _softmax_scale(scale, d), 0,
-                           max_seq_len, total_blocks, ws.data_ptr(), ws.numel() * ws.element_size(), _err_word(err, dev))
-    _call(lib.bl_paged_prefill_fp8, a, dev)
+    ws = _scratch(ws, prefill_fp8_workspace_bytes(dtype, batch, hq, hkv, d, bs, max_seq_len, total_blocks), q)
+    a = nat.pack_prefill_fp8_args(*fields, q.data_ptr(), 0 if packed else qst[0], qst[2], qst[1], out.data_ptr(),
+                                  0 if packed else ost[0], ost[2], ost[1], q_offsets.data_ptr() if packed else 0,
+                                  seq_lens.data_ptr(), batch, hq, mq, _softmax_scale(scale, d), 0, max_seq_len, total_blocks,
+                                  ws.data_ptr(), ws.nbytes, _err_word(err, dev))
+    _call(nat.load().bl_paged_prefill_fp8, a, dev)
     return out
 
 
-def _block_ids(ids, name: str, num_blocks: int) -> np.ndarray:
+def _block_ids(ids, name: str) -> np.ndarray:
+    """Host block ids as int64 (the library checks their range)."""
     a = np.asarray(ids)
-    if a.size == 0:
-        return np.zeros(0, dtype=np.int32)
-    _check(a.ndim == 1 and a.dtype.kind in "iu", f"{name} must be a sequence of block ids")
-    _check(int(a.min()) >= 0 and int(a.max()) < num_blocks, f"{name} holds a block id outside the pool")
-    return np.ascontiguousarray(a, dtype=np.int32)
+    if a.dtype != np.int64:
+        _check(a.dtype.kind in "iu" or a.size == 0, f"{name} must be a sequence of block ids")
+        a = a.astype(np.int64)
+    _check(a.ndim == 1, f"{name} must be a sequence of block ids")
+    return np.ascontiguousarray(a)
 
 
 def copy_blocks(
@@ -1001,26 +1048,29 @@ def copy_blocks(
     them out).  A block that would be written twice, or both read and written,
     raises ``ValueError`` before anything is copied."""
     _require_cuda(key_cache, "key_cache")
-    _check(key_cache.ndim == 5, "K/V pool must have shape [L, P, H, S, D]")
-    _check(key_cache.shape == value_cache.shape, "K/V pools must have identical shape")
-    _check(key_cache.dtype == value_cache.dtype, "K/V dtype must match")
-    _check(key_cache.device == value_cache.device, "K/V device must match")
+    shape, dev, dtype = key_cache.shape, key_cache.get_device(), key_cache.dtype
+    _check(len(shape) == 5, "K/V pool must have shape [L, P, H, S, D]")
+    _check(shape == value_cache.shape, "K/V pools must have identical shape")
+    _check(dtype is value_cache.dtype, "K/V dtype must match")
+    _check(dev == value_cache.get_device(), "K/V device must match")
     _check(key_cache.is_contiguous() and value_cache.is_contiguous(), "K/V pools must be contiguous")
-    _check(key_cache.dtype in DTYPE_CODE or key_cache.dtype is FP8_DTYPE, f"unsupported dtype {key_cache.dtype}")
-    _check((key_cache.dtype is FP8_DTYPE) == (key_scale is not None) == (value_scale is not None),
-           "8-bit pools, and only they, are copied with their scales")
-    l, p, h, s, d = key_cache.shape
-    for t, name in ((key_scale, "key_scale"), (value_scale, "value_scale")):
-        _check(t is None or (t.shape == (l, p, h) and t.dtype is torch.float32 and t.device == key_cache.device
-                             and t.is_contiguous()),
-               f"{name} must be a contiguous float32 [L, P, H] tensor on the pool's device")
-    sa, da = _block_ids(src, "src", p), _block_ids(dst, "dst", p)
-    _check(sa.size == da.size, "src and dst must have the same length")
-    if sa.size == 0:
+    fp8 = dtype is FP8_DTYPE
+    _check(fp8 or dtype in DTYPE_CODE, f"unsupported dtype {dtype}")
+    _check(fp8 == (key_scale is not None) == (value_scale is not None), "8-bit pools, and only they, are copied with their scales")
+    kp = vp = 0
+    if fp8:
+        for t, name in ((key_scale, "key_scale"), (value_scale, "value_scale")):
+            _check(t.shape == shape[:3] and t.dtype is _F32 and t.get_device() == dev and t.is_contiguous(),
+                   f"{name} must be a contiguous float32 [L, P, H] tensor on the pool's device")
+        kp, vp = key_scale.data_ptr(), value_scale.data_ptr()
+    sa, da = _block_ids(src, "src"), _block_ids(dst, "dst")
+    n = len(sa)
+    _check(n == len(da), "src and dst must have the same length")
+    if n == 0:
         return
-    a = nat.CopyBlocksArgs(key_cache.data_ptr(), value_cache.data_ptr(), _ptr(key_scale), _ptr(value_scale), l, p, h, s, d,
-                           key_cache.element_size(), sa.ctypes.data, da.ctypes.data, sa.size)
-    _call(nat.load().bl_copy_blocks, a, key_cache.device)
+    a = nat.pack_copy_blocks_args(key_cache.data_ptr(), value_cache.data_ptr(), kp, vp, *shape, key_cache.element_size(),
+                                  sa.ctypes.data, da.ctypes.data, n)
+    _call(nat.load().bl_copy_blocks, a, dev)
 
 
 def decode_path(dtype: torch.dtype, head_dim: int, block_size: int, num_q_heads: int, num_kv_heads: int) -> int:

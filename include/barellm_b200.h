@@ -522,8 +522,8 @@ typedef struct bl_copy_blocks_args {
   int64_t block_size;
   int64_t head_dim;
   int64_t elem_bytes;
-  const int32_t* src;
-  const int32_t* dst;
+  const int64_t* src; /* [count], host */
+  const int64_t* dst; /* [count], host */
   int64_t count;
 } bl_copy_blocks_args;
 

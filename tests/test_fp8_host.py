@@ -112,10 +112,36 @@ def test_bad_arguments_are_refused(native_lib, name, change, rc):
     (list(range(8)) + [0], [0] * 9, "more pairs"),
 ])
 def test_bad_copy_pairs_are_refused(native_lib, src, dst, text):
-    s, d = np.asarray(src, dtype=np.int32), np.asarray(dst, dtype=np.int32)
+    s, d = np.asarray(src, dtype=np.int64), np.asarray(dst, dtype=np.int64)
     a = nat.CopyBlocksArgs(4096, 4096, None, None, 2, 8, 2, 16, 128, 2, s.ctypes.data, d.ctypes.data, len(src))
     assert native_lib.bl_copy_blocks(ctypes.byref(a), None) == nat.BL_ERR_ARG
     assert text in nat.last_error()
+
+
+def test_packed_arguments_are_the_structures(native_lib):
+    """The byte strings that ops passes are the ctypes structures, field for field."""
+    rs = np.random.RandomState(0)
+    for name, cls in nat.STRUCTS.items():
+        if not hasattr(nat, "pack_" + name[3:]):
+            continue
+        pack = getattr(nat, "pack_" + name[3:])
+
+        def fields(c):
+            for f, t in c._fields_:
+                if issubclass(t, ctypes.Structure):
+                    yield from ((f + "." + g, u) for g, u in fields(t))
+                else:
+                    yield f, t
+
+        vals = [float(rs.randint(1, 100)) if t is ctypes.c_float else int(rs.randint(1, 1 << 30)) for _, t in fields(cls)]
+        data = pack(*vals)
+        assert len(data) == ctypes.sizeof(cls), name
+        got = cls.from_buffer_copy(data)
+        for (path, _), v in zip(fields(cls), vals):
+            x = got
+            for part in path.split("."):
+                x = getattr(x, part)
+            assert x == v, (name, path)
 
 
 def test_copy_of_nothing_is_nothing(native_lib):
