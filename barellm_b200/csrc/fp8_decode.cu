@@ -58,7 +58,7 @@ WsLayout ws_layout(int64_t batch, int64_t hq, int64_t d, int64_t max_seq_len) {
   WsLayout w;
   w.max_units = batch * ((max_seq_len + kChunk - 1) / kChunk);
   size_t off = 0;
-  w.hdr = off;      off += align256(4 * sizeof(int32_t));
+  w.hdr = off;      off += align256(8 * sizeof(int32_t));
   w.row_base = off; off += align256((batch + 1) * sizeof(int32_t));
   w.units = off;    off += align256(w.max_units * sizeof(Unit));
   // a row of one chunk leaves no partial
@@ -79,7 +79,7 @@ struct PlanArgs {
   const int32_t* row_ids;
   int32_t batch, max_units;
   int64_t cap;        // tokens a table row covers
-  int32_t* hdr;       // [0] units, [1] magic, [2] batch, [3] max_units
+  int32_t* hdr;       // [0] units, [1] magic, [2] batch, [3] max_units, [4..5] items claimed, [6] CTAs done
   int32_t* row_base;  // [batch + 1]
   Unit* units;        // [max_units]
   int32_t* err;
@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(kPlanThreads) fp8_decode_plan_kernel(const Pla
     a.hdr[1] = kPlanMagic;
     a.hdr[2] = a.batch;
     a.hdr[3] = a.max_units;
+    a.hdr[4] = a.hdr[5] = a.hdr[6] = 0;
   }
   __syncthreads();
   // (the order among chunks of one size is left to the atomics: it changes no result)
@@ -185,7 +186,7 @@ struct Args {
   int32_t batch, hq, hkv, g, head_tiles, bs, d;
   int32_t q_vec, o_vec;  // q / out rows can be read / written four 16-bit elements at a time
   float scale_log2;
-  const int32_t* hdr;
+  int32_t* hdr;
   const int32_t* row_base;
   const Unit* units;
   float* ws_lse;
@@ -338,9 +339,9 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, in
   }
 }
 
-// An item on its way to the ring: lane i holds tile i of the chunk.  begin()
-// issues the loads that the plan's record leads to, finish() those behind the
-// block id; a whole item lies between them, so neither is waited for.
+// An item on its way to the consumers: lane i holds tile i of the chunk.  begin()
+// makes the loads that the plan's record leads to, finish() those behind the
+// block id.
 template <typename T, int D>
 struct Pending {
   Item it;
@@ -458,31 +459,40 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
 
   if (warp == kNW) {
     // ------------------------------ planner ------------------------------
-    // Describes item by item to the consumers, one item ahead of them; the loads
-    // behind the item after that one are in flight meanwhile.
-    int n_item = 0;
+    // Describes item by item to the consumers, one item ahead of them.  After its
+    // first item a CTA claims the next one that nobody has: the plan lists the
+    // chunks by decreasing size, so the CTAs finish together.  (A claim is made
+    // when the consumers begin the item before it, late enough to be fair and a
+    // whole item's time ahead of its use.)
+    unsigned long long* claimed = reinterpret_cast<unsigned long long*>(a.hdr + 4);
+    Pending<T, D> p;
     int64_t item = blockIdx.x;
-    Pending<T, D> cur, nxt;
-    Unit unit = {};
-    if (item < items) {
-      cur.begin(a, item, load_unit(a, item), lane);
-      if (item + gridDim.x < items) unit = load_unit(a, item + gridDim.x);
-      cur.finish(a);
-    }
-    for (; item < items; ++n_item) {
-      if (!cur.valid && lane == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
-      item += gridDim.x;
-      if (item < items) {
-        nxt.begin(a, item, unit, lane);
-        if (item + gridDim.x < items) unit = load_unit(a, item + gridDim.x);
-      }
+    for (int n_item = 0;; ++n_item) {
       const int k = n_item & 1;
       if (!__all_sync(0xffffffffu, wait_or_abort(&sh->item_empty[k], ((n_item >> 1) & 1) ^ 1, &sh->abort, a.err))) break;
-      cur.stage(a, lane, sh->items[k], qs + k * C::kKS * room);
+      if (n_item > 0) {
+        unsigned long long c = 0;
+        if (lane == 0) c = atomicAdd(claimed, 1ull);
+        item = (int64_t)__shfl_sync(0xffffffffu, c, 0) + gridDim.x;
+      }
+      const bool end = item >= items;
+      if (end) {
+        if (lane == 0) sh->items[k].it.heads = -1;
+      } else {
+        p.begin(a, item, load_unit(a, item), lane);
+        p.finish(a);
+        if (!p.valid && lane == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
+        p.stage(a, lane, sh->items[k], qs + k * C::kKS * room);
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->item_full[k]);
-      if (item < items) nxt.finish(a);
-      cur = nxt;
+      if (end) break;
+    }
+    // The last CTA to make its last claim leaves the counters as the plan did, for
+    // the next layer's call with the same plan.
+    if (lane == 0 && atomicAdd(a.hdr + 6, 1) == (int)gridDim.x - 1) {
+      a.hdr[6] = 0;
+      *claimed = 0;
     }
     return;
   }
@@ -504,7 +514,6 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
   float4* const mine = reinterpret_cast<float4*>(comb) + g_row * pairs + t4;
   const int comb_vec = 8 * pairs;  // float4s between a lane's own
   const uint64_t policy = policy_evict_first();
-  const int my_items = items > blockIdx.x ? (int)((items - blockIdx.x + gridDim.x - 1) / gridDim.x) : 0;
 
   // A warp issues its own copies into a ring of its own: kDepth steps of 32
   // tokens.  One producer warp for the CTA had to pass every step through two
@@ -515,6 +524,7 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
   int issued = 0, taken = 0;       // steps
   int at_item = -1, at_step = 0, at_steps = 0;
   int at_tiles = 0;
+  bool at_end = false;
   // Issues the next step if there is one; `may_wait` false: only if its item is
   // described already.  n_item: the item being consumed; the cursor goes at most
   // one item further, since the planner describes that one only after this warp
@@ -522,15 +532,19 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
   auto issue = [&](int n_item, bool may_wait) -> bool {
     while (at_step >= at_steps) {
       const int next = at_item + 1;
-      if (next >= my_items || next > n_item + 1) return false;
+      if (at_end || next > n_item + 1) return false;
       const int k = next & 1;
       if (!may_wait) {
         if (!__all_sync(0xffffffffu, mbar_try_wait(&sh->item_full[k], (next >> 1) & 1))) return false;
       } else if (!__all_sync(0xffffffffu, wait_or_abort(&sh->item_full[k], (next >> 1) & 1, &sh->abort, a.err))) {
         return false;
       }
-      at_item = next;
       const Item& it = sh->items[k].it;
+      if (it.heads < 0) {
+        at_end = true;
+        return false;
+      }
+      at_item = next;
       at_tiles = (it.t1 - it.t0 + 15) / 16;
       at_steps = (at_tiles + 1) / 2;
       at_step = (warp + next) & (kNW - 1);
@@ -563,12 +577,13 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
   };
   bool ok = true;
 
-  for (int n_item = 0; n_item < my_items && ok; ++n_item) {
+  for (int n_item = 0; ok; ++n_item) {
     // all waits are per warp and bounded; a CTA that gave up leaves them at once
     const int slot_i = n_item & 1;
     ok = __all_sync(0xffffffffu, wait_or_abort(&sh->item_full[slot_i], (n_item >> 1) & 1, &sh->abort, a.err));
     if (!ok) break;
     const Item it = sh->items[slot_i].it;
+    if (it.heads < 0) break;  // no more items
     const float2 fs = sh->items[slot_i].f[t4];
     uint2 qf[kKS];
 #pragma unroll
@@ -1267,7 +1282,7 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
   k.q_vec = ((uintptr_t)a.q & 7) == 0 && a.q_stride_b % 4 == 0 && a.q_stride_h % 4 == 0;
   k.o_vec = ((uintptr_t)a.out & 7) == 0 && a.out_stride_b % 4 == 0 && a.out_stride_h % 4 == 0;
   k.scale_log2 = a.scale * kLog2e;
-  k.hdr = (const int32_t*)(ws + w.hdr);
+  k.hdr = (int32_t*)(ws + w.hdr);
   k.row_base = (const int32_t*)(ws + w.row_base);
   k.units = (const Unit*)(ws + w.units);
   k.ws_lse = (float*)(ws + w.lse);
