@@ -72,7 +72,7 @@ WsLayout ws_layout(int64_t batch, int64_t hq, int64_t d, int64_t max_seq_len) {
 // ---------------------------------------------------------------------------
 // plan
 // ---------------------------------------------------------------------------
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024;  // at most; a batch of fewer rows takes fewer
 
 struct PlanArgs {
   const int32_t* seq_lens;
@@ -85,7 +85,7 @@ struct PlanArgs {
   int32_t* err;
 };
 
-// Exclusive sums of v over the CTA's 32 warps; total over all.  s: 32 ints.
+// Exclusive sums of v over the CTA; total over all.  s: an int per warp.
 __device__ __forceinline__ int cta_exclusive(int v, int* s, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int x = v;
@@ -98,8 +98,7 @@ __device__ __forceinline__ int cta_exclusive(int v, int* s, int& total) {
   __syncthreads();
   int before = 0;
   total = 0;
-#pragma unroll
-  for (int w = 0; w < kPlanThreads / 32; ++w) {
+  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
     const int t = s[w];
     if (w < warp) before += t;
     total += t;
@@ -126,7 +125,7 @@ __global__ void __launch_bounds__(kPlanThreads) fp8_decode_plan_kernel(const Pla
     return (int)min(max(len, (int64_t)0), a.cap);
   };
   int all = 0, full = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kPlanThreads) {
+  for (int b0 = 0; b0 < a.batch; b0 += blockDim.x) {
     const int b = b0 + tid;
     const int len = b < a.batch ? length(b) : 0;
     if (b < a.batch && a.seq_lens[b] > a.cap) raise_dev(a.err, BL_DEVERR_TABLE);
@@ -160,7 +159,7 @@ __global__ void __launch_bounds__(kPlanThreads) fp8_decode_plan_kernel(const Pla
   }
   __syncthreads();
   // (the order among chunks of one size is left to the atomics: it changes no result)
-  for (int b = tid; b < a.batch; b += kPlanThreads) {
+  for (int b = tid; b < a.batch; b += blockDim.x) {
     const int len = length(b), nfull = len / kChunk, rest = len - nfull * kChunk;
     if (rest > 0)
       put(atomicAdd(&s_next[(rest + 15) / 16 - 1], 1), b, nfull, len, a.row_base[b], a.row_ids ? a.row_ids[b] : b);
@@ -192,6 +191,7 @@ struct Args {
   float* ws_lse;
   float* ws_o;
   int32_t max_units, has_parts;
+  int32_t planned;  // 0: a small call without a plan; every CTA has at most one item
   int32_t* err;
 };
 
@@ -202,6 +202,34 @@ struct Item {
   int nch, part;  // chunks of the row, slot of this one's partial
   int table_row;
 };
+
+// Unit u of a small batch (at most 32 rows), found by one warp from the lengths
+// alone: row by row, chunk by chunk, as the plan numbers the partials.  Lane b
+// stands for row b.  `units`: their number.
+__device__ __forceinline__ Unit find_unit(const Args& a, int u, int lane, int& units) {
+  int64_t len = lane < a.batch ? (int64_t)a.seq_lens[lane] : 0;
+  const int64_t cap = a.bt_width * a.bs;
+  if (len > cap) {
+    if (blockIdx.x == 0) raise_dev(a.err, BL_DEVERR_TABLE);
+    len = cap;
+  }
+  const int n = len > 0 ? (int)((len + kChunk - 1) / kChunk) : 0;
+  int incl = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  units = __shfl_sync(0xffffffffu, incl, 31);
+  const uint32_t past = __ballot_sync(0xffffffffu, incl > u);
+  Unit r = {};
+  r.row = past ? __ffs(past) - 1 : 0;
+  r.chunk = u - __shfl_sync(0xffffffffu, incl - n, r.row);
+  r.len = __shfl_sync(0xffffffffu, (int)len, r.row);
+  r.part = u;
+  r.table_row = a.row_ids ? a.row_ids[r.row] : r.row;
+  return r;
+}
 
 __device__ __forceinline__ Unit load_unit(const Args& a, int64_t item) {
   const int4* p = reinterpret_cast<const int4*>(a.units + item / (a.hkv * a.head_tiles));
@@ -229,10 +257,10 @@ __device__ __forceinline__ bool make_item(const Args& a, int64_t item, const Uni
   return ok;
 }
 
-__device__ __forceinline__ int plan_units(const Args& a) {
+__device__ __forceinline__ int plan_units(const Args& a, bool tell) {
   const int units = a.hdr[0];
   if (a.hdr[1] != kPlanMagic || a.hdr[2] != a.batch || a.hdr[3] != a.max_units || units < 0 || units > a.max_units) {
-    if (threadIdx.x == 0 && blockIdx.x == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
+    if (tell && blockIdx.x == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
     return 0;
   }
   return units;
@@ -454,8 +482,10 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
   }
   __syncthreads();
 
-  pdl_wait();  // the plan (and all work before it) is complete and visible
-  const int64_t items = (int64_t)plan_units(a) * a.hkv * a.head_tiles;
+  pdl_wait();     // the plan (and all work before it) is complete and visible
+  // In a small call the join kernel's launch may overlap this one (it waits for
+  // this grid).  In a large one its CTAs would wait in places that others need.
+  if (!a.planned) pdl_trigger();
 
   if (warp == kNW) {
     // ------------------------------ planner ------------------------------
@@ -466,20 +496,35 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
     // whole item's time ahead of its use.)
     unsigned long long* claimed = reinterpret_cast<unsigned long long*>(a.hdr + 4);
     Pending<T, D> p;
-    int64_t item = blockIdx.x;
+    int64_t item = blockIdx.x, items = 0;
+    if (a.planned) items = (int64_t)plan_units(a, lane == 0) * a.hkv * a.head_tiles;
     for (int n_item = 0;; ++n_item) {
       const int k = n_item & 1;
       if (!__all_sync(0xffffffffu, wait_or_abort(&sh->item_empty[k], ((n_item >> 1) & 1) ^ 1, &sh->abort, a.err))) break;
-      if (n_item > 0) {
-        unsigned long long c = 0;
-        if (lane == 0) c = atomicAdd(claimed, 1ull);
-        item = (int64_t)__shfl_sync(0xffffffffu, c, 0) + gridDim.x;
+      Unit unit = {};
+      bool end;
+      if (a.planned) {
+        if (n_item > 0) {
+          unsigned long long c = 0;
+          if (lane == 0) c = atomicAdd(claimed, 1ull);
+          item = (int64_t)__shfl_sync(0xffffffffu, c, 0) + gridDim.x;
+        }
+        end = item >= items;
+        if (!end) unit = load_unit(a, item);
+      } else {
+        end = n_item > 0;
+        if (!end) {
+          const int per_unit = a.hkv * a.head_tiles;
+          int units;
+          unit = find_unit(a, (int)(item / per_unit), lane, units);
+          end = item >= (int64_t)units * per_unit;
+          if (units > a.max_units && blockIdx.x == 0 && lane == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
+        }
       }
-      const bool end = item >= items;
       if (end) {
         if (lane == 0) sh->items[k].it.heads = -1;
       } else {
-        p.begin(a, item, load_unit(a, item), lane);
+        p.begin(a, item, unit, lane);
         p.finish(a);
         if (!p.valid && lane == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
         p.stage(a, lane, sh->items[k], qs + k * C::kKS * room);
@@ -490,7 +535,7 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
     }
     // The last CTA to make its last claim leaves the counters as the plan did, for
     // the next layer's call with the same plan.
-    if (lane == 0 && atomicAdd(a.hdr + 6, 1) == (int)gridDim.x - 1) {
+    if (a.planned && lane == 0 && atomicAdd(a.hdr + 6, 1) == (int)gridDim.x - 1) {
       a.hdr[6] = 0;
       *claimed = 0;
     }
@@ -930,7 +975,7 @@ __global__ void __launch_bounds__(kSimtThreads) fp8_decode_simt_kernel(const Arg
   const int vd = tid % dp, vh0 = tid / dp, vstep = kSimtThreads / dp;
 
   pdl_wait();
-  const int64_t items = (int64_t)plan_units(a) * a.hkv * a.head_tiles;
+  const int64_t items = (int64_t)plan_units(a, tid == 0) * a.hkv * a.head_tiles;
   zero_empty_rows<T>(a, kSimtThreads);
 
   auto load_tile = [&](const uint8_t* pool, const float* sc) {
@@ -1071,7 +1116,13 @@ __global__ void __launch_bounds__(kReduceThreads) fp8_decode_reduce_kernel(const
   const int64_t len = min((int64_t)a.seq_lens[b], a.bt_width * a.bs);
   if (len <= kChunk) return;
   const int nch = (int)((len + kChunk - 1) / kChunk);
-  const int64_t base = a.row_base[b];
+  int64_t base = 0;
+  if (a.planned) {
+    base = a.row_base[b];
+  } else {
+    for (int r = 0; r < b; ++r)
+      base += (min(max((int64_t)a.seq_lens[r], (int64_t)0), a.bt_width * a.bs) + kChunk - 1) / kChunk;
+  }
   if (base < 0 || base + nch > a.max_units) return;  // flagged by the plan or the attention kernel
   __shared__ float s_w[kReduceTile];
   __shared__ float s_red[kWarps];
@@ -1291,7 +1342,11 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
   k.has_parts = a.max_seq_len > kChunk;
   k.err = a.err;
 
-  if (!a.plan_ready) {
+  // A call whose items all fit the GPU at once needs no plan: the order and the
+  // claims that it brings would change nothing, and its launch is a fifth of
+  // such a call (one request of 777 tokens: MEASURED).
+  k.planned = !(use_tc(kv) && a.batch <= 32 && (int64_t)k.max_units * k.hkv * k.head_tiles <= num_sms());
+  if (k.planned && !a.plan_ready) {
     PlanArgs p;
     p.seq_lens = a.seq_lens;
     p.row_ids = kv.row_ids;
@@ -1302,7 +1357,8 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
     p.row_base = (int32_t*)(ws + w.row_base);
     p.units = (Unit*)(ws + w.units);
     p.err = a.err;
-    if (launch_pdl(fp8_decode_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p) != cudaSuccess) {
+    const int threads = std::min(kPlanThreads, (k.batch + 31) / 32 * 32);  // >= kChunkTiles
+    if (launch_pdl(fp8_decode_plan_kernel, dim3(1), dim3(threads), 0, s, p) != cudaSuccess) {
       set_error("fp8_decode_plan_kernel: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
       return BL_ERR_LAUNCH;
     }

@@ -166,8 +166,35 @@ def test_decode_reports_what_it_cannot_do(cuda, native_lib):
     assert word(bt=bad) == nat.BL_DEVERR_BLOCK_ID
     assert word(bt=bt[:, :20].contiguous()) & nat.BL_DEVERR_TABLE
     assert word(n=100) & nat.BL_DEVERR_WORKSPACE  # a row longer than max_seq_len
-    blank = torch.zeros(ops.decode_fp8_workspace_bytes(2, 4, 128, 600), dtype=torch.uint8, device=cuda)
-    assert word(ws=blank, plan_ready=True) == nat.BL_DEVERR_WORKSPACE
+    # a plan that was never made, or made for another call (40 rows: more items than a call without a plan takes)
+    lens = [600] * 40
+    pool, table, bt = filled(cuda, lens, 2, 16, 128, BF16)
+    q, seq = torch.randn(40, 4, 128, device=cuda).to(BF16), i32(lens, cuda)
+    ws = torch.zeros(ops.decode_fp8_workspace_bytes(40, 4, 128, 600), dtype=torch.uint8, device=cuda)
+
+    def planned(n):
+        err.zero_()
+        ops.paged_decode_fp8(q[:n], *pool.args, 1, bt, seq[:n], 600, ws=ws, plan_ready=True, err=err)
+        return int(err)
+
+    assert planned(40) == nat.BL_DEVERR_WORKSPACE
+    ops.paged_decode_fp8(q, *pool.args, 1, bt, seq, 600, ws=ws)
+    assert planned(40) == 0 and planned(39) == nat.BL_DEVERR_WORKSPACE
+
+
+@pytest.mark.parametrize("batch", [1, 9, 32, 33])
+def test_decode_small_and_large_calls_agree(cuda, native_lib, batch):
+    """Calls with and without a plan, on both sides of the border, and the reuse of a plan by many layers' calls."""
+    lens = [(37 * b * b) % 1500 for b in range(batch)]
+    pool, table, bt = filled(cuda, lens, 2, 16, 128, BF16)
+    q, seq = torch.randn(batch, 8, 128, device=cuda).to(BF16), i32(lens, cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    ws = torch.empty(ops.decode_fp8_workspace_bytes(batch, 8, 128, 60000), dtype=torch.uint8, device=cuda)
+    small = ops.paged_decode_fp8(q, *pool.args, 1, bt, seq, 1500, err=err)
+    check_decode(small, q, pool, table, lens, 1)
+    for n in range(6):  # a bound of 60000 tokens needs a plan
+        assert torch.equal(ops.paged_decode_fp8(q, *pool.args, 1, bt, seq, 60000, ws=ws, plan_ready=n > 0, err=err), small)
+    assert int(err) == 0
 
 
 def prefill_case(device, prefixes, chunks, hq, hkv, bs, d, dtype, seed=0):
