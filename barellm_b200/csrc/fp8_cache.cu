@@ -16,7 +16,7 @@
 namespace bl {
 namespace {
 
-constexpr int kAppendWarps = 8;
+constexpr int kAppendWarps = 4;
 
 struct AppendFp8Args {
   uint8_t* k_pool;
@@ -34,6 +34,7 @@ struct AppendFp8Args {
   const int32_t* new_offsets;
   int64_t max_new;
   int32_t hkv, bs, d;
+  int32_t vpr_shift;  // log2 of a token's 16-byte vectors, or -1
   int32_t* err;
 };
 
@@ -65,10 +66,39 @@ __device__ __forceinline__ void store_codes(uint8_t* dst, const float* f, float 
   }
 }
 
+// The largest magnitude in a 16-byte vector as an integer that orders as the
+// magnitudes do: the values' bits without the sign.  16-bit elements go two
+// at a time (the result's halves are separate maxima).
+template <typename T>
+__device__ __forceinline__ uint32_t max_bits(uint32_t m, const uint4& v) {
+  if constexpr (sizeof(T) == 2) {
+    m = __vmaxu2(m, v.x & 0x7fff7fffu);
+    m = __vmaxu2(m, v.y & 0x7fff7fffu);
+    m = __vmaxu2(m, v.z & 0x7fff7fffu);
+    return __vmaxu2(m, v.w & 0x7fff7fffu);
+  } else {
+    m = max(m, v.x & 0x7fffffffu);
+    m = max(m, v.y & 0x7fffffffu);
+    m = max(m, v.z & 0x7fffffffu);
+    return max(m, v.w & 0x7fffffffu);
+  }
+}
+// The magnitude that max_bits' result (joined over its halves) stands for;
+// +inf or NaN where the vector holds one.
+template <typename T> __device__ __forceinline__ float bits_to_magnitude(uint32_t m);
+template <> __device__ __forceinline__ float bits_to_magnitude<float>(uint32_t m) { return __uint_as_float(m); }
+template <> __device__ __forceinline__ float bits_to_magnitude<__nv_bfloat16>(uint32_t m) {
+  return __uint_as_float(max(m & 0xffffu, m >> 16) << 16);
+}
+template <> __device__ __forceinline__ float bits_to_magnitude<__half>(uint32_t m) {
+  return __half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16)));
+}
+
 // grid: (touched blocks, ceil(2 * hkv / kAppendWarps), batch)
 // VEC: rows move as 16-byte vectors (head_dim a multiple of one, everything
 // aligned); up to kHeld of them per lane stay in registers between the maximum
 // and the store (a 16-token block of head_dim 128 fits), more are read twice.
+// Measured at 40k packed tokens (8 KV heads, head_dim 128, bf16): MEASURED.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kAppendWarps * 32) append_fp8_kernel(const AppendFp8Args a) {
   pdl_trigger();  // a dependent launch (the decode plan) may start; it waits for this grid
@@ -93,6 +123,27 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_fp8_kernel(const App
   const int64_t lb = start / a.bs + blockIdx.x;
   const int64_t p0 = max(start, lb * a.bs), p1 = min(start + n, (lb + 1) * a.bs);
   if (p0 >= p1) return;
+  const int64_t st = is_v ? a.vst : a.kst;
+  const T* src = reinterpret_cast<const T*>(is_v ? a.v_new : a.k_new) + b * (is_v ? a.vsb : a.ksb) +
+                 (int64_t)h * (is_v ? a.vsh : a.ksh) + (off + p0 - start) * st;
+  const int vpr = a.d / E;                  // vectors per token
+  const int total = (int)(p1 - p0) * vpr;  // block_size * head_dim <= 2^24
+  auto token_of = [&](int idx) { return a.vpr_shift >= 0 ? idx >> a.vpr_shift : idx / vpr; };
+  auto vector_at = [&](int idx) {
+    const int t = token_of(idx);
+    return src + t * st + (idx - t * vpr) * E;
+  };
+  // the tokens are on their way while the block is looked up
+  uint4 held[kHeld];
+  const bool fits = VEC && total <= kHeld * 32;
+  if (fits) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int idx = lane + 32 * i;
+      held[i] = make_uint4(0, 0, 0, 0);
+      if (idx < total) held[i] = *reinterpret_cast<const uint4*>(vector_at(idx));
+    }
+  }
   if (lb >= a.bt_width) {
     if (lane == 0) raise_dev(a.err, BL_DEVERR_TABLE);
     return;
@@ -103,52 +154,37 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_fp8_kernel(const App
     if (lane == 0) raise_dev(a.err, BL_DEVERR_BLOCK_ID);
     return;
   }
-  const int64_t st = is_v ? a.vst : a.kst;
-  const T* src = reinterpret_cast<const T*>(is_v ? a.v_new : a.k_new) + b * (is_v ? a.vsb : a.ksb) +
-                 (int64_t)h * (is_v ? a.vsh : a.ksh) + (off + p0 - start) * st;
   const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + h;
   uint8_t* page = (is_v ? a.v_pool : a.k_pool) + slot * a.bs * a.d;
   float* scale_p = (is_v ? a.v_scale : a.k_scale) + slot;
   const int kept = (int)(p0 - lb * a.bs);  // tokens the block holds already
   const float old_scale = kept > 0 ? *scale_p : 0.f;
   uint8_t* dst = page + (int64_t)kept * a.d;
-  const int vpr = a.d / E;                  // vectors per token
-  const int total = (int)(p1 - p0) * vpr;  // block_size * head_dim <= 2^24
 
   // largest finite magnitude of the new tokens
   float amax = 0.f;
-  uint4 held[kHeld];
-  const bool fits = VEC && total <= kHeld * 32;
-  if (fits) {
+  if constexpr (VEC) {
+    uint32_t bits = 0;
+    if (fits) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const int idx = lane + 32 * i;
-      held[i] = make_uint4(0, 0, 0, 0);
-      if (idx < total) {
-        const int t = idx / vpr;
-        held[i] = *reinterpret_cast<const uint4*>(src + t * st + (idx - t * vpr) * E);
-      }
+      for (int i = 0; i < kHeld; ++i) bits = max_bits<T>(bits, held[i]);
+    } else {
+#pragma unroll 4
+      for (int idx = lane; idx < total; idx += 32) bits = max_bits<T>(bits, *reinterpret_cast<const uint4*>(vector_at(idx)));
     }
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      float f[8];
-      unpack16<T>(held[i], f);
-#pragma unroll
-      for (int e = 0; e < 16 / (int)sizeof(T); ++e) amax = fmaxf(amax, finite_abs(f[e]));
-    }
-  } else {
-    for (int idx = lane; idx < total; idx += 32) {
-      const int t = idx / vpr;
-      const T* p = src + t * st + (idx - t * vpr) * E;
-      if constexpr (VEC) {
+    amax = bits_to_magnitude<T>(bits);
+    if (__any_sync(0xffffffffu, !(amax < INFINITY))) {
+      // an infinity or a NaN among the tokens: again, leaving those out
+      amax = 0.f;
+      for (int idx = lane; idx < total; idx += 32) {
         float f[8];
-        unpack16<T>(*reinterpret_cast<const uint4*>(p), f);
+        unpack16<T>(*reinterpret_cast<const uint4*>(vector_at(idx)), f);
 #pragma unroll
         for (int e = 0; e < E; ++e) amax = fmaxf(amax, finite_abs(f[e]));
-      } else {
-        amax = fmaxf(amax, finite_abs(to_f32<T>(*p)));
       }
     }
+  } else {
+    for (int idx = lane; idx < total; idx += 32) amax = fmaxf(amax, finite_abs(to_f32<T>(*vector_at(idx))));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
@@ -186,8 +222,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_fp8_kernel(const App
     }
   } else {
     for (int idx = lane; idx < total; idx += 32) {
-      const int t = idx / vpr;
-      const T* p = src + t * st + (idx - t * vpr) * E;
+      const T* p = vector_at(idx);
       if constexpr (VEC) {
         float f[8];
         unpack16<T>(*reinterpret_cast<const uint4*>(p), f);
@@ -213,27 +248,32 @@ struct GatherFp8Args {
   const int32_t* row_ids;
   const int32_t* seq_lens;
   int64_t max_len;
-  int32_t hkv, bs, d, nvec, zero_fill;
+  int32_t hkv, bs, bs_shift, d, nvec, zero_fill;
   int32_t* err;
 };
 
-// E consecutive codes times scale, as one store of E elements of T
+// E consecutive codes
+template <int E> struct CodesT;
+template <> struct CodesT<8> { using type = uint2; };
+template <> struct CodesT<4> { using type = uint32_t; };
+template <> struct CodesT<1> { using type = uint8_t; };
+template <int E> using Codes = typename CodesT<E>::type;
+
+// E codes times scale, as one store of E elements of T
 template <typename T, int E>
-__device__ __forceinline__ void dequant_store(T* dst, const uint8_t* src, float scale) {
+__device__ __forceinline__ void dequant_store(T* dst, const Codes<E>& c, float scale) {
   if constexpr (E == 1) {
-    *dst = dequant_to<T>(e4m3_to_float(*src) * scale);
+    *dst = dequant_to<T>(e4m3_to_float(c) * scale);
   } else {
     float f[E];
     uint32_t w[E / 4];
-    if constexpr (E == 8) {
-      const uint2 c = *reinterpret_cast<const uint2*>(src);
+    if constexpr (E == 8)
       w[0] = c.x, w[1] = c.y;
-    } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(src);
-    }
+    else
+      w[0] = c;
 #pragma unroll
     for (int i = 0; i < E / 4; ++i) {
-      const float2 x = e4m3x2_to_float2((uint16_t)w[i]), y = e4m3x2_to_float2((uint16_t)(w[i] >> 16));
+      const float2 x = unpack2<__half>(e4m3lo_to_f16x2(w[i])), y = unpack2<__half>(e4m3hi_to_f16x2(w[i]));
       f[4 * i] = x.x * scale, f[4 * i + 1] = x.y * scale, f[4 * i + 2] = y.x * scale, f[4 * i + 3] = y.y * scale;
     }
     union {
@@ -254,42 +294,63 @@ __device__ __forceinline__ void zero_store(T* dst) {
     *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
 }
 
-// grid: (ceil(max_len / blockDim.y), hkv, batch); threadIdx.x walks the vectors
-// of a token, threadIdx.y the tokens
+constexpr int kGatherTok = 2;  // tokens of a thread: their loads are in flight together
+
+// grid: (ceil(max_len / (kGatherTok * blockDim.y)), hkv, batch); threadIdx.x walks the
+// vectors of a token, threadIdx.y the tokens
 template <typename T, int E>
 __global__ void __launch_bounds__(256) gather_fp8_kernel(const GatherFp8Args a) {
   const int64_t b = blockIdx.z;
   const int h = blockIdx.y;
-  const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (t >= a.max_len) return;
-  T* ko = reinterpret_cast<T*>(a.k_out) + b * a.osb + h * a.osh + t * a.ost;
-  T* vo = reinterpret_cast<T*>(a.v_out) + b * a.osb + h * a.osh + t * a.ost;
+  const int64_t t0 = (int64_t)blockIdx.x * (kGatherTok * blockDim.y) + threadIdx.y;
   const int64_t len = a.seq_lens[b];
-  if (t >= len) {
-    if (a.zero_fill)
-      for (int v = threadIdx.x; v < a.nvec; v += blockDim.x) {
-        zero_store<T, E>(ko + v * E);
-        zero_store<T, E>(vo + v * E);
-      }
-    return;
-  }
-  const int64_t lb = t / a.bs;
-  if (lb >= a.bt_width) {
-    raise_dev(a.err, BL_DEVERR_TABLE);
-    return;
-  }
   const int64_t row = a.row_ids ? (int64_t)a.row_ids[b] : b;
-  const int64_t phys = a.block_tables[row * a.bt_stride + lb];
-  if (phys < 0 || phys >= a.num_blocks) {
-    raise_dev(a.err, BL_DEVERR_BLOCK_ID);
-    return;
+  T* ko = reinterpret_cast<T*>(a.k_out) + b * a.osb + h * a.osh;
+  T* vo = reinterpret_cast<T*>(a.v_out) + b * a.osb + h * a.osh;
+  int64_t src[kGatherTok];
+  float ks[kGatherTok], vs[kGatherTok];
+#pragma unroll
+  for (int i = 0; i < kGatherTok; ++i) {
+    const int64_t t = t0 + i * blockDim.y;
+    src[i] = -1;
+    if (t >= len || t >= a.max_len) continue;
+    const int64_t lb = a.bs_shift >= 0 ? t >> a.bs_shift : t / a.bs;
+    if (lb >= a.bt_width) {
+      raise_dev(a.err, BL_DEVERR_TABLE);
+      src[i] = -2;
+      continue;
+    }
+    const int64_t phys = a.block_tables[row * a.bt_stride + lb];
+    if (phys < 0 || phys >= a.num_blocks) {
+      raise_dev(a.err, BL_DEVERR_BLOCK_ID);
+      src[i] = -2;
+      continue;
+    }
+    const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + h;
+    src[i] = (slot * a.bs + (t - lb * a.bs)) * a.d;
+    ks[i] = a.k_scale[slot];
+    vs[i] = a.v_scale[slot];
   }
-  const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + h;
-  const int64_t src = (slot * a.bs + (t - lb * a.bs)) * a.d;
-  const float ks = a.k_scale[slot], vs = a.v_scale[slot];
   for (int v = threadIdx.x; v < a.nvec; v += blockDim.x) {
-    dequant_store<T, E>(ko + v * E, a.k_pool + src + v * E, ks);
-    dequant_store<T, E>(vo + v * E, a.v_pool + src + v * E, vs);
+    Codes<E> kc[kGatherTok], vc[kGatherTok];
+#pragma unroll
+    for (int i = 0; i < kGatherTok; ++i)
+      if (src[i] >= 0) {
+        kc[i] = *reinterpret_cast<const Codes<E>*>(a.k_pool + src[i] + v * E);
+        vc[i] = *reinterpret_cast<const Codes<E>*>(a.v_pool + src[i] + v * E);
+      }
+#pragma unroll
+    for (int i = 0; i < kGatherTok; ++i) {
+      const int64_t t = t0 + i * blockDim.y;
+      if (t >= a.max_len) break;
+      if (src[i] >= 0) {
+        dequant_store<T, E>(ko + t * a.ost + v * E, kc[i], ks[i]);
+        dequant_store<T, E>(vo + t * a.ost + v * E, vc[i], vs[i]);
+      } else if (src[i] == -1 && a.zero_fill) {
+        zero_store<T, E>(ko + t * a.ost + v * E);
+        zero_store<T, E>(vo + t * a.ost + v * E);
+      }
+    }
   }
 }
 
@@ -309,7 +370,7 @@ int launch_gather(GatherFp8Args k, bool vec, int64_t batch, cudaStream_t s) {
   k.nvec = vec ? k.d / E : k.d;
   const int bx = std::min(k.nvec, 256);
   const int by = 256 / bx;
-  const int64_t gx = (k.max_len + by - 1) / by;
+  const int64_t gx = (k.max_len + kGatherTok * by - 1) / (kGatherTok * by);
   dim3 grid((unsigned)gx, (unsigned)k.hkv, (unsigned)batch), block((unsigned)bx, (unsigned)by);
   if (vec)
     gather_fp8_kernel<T, E><<<grid, block, 0, s>>>(k);
@@ -362,6 +423,9 @@ extern "C" int bl_paged_append_fp8(const bl_append_fp8_args* args, void* stream)
   const int E = 16 / es;
   bool vec = kv.head_dim % E == 0 && ((uintptr_t)a.k_new & 15) == 0 && ((uintptr_t)a.v_new & 15) == 0;
   for (int64_t st : {k.ksb, k.ksh, k.kst, k.vsb, k.vsh, k.vst}) vec = vec && st % E == 0;
+  k.vpr_shift = -1;
+  for (int i = 0; i < 8; ++i)
+    if (vec && kv.head_dim / E == 1 << i) k.vpr_shift = i;
   // blocks that n tokens can touch, from any offset in a block
   const int64_t touched = (a.max_new_tokens + kv.block_size - 2) / kv.block_size + 1;
   dim3 grid((unsigned)touched, (unsigned)((2 * k.hkv + kAppendWarps - 1) / kAppendWarps), (unsigned)a.batch);
@@ -406,6 +470,9 @@ extern "C" int bl_paged_gather_fp8(const bl_gather_fp8_args* args, void* stream)
   k.bs = (int32_t)kv.block_size;
   k.d = (int32_t)kv.head_dim;
   k.nvec = 0;
+  k.bs_shift = -1;
+  for (int i = 0; i < 17; ++i)
+    if (kv.block_size == (int64_t)1 << i) k.bs_shift = i;
   k.zero_fill = a.zero_fill;
   k.err = a.err;
   const int E = 16 / es;

@@ -36,7 +36,7 @@ inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 // head repeated `dup` times.
 struct Scratch {
   int64_t width, pages, heads, dup;
-  size_t table, k, v, total;
+  size_t table, order, k, v, total;
 };
 
 bool use_tc(int32_t dtype, int64_t d) { return (dtype == BL_BF16 || dtype == BL_F16) && d == kTCDim; }
@@ -54,9 +54,11 @@ bool plan_scratch(int64_t batch, int64_t hq, int64_t hkv, int64_t bs, int64_t ma
   const double bound = (double)total_blocks * (double)bs / kPage + (double)batch + 1;
   w->pages = (int64_t)std::min(bound, (double)batch * (double)w->width);
   if ((double)w->pages * w->heads * kPage > (double)(INT32_MAX - 64) || w->heads > 65535) return false;
-  size_t off = align256((size_t)batch * w->width * sizeof(int32_t));
+  const size_t table_bytes = align256((size_t)batch * w->width * sizeof(int32_t));
+  const size_t off = table_bytes + align256((size_t)batch * sizeof(int32_t));
   const size_t half = align256((size_t)w->pages * w->heads * kPage * kTCDim * 2);
   w->table = 0;
+  w->order = table_bytes;
   w->k = off;
   w->v = off + half;
   w->total = off + 2 * half;
@@ -71,6 +73,7 @@ struct ExpandArgs {
   void* k_out;
   void* v_out;
   int32_t* table;  // [batch][width]
+  int32_t* order;  // [batch] rows, the longest first
   int64_t num_blocks, layer, width, pages, bt_stride, bt_width;
   const int32_t* block_tables;
   const int32_t* row_ids;
@@ -103,22 +106,22 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(const Expand
         reinterpret_cast<T*>(a.out)[b * a.o_sb + (qo + i) * a.o_st + (int64_t)(e / kTCDim) * a.o_sh + e % kTCDim] =
             from_f32<T>(0.f);
     if (tid == 0 && len > a.width * kPage) raise_dev(a.err, BL_DEVERR_WORKSPACE);  // longer than max_seq_len
+    // The attention kernel's CTAs start in the order of their rows, and one CTA's
+    // time goes with its row's length: the longest rows go first.
+    __shared__ int s_rank;
+    if (tid == 0) s_rank = 0;
+    __syncthreads();
+    int longer = 0;
+    for (int64_t r = tid; r < (int64_t)gridDim.z; r += kExpandThreads) {
+      const int64_t l = max((int64_t)a.seq_lens[r], (int64_t)0);
+      longer += l > len || (l == len && r < b);
+    }
+    atomicAdd(&s_rank, longer);
+    __syncthreads();
+    if (tid == 0) a.order[s_rank] = (int32_t)b;
   }
   const int64_t j0 = (int64_t)blockIdx.x * kExpandPages;
   if (j0 * kPage >= len) return;
-
-  // first scratch page of the row: the pages of the rows before it
-  __shared__ int64_t s_sum[kExpandThreads / 32];
-  int64_t base = 0;
-  for (int64_t r = tid; r < b; r += kExpandThreads)
-    base += (min(max((int64_t)a.seq_lens[r], (int64_t)0), a.width * kPage) + kPage - 1) / kPage;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o);
-  if ((tid & 31) == 0) s_sum[tid >> 5] = base;
-  __syncthreads();
-  base = 0;
-#pragma unroll
-  for (int w = 0; w < kExpandThreads / 32; ++w) base += s_sum[w];
 
   const int64_t row = a.row_ids ? (int64_t)a.row_ids[b] : b;
   const int tok = tid >> 4, v = tid & 15;
@@ -129,13 +132,7 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(const Expand
   for (int p = 0; p < kExpandPages; ++p) {
     const int64_t j = j0 + p, t = j * kPage + tok;
     ok[p] = false;
-    if (j >= a.width || j * kPage >= len) continue;
-    const bool fits = base + j < a.pages;
-    if (h == 0 && tid == 0) {
-      a.table[b * a.width + j] = fits ? (int32_t)(base + j) : -1;
-      if (!fits) raise_dev(a.err, BL_DEVERR_WORKSPACE);
-    }
-    if (!fits || t >= len) continue;
+    if (j >= a.width || t >= len) continue;
     const int64_t lb = t / a.bs;
     if (lb >= a.bt_width) {
       raise_dev(a.err, BL_DEVERR_TABLE);
@@ -153,6 +150,23 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(const Expand
     ks[p] = a.k_scale[slot];
     vs[p] = a.v_scale[slot];
     ok[p] = true;
+  }
+  // meanwhile, the first scratch page of the row: the pages of the rows before it
+  __shared__ int64_t s_sum[kExpandThreads / 32];
+  int64_t base = 0;
+  for (int64_t r = tid; r < b; r += kExpandThreads)
+    base += (min(max((int64_t)a.seq_lens[r], (int64_t)0), a.width * kPage) + kPage - 1) / kPage;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o);
+  if ((tid & 31) == 0) s_sum[tid >> 5] = base;
+  __syncthreads();
+  base = 0;
+#pragma unroll
+  for (int w = 0; w < kExpandThreads / 32; ++w) base += s_sum[w];
+  if (h == 0 && tid < kExpandPages && j0 + tid < a.width && (j0 + tid) * kPage < len) {
+    const bool fits = base + j0 + tid < a.pages;
+    a.table[b * a.width + j0 + tid] = fits ? (int32_t)(base + j0 + tid) : -1;
+    if (!fits) raise_dev(a.err, BL_DEVERR_WORKSPACE);
   }
 #pragma unroll
   for (int p = 0; p < kExpandPages; ++p) {
@@ -466,6 +480,7 @@ int launch_tc(const bl_prefill_fp8_args& a, const Scratch& w, cudaStream_t s) {
   e.k_out = ws + w.k;
   e.v_out = ws + w.v;
   e.table = (int32_t*)(ws + w.table);
+  e.order = (int32_t*)(ws + w.order);
   e.num_blocks = kv.num_blocks;
   e.layer = kv.layer;
   e.width = w.width;
@@ -514,7 +529,7 @@ int launch_tc(const bl_prefill_fp8_args& a, const Scratch& w, cudaStream_t s) {
   p.max_q_len = a.max_q_len;
   p.scale = a.scale;
   p.err = a.err;
-  return prefill_tc_launch(p, s);
+  return prefill_tc_launch(p, s, e.order);
 }
 
 // Strides and pointers that the tcgen05 kernel reads pairs of elements through.

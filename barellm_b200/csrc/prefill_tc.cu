@@ -90,6 +90,7 @@ struct Args {
   int64_t bt_stride;
   int32_t bt_width;
   const int32_t* row_ids;
+  const int32_t* row_order;  // row of each blockIdx.z, or null: in order
   const uint16_t* k_pool;
   const uint16_t* v_pool;
   int32_t q_vec16;  // q rows start on 16-byte boundaries (pointer and strides)
@@ -128,7 +129,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // ---- which rows: heaviest query tiles first ----
   const int64_t qtile = (int64_t)gridDim.x - 1 - blockIdx.x;
   const int h = blockIdx.y;
-  const int64_t b = blockIdx.z;
+  const int64_t b = a.row_order ? (int64_t)a.row_order[blockIdx.z] : (int64_t)blockIdx.z;
   int64_t qo = 0, nq = a.max_q;
   if (a.q_offsets) {
     qo = a.q_offsets[b];
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 size_t smem_bytes() { return 1024 + kSmemData + sizeof(Shared); }
 
 template <bool BF16>
-int launch(const bl_prefill_args& a, cudaStream_t s) {
+int launch(const bl_prefill_args& a, const int32_t* row_order, cudaStream_t s) {
   // the attribute belongs to one device's copy of the kernel: set once per device
   static std::atomic<bool> attr_done[64];
   int dev = 0;
@@ -583,6 +584,7 @@ int launch(const bl_prefill_args& a, cudaStream_t s) {
   k.bt_stride = a.kv.bt_stride;
   k.bt_width = (int32_t)std::min<int64_t>(a.kv.bt_width, INT32_MAX);
   k.row_ids = a.kv.row_ids;
+  k.row_order = row_order;
   k.hkv = (int32_t)a.kv.num_kv_heads;
   k.g = (int32_t)(a.num_q_heads / a.kv.num_kv_heads);
   k.bq = kRows / k.g;
@@ -618,7 +620,7 @@ bool prefill_tc_supported(int32_t dtype, int64_t head_dim, int64_t block_size, i
   return g == 1 || g == 2 || g == 4 || g == 8;
 }
 
-int prefill_tc_launch(const bl_prefill_args& a, cudaStream_t s) {
+int prefill_tc_launch(const bl_prefill_args& a, cudaStream_t s, const int32_t* row_order) {
   const uint64_t rows = (uint64_t)a.kv.num_layers * a.kv.num_blocks * a.kv.num_kv_heads * kBS;
   BL_CHECK_ARG(rows + kBS <= (uint64_t)INT32_MAX, "bl_paged_prefill: pool has more than 2^31 rows");
   BL_CHECK_ARG(((uintptr_t)a.kv.k_pool & 15) == 0 && ((uintptr_t)a.kv.v_pool & 15) == 0,
@@ -627,8 +629,8 @@ int prefill_tc_launch(const bl_prefill_args& a, cudaStream_t s) {
                    a.q_stride_t % 2 == 0 && a.q_stride_h % 2 == 0 && a.out_stride_b % 2 == 0 &&
                    a.out_stride_t % 2 == 0 && a.out_stride_h % 2 == 0,
                "bl_paged_prefill: q/out must be 4-byte aligned with even strides");
-  if (a.kv.dtype == BL_BF16) return launch<true>(a, s);
-  return launch<false>(a, s);
+  if (a.kv.dtype == BL_BF16) return launch<true>(a, row_order, s);
+  return launch<false>(a, row_order, s);
 }
 
 }  // namespace bl

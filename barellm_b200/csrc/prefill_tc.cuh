@@ -5,6 +5,8 @@
 namespace bl {
 
 bool prefill_tc_supported(int32_t dtype, int64_t head_dim, int64_t block_size, int64_t hq, int64_t hkv);
-int prefill_tc_launch(const bl_prefill_args& a, cudaStream_t s);
+// row_order: device array, the row that each blockIdx.z works on (a permutation
+// of the batch), or null.
+int prefill_tc_launch(const bl_prefill_args& a, cudaStream_t s, const int32_t* row_order = nullptr);
 
 }  // namespace bl
