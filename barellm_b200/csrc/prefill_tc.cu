@@ -126,6 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Shared* sh = reinterpret_cast<Shared*>(smem + kSmemData);
 
+  pdl_wait();  // (launched so behind the expansion of an 8-bit cache; else a no-op)
   // ---- which rows: heaviest query tiles first ----
   const int64_t qtile = (int64_t)gridDim.x - 1 - blockIdx.x;
   const int h = blockIdx.y;
@@ -605,6 +606,15 @@ int launch(const bl_prefill_args& a, const int32_t* row_order, cudaStream_t s) {
   k.err = a.err;
   const int64_t tiles = (a.max_q_len + k.bq - 1) / k.bq;
   dim3 grid((unsigned)tiles, (unsigned)a.kv.num_kv_heads, (unsigned)a.batch);
+  if (row_order) {
+    // the kernel before it on the stream is the expansion: this launch is prepared
+    // while that one runs
+    if (launch_pdl(prefill_tc_kernel<BF16>, grid, dim3(kThreads), smem_bytes(), s, k, kmap, vmap) != cudaSuccess) {
+      set_error("prefill_tc_kernel: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+      return BL_ERR_LAUNCH;
+    }
+    return BL_OK;
+  }
   prefill_tc_kernel<BF16><<<grid, kThreads, smem_bytes(), s>>>(k, kmap, vmap);
   BL_CHECK_LAUNCH("prefill_tc_kernel");
   return BL_OK;
