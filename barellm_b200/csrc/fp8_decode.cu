@@ -483,9 +483,6 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
   __syncthreads();
 
   pdl_wait();     // the plan (and all work before it) is complete and visible
-  // In a small call the join kernel's launch may overlap this one (it waits for
-  // this grid).  In a large one its CTAs would wait in places that others need.
-  if (!a.planned) pdl_trigger();
 
   if (warp == kNW) {
     // ------------------------------ planner ------------------------------
@@ -497,7 +494,11 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
     unsigned long long* claimed = reinterpret_cast<unsigned long long*>(a.hdr + 4);
     Pending<T, D> p;
     int64_t item = blockIdx.x, items = 0;
-    if (a.planned) items = (int64_t)plan_units(a, lane == 0) * a.hkv * a.head_tiles;
+    Unit first = {};
+    if (a.planned) {
+      first = load_unit(a, item);  // (the grid is no larger than the plan has room for)
+      items = (int64_t)plan_units(a, lane == 0) * a.hkv * a.head_tiles;
+    }
     for (int n_item = 0;; ++n_item) {
       const int k = n_item & 1;
       if (!__all_sync(0xffffffffu, wait_or_abort(&sh->item_empty[k], ((n_item >> 1) & 1) ^ 1, &sh->abort, a.err))) break;
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
           item = (int64_t)__shfl_sync(0xffffffffu, c, 0) + gridDim.x;
         }
         end = item >= items;
-        if (!end) unit = load_unit(a, item);
+        if (!end) unit = n_item > 0 ? load_unit(a, item) : first;
       } else {
         end = n_item > 0;
         if (!end) {
@@ -522,6 +523,7 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
         }
       }
       if (end) {
+        pdl_trigger();  // the join kernel's launch may overlap this grid's end, for which it waits
         if (lane == 0) sh->items[k].it.heads = -1;
       } else {
         p.begin(a, item, unit, lane);
