@@ -18,6 +18,8 @@ with one scatter kernel and attends straight from the pages:
     packed on the token axis): one packed append, one paged prefill;
   * None (uncached full forward): the new K/V are paged into a scratch pool
     and attended causally by the same prefill kernel.
+An 8-bit cache (``PagedKVCache(kv_dtype=torch.float8_e4m3fn)``) takes the 8-bit
+form of the same ops.
 There is no CPU path: a CPU tensor or an unknown cache type raises.
 """
 
@@ -100,6 +102,8 @@ class CudaPagedAttentionBackend:
         s = layer.storage()
         idx = layer.layer_idx
         b, hq, t, d = q.shape
+        if s.quantized:
+            return self._batched_attend_fp8(q, layer, meta)
         if t == 1:
             out = torch.empty((b, hq, 1, d), dtype=q.dtype, device=q.device)
             serial = ops.plan_serial(s.device)
@@ -120,6 +124,22 @@ class CudaPagedAttentionBackend:
         return ops.paged_prefill(q, s.key_cache, s.value_cache, idx, s.arena.table, meta.seq_lens,
                                  row_ids=meta.rows, err=s.err)
 
+    def _batched_attend_fp8(self, q, layer: BatchLayerKV, meta) -> torch.Tensor:
+        s, idx = layer.storage(), layer.layer_idx
+        b, hq, t, d = q.shape
+        if t > 1:
+            return ops.paged_prefill_fp8(q, *s.pools, idx, s.arena.table, meta.seq_lens, meta.max_seq_len,
+                                         total_blocks=meta.total_blocks(s.block_size), row_ids=meta.rows, err=s.err)
+        # the step's first layer makes the plan, in a workspace that belongs to
+        # this step's metadata; its later layers read it
+        first = meta.plan_ws is None or meta.plan_heads != hq
+        if first:
+            n = ops.decode_fp8_workspace_bytes(b, hq, d, meta.max_seq_len)
+            meta.plan_ws, meta.plan_heads = torch.empty(n, dtype=torch.uint8, device=q.device), hq
+        out = ops.paged_decode_fp8(q, *s.pools, idx, s.arena.table, meta.seq_lens, meta.max_seq_len, row_ids=meta.rows,
+                                   ws=meta.plan_ws, plan_ready=not first, err=s.err)
+        return out.unsqueeze(2)
+
     def _single(self, q, new_k, new_v, layer: PagedLayerKV) -> torch.Tensor:
         check(q.shape[0] == 1, "PagedKVCache currently supports batch size 1")
         layer.append_only(new_k, new_v)
@@ -130,6 +150,11 @@ class CudaPagedAttentionBackend:
         n = layer.seq_len
         rows = _i32([layer._request.row], s.device)
         seq = _i32([n], s.device)
+        if s.quantized:
+            if q.shape[2] == 1:
+                return ops.paged_decode_fp8(q, *s.pools, layer.layer_idx, s.arena.table, seq, n, row_ids=rows,
+                                            err=s.err).unsqueeze(2)
+            return ops.paged_prefill_fp8(q, *s.pools, layer.layer_idx, s.arena.table, seq, n, row_ids=rows, err=s.err)
         if q.shape[2] == 1:
             out = ops.paged_decode(q, s.key_cache, s.value_cache, layer.layer_idx, s.arena.table, seq, n,
                                    row_ids=rows, err=s.err)
@@ -141,6 +166,10 @@ class CudaPagedAttentionBackend:
         """Chunked prefill of a packed batch: each row's chunk attends over its
         cached prefix and itself (bottom-right causal), one kernel."""
         s = layer.owner.storage
+        if s.quantized:
+            return ops.paged_prefill_fp8(q, *s.pools, layer.layer_idx, s.arena.table, meta.seq_lens, meta.max_seq_len,
+                                         total_blocks=meta.total_blocks, q_offsets=meta.offsets, max_q_len=meta.max_chunk,
+                                         row_ids=meta.rows, err=s.err)
         return ops.paged_prefill(q, s.key_cache, s.value_cache, layer.layer_idx, s.arena.table, meta.seq_lens,
                                  q_offsets=meta.offsets, max_q_len=meta.max_chunk, row_ids=meta.rows, err=s.err)
 

@@ -19,7 +19,6 @@ from operator import attrgetter
 import numpy as np
 import torch
 
-from . import ops
 from .paged_kv_cache import PagedBatchKVMetadata, PagedKVCache, PagedKVCacheView, PagedLayerKV, check
 
 
@@ -54,6 +53,13 @@ class StepMeta:
         self.plan_ws: torch.Tensor | None = None
         self.plan_heads = 0
         self.plan_token = -1
+
+    def total_blocks(self, block_size: int) -> int:
+        """Host-side bound on the rows' blocks together (in static mode for any
+        lengths up to the captured bound)."""
+        if self.static:
+            return len(self._rows) * -(-self.max_seq_len // block_size)
+        return int((-(-self.seq_lens_host // block_size)).sum())
 
     def _fill(self, starts: np.ndarray, new_tokens: int) -> torch.Tensor:
         host = torch.empty((3, len(self._rows)), dtype=torch.int32, pin_memory=self._pin)
@@ -226,8 +232,7 @@ class BatchLayerKV:
         per-row appends, batched_kv_cache.py:40-63).  Returns the step metadata
         whose ``seq_lens`` are the post-append lengths."""
         s, rows, ends, meta = self._begin_append(key, value)
-        ops.paged_append(s.key_cache, s.value_cache, self.layer_idx, s.arena.table, meta.starts, key, value,
-                         row_ids=meta.rows, err=s.err)
+        s.write(self.layer_idx, meta.starts, key, value, row_ids=meta.rows)
         s.arena.lens[rows, self.layer_idx] = ends
         return meta
 
@@ -238,9 +243,8 @@ class BatchLayerKV:
         ``ops.qk_norm_rope_append``).  Returns the step metadata and the
         prepared q."""
         s, rows, ends, meta = self._begin_append(key, value)
-        q_out = ops.qk_norm_rope_append(q, key, value, q_norm_weight, k_norm_weight, cos, sin, eps, s.key_cache,
-                                        s.value_cache, self.layer_idx, s.arena.table, meta.starts,
-                                        row_ids=meta.rows, err=s.err)
+        q_out = s.write_prepped(self.layer_idx, meta.starts, q, key, value, q_norm_weight, k_norm_weight, cos, sin, eps,
+                                row_ids=meta.rows)
         s.arena.lens[rows, self.layer_idx] = ends
         return meta, q_out
 
@@ -260,8 +264,7 @@ class BatchLayerKV:
         check(bool((self.starts() > 0).all()), "KV cache is empty")
         s = self.storage()
         meta = self.current_meta()
-        return ops.paged_gather(s.key_cache, s.value_cache, self.layer_idx, s.arena.table, meta.seq_lens,
-                                meta.max_seq_len, row_ids=meta.rows, err=s.err)
+        return s.gather(self.layer_idx, meta.seq_lens, meta.max_seq_len, meta.rows)
 
     def attention_mask(self, q_len: int) -> torch.Tensor:
         """``[B, 1, q_len, Tmax]`` valid-key mask (batched_kv_cache.py:97-102)."""
@@ -283,7 +286,7 @@ class BatchLayerKV:
         limit = torch.from_numpy(counts.copy()).to(s.device).unsqueeze(1)
         tables.masked_fill_(col >= limit, -1)
         return PagedBatchKVMetadata(s.key_cache, s.value_cache, self.layer_idx, tables, meta.seq_lens.clone(),
-                                    s.block_size)
+                                    s.block_size, s.key_scale, s.value_scale)
 
 
 class PackedBatchKVCache:
@@ -343,6 +346,9 @@ class PackedStepMeta:
         self.rows, self.starts, self.seq_lens, self.offsets = dev[0, :b], dev[1, :b], dev[2, :b], dev[3]
         self.starts_host = np.array(starts, dtype=np.int64)
         self.max_chunk = int(chunk_lens.max())
+        ends = self.starts_host + chunk_lens
+        self.max_seq_len = int(ends.max())
+        self.total_blocks = int((-(-ends // storage.block_size)).sum())
 
 
 class PackedBatchLayerKV:
@@ -367,17 +373,15 @@ class PackedBatchLayerKV:
 
     def append_only(self, key: torch.Tensor, value: torch.Tensor) -> PackedStepMeta:
         s, ends, meta = self._begin(key, value)
-        ops.paged_append(s.key_cache, s.value_cache, self.layer_idx, s.arena.table, meta.starts, key, value,
-                         row_ids=meta.rows, new_offsets=meta.offsets, max_new_tokens=meta.max_chunk, err=s.err)
+        s.write(self.layer_idx, meta.starts, key, value, row_ids=meta.rows, new_offsets=meta.offsets,
+                max_new_tokens=meta.max_chunk)
         s.arena.lens[self.owner.rows, self.layer_idx] = ends
         return meta
 
     def append_only_prepped(self, q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, q_norm_weight,
                             k_norm_weight, cos, sin, eps: float) -> tuple[PackedStepMeta, torch.Tensor]:
         s, ends, meta = self._begin(key, value)
-        q_out = ops.qk_norm_rope_append(q, key, value, q_norm_weight, k_norm_weight, cos, sin, eps, s.key_cache,
-                                        s.value_cache, self.layer_idx, s.arena.table, meta.starts,
-                                        row_ids=meta.rows, new_offsets=meta.offsets, max_new_tokens=meta.max_chunk,
-                                        err=s.err)
+        q_out = s.write_prepped(self.layer_idx, meta.starts, q, key, value, q_norm_weight, k_norm_weight, cos, sin, eps,
+                                row_ids=meta.rows, new_offsets=meta.offsets, max_new_tokens=meta.max_chunk)
         s.arena.lens[self.owner.rows, self.layer_idx] = ends
         return meta, q_out

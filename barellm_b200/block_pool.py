@@ -5,6 +5,10 @@ Same contract as the reference's BlockPool (src/barellm/engine/block_pool.py:9-2
 returns ``[]`` when the pool cannot satisfy the request; ``free`` returns blocks
 to the top of the stack.  Keeping that order keeps block tables identical to
 the reference's for the same sequence of calls.
+
+Blocks may have several holders (requests forked from one another): ``share``
+adds one, and ``free`` returns a block to the stack when its last holder frees
+it.
 """
 
 from __future__ import annotations
@@ -22,6 +26,7 @@ class BlockPool:
         self.blocks = [KVCacheBlock(i) for i in range(max_blocks)]
         # stack of free ids; the top of the stack is the end of the list
         self.free_ids: list[int] = list(range(max_blocks))
+        self.extra_holders: dict[int, int] = {}  # block id -> holders beyond the first
 
     @property
     def num_free(self) -> int:
@@ -39,5 +44,20 @@ class BlockPool:
         del self.free_ids[-num_blocks:]
         return [self.blocks[i] for i in reversed(taken)]
 
+    def share(self, blocks: list[KVCacheBlock]) -> None:
+        """Adds a holder to each block; ``free`` has to be called once more for it."""
+        for b in blocks:
+            self.extra_holders[b.block_id] = self.extra_holders.get(b.block_id, 0) + 1
+
     def free(self, blocks: list[KVCacheBlock]) -> None:
-        self.free_ids.extend(b.block_id for b in blocks)
+        if not self.extra_holders:
+            self.free_ids.extend(b.block_id for b in blocks)
+            return
+        for b in blocks:
+            n = self.extra_holders.get(b.block_id, 0)
+            if n > 1:
+                self.extra_holders[b.block_id] = n - 1
+            elif n == 1:
+                del self.extra_holders[b.block_id]
+            else:
+                self.free_ids.append(b.block_id)

@@ -284,10 +284,11 @@ class PagedEngine:
     chunked prefill, docs/ROADMAP.md:131).  ``prefill_tokens=0`` prefills each
     request on its own through the single-request PagedLayerKV path, as the
     reference does.  Every decode step then runs all requests as one
-    BatchKVCache batch (engine.py:458-488)."""
+    BatchKVCache batch (engine.py:458-488).  ``kv_dtype=torch.float8_e4m3fn``
+    keeps the cache in 8 bits."""
 
     def __init__(self, model: Qwen3, num_blocks: int, block_size: int = 16, max_requests: int = 256,
-                 prefill_tokens: int = 8192) -> None:
+                 prefill_tokens: int = 8192, kv_dtype: torch.dtype | None = None) -> None:
         s = model.s
         dev = next(model.parameters()).device
         dtype = next(model.parameters()).dtype
@@ -295,7 +296,7 @@ class PagedEngine:
         model.fuse_projections()
         self.block_size = block_size
         self.cache = PagedKVCache(s.num_layers, num_blocks, s.num_kv_heads, block_size, s.head_dim, dtype=dtype,
-                                  device=dev, max_requests=max_requests)
+                                  device=dev, max_requests=max_requests, kv_dtype=kv_dtype)
         self.pool = BlockPool(num_blocks)
         self.manager = KVCacheManager(block_size, self.pool, self.cache)
         self.device = dev

@@ -696,7 +696,7 @@ def _call(fn, args: bytes, dev: int) -> None:
 
 
 def _vector_i32(t: torch.Tensor, dev: int, n: int, name: str) -> None:
-    if not (t.dtype is _I32 and t.get_device() == dev and t.shape == (n,) and (n == 1 or t.stride(0) == 1)):
+    if not (t.dtype is _I32 and t.get_device() == dev and t.shape == (n,) and t.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous int32 [{n}] tensor on cuda:{dev}")
 
 
@@ -733,7 +733,7 @@ def _fp8_layer(key_cache, value_cache, key_scale, value_scale, layer, block_tabl
     code = DTYPE_CODE.get(dtype)
     if not (dev >= 0 and len(shape) == 5 and key_cache.dtype is FP8_DTYPE and value_cache.dtype is FP8_DTYPE
             and value_cache.shape == shape and value_cache.get_device() == dev and key_cache.is_contiguous()
-            and value_cache.is_contiguous() and key_scale.shape == shape[:3] and value_scale.shape == shape[:3]
+            and value_cache.is_contiguous() and shape[:3] == key_scale.shape == value_scale.shape
             and key_scale.dtype is _F32 and value_scale.dtype is _F32 and key_scale.get_device() == dev
             and value_scale.get_device() == dev and key_scale.is_contiguous() and value_scale.is_contiguous()
             and code is not None and 0 <= layer < shape[0] and block_tables.dtype is _I32

@@ -128,6 +128,8 @@ class PagedKVMetadata:
     block_table: torch.Tensor
     seq_len: int
     block_size: int
+    key_scale: torch.Tensor | None = None  # 8-bit pools
+    value_scale: torch.Tensor | None = None
 
 
 @dataclass(frozen=True)
@@ -140,6 +142,8 @@ class PagedBatchKVMetadata:
     block_tables: torch.Tensor
     seq_lens: torch.Tensor
     block_size: int
+    key_scale: torch.Tensor | None = None  # 8-bit pools
+    value_scale: torch.Tensor | None = None
 
 
 class _RowSet:
@@ -154,7 +158,13 @@ class _RowSet:
 
 
 class PagedKVCache:
-    """Paged K/V storage for one GPU (one BlockPool shard)."""
+    """Paged K/V storage for one GPU (one BlockPool shard).
+
+    ``kv_dtype=torch.float8_e4m3fn`` stores the tokens as 8-bit codes with one
+    fp32 power-of-two scale per (layer, block, KV head) in ``key_scale`` /
+    ``value_scale`` ``[L, P, Hkv]``; ``dtype`` stays the type of the tensors that
+    go in and come out.  Half the bytes of a 16-bit cache, for twice the tokens
+    in the same memory and half the traffic of a decode step."""
 
     def __init__(
         self,
@@ -167,6 +177,7 @@ class PagedKVCache:
         device: torch.device | str = "cpu",
         *,
         max_requests: int = 64,
+        kv_dtype: torch.dtype | None = None,
     ) -> None:
         check(num_layers > 0, "num_layers must be positive")
         check(max_blocks > 0, "max_blocks must be positive")
@@ -180,9 +191,18 @@ class PagedKVCache:
         self.block_size = block_size
         self.head_dim = head_dim
         self.dtype = dtype
+        check(kv_dtype is None or kv_dtype is dtype or kv_dtype is ops.FP8_DTYPE,
+              "kv_dtype must be the cache's dtype or torch.float8_e4m3fn")
+        self.quantized = kv_dtype is ops.FP8_DTYPE
+        self.kv_dtype = ops.FP8_DTYPE if self.quantized else dtype
+        check(not self.quantized or (dtype in ops.DTYPE_CODE and head_dim <= 256 and block_size <= 65536),
+              "an 8-bit cache needs a bf16, fp16 or fp32 dtype, head_dim <= 256 and block_size <= 65536")
         shape = (num_layers, max_blocks, num_kv_heads, block_size, head_dim)
-        self.key_cache = torch.empty(shape, dtype=dtype, device=device)
+        self.key_cache = torch.empty(shape, dtype=self.kv_dtype, device=device)
         self.value_cache = torch.empty_like(self.key_cache)
+        # (a block's scale means something once the block holds a token)
+        self.key_scale = torch.ones(shape[:3], dtype=torch.float32, device=device) if self.quantized else None
+        self.value_scale = torch.ones_like(self.key_scale) if self.quantized else None
         self.device = self.key_cache.device
         self.request_pages: dict[str, _RequestPages] = {}
         self.arena = BlockTableArena(self.device, rows=max_requests, width=64, num_layers=num_layers)
@@ -209,6 +229,59 @@ class PagedKVCache:
         if code:
             self._err.zero_()
             raise RuntimeError("paged-KV kernel reported " + ops.describe_device_error(code))
+
+    # -- the kernels, by kind of pool ------------------------------------------
+    @property
+    def pools(self) -> tuple[torch.Tensor, ...]:
+        """The pool arguments of the tensor-level ops: K and V, and an 8-bit
+        pool's two scale tables."""
+        if self.quantized:
+            return self.key_cache, self.value_cache, self.key_scale, self.value_scale
+        return self.key_cache, self.value_cache
+
+    def write(self, layer_idx: int, starts: torch.Tensor, key: torch.Tensor, value: torch.Tensor, **kw) -> None:
+        """Appends tokens to one layer (``ops.paged_append`` or its 8-bit form)."""
+        fn = ops.paged_append_fp8 if self.quantized else ops.paged_append
+        fn(*self.pools, layer_idx, self.arena.table, starts, key, value, err=self.err, **kw)
+
+    def write_prepped(self, layer_idx: int, starts: torch.Tensor, q, key, value, q_norm_weight, k_norm_weight, cos, sin,
+                      eps: float, *, row_ids: torch.Tensor, new_offsets: torch.Tensor | None = None,
+                      max_new_tokens: int | None = None) -> torch.Tensor:
+        """``write`` of the QK-normalised, rotated key; returns q normalised and
+        rotated.  A 16-bit pool takes both in one kernel.  For an 8-bit pool the
+        same kernel leaves the prepared key in a scratch pool of one block per
+        row (packed: of one block), from where it is quantised into its pages."""
+        if not self.quantized:
+            return ops.qk_norm_rope_append(q, key, value, q_norm_weight, k_norm_weight, cos, sin, eps, self.key_cache,
+                                           self.value_cache, layer_idx, self.arena.table, starts, row_ids=row_ids,
+                                           new_offsets=new_offsets, max_new_tokens=max_new_tokens, err=self.err)
+        b, h, t, d = key.shape
+        batch = starts.shape[0]
+        k_prep = torch.empty((1, b, h, t, d), dtype=key.dtype, device=key.device)
+        v_copy = torch.empty_like(k_prep)
+        if new_offsets is None:
+            table = torch.arange(b, dtype=torch.int32, device=key.device).view(b, 1)
+            at = torch.zeros(b, dtype=torch.int32, device=key.device)
+        else:
+            table = torch.zeros((batch, 1), dtype=torch.int32, device=key.device)
+            at = new_offsets[:-1]
+        q_out = ops.qk_norm_rope_append(q, key, value, q_norm_weight, k_norm_weight, cos, sin, eps, k_prep, v_copy, 0, table,
+                                        at, new_offsets=new_offsets, max_new_tokens=max_new_tokens, err=self.err)
+        self.write(layer_idx, starts, k_prep[0], value, row_ids=row_ids, new_offsets=new_offsets,
+                   max_new_tokens=max_new_tokens)
+        return q_out
+
+    def gather(self, layer_idx: int, seq_lens: torch.Tensor, max_len: int,
+               row_ids: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """Dense zero-padded read in ``dtype``."""
+        if self.quantized:
+            return ops.paged_gather_fp8(*self.pools, layer_idx, self.arena.table, seq_lens, max_len, dtype=self.dtype,
+                                        row_ids=row_ids, err=self.err)
+        return ops.paged_gather(*self.pools, layer_idx, self.arena.table, seq_lens, max_len, row_ids=row_ids, err=self.err)
+
+    def copy_blocks(self, src: list[int], dst: list[int]) -> None:
+        """Copies whole blocks (every layer, K, V and scales); see ``ops.copy_blocks``."""
+        ops.copy_blocks(self.key_cache, self.value_cache, src, dst, key_scale=self.key_scale, value_scale=self.value_scale)
 
     def register_request(self, request_id: str, blocks: list[KVCacheBlock]) -> None:
         pages = self.request_pages.get(request_id)
@@ -323,8 +396,7 @@ class PagedLayerKV:
         s = self.storage
         req = self._request
         start = int(req.layer_seq_lens[self.layer_idx])
-        ops.paged_append(s.key_cache, s.value_cache, self.layer_idx, s.arena.table,
-                         _i32([start], s.device), key, value, row_ids=_i32([req.row], s.device), err=s.err)
+        s.write(self.layer_idx, _i32([start], s.device), key, value, row_ids=_i32([req.row], s.device))
         req.layer_seq_lens[self.layer_idx] = start + key.shape[2]
 
     def append_only_prepped(self, q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, q_norm_weight,
@@ -336,9 +408,8 @@ class PagedLayerKV:
         s = self.storage
         req = self._request
         start = int(req.layer_seq_lens[self.layer_idx])
-        q_out = ops.qk_norm_rope_append(q, key, value, q_norm_weight, k_norm_weight, cos, sin, eps, s.key_cache,
-                                        s.value_cache, self.layer_idx, s.arena.table, _i32([start], s.device),
-                                        row_ids=_i32([req.row], s.device), err=s.err)
+        q_out = s.write_prepped(self.layer_idx, _i32([start], s.device), q, key, value, q_norm_weight, k_norm_weight, cos,
+                                sin, eps, row_ids=_i32([req.row], s.device))
         req.layer_seq_lens[self.layer_idx] = start + key.shape[2]
         return q_out
 
@@ -346,15 +417,14 @@ class PagedLayerKV:
         check(self.seq_len > 0, "KV cache is empty")
         s = self.storage
         return PagedKVMetadata(s.key_cache, s.value_cache, self.layer_idx, self._request.block_table,
-                               self.seq_len, s.block_size)
+                               self.seq_len, s.block_size, s.key_scale, s.value_scale)
 
     def read(self) -> tuple[torch.Tensor, torch.Tensor]:
         check(self.seq_len > 0, "KV cache is empty")
         s = self.storage
         n = self.seq_len
         req = self._request
-        return ops.paged_gather(s.key_cache, s.value_cache, self.layer_idx, s.arena.table, _i32([n], s.device), n,
-                                row_ids=_i32([req.row], s.device), err=s.err)
+        return s.gather(self.layer_idx, _i32([n], s.device), n, _i32([req.row], s.device))
 
     def attention_mask(self, q_len: int) -> torch.Tensor | None:
         del q_len
