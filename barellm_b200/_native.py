@@ -307,6 +307,7 @@ class PrefillFp8Args(Structure):
         ("max_q_len", c_int64),
         ("scale", c_float),
         ("pad0", c_int32),
+        ("total_q_len", c_int64),
         ("max_seq_len", c_int64),
         ("total_blocks", c_int64),
         ("workspace", c_void_p),
@@ -422,7 +423,7 @@ def load() -> ctypes.CDLL:
     lib.bl_paged_decode_fp8_workspace_bytes.restype = c_size_t
     lib.bl_paged_decode_fp8.argtypes = [c_void_p, c_void_p]  # a packed DecodeFp8Args, or a reference to one
     lib.bl_paged_decode_fp8.restype = c_int
-    lib.bl_paged_prefill_fp8_workspace_bytes.argtypes = [c_int32] + [c_int64] * 7
+    lib.bl_paged_prefill_fp8_workspace_bytes.argtypes = [c_int32] + [c_int64] * 8
     lib.bl_paged_prefill_fp8_workspace_bytes.restype = c_size_t
     lib.bl_paged_prefill_fp8.argtypes = [c_void_p, c_void_p]  # a packed PrefillFp8Args, or a reference to one
     lib.bl_paged_prefill_fp8.restype = c_int

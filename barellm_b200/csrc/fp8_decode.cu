@@ -824,8 +824,10 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
       }
       const float r0 = sc.z * vinv, r1 = sc.w * vinv;
       if (fminf(r0, r1) >= 0.015625f) {
+        if (r0 != 1.f || r1 != 1.f) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][e] *= r0, s[1][e] *= r1;
+          for (int e = 0; e < 4; ++e) s[0][e] *= r0, s[1][e] *= r1;
+        }
         pv(0, 1.f, std::false_type());
         pv(1, 1.f, std::false_type());
       } else {

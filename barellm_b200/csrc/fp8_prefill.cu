@@ -4,7 +4,7 @@
 // src/barellm/attention/backend.py:52-61 over a dense read of the cache.
 //
 // Two ways, chosen by shape (use_tc below):
-//   expand + prefill_tc_kernel  16-bit q, head_dim 128.  The rows' pages are
+//   expand + prefill_tc_kernel  16-bit q, head_dim a multiple of 8 up to 128.  The rows' pages are
 //       dequantised once into a 16-bit paged scratch (exact in bf16: a code has
 //       four significant bits), which the tcgen05 kernel of prefill_tc.cu then
 //       reads.  The expansion moves 1 + 2 bytes per cached element once; a
@@ -13,7 +13,9 @@
 //       kernel would repeat the conversion for every query tile.  Block sizes
 //       other than 16 become 16-token pages on the way, and a query group
 //       that the kernel is not built for (3, 5, 16, ...) becomes several KV heads
-//       with the same contents and a group of 8, 4, 2 or 1.
+//       with the same contents and a group of 8, 4, 2 or 1.  A head_dim below
+//       128 is widened with zeros, which change neither scores nor outputs: K
+//       and V on the way, q and out through copies.
 //   fp8_prefill_simt_kernel     any element type, head_dim <= 256, block size
 //       and group: 64 queries x 64 keys a tile in fp32, pages dequantised
 //       into shared memory.
@@ -33,17 +35,19 @@ constexpr int kTCDim = 128;
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // How a call's scratch looks: 16-token pages of `heads` KV heads, each cached
-// head repeated `dup` times.
+// head repeated `dup` times; q and out widened to 128 dims where head_dim is less.
 struct Scratch {
   int64_t width, pages, heads, dup;
-  size_t table, order, k, v, total;
+  size_t table, order, k, v, q, out, total;
 };
 
-bool use_tc(int32_t dtype, int64_t d) { return (dtype == BL_BF16 || dtype == BL_F16) && d == kTCDim; }
+bool use_tc(int32_t dtype, int64_t d) {
+  return (dtype == BL_BF16 || dtype == BL_F16) && d > 0 && d <= kTCDim && d % 8 == 0;
+}
 
 // False when the scratch would not fit the tcgen05 kernel's 32-bit row coordinates.
-bool plan_scratch(int64_t batch, int64_t hq, int64_t hkv, int64_t bs, int64_t max_seq_len, int64_t total_blocks,
-                  Scratch* w) {
+bool plan_scratch(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t bs, int64_t total_q, int64_t max_seq_len,
+                  int64_t total_blocks, Scratch* w) {
   const int64_t g = hq / hkv;
   int64_t gt = 8;
   while (g % gt) gt /= 2;
@@ -61,7 +65,10 @@ bool plan_scratch(int64_t batch, int64_t hq, int64_t hkv, int64_t bs, int64_t ma
   w->order = table_bytes;
   w->k = off;
   w->v = off + half;
-  w->total = off + 2 * half;
+  const size_t wide = d < kTCDim ? align256((size_t)total_q * hq * kTCDim * 2) : 0;
+  w->q = off + 2 * half;
+  w->out = w->q + wide;
+  w->total = w->out + wide;
   return true;
 }
 
@@ -81,7 +88,7 @@ struct ExpandArgs {
   const int32_t* q_offsets;
   int64_t max_q, o_sb, o_st, o_sh;
   void* out;
-  int32_t hkv, bs, dup, hq;
+  int32_t hkv, bs, d, dup, hq;
   int32_t* err;
 };
 
@@ -144,7 +151,8 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(const Expand
       continue;
     }
     const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + h;
-    const int64_t src = (slot * a.bs + (t - lb * a.bs)) * kTCDim + v * 8;
+    if (v * 8 >= a.d) continue;  // (dims that head_dim does not have are zeros)
+    const int64_t src = (slot * a.bs + (t - lb * a.bs)) * a.d + v * 8;
     kc[p] = *reinterpret_cast<const uint2*>(a.k_pool + src);
     vc[p] = *reinterpret_cast<const uint2*>(a.v_pool + src);
     ks[p] = a.k_scale[slot];
@@ -196,6 +204,52 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(const Expand
       *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.v_out) + dst) = vo.u;
     }
   }
+}
+
+// q rows of head_dim d widened to 128 dims with zeros (IN), or the widened out
+// rows cut back to d.  One warp per (token, head) row, four dims a lane.  Tokens:
+// packed on one axis, or [batch, max_q].
+struct WidenArgs {
+  void* narrow;
+  void* wide;  // [total, hq, 128]
+  int64_t sb, st, sh;
+  const int32_t* offsets;  // packed: tokens [offsets[0], offsets[batch]) belong to rows
+  int64_t batch, max_q, total;
+  int32_t hq, d;
+};
+
+template <typename T, bool IN>
+__global__ void __launch_bounds__(256) fp8_widen_kernel(const WidenArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t n = r / a.hq;
+  if (n >= a.total) return;
+  const int h = (int)(r - n * a.hq);
+  int64_t b = 0, t = n;
+  if (a.offsets) {
+    if (n < a.offsets[0] || n >= a.offsets[a.batch]) return;
+  } else {
+    b = n / a.max_q;
+    t = n - b * a.max_q;
+  }
+  T* x = reinterpret_cast<T*>(a.narrow) + b * a.sb + t * a.st + (int64_t)h * a.sh;
+  T* y = reinterpret_cast<T*>(a.wide) + r * kTCDim + 4 * lane;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int d = 4 * lane + e;
+    if (IN)
+      y[e] = d < a.d ? x[d] : from_f32<T>(0.f);
+    else if (d < a.d)
+      x[d] = y[e];
+  }
+}
+
+template <typename T, bool IN>
+int launch_widen(const WidenArgs& k, cudaStream_t s) {
+  const int64_t rows = k.total * k.hq;
+  fp8_widen_kernel<T, IN><<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(k);
+  BL_CHECK_LAUNCH("fp8_widen_kernel");
+  return BL_OK;
 }
 
 // ---------------------------------------------------------------------------
@@ -472,6 +526,31 @@ template <typename T>
 int launch_tc(const bl_prefill_fp8_args& a, const Scratch& w, cudaStream_t s) {
   const bl_paged_layer& kv = a.layer.kv;
   char* ws = (char*)a.workspace;
+  // the attention kernel's q and out: the caller's, or widened copies
+  const bool wide = kv.head_dim < kTCDim;
+  const void* q = a.q;
+  void* out = a.out;
+  int64_t q_sb = a.q_stride_b, q_st = a.q_stride_t, q_sh = a.q_stride_h;
+  int64_t o_sb = a.out_stride_b, o_st = a.out_stride_t, o_sh = a.out_stride_h;
+  WidenArgs x;
+  if (wide) {
+    x.offsets = a.q_offsets;
+    x.batch = a.batch;
+    x.max_q = a.max_q_len;
+    x.total = a.total_q_len;
+    x.hq = (int32_t)a.num_q_heads;
+    x.d = (int32_t)kv.head_dim;
+    x.narrow = const_cast<void*>(a.q);
+    x.wide = ws + w.q;
+    x.sb = q_sb, x.st = q_st, x.sh = q_sh;
+    const int rc = launch_widen<T, true>(x, s);
+    if (rc) return rc;
+    q = ws + w.q;
+    out = ws + w.out;
+    q_sh = o_sh = kTCDim;
+    q_st = o_st = a.num_q_heads * kTCDim;
+    q_sb = o_sb = a.q_offsets ? 0 : a.max_q_len * q_st;
+  }
   ExpandArgs e;
   e.k_pool = (const uint8_t*)kv.k_pool;
   e.v_pool = (const uint8_t*)kv.v_pool;
@@ -492,10 +571,11 @@ int launch_tc(const bl_prefill_fp8_args& a, const Scratch& w, cudaStream_t s) {
   e.seq_lens = a.seq_lens;
   e.q_offsets = a.q_offsets;
   e.max_q = a.max_q_len;
-  e.out = a.out;
-  e.o_sb = a.out_stride_b, e.o_st = a.out_stride_t, e.o_sh = a.out_stride_h;
+  e.out = out;
+  e.o_sb = o_sb, e.o_st = o_st, e.o_sh = o_sh;
   e.hkv = (int32_t)kv.num_kv_heads;
   e.bs = (int32_t)kv.block_size;
+  e.d = (int32_t)kv.head_dim;
   e.dup = (int32_t)w.dup;
   e.hq = (int32_t)a.num_q_heads;
   e.err = a.err;
@@ -518,10 +598,10 @@ int launch_tc(const bl_prefill_fp8_args& a, const Scratch& w, cudaStream_t s) {
   p.kv.bt_stride = w.width;
   p.kv.bt_width = w.width;
   p.kv.row_ids = nullptr;
-  p.q = a.q;
-  p.q_stride_b = a.q_stride_b, p.q_stride_t = a.q_stride_t, p.q_stride_h = a.q_stride_h;
-  p.out = a.out;
-  p.out_stride_b = a.out_stride_b, p.out_stride_t = a.out_stride_t, p.out_stride_h = a.out_stride_h;
+  p.q = q;
+  p.q_stride_b = q_sb, p.q_stride_t = q_st, p.q_stride_h = q_sh;
+  p.out = out;
+  p.out_stride_b = o_sb, p.out_stride_t = o_st, p.out_stride_h = o_sh;
   p.q_offsets = a.q_offsets;
   p.seq_lens = a.seq_lens;
   p.batch = a.batch;
@@ -529,11 +609,18 @@ int launch_tc(const bl_prefill_fp8_args& a, const Scratch& w, cudaStream_t s) {
   p.max_q_len = a.max_q_len;
   p.scale = a.scale;
   p.err = a.err;
-  return prefill_tc_launch(p, s, e.order);
+  const int rc = prefill_tc_launch(p, s, e.order);
+  if (rc || !wide) return rc;
+  x.narrow = a.out;
+  x.wide = out;
+  x.sb = a.out_stride_b, x.st = a.out_stride_t, x.sh = a.out_stride_h;
+  return launch_widen<T, false>(x, s);
 }
 
-// Strides and pointers that the tcgen05 kernel reads pairs of elements through.
+// Strides and pointers that the tcgen05 kernel reads pairs of elements through
+// (widened copies have them by themselves).
 bool tc_alignment(const bl_prefill_fp8_args& a) {
+  if (a.layer.kv.head_dim < kTCDim) return true;
   return ((uintptr_t)a.q & 3) == 0 && ((uintptr_t)a.out & 3) == 0 && a.q_stride_b % 2 == 0 && a.q_stride_t % 2 == 0 &&
          a.q_stride_h % 2 == 0 && a.out_stride_b % 2 == 0 && a.out_stride_t % 2 == 0 && a.out_stride_h % 2 == 0;
 }
@@ -545,12 +632,14 @@ using namespace bl;
 
 extern "C" size_t bl_paged_prefill_fp8_workspace_bytes(int32_t dtype, int64_t batch, int64_t num_q_heads,
                                                        int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
-                                                       int64_t max_seq_len, int64_t total_blocks) {
-  if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || block_size <= 0 ||
+                                                       int64_t total_q_len, int64_t max_seq_len, int64_t total_blocks) {
+  if (batch <= 0 || total_q_len <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || block_size <= 0 ||
       max_seq_len <= 0 || total_blocks <= 0 || !use_tc(dtype, head_dim))
     return 0;
   Scratch w;
-  return plan_scratch(batch, num_q_heads, num_kv_heads, block_size, max_seq_len, total_blocks, &w) ? w.total : 0;
+  return plan_scratch(batch, num_q_heads, num_kv_heads, head_dim, block_size, total_q_len, max_seq_len, total_blocks, &w)
+             ? w.total
+             : 0;
 }
 
 extern "C" int bl_paged_prefill_fp8(const bl_prefill_fp8_args* args, void* stream) {
@@ -567,13 +656,16 @@ extern "C" int bl_paged_prefill_fp8(const bl_prefill_fp8_args* args, void* strea
   BL_CHECK_ARG(a.max_q_len > 0 && a.max_q_len <= INT32_MAX, "K/V sequence length must be greater than zero");
   BL_CHECK_ARG(a.max_seq_len > 0 && a.max_seq_len <= INT32_MAX, "%s: max_seq_len must be in [1, 2^31)", who);
   BL_CHECK_ARG(a.total_blocks > 0, "%s: total_blocks must be positive", who);
+  BL_CHECK_ARG(a.total_q_len >= (a.q_offsets ? 1 : a.batch * a.max_q_len) && a.total_q_len <= INT32_MAX,
+               "%s: total_q_len does not cover the queries", who);
   const int es = elem_size(kv.dtype);
   BL_CHECK_ARG(((uintptr_t)a.q % es) == 0 && ((uintptr_t)a.out % es) == 0,
                "%s: q/out must be aligned to their element type", who);
   cudaStream_t s = (cudaStream_t)stream;
   Scratch w;
   if (use_tc(kv.dtype, kv.head_dim) && tc_alignment(a) &&
-      plan_scratch(a.batch, a.num_q_heads, kv.num_kv_heads, kv.block_size, a.max_seq_len, a.total_blocks, &w)) {
+      plan_scratch(a.batch, a.num_q_heads, kv.num_kv_heads, kv.head_dim, kv.block_size, a.total_q_len, a.max_seq_len,
+                   a.total_blocks, &w)) {
     if (!a.workspace || a.workspace_bytes < w.total) {
       set_error("%s: workspace too small (%zu < %zu bytes)", who, a.workspace ? a.workspace_bytes : (size_t)0, w.total);
       return BL_ERR_CAPACITY;

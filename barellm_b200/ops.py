@@ -946,9 +946,9 @@ def paged_decode_fp8(
 
 @functools.lru_cache(maxsize=256)
 def prefill_fp8_workspace_bytes(dtype: torch.dtype, batch: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
-                                block_size: int, max_seq_len: int, total_blocks: int) -> int:
+                                block_size: int, total_q_len: int, max_seq_len: int, total_blocks: int) -> int:
     return int(nat.load().bl_paged_prefill_fp8_workspace_bytes(DTYPE_CODE[dtype], batch, num_q_heads, num_kv_heads, head_dim,
-                                                               block_size, max_seq_len, total_blocks))
+                                                               block_size, total_q_len, max_seq_len, total_blocks))
 
 
 def paged_prefill_fp8(
@@ -1013,10 +1013,10 @@ def paged_prefill_fp8(
     ost = out.stride()
     _check(out.shape == qs and (ost[3] == 1 or d == 1) and out.dtype is dtype and out.get_device() == dev,
            "prefill output must match q's shape, D contiguous")
-    ws = _scratch(ws, prefill_fp8_workspace_bytes(dtype, batch, hq, hkv, d, bs, max_seq_len, total_blocks), q)
+    ws = _scratch(ws, prefill_fp8_workspace_bytes(dtype, batch, hq, hkv, d, bs, b0 * t, max_seq_len, total_blocks), q)
     a = nat.pack_prefill_fp8_args(*fields, q.data_ptr(), 0 if packed else qst[0], qst[2], qst[1], out.data_ptr(),
                                   0 if packed else ost[0], ost[2], ost[1], q_offsets.data_ptr() if packed else 0,
-                                  seq_lens.data_ptr(), batch, hq, mq, _softmax_scale(scale, d), 0, max_seq_len, total_blocks,
+                                  seq_lens.data_ptr(), batch, hq, mq, _softmax_scale(scale, d), 0, b0 * t, max_seq_len, total_blocks,
                                   ws.data_ptr(), ws.nbytes, _err_word(err, dev))
     _call(nat.load().bl_paged_prefill_fp8, a, dev)
     return out

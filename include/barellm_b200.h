@@ -472,8 +472,11 @@ BL_API int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream);
 /* of a row with C queries sees keys 0 .. seq_len - C + i.  Queries of a row  */
 /* that see no key get zeros.                                                */
 /* max_seq_len and total_blocks are host upper bounds on seq_lens[] and on   */
-/* the sum over the rows of ceil(seq_len / block_size); they size the        */
-/* workspace (0 bytes where the call needs none).                            */
+/* the sum over the rows of ceil(seq_len / block_size); total_q_len is the   */
+/* number of query tokens that q and out have room for (packed: the token    */
+/* axis; else batch * max_q_len).  They size the workspace (0 bytes where    */
+/* the call needs none).  Tokens of a packed q that no row has are left as   */
+/* they were in out.                                                         */
 typedef struct bl_prefill_fp8_args {
   bl_fp8_layer layer;
   const void* q;
@@ -491,6 +494,7 @@ typedef struct bl_prefill_fp8_args {
   int64_t max_q_len;
   float scale;
   int32_t pad0;
+  int64_t total_q_len;
   int64_t max_seq_len;
   int64_t total_blocks;
   void* workspace; /* device scratch, >= bl_paged_prefill_fp8_workspace_bytes, 256-byte aligned */
@@ -500,7 +504,7 @@ typedef struct bl_prefill_fp8_args {
 
 BL_API size_t bl_paged_prefill_fp8_workspace_bytes(int32_t dtype, int64_t batch, int64_t num_q_heads,
                                                    int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
-                                                   int64_t max_seq_len, int64_t total_blocks);
+                                                   int64_t total_q_len, int64_t max_seq_len, int64_t total_blocks);
 BL_API int bl_paged_prefill_fp8(const bl_prefill_fp8_args* args, void* stream);
 
 /* ------------------------------------------------------------------------ */

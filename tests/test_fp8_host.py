@@ -65,7 +65,7 @@ def entry_points(layer):
     dec = nat.DecodeFp8Args(layer=layer, q=4096, out=4096, seq_lens=4096, batch=1, num_q_heads=4, scale=1.0, max_seq_len=16,
                             workspace=4096, workspace_bytes=1 << 30)
     pre = nat.PrefillFp8Args(layer=layer, q=4096, out=4096, seq_lens=4096, batch=1, num_q_heads=4, max_q_len=2, scale=1.0,
-                             max_seq_len=16, total_blocks=1, workspace=4096, workspace_bytes=1 << 30)
+                             total_q_len=2, max_seq_len=16, total_blocks=1, workspace=4096, workspace_bytes=1 << 30)
     return {"bl_paged_append_fp8": app, "bl_paged_gather_fp8": gat, "bl_paged_decode_fp8": dec, "bl_paged_prefill_fp8": pre}
 
 
@@ -92,6 +92,7 @@ def test_bad_layers_are_refused(native_lib, change, rc, text):
     ("bl_paged_decode_fp8", dict(q=4097), nat.BL_ERR_ARG),
     ("bl_paged_prefill_fp8", dict(max_q_len=0), nat.BL_ERR_ARG),
     ("bl_paged_prefill_fp8", dict(total_blocks=0), nat.BL_ERR_ARG),
+    ("bl_paged_prefill_fp8", dict(total_q_len=1), nat.BL_ERR_ARG),
     ("bl_paged_prefill_fp8", dict(workspace_bytes=100), nat.BL_ERR_CAPACITY),
     ("bl_paged_prefill_fp8", dict(num_q_heads=5), nat.BL_ERR_ARG),
 ])
@@ -157,11 +158,14 @@ def test_workspace_sizes(native_lib):
     assert ops.decode_fp8_workspace_bytes(64, 16, 128, 513) >= 64 * 2 * 16 * 129 * 4
     assert ops.decode_fp8_workspace_bytes(0, 16, 128, 512) == 0
     f = native_lib.bl_paged_prefill_fp8_workspace_bytes
-    one = f(nat.BL_BF16, 4, 16, 8, 128, 16, 1000, 40)
+    one = f(nat.BL_BF16, 4, 16, 8, 128, 16, 500, 1000, 40)
     assert one >= 2 * 40 * 8 * 16 * 128 * 2
-    assert f(nat.BL_BF16, 4, 24, 8, 128, 16, 1000, 40) > 2 * one  # group 3: every KV head three times
-    assert f(nat.BL_F32, 4, 16, 8, 128, 16, 1000, 40) == 0
-    assert f(nat.BL_BF16, 4, 16, 8, 64, 16, 1000, 40) == 0
+    assert f(nat.BL_BF16, 4, 24, 8, 128, 16, 500, 1000, 40) > 2 * one  # group 3: every KV head three times
+    # narrower heads: q and out widened to 128 dims as well
+    assert f(nat.BL_BF16, 4, 16, 8, 64, 16, 500, 1000, 40) >= one + 2 * 500 * 16 * 128 * 2
+    assert f(nat.BL_F32, 4, 16, 8, 128, 16, 500, 1000, 40) == 0
+    assert f(nat.BL_BF16, 4, 16, 8, 256, 16, 500, 1000, 40) == 0
+    assert f(nat.BL_BF16, 4, 16, 8, 12, 16, 500, 1000, 40) == 0
 
 
 def test_cpu_tensors_are_refused():

@@ -227,7 +227,20 @@ def test_prefill(cuda, native_lib, dtype, hq, hkv, bs, d):
     out = ops.paged_prefill_fp8(q, *pool.args, 1, bt, i32(lens, cuda), max(lens), total_blocks=total, q_offsets=off,
                                 max_q_len=max(chunks), err=err)
     assert int(err) == 0
-    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32 and d == 128)
+    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32)
+
+
+@pytest.mark.parametrize("d", [128, 80])
+def test_prefill_leaves_tokens_of_no_row(cuda, native_lib, d):
+    """A packed q with room behind its last row: those outputs stay as they were; narrow, strided q and out."""
+    chunks, lens = [5, 20], [30, 20]
+    pool, table, bt = filled(cuda, lens, 2, 16, d, BF16)
+    q = torch.randn(1, 40, 8, d + 4, device=cuda).to(BF16)[..., :d].transpose(1, 2)
+    out = torch.full((1, 40, 8, d + 4), 3.0, dtype=BF16, device=cuda)
+    view = out[..., :d].transpose(1, 2)
+    ops.paged_prefill_fp8(q, *pool.args, 1, bt, i32(lens, cuda), 30, q_offsets=i32([0, 5, 25], cuda), max_q_len=20, out=view)
+    check_prefill(view[:, :, :25], q[:, :, :25], pool, table, lens, chunks, 1)
+    assert bool((out[:, 25:] == 3).all()) and bool((out[..., d:] == 3).all())
 
 
 @pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64), (F32, 128)])
@@ -239,7 +252,7 @@ def test_prefill_queries_that_see_no_key(cuda, native_lib, dtype, d):
     off = i32(np.concatenate([[0], np.cumsum(chunks)]), cuda)
     out = torch.full_like(q, 5.0)
     ops.paged_prefill_fp8(q, *pool.args, 1, bt, i32(lens, cuda), 13, q_offsets=off, max_q_len=300, out=out)
-    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32 and d == 128)
+    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32)
     assert bool((out[0, :, :27] == 0).all()) and bool((out[0, :, 40:47] == 0).all())
 
 
@@ -330,6 +343,7 @@ def test_refusals(cuda, native_lib):
     pre = lambda **kw: ops.paged_prefill_fp8(kw.pop("q", q.unsqueeze(2)), *pool.args, 1, bt, seq, kw.pop("n", 40), **kw)
     pre()
     bad(lambda: pre(n=0))
+    bad(lambda: pre(ws=torch.empty(64, dtype=torch.uint8, device=cuda)))
     bad(lambda: pre(total_blocks=0))
     bad(lambda: pre(q=q))
     bad(lambda: pre(scale=-1.0))
