@@ -955,51 +955,109 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
 // SIMT kernel: any element type, head_dim <= 256, any block size
 // ---------------------------------------------------------------------------
 constexpr int kSimtThreads = 256;
-constexpr int kSimtTokens = 32;  // tokens per tile: one per lane in the score phase
+constexpr int kSimtMaxTokens = 128;
+constexpr int kSimtWords = 16;  // four-code words a thread holds of a tile
 
-struct SimtShared {
-  int64_t row[kSimtTokens];  // byte offset of the token's codes, -1: none
-  float ks[kSimtTokens], vs[kSimtTokens];
-  float p[8][kSimtTokens];
+// tokens of a tile: what 256 threads hold in kSimtWords words each
+__host__ __device__ constexpr int simt_tokens(int d) { return d <= 128 ? 128 : 64; }
+// floats between a tile's rows: whole 16-byte vectors, an odd number of them, so
+// that 32 lanes reading a vector of a row each meet no bank twice
+__host__ __device__ constexpr int simt_stride(int d) { return ((d + 3) / 4 | 1) * 4; }
+
+struct alignas(16) SimtShared {  // float4 arrays follow
+  int64_t row[2][kSimtMaxTokens];  // byte offset of the token's codes, -1: none; this tile and the next
+  float ks[2][kSimtMaxTokens], vs[2][kSimtMaxTokens];
+  float p[kSimtMaxTokens][8];  // scores, then weights, of the eight heads
   float alpha[8], l[8], m[8];
 };
 
-// Eight warps: in the score phase warp w owns query head w and lane i token i;
-// in the P V phase a thread owns one dim of every (256 / Dp)-th head.
+// A tile's K becomes fp32 in shared memory, a warp scores 32 tokens with one head
+// (a lane each), warp h takes head h's softmax, then the tile's V replaces K and
+// a thread owns one dim of every head over a share of the tokens.  The next
+// codes are on their way from HBM meanwhile, in registers.
 template <typename T>
-__global__ void __launch_bounds__(kSimtThreads) fp8_decode_simt_kernel(const Args a) {
+__global__ void __launch_bounds__(kSimtThreads, 2) fp8_decode_simt_kernel(const Args a) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   SimtShared* sh = reinterpret_cast<SimtShared*>(smem_raw);
-  const int dp1 = a.d + 1;
-  float* qs = reinterpret_cast<float*>(smem_raw + sizeof(SimtShared));  // [8][d]
-  float* tile = qs + 8 * a.d;                                          // [32][d + 1]
+  const int ts = simt_stride(a.d), ntok = simt_tokens(a.d), dq = (a.d + 3) / 4 * 4;
+  float* qs = reinterpret_cast<float*>(smem_raw + sizeof(SimtShared));  // [8][dq], zeros behind head_dim
+  float* tile = qs + 8 * dq;                                           // [ntok][ts]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int dp = 32;
   while (dp < a.d) dp *= 2;
-  const int vd = tid % dp, vh0 = tid / dp, vstep = kSimtThreads / dp;
+  const int vd = tid % dp, vgroup = tid / dp, vgroups = kSimtThreads / dp;
+  // words of a token: thread tid has word `col` of tokens row0, row0 + step, ...
+  const bool words = (a.d & 3) == 0;
+  int wsh = 0;
+  while ((4 << wsh) < a.d) ++wsh;
+  const int col = tid & ((1 << wsh) - 1), row0 = tid >> wsh, step = kSimtThreads >> wsh;
+  const bool has_col = 4 * col < a.d;
 
   pdl_wait();
   const int64_t items = (int64_t)plan_units(a, tid == 0) * a.hkv * a.head_tiles;
   zero_empty_rows<T>(a, kSimtThreads);
 
-  auto load_tile = [&](const uint8_t* pool, const float* sc) {
-    const bool words = (a.d & 3) == 0;
-    const int per = words ? a.d / 4 : a.d;
-    for (int e = tid; e < kSimtTokens * per; e += kSimtThreads) {
-      const int t = e / per, c = e - t * per;
-      const int64_t r = sh->row[t];
-      if (words) {
-        float2 x = make_float2(0.f, 0.f), y = x;
-        if (r >= 0) {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(pool + r + 4 * c);
-          x = e4m3x2_to_float2((uint16_t)w), y = e4m3x2_to_float2((uint16_t)(w >> 16));
-        }
-        const float s = r >= 0 ? sc[t] : 0.f;
-        float* p = tile + t * dp1 + 4 * c;
-        p[0] = x.x * s, p[1] = x.y * s, p[2] = y.x * s, p[3] = y.y * s;
+  // where the tokens [t0, t0 + ntok) of the item are
+  auto locate = [&](const Item& it, int t0, int buf) {
+    if (tid >= ntok) return;
+    const int t = t0 + tid;
+    int64_t r = -1;
+    if (t < it.t1) {
+      const int lb = t / a.bs;
+      const int64_t phys = a.block_tables[(int64_t)it.table_row * a.bt_stride + lb];
+      if (phys < 0 || phys >= a.num_blocks) {
+        raise_dev(a.err, BL_DEVERR_BLOCK_ID);
       } else {
-        tile[t * dp1 + c] = r >= 0 ? e4m3_to_float(pool[r + c]) * sc[t] : 0.f;
+        const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + it.h;
+        r = (slot * a.bs + (t - lb * a.bs)) * a.d;
+        sh->ks[buf][tid] = a.k_scale[slot];
+        sh->vs[buf][tid] = a.v_scale[slot];
       }
+    }
+    sh->row[buf][tid] = r;
+  };
+  auto fetch = [&](const uint8_t* pool, int buf, uint32_t (&w)[kSimtWords]) {
+    if (!words) return;
+#pragma unroll
+    for (int i = 0; i < kSimtWords; ++i) {
+      const int t = row0 + i * step;
+      w[i] = 0;
+      if (t < ntok && has_col) {
+        const int64_t r = sh->row[buf][t];
+        if (r >= 0) w[i] = *reinterpret_cast<const uint32_t*>(pool + r + 4 * col);
+      }
+    }
+  };
+  auto expand = [&](const uint8_t* pool, const float* sc, int buf, const uint32_t (&w)[kSimtWords]) {
+    if (words) {
+#pragma unroll
+      for (int i = 0; i < kSimtWords; ++i) {
+        const int t = row0 + i * step;
+        if (t < ntok && has_col) {
+          const float s = sh->row[buf][t] >= 0 ? sc[t] : 0.f;
+          const float2 x = e4m3x2_to_float2((uint16_t)w[i]), y = e4m3x2_to_float2((uint16_t)(w[i] >> 16));
+          *reinterpret_cast<float4*>(tile + t * ts + 4 * col) = make_float4(x.x * s, x.y * s, y.x * s, y.y * s);
+        }
+      }
+    } else {
+      for (int e = tid; e < ntok * dq; e += kSimtThreads) {
+        const int t = e / dq, c = e - t * dq;
+        const int64_t r = sh->row[buf][t];
+        tile[t * ts + c] = r >= 0 && c < a.d ? e4m3_to_float(pool[r + c]) * sc[t] : 0.f;
+      }
+    }
+  };
+  // acc = acc * alpha + sum over this thread's tokens of p[t][h] * V[t][vd], heads [0, N)
+  float acc[8];
+  auto add_values = [&](auto n) {
+    constexpr int N = decltype(n)::value;
+#pragma unroll
+    for (int h = 0; h < N; ++h) acc[h] *= sh->alpha[h];
+#pragma unroll 8
+    for (int t = vgroup; t < ntok; t += vgroups) {
+      const float v = tile[t * ts + vd];
+#pragma unroll
+      for (int h = 0; h < N; ++h) acc[h] = fmaf(sh->p[t][h], v, acc[h]);
     }
   };
 
@@ -1010,99 +1068,112 @@ __global__ void __launch_bounds__(kSimtThreads) fp8_decode_simt_kernel(const Arg
       continue;
     }
     __syncthreads();  // the previous item's shared state is no longer read
-    for (int e = tid; e < it.heads * a.d; e += kSimtThreads) {
-      const int h = e / a.d;
-      qs[e] = to_f32<T>(reinterpret_cast<const T*>(a.q)[(int64_t)it.b * a.q_sb + (int64_t)(it.hq0 + h) * a.q_sh + (e - h * a.d)]) *
-              a.scale_log2;
+    for (int e = tid; e < it.heads * dq; e += kSimtThreads) {
+      const int h = e / dq, d = e - h * dq;
+      qs[e] = d < a.d ? to_f32<T>(reinterpret_cast<const T*>(a.q)[(int64_t)it.b * a.q_sb + (int64_t)(it.hq0 + h) * a.q_sh + d]) *
+                            a.scale_log2
+                      : 0.f;
     }
-    float m = -INFINITY, l = 0.f;  // warp w: head w
-    float acc[8];
+    float m = -INFINITY, l = 0.f;  // warp h: head h
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[k] = 0.f;
-    const int64_t row = it.table_row;
-    for (int t0 = it.t0; t0 < it.t1; t0 += kSimtTokens) {
-      __syncthreads();  // the previous tile is no longer read; qs is complete
-      if (tid < kSimtTokens) {
-        const int t = t0 + tid;
-        int64_t r = -1;
-        if (t < it.t1) {
-          const int lb = t / a.bs;
-          const int64_t phys = a.block_tables[row * a.bt_stride + lb];
-          if (phys < 0 || phys >= a.num_blocks) {
-            raise_dev(a.err, BL_DEVERR_BLOCK_ID);
-          } else {
-            const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + it.h;
-            r = (slot * a.bs + (t - lb * a.bs)) * a.d;
-            sh->ks[tid] = a.k_scale[slot];
-            sh->vs[tid] = a.v_scale[slot];
-          }
+    // (heads that the item does not have are weighted too, up to the next power of two: with zeros)
+    if (tid < 8) sh->alpha[tid] = 0.f;
+    for (int e = tid; e < kSimtMaxTokens * 8; e += kSimtThreads) (&sh->p[0][0])[e] = 0.f;
+    uint32_t kw[kSimtWords], vw[kSimtWords];
+    locate(it, it.t0, 0);
+    __syncthreads();
+    fetch(a.k_pool, 0, kw);
+    int buf = 0;
+    for (int t0 = it.t0; t0 < it.t1; t0 += ntok, buf ^= 1) {
+      const bool more = t0 + ntok < it.t1;
+      expand(a.k_pool, sh->ks[buf], buf, kw);
+      fetch(a.v_pool, buf, vw);
+      if (more) locate(it, t0 + ntok, buf ^ 1);
+      __syncthreads();
+      for (int u = warp; u < it.heads * (ntok / 32); u += kSimtThreads / 32) {
+        const int h = u / (ntok / 32), t = (u - h * (ntok / 32)) * 32 + lane;
+        const float4* qh = reinterpret_cast<const float4*>(qs + h * dq);
+        const float4* kt = reinterpret_cast<const float4*>(tile + t * ts);
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll 4
+        for (int d = 0; d < dq / 4; ++d) {
+          const float4 x = qh[d], y = kt[d];
+          s0 = fmaf(x.x, y.x, s0), s1 = fmaf(x.y, y.y, s1), s2 = fmaf(x.z, y.z, s2), s3 = fmaf(x.w, y.w, s3);
         }
-        sh->row[tid] = r;
+        sh->p[t][h] = sh->row[buf][t] < 0 ? -INFINITY : (s0 + s1) + (s2 + s3);
       }
       __syncthreads();
-      load_tile(a.k_pool, sh->ks);
-      __syncthreads();
       if (warp < it.heads) {
-        const float* qh = qs + warp * a.d;
-        const float* kt = tile + lane * dp1;
-        float s = 0.f;
-        for (int d = 0; d < a.d; ++d) s = fmaf(qh[d], kt[d], s);
-        if (sh->row[lane] < 0) s = -INFINITY;
-        float mx = s;
+        float s[kSimtMaxTokens / 32], mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kSimtMaxTokens / 32; ++i)
+          if (i < ntok / 32) mx = fmaxf(mx, s[i] = sh->p[lane + 32 * i][warp]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float mn = fmaxf(m, mx);
+        const float mn = fmaxf(m, mx), u = mn == -INFINITY ? 0.f : mn;
         const float al = mn == m ? 1.f : fast_exp2(m - mn);
-        const float p = fast_exp2(s - (mn == -INFINITY ? 0.f : mn));
-        float ps = p;
+        float ps = 0.f;
+#pragma unroll
+        for (int i = 0; i < kSimtMaxTokens / 32; ++i)
+          if (i < ntok / 32) {
+            const float p = fast_exp2(s[i] - u);
+            ps += p;
+            sh->p[lane + 32 * i][warp] = p;
+          }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
         m = mn;
         l = l * al + ps;
-        sh->p[warp][lane] = p;
         if (lane == 0) sh->alpha[warp] = al;
       }
+      expand(a.v_pool, sh->vs[buf], buf, vw);  // (K's tile was last read before the barrier above)
       __syncthreads();
-      load_tile(a.v_pool, sh->vs);
-      __syncthreads();
+      if (more) fetch(a.k_pool, buf ^ 1, kw);
       if (vd < a.d) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int h = vh0 + k * vstep;
-          if (h >= it.heads) break;
-          float x = acc[k] * sh->alpha[h];
-#pragma unroll 8
-          for (int t = 0; t < kSimtTokens; ++t) x = fmaf(sh->p[h][t], tile[t * dp1 + vd], x);
-          acc[k] = x;
-        }
+        if (it.heads == 1)
+          add_values(std::integral_constant<int, 1>());
+        else if (it.heads == 2)
+          add_values(std::integral_constant<int, 2>());
+        else if (it.heads <= 4)
+          add_values(std::integral_constant<int, 4>());
+        else
+          add_values(std::integral_constant<int, 8>());
       }
+      __syncthreads();  // the tile and the weights are no longer read
     }
+    // join the threads that share a dim, and the heads' sums
     if (warp < it.heads && lane == 0) {
       sh->m[warp] = m;
       sh->l[warp] = l;
     }
-    __syncthreads();
     if (vd < a.d) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int h = vh0 + k * vstep;
-        if (h >= it.heads) break;
-        const int hq = it.hq0 + h;
-        const float L = sh->l[h], val = L == 0.f ? 0.f : acc[k] / L;  // a NaN sum stays NaN
-        if (it.nch <= 1) {
-          reinterpret_cast<T*>(a.out)[(int64_t)it.b * a.o_sb + (int64_t)hq * a.o_sh + vd] = from_f32<T>(val);
-        } else if (!has_part(a, it)) {
-          if (vd == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
-        } else {
-          a.ws_o[((int64_t)it.part * a.hq + hq) * a.d + vd] = val;
-          if (vd == 0) a.ws_lse[(int64_t)it.part * a.hq + hq] = L == 0.f ? -INFINITY : sh->m[h] + __log2f(L);
-        }
+      for (int h = 0; h < 8; ++h)
+        if (h < it.heads) tile[(vgroup * 8 + h) * a.d + vd] = acc[h];
+    }
+    __syncthreads();
+    for (int e = tid; e < it.heads * a.d; e += kSimtThreads) {
+      const int h = e / a.d, d = e - h * a.d, hq = it.hq0 + h;
+      float x = 0.f;
+      for (int g = 0; g < vgroups; ++g) x += tile[(g * 8 + h) * a.d + d];
+      const float L = sh->l[h], val = L == 0.f ? 0.f : x / L;  // a NaN sum stays NaN
+      if (it.nch <= 1) {
+        reinterpret_cast<T*>(a.out)[(int64_t)it.b * a.o_sb + (int64_t)hq * a.o_sh + d] = from_f32<T>(val);
+      } else if (!has_part(a, it)) {
+        if (d == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
+      } else {
+        a.ws_o[((int64_t)it.part * a.hq + hq) * a.d + d] = val;
+        if (d == 0) a.ws_lse[(int64_t)it.part * a.hq + hq] = L == 0.f ? -INFINITY : sh->m[h] + __log2f(L);
       }
     }
   }
 }
 
-size_t simt_smem(int d) { return sizeof(SimtShared) + sizeof(float) * (8 * (size_t)d + kSimtTokens * (d + 1)); }
+// (the join's [groups][8][d] sums fit the tile: groups * 8 <= tokens of a tile)
+size_t simt_smem(int d) {
+  return sizeof(SimtShared) + sizeof(float) * (8 * (size_t)((d + 3) / 4 * 4) + (size_t)simt_tokens(d) * simt_stride(d));
+}
 
 // ---------------------------------------------------------------------------
 // reduce: rows of several chunks
@@ -1243,8 +1314,10 @@ template <typename T>
 int launch_simt(const Args& k, cudaStream_t s) {
   const size_t smem = simt_smem(k.d);
   const int64_t items = (int64_t)k.max_units * k.hkv * k.head_tiles;
-  const int64_t grid = std::min<int64_t>((int64_t)num_sms() * 4, items);
-  if (launch_pdl(fp8_decode_simt_kernel<T>, dim3((unsigned)grid), dim3(kSimtThreads), smem, s, k) != cudaSuccess) {
+  const int64_t grid = std::min<int64_t>((int64_t)num_sms() * 2, items);
+  if (cudaFuncSetAttribute(fp8_decode_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+          cudaSuccess ||
+      launch_pdl(fp8_decode_simt_kernel<T>, dim3((unsigned)grid), dim3(kSimtThreads), smem, s, k) != cudaSuccess) {
     set_error("fp8_decode_simt_kernel: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
     return BL_ERR_LAUNCH;
   }

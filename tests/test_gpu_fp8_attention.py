@@ -227,7 +227,7 @@ def test_prefill(cuda, native_lib, dtype, hq, hkv, bs, d):
     out = ops.paged_prefill_fp8(q, *pool.args, 1, bt, i32(lens, cuda), max(lens), total_blocks=total, q_offsets=off,
                                 max_q_len=max(chunks), err=err)
     assert int(err) == 0
-    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32)
+    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32 and d <= 128 and d % 8 == 0)
 
 
 @pytest.mark.parametrize("d", [128, 80])
@@ -252,7 +252,7 @@ def test_prefill_queries_that_see_no_key(cuda, native_lib, dtype, d):
     off = i32(np.concatenate([[0], np.cumsum(chunks)]), cuda)
     out = torch.full_like(q, 5.0)
     ops.paged_prefill_fp8(q, *pool.args, 1, bt, i32(lens, cuda), 13, q_offsets=off, max_q_len=300, out=out)
-    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32)
+    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32 and d <= 128 and d % 8 == 0)
     assert bool((out[0, :, :27] == 0).all()) and bool((out[0, :, 40:47] == 0).all())
 
 
