@@ -53,35 +53,38 @@ __global__ void __launch_bounds__(kThreads) copy_blocks_kernel(const __grid_cons
 }
 
 // Refuses ids outside the pool, a destination named twice and a block that is
-// both source and destination.
+// both source and destination.  A few pairs are compared with one another; for
+// more, a byte per block of the pool says what was seen.
 int check_pairs(const bl_copy_blocks_args& a) {
-  uint8_t* seen = static_cast<uint8_t*>(calloc((size_t)a.num_blocks, 1));  // 1: read, 2: written
-  if (!seen) {
-    set_error("bl_copy_blocks: out of host memory");
-    return BL_ERR_CAPACITY;
-  }
-  int rc = BL_OK;
-  for (int64_t i = 0; i < a.count && rc == BL_OK; ++i) {
-    const int64_t s = a.src[i], d = a.dst[i];
-    if (s < 0 || s >= a.num_blocks || d < 0 || d >= a.num_blocks) {
-      set_error("bl_copy_blocks: block id outside the pool (pair %lld: %lld -> %lld, %lld blocks)", (long long)i,
-                (long long)s, (long long)d, (long long)a.num_blocks);
-      rc = BL_ERR_ARG;
-    } else if (seen[d] & 2) {
-      set_error("bl_copy_blocks: block %lld is written twice", (long long)d);
-      rc = BL_ERR_ARG;
-    } else {
-      seen[s] |= 1;
-      seen[d] |= 2;
+  for (int64_t i = 0; i < a.count; ++i)
+    BL_CHECK_ARG(a.src[i] >= 0 && a.src[i] < a.num_blocks && a.dst[i] >= 0 && a.dst[i] < a.num_blocks,
+                 "bl_copy_blocks: block id outside the pool (pair %lld: %lld -> %lld, %lld blocks)", (long long)i,
+                 (long long)a.src[i], (long long)a.dst[i], (long long)a.num_blocks);
+  int64_t twice = -1, both = -1;
+  if (a.count <= 32) {
+    for (int64_t i = 0; i < a.count; ++i)
+      for (int64_t j = 0; j < a.count; ++j) {
+        if (j < i && a.dst[i] == a.dst[j]) twice = a.dst[i];
+        if (a.dst[i] == a.src[j]) both = a.dst[i];
+      }
+  } else {
+    uint8_t* seen = static_cast<uint8_t*>(calloc((size_t)a.num_blocks, 1));  // 1: read, 2: written
+    if (!seen) {
+      set_error("bl_copy_blocks: out of host memory");
+      return BL_ERR_CAPACITY;
     }
-  }
-  for (int64_t i = 0; i < a.count && rc == BL_OK; ++i)
-    if (seen[a.dst[i]] & 1) {
-      set_error("bl_copy_blocks: block %lld is both read and written", (long long)a.dst[i]);
-      rc = BL_ERR_ARG;
+    for (int64_t i = 0; i < a.count; ++i) {
+      if (seen[a.dst[i]] & 2) twice = a.dst[i];
+      seen[a.src[i]] |= 1;
+      seen[a.dst[i]] |= 2;
     }
-  free(seen);
-  return rc;
+    for (int64_t i = 0; i < a.count; ++i)
+      if (seen[a.dst[i]] & 1) both = a.dst[i];
+    free(seen);
+  }
+  BL_CHECK_ARG(twice < 0, "bl_copy_blocks: block %lld is written twice", (long long)twice);
+  BL_CHECK_ARG(both < 0, "bl_copy_blocks: block %lld is both read and written", (long long)both);
+  return BL_OK;
 }
 
 }  // namespace

@@ -111,10 +111,14 @@ def test_bad_arguments_are_refused(native_lib, name, change, rc):
     ([0], [8], "outside the pool"),
     ([-1], [2], "outside the pool"),
     (list(range(8)) + [0], [0] * 9, "more pairs"),
+    (list(range(40)), list(range(50, 89)) + [50], "written twice"),  # (many pairs are checked another way)
+    (list(range(40)), list(range(50, 89)) + [7], "read and written"),
+    (list(range(40)), list(range(61, 101)), "outside the pool"),
 ])
 def test_bad_copy_pairs_are_refused(native_lib, src, dst, text):
     s, d = np.asarray(src, dtype=np.int64), np.asarray(dst, dtype=np.int64)
-    a = nat.CopyBlocksArgs(4096, 4096, None, None, 2, 8, 2, 16, 128, 2, s.ctypes.data, d.ctypes.data, len(src))
+    blocks = 8 if len(src) < 40 else 100
+    a = nat.CopyBlocksArgs(4096, 4096, None, None, 2, blocks, 2, 16, 128, 2, s.ctypes.data, d.ctypes.data, len(src))
     assert native_lib.bl_copy_blocks(ctypes.byref(a), None) == nat.BL_ERR_ARG
     assert text in nat.last_error()
 
