@@ -10,10 +10,11 @@
 //                          decreasing size.  A unit's record holds all that the
 //                          attention kernel's producer needs to start on it.
 //   fp8_decode_tc_kernel   bf16 / fp16 q, head_dim 64, 128 or 256, block_size a
-//                          multiple of 16.  Persistent CTAs walk (chunk, KV head,
-//                          8 query heads) items.  One producer warp streams 32
-//                          tokens of K and V codes a step through a TMA ring;
-//                          four consumer warps take every fourth step.
+//                          multiple of 16.  Persistent CTAs claim (chunk, KV head,
+//                          8 query heads) items.  A planner warp describes the
+//                          next item (query fragments, page rows, scales) while
+//                          four consumer warps work on one, each on every fourth
+//                          step of 32 tokens, copied by TMA into a ring of its own.
 //   fp8_decode_simt_kernel everything else (fp32 q, other head_dims and block
 //                          sizes, pools past the tensor map's 2^31 rows): the
 //                          same chunks, fp32 multiplies on dequantised tiles.
@@ -25,7 +26,19 @@
 // (its largest magnitude lands in [1, 2)), so a bf16 element keeps all its bits
 // down to 2^-16 of the head's largest and loses at most 2^-25 of that below.
 // k_scale multiplies the score in fp32.  P (<= 2^8, see below) is rounded to
-// fp16, 2^-12 relative.  V's scales are applied to the fp32 sums.
+// fp16, half a step of 2^-11 relative.  V's scales are powers of two: a tile's is
+// folded into its P relative to the tile that set the sums' unit, or applied to
+// sums of its own where it is far smaller.
+//
+// What bounds it (64 requests of 1k..32k tokens, 32 / 8 heads, head_dim 128, bf16:
+// 2.12 GB): HBM.  Plan, attention and join together 354 us, 5.98 TB/s, the
+// attention kernel alone 339 us, 6.25 TB/s (a copy on this card: 6.56).  Under a
+// load that goes on for 100 ms the card reaches its power cap and the SM
+// clock falls to 1.6 GHz; the conversions and products then take longer than
+// the copies (380..410 us; without them 343 us).  Measured and not kept: one
+// producer warp for the CTA (375 us without any arithmetic), rings of 4 steps a
+// warp or 2 CTAs per SM with larger rings (more than 96 KB in flight per SM is
+// slower), 4 CTAs of 96 registers (425 us), static rounds in place of claims (373 us).
 #include <cstddef>
 #include <cstring>
 #include <mutex>
@@ -288,10 +301,10 @@ __device__ __forceinline__ bool has_part(const Args& a, const Item& it) {
 // tensor-core kernel
 // ---------------------------------------------------------------------------
 constexpr int kNW = 4;                      // consumer warps
-constexpr int kThreadsTC = (kNW + 1) * 32;  // + the producer warp
+constexpr int kThreadsTC = (kNW + 1) * 32;  // + the planner warp
 constexpr int kStepTokens = 32;             // tokens a consumer warp takes at a time: two 16-token tiles
-constexpr int kTiles = kChunk / 16;         // 16-token tiles of a chunk, one per producer lane
-static_assert(kTiles == 32, "a producer lane holds one tile of the chunk");
+constexpr int kTiles = kChunkTiles;         // 16-token tiles of a chunk, one per planner lane
+static_assert(kTiles == 32, "a planner lane holds one tile of the chunk");
 
 template <int D>
 struct Cfg {
@@ -839,6 +852,12 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
     }
     __syncwarp();
     if (!ok) break;
+    // The slot's description is gone once every warp has arrived here: a cursor
+    // that has not passed this item (it has no step for this warp) passes it now.
+    if (at_item < n_item) {
+      at_item = n_item;
+      at_step = at_steps = 0;
+    }
     if (lane == 0) mbar_arrive(&sh->item_empty[slot_i]);
 
     // ---- merge the warps: the one with class 0 joins the others' sums to its own ----
@@ -1367,7 +1386,7 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
   BL_CHECK_ARG(a.num_q_heads > 0 && a.num_q_heads <= 65535 && a.num_q_heads % kv.num_kv_heads == 0,
                "num_heads must divide evenly by num_kv_heads");
   BL_CHECK_ARG(a.max_seq_len > 0, "KV cache is empty");
-  BL_CHECK_ARG(a.max_seq_len <= INT32_MAX, "%s: max_seq_len does not fit in int32", who);
+  BL_CHECK_ARG(a.max_seq_len <= INT32_MAX - kChunk, "%s: max_seq_len does not fit in int32", who);
   const int es = elem_size(kv.dtype);
   BL_CHECK_ARG(((uintptr_t)a.q % es) == 0 && ((uintptr_t)a.out % es) == 0,
                "%s: q/out must be aligned to their element type", who);
@@ -1420,8 +1439,8 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
   k.err = a.err;
 
   // A call whose items all fit the GPU at once needs no plan: the order and the
-  // claims that it brings would change nothing, and its launch is a fifth of
-  // such a call (one request of 777 tokens: MEASURED).
+  // claims that it brings would change nothing (one request of 777 tokens: 14.4 us
+  // on the device without it, 20.5 us with it).
   k.planned = !(use_tc(kv) && a.batch <= 32 && (int64_t)k.max_units * k.hkv * k.head_tiles <= num_sms());
   if (k.planned && !a.plan_ready) {
     PlanArgs p;

@@ -149,6 +149,24 @@ def test_decode_layouts_plan_reuse_and_batch_invariance(cuda, native_lib):
     assert torch.equal(ops.paged_decode_fp8(q, *pool.args, 1, bt, seq, 2000, ws=ws, plan_ready=True), base)
 
 
+@pytest.mark.parametrize("lens,hkv", [
+    ([1 + (b * 29) % 70 for b in range(1500)], 8),  # dozens of items a CTA, most with steps for some of its warps only
+    ([(b * b * 131) % 2100 for b in range(200)], 4),  # full chunks, partial ones of every size, empty rows
+], ids=["short", "ragged"])
+def test_decode_many_items(cuda, native_lib, lens, hkv):
+    pool, table, bt = filled(cuda, lens, hkv, 16, 128, BF16, layers=1, layer=0)
+    q = torch.randn(len(lens), 2 * hkv, 128, generator=torch.Generator().manual_seed(0)).to(BF16).to(cuda)
+    seq, err = i32(lens, cuda), torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = ops.paged_decode_fp8(q, *pool.args, 0, bt, seq, max(lens), err=err)
+    assert int(err) == 0
+    pick = list(range(0, len(lens), 23))
+    check_decode(out[pick], q[pick], pool, table[pick], [lens[i] for i in pick], 0)
+    # which CTA takes which item does not change a bit
+    for _ in range(10):
+        assert torch.equal(ops.paged_decode_fp8(q, *pool.args, 0, bt, seq, max(lens), err=err), out)
+    assert int(err) == 0
+
+
 def test_decode_reports_what_it_cannot_do(cuda, native_lib):
     pool, table, bt = filled(cuda, [40, 600], 2, 16, 128, BF16)
     q = torch.randn(2, 4, 128, device=cuda).to(BF16)
