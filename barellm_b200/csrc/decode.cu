@@ -41,13 +41,15 @@
 #include <mutex>
 
 #include "common.cuh"
-#include "decode_plan.cuh"
 
 namespace bl {
 namespace {
 
-constexpr int kChunkTokens = kDecodeChunkTokens;
-constexpr int32_t kPlanMagic = kDecodePlanMagic;
+constexpr int kChunkTokens = 512;  // split-K chunk; fixed so results are batch-invariant
+// The plan kernel stamps its header with this value and the batch size; the
+// attention kernel runs a plan only when both match, so a workspace that holds
+// no plan (or another batch's) yields an error word, not stray reads.
+constexpr int32_t kPlanMagic = 0x4e414c50;
 
 // ---------------------------------------------------------------------------
 // workspace layout
@@ -106,7 +108,14 @@ __device__ __forceinline__ int block_excl_scan(int v, int* warp_tot, int& total)
   return warp_excl + x - v;
 }
 
-using PlanArgs = DecodePlanArgs;
+struct PlanArgs {
+  const int32_t* seq_lens;
+  int32_t batch, bs, chunk_blocks, bt_width, max_units;
+  int32_t* hdr;       // [0] total units
+  int32_t* row_base;  // [batch + 1]
+  int2* exec;         // [max_units] (row, chunk)
+  int32_t* err;
+};
 
 __device__ __forceinline__ int row_blocks(int len, int bs, int bt_width, int32_t* err) {
   if (len <= 0) return 0;
@@ -913,19 +922,14 @@ extern "C" int bl_paged_decode_plan(const bl_decode_args* args, void* stream) {
   p.row_base = (int32_t*)(ws + w.row_base);
   p.exec = (int2*)(ws + w.exec);
   p.err = a.err;
-  return launch_decode_plan(p, (cudaStream_t)stream);
-}
-
-namespace bl {
-
-int launch_decode_plan(const DecodePlanArgs& p, cudaStream_t s) {
-  if (launch_pdl(decode_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p) != cudaSuccess) {
+  if (launch_pdl(decode_plan_kernel, dim3(1), dim3(kPlanThreads), 0, (cudaStream_t)stream, p) != cudaSuccess) {
     set_error("decode_plan_kernel: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
     return BL_ERR_LAUNCH;
   }
   return BL_OK;
 }
 
+namespace bl {
 namespace {
 
 // Validates the tensor-core-path specifics and the workspace; fills `w`.

@@ -10,7 +10,8 @@
 // gather   dense code * scale in the caller's type, zeros behind each length.
 //          Counterpart of PagedLayerKV.read (paged_kv_cache.py:215-240).
 // Both are bound by HBM: append reads E bytes and writes 1 per element, gather
-// reads 1 and writes E.
+// reads 1 and writes E.  A call of a few tokens is bound by its launch and three
+// dependent loads (row, table entry, tokens): 4.2 us for 4 rows of one token.
 #include "fp8.cuh"
 
 namespace bl {
@@ -98,7 +99,9 @@ template <> __device__ __forceinline__ float bits_to_magnitude<__half>(uint32_t 
 // VEC: rows move as 16-byte vectors (head_dim a multiple of one, everything
 // aligned); up to kHeld of them per lane stay in registers between the maximum
 // and the store (a 16-token block of head_dim 128 fits), more are read twice.
-// Measured at 40k packed tokens (8 KV heads, head_dim 128, bf16): MEASURED.
+// A warp per block and head, not per token: the block's scale needs all of its new
+// tokens.  40k packed tokens (8 KV heads, head_dim 128, bf16, 247 MB): 47.4 us,
+// 5.2 TB/s; with the tokens read twice 69.8 us.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kAppendWarps * 32) append_fp8_kernel(const AppendFp8Args a) {
   pdl_trigger();  // a dependent launch (the decode plan) may start; it waits for this grid
@@ -297,7 +300,8 @@ __device__ __forceinline__ void zero_store(T* dst) {
 constexpr int kGatherTok = 2;  // tokens of a thread: their loads are in flight together
 
 // grid: (ceil(max_len / (kGatherTok * blockDim.y)), hkv, batch); threadIdx.x walks the
-// vectors of a token, threadIdx.y the tokens
+// vectors of a token, threadIdx.y the tokens.  64 rows of up to 4k tokens (8 KV
+// heads, head_dim 128, bf16, 1.35 GB): 215 us, 6.28 TB/s; one token a thread 236 us.
 template <typename T, int E>
 __global__ void __launch_bounds__(256) gather_fp8_kernel(const GatherFp8Args a) {
   const int64_t b = blockIdx.z;

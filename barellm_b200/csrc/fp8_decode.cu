@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kPlanThreads) fp8_decode_plan_kernel(const Pla
   if (tid < kChunkTiles) s_count[tid] = 0;
   __syncthreads();
   auto put = [&](int pos, int row, int chunk, int len, int base, int table_row) {
-    if (pos >= a.max_units) return;
+    if ((uint32_t)pos >= (uint32_t)a.max_units) return;  // (rows far past max_seq_len may wrap the sums)
     int4* u = reinterpret_cast<int4*>(a.units + pos);
     u[0] = make_int4(row, chunk, len, base + chunk);
     u[1] = make_int4(table_row, 0, 0, 0);
@@ -1414,7 +1414,7 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
   k.v_scale = a.layer.v_scale;
   k.block_tables = kv.block_tables;
   k.bt_stride = kv.bt_stride;
-  k.bt_width = kv.bt_width;
+  k.bt_width = std::min(kv.bt_width, (int64_t)(INT32_MAX - kChunk) / kv.block_size);  // positions are 32-bit
   k.row_ids = kv.row_ids;
   k.seq_lens = a.seq_lens;
   k.num_blocks = kv.num_blocks;
@@ -1448,7 +1448,7 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
     p.row_ids = kv.row_ids;
     p.batch = k.batch;
     p.max_units = k.max_units;
-    p.cap = kv.bt_width * kv.block_size;
+    p.cap = k.bt_width * kv.block_size;
     p.hdr = (int32_t*)(ws + w.hdr);
     p.row_base = (int32_t*)(ws + w.row_base);
     p.units = (Unit*)(ws + w.units);

@@ -908,8 +908,9 @@ def paged_decode_fp8(
     upper bound on them.  ``ws``: at least :func:`decode_fp8_workspace_bytes`;
     by default every call takes its own from torch's allocator.  With
     ``plan_ready`` the (required) ``ws`` still holds the plan of an earlier call
-    with the same ``seq_lens``, ``max_seq_len`` and q shape, as a step's later
-    layers have it.
+    with the same ``seq_lens``, ``row_ids`` (their contents too), table width,
+    pool shape, ``max_seq_len`` and q shape, as a step's later layers have it.
+    Calls that share a ``ws`` must be ordered, in one stream or by events.
     """
     _require_cuda(q, "q")
     qs, qst = q.shape, q.stride()

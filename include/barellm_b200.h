@@ -443,8 +443,11 @@ BL_API int bl_paged_gather_fp8(const bl_gather_fp8_args* args, void* stream);
 /* Decode attention over the 8-bit pages (bl_paged_decode), one query token  */
 /* per request.  A row of length 0 gets zeros.  Rows are split into fixed    */
 /* 512-token chunks, as there: a row's result does not depend on the batch.  */
-/* plan_ready: the workspace holds the plan that an earlier call with the    */
-/* same seq_lens, batch, num_q_heads, head_dim and max_seq_len left there.   */
+/* plan_ready: the workspace holds the plan that an earlier call left there  */
+/* with the same seq_lens, row_ids, table width, pool shape, batch,          */
+/* num_q_heads and max_seq_len (the contents of seq_lens and row_ids         */
+/* included; the layer, q, out and the table's entries may differ).  Calls   */
+/* that use one workspace must be ordered, in one stream or by events.       */
 typedef struct bl_decode_fp8_args {
   bl_fp8_layer layer;
   const void* q;
