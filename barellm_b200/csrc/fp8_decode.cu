@@ -9,8 +9,9 @@
 //                          the units, full chunks first, then partial ones by
 //                          decreasing size.  A unit's record holds all that the
 //                          attention kernel's producer needs to start on it.
-//   fp8_decode_tc_kernel   bf16 / fp16 q, head_dim 64, 128 or 256, block_size a
-//                          multiple of 16.  Persistent CTAs claim (chunk, KV head,
+//   fp8_decode_tc_kernel   bf16 / fp16 q, head_dim and block_size multiples of 16
+//                          (built for 64, 128 and 256 dims; the copies fill the
+//                          dims up to the next of these with zeros).  Persistent CTAs claim (chunk, KV head,
 //                          8 query heads) items.  A planner warp describes the
 //                          next item (query fragments, page rows, scales) while
 //                          four consumer warps work on one, each on every fourth
@@ -403,7 +404,9 @@ struct Pending {
                   (int64_t)(it.hq0 + (g_row < it.heads ? g_row : 0)) * a.q_sh + 4 * t4;
 #pragma unroll
     for (int k = 0; k < Cfg<D>::kKS; ++k) {
-      if (a.q_vec) {
+      if (k * 16 >= a.d) {
+        q[k] = make_uint2(0u, 0u);  // (the codes there are zeros)
+      } else if (a.q_vec) {
         q[k] = *reinterpret_cast<const uint2*>(qp + k * 16);
       } else {
         const T* p = qp + k * 16;
@@ -938,7 +941,7 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
           const int hq = it.hq0 + (c ? h1 : h0);
           const float inv = c ? i1 : i0;
           T* dst = reinterpret_cast<T*>(a.out) + (int64_t)it.b * a.o_sb + (int64_t)hq * a.o_sh;
-          float* part = a.ws_o + ((int64_t)it.part * a.hq + hq) * D;
+          float* part = a.ws_o + ((int64_t)it.part * a.hq + hq) * a.d;
           if (parts && g_row == 0)
             a.ws_lse[(int64_t)it.part * a.hq + hq] = c ? (L1 == 0.f ? -INFINITY : M1 + __log2f(L1))
                                                        : (L0 == 0.f ? -INFINITY : M0 + __log2f(L0));
@@ -947,6 +950,7 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
 #pragma unroll
             for (int j = 0; j < 2 * kWords; j += 2) {
               const int d = hf * 128 + g_row * kLaneDims + 2 * j;
+              if (d >= a.d) break;
               const float v0 = o[hf][j][c] * inv, v1 = o[hf][j][2 + c] * inv;
               const float v2 = o[hf][j + 1][c] * inv, v3 = o[hf][j + 1][2 + c] * inv;
               if (parts) {
@@ -1276,11 +1280,13 @@ __global__ void __launch_bounds__(kReduceThreads) fp8_decode_reduce_kernel(const
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-// The tensor-core kernel: 16-bit q, a head_dim it is built for, whole 16-token
-// tiles in a block, and pool rows within the tensor map's 32-bit coordinates.
+// The tensor-core kernel: 16-bit q, pool rows of whole 16-byte units (a tensor
+// map's stride), whole 16-token tiles in a block, and pool rows within the
+// tensor map's 32-bit coordinates.  Columns behind head_dim lie outside the map,
+// so that the copies fill them with zeros; they cost products but no bytes.
 bool use_tc(const bl_paged_layer& kv) {
   const double rows = (double)kv.num_layers * kv.num_blocks * kv.num_kv_heads * kv.block_size;
-  return (kv.dtype == BL_BF16 || kv.dtype == BL_F16) && (kv.head_dim == 64 || kv.head_dim == 128 || kv.head_dim == 256) &&
+  return (kv.dtype == BL_BF16 || kv.dtype == BL_F16) && kv.head_dim % 16 == 0 && kv.head_dim <= 256 &&
          kv.block_size % 16 == 0 && rows <= (double)INT32_MAX;
 }
 
@@ -1289,8 +1295,9 @@ int launch_tc(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
   using C = Cfg<D>;
   CUtensorMap kmap, vmap;
   const uint64_t rows = (uint64_t)kv.num_layers * kv.num_blocks * kv.num_kv_heads * kv.block_size;
-  if (!make_tmap_rows_8bit(&kmap, kv.k_pool, D, rows, C::kRow, 16) ||
-      !make_tmap_rows_8bit(&vmap, kv.v_pool, D, rows, C::kRow, 16))
+  const uint64_t row_bytes = (uint64_t)kv.head_dim;
+  if (!make_tmap_rows_8bit(&kmap, kv.k_pool, row_bytes, rows, C::kRow, 16) ||
+      !make_tmap_rows_8bit(&vmap, kv.v_pool, row_bytes, rows, C::kRow, 16))
     return BL_ERR_LAUNCH;
   const auto smem_for = [](int g) {
     const size_t heads = std::min(g, 8);
@@ -1348,7 +1355,7 @@ int launch_all(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
   int rc = BL_ERR_UNSUPPORTED;
   if constexpr (sizeof(T) == 2) {
     if (use_tc(kv))
-      rc = k.d == 64 ? launch_tc<T, 64>(k, kv, s) : k.d == 128 ? launch_tc<T, 128>(k, kv, s) : launch_tc<T, 256>(k, kv, s);
+      rc = k.d <= 64 ? launch_tc<T, 64>(k, kv, s) : k.d <= 128 ? launch_tc<T, 128>(k, kv, s) : launch_tc<T, 256>(k, kv, s);
     else
       rc = launch_simt<T>(k, s);
   } else {

@@ -68,6 +68,22 @@ def test_decode_long_row(cuda, native_lib, dtype):
     check_decode(out, q, pool, table, lens, 0)
 
 
+@pytest.mark.parametrize("d", [16, 48, 80, 96, 112, 144, 208, 240])
+@pytest.mark.parametrize("pad", [0, 4, 1])
+def test_decode_head_dims_between(cuda, native_lib, d, pad):
+    """Head dims that are multiples of 16: the columns behind them are neither read as values nor written."""
+    lens = [3, 0, 512, 1100, 40]
+    pool, table, bt = filled(cuda, lens, 2, 16, d, BF16)
+    q = torch.full((len(lens), 6, d + pad), float("nan"), dtype=BF16, device=cuda)[..., :d]
+    q.copy_(torch.randn(len(lens), 6, d, generator=torch.Generator().manual_seed(d)).to(BF16))
+    whole = torch.full((len(lens), 6, d + pad), 9.0, dtype=BF16, device=cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    ops.paged_decode_fp8(q, *pool.args, 1, bt, i32(lens, cuda), 1100, out=whole[..., :d], err=err)
+    assert int(err) == 0
+    check_decode(whole[..., :d], q, pool, table, lens, 1)
+    assert bool((whole[..., d:] == 9.0).all())
+
+
 @pytest.mark.parametrize("spread", [4.0, 12.0])
 def test_decode_scales_far_apart(cuda, native_lib, spread):
     """Blocks whose V scales differ by many binades: the running reference moves up, and small blocks are added apart."""
