@@ -196,8 +196,9 @@ struct Args {
   const int32_t* row_ids;
   const int32_t* seq_lens;
   int64_t num_blocks, layer;
-  int32_t batch, hq, hkv, g, head_tiles, bs, d;
-  int32_t q_vec, o_vec;  // q / out rows can be read / written four 16-bit elements at a time
+  int32_t batch, hq, hkv, g, bs, d;
+  int32_t tile_heads, head_tiles;  // query heads of an item, at most; items of a KV head
+  int32_t q_vec, o_vec;  // q (of a head_dim that the kernel is built for) / out go four 16-bit elements at a time
   float scale_log2;
   int32_t* hdr;
   const int32_t* row_base;
@@ -209,7 +210,7 @@ struct Args {
   int32_t* err;
 };
 
-// One item: a chunk of a row, a KV head and up to eight of its query heads.
+// One item: a chunk of a row, a KV head and up to tile_heads of its query heads.
 struct Item {
   int b, h, hq0, heads;
   int t0, t1;     // the chunk's tokens are [t0, t1)
@@ -258,8 +259,8 @@ __device__ __forceinline__ bool make_item(const Args& a, int64_t item, const Uni
   const int r = (int)(item % (a.hkv * a.head_tiles));
   it.h = r / a.head_tiles;
   const int ht = r - it.h * a.head_tiles;
-  it.hq0 = it.h * a.g + ht * 8;
-  it.heads = min(8, a.g - ht * 8);
+  it.hq0 = it.h * a.g + ht * a.tile_heads;
+  it.heads = min(a.tile_heads, a.g - ht * a.tile_heads);
   it.b = u.row;
   it.table_row = u.table_row;
   it.part = u.part;
@@ -404,10 +405,10 @@ struct Pending {
                   (int64_t)(it.hq0 + (g_row < it.heads ? g_row : 0)) * a.q_sh + 4 * t4;
 #pragma unroll
     for (int k = 0; k < Cfg<D>::kKS; ++k) {
-      if (k * 16 >= a.d) {
-        q[k] = make_uint2(0u, 0u);  // (the codes there are zeros)
-      } else if (a.q_vec) {
+      if (a.q_vec) {
         q[k] = *reinterpret_cast<const uint2*>(qp + k * 16);
+      } else if (k * 16 >= a.d) {
+        q[k] = make_uint2(0u, 0u);  // (the codes there are zeros)
       } else {
         const T* p = qp + k * 16;
         q[k] = make_uint2(pack2<T>(to_f32<T>(p[0]), to_f32<T>(p[1])), pack2<T>(to_f32<T>(p[2]), to_f32<T>(p[3])));
@@ -977,110 +978,98 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
 // ---------------------------------------------------------------------------
 // SIMT kernel: any element type, head_dim <= 256, any block size
 // ---------------------------------------------------------------------------
-constexpr int kSimtThreads = 256;
-constexpr int kSimtMaxTokens = 128;
-constexpr int kSimtWords = 16;  // four-code words a thread holds of a tile
+constexpr int kSimtThreads = 128;
+constexpr int kSimtWarps = kSimtThreads / 32;
+constexpr int kSimtTok = 4;    // tokens a lane group has in hand
+// resident CTAs per SM that the registers of HG heads allow
+__host__ __device__ constexpr int simt_ctas(int heads) { return heads == 4 ? 2 : heads == 2 ? 3 : 4; }
+constexpr int kSimtHeads = 4;  // query heads of an item, at most
 
-// tokens of a tile: what 256 threads hold in kSimtWords words each
-__host__ __device__ constexpr int simt_tokens(int d) { return d <= 128 ? 128 : 64; }
-// floats between a tile's rows: whole 16-byte vectors, an odd number of them, so
-// that 32 lanes reading a vector of a row each meet no bank twice
-__host__ __device__ constexpr int simt_stride(int d) { return ((d + 3) / 4 | 1) * 4; }
+// two fp32 values side by side: one instruction multiplies and adds both
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 un2(F2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// the four codes of a word, times s
+__device__ __forceinline__ void decode4(uint32_t w, F2 s, F2 (&x)[2]) {
+  const float2 lo = unpack2<__half>(e4m3lo_to_f16x2(w)), hi = unpack2<__half>(e4m3hi_to_f16x2(w));
+  x[0] = mul2(f2(lo.x, lo.y), s);
+  x[1] = mul2(f2(hi.x, hi.y), s);
+}
 
-struct alignas(16) SimtShared {  // float4 arrays follow
-  int64_t row[2][kSimtMaxTokens];  // byte offset of the token's codes, -1: none; this tile and the next
-  float ks[2][kSimtMaxTokens], vs[2][kSimtMaxTokens];
-  float p[kSimtMaxTokens][8];  // scores, then weights, of the eight heads
-  float alpha[8], l[8], m[8];
+template <int HG>
+struct alignas(16) SimtShared {
+  float4 q[HG][4][16];          // dims 16 l + 4 c + {0..3} of a head at [c][l]: lanes side by side read side by side
+  int64_t row[kChunk];          // byte offset of a token's codes, -1: none
+  float ks[kChunk], vs[kChunk];
+  float2 ml[kSimtWarps][HG];    // maximum and sum of each warp
+  float o[kSimtWarps][HG][256];
 };
 
-// A tile's K becomes fp32 in shared memory, a warp scores 32 tokens with one head
-// (a lane each), warp h takes head h's softmax, then the tile's V replaces K and
-// a thread owns one dim of every head over a share of the tokens.  The next
-// codes are on their way from HBM meanwhile, in registers.
-template <typename T>
-__global__ void __launch_bounds__(kSimtThreads, 2) fp8_decode_simt_kernel(const Args a) {
-  extern __shared__ __align__(1024) unsigned char smem_raw[];
-  SimtShared* sh = reinterpret_cast<SimtShared*>(smem_raw);
-  const int ts = simt_stride(a.d), ntok = simt_tokens(a.d), dq = (a.d + 3) / 4 * 4;
-  float* qs = reinterpret_cast<float*>(smem_raw + sizeof(SimtShared));  // [8][dq], zeros behind head_dim
-  float* tile = qs + 8 * dq;                                           // [ntok][ts]
+// A group of lanes has a token, each lane 16 dims of it, straight from the pool:
+// the codes never pass through shared memory.  HG heads' products with them in
+// registers (q from shared memory, the sums of the output in registers), the
+// lanes' shares of a score joined by shuffles; every group keeps a softmax of its
+// own, and the groups and warps are joined once per chunk.  K codes of the next
+// step are on their way during the V half of this one, V codes during the K half.
+// What bounds it (64 requests of 1k..8k tokens, 32 / 8 heads of 128 dims, fp32 q,
+// 617 MB): SIMT_MEASURED.
+// WIDE: head_dim and the pool's rows in whole 16-byte units.
+template <typename T, int HG, bool WIDE>
+__global__ void __launch_bounds__(kSimtThreads, simt_ctas(HG)) fp8_decode_simt_kernel(const Args a) {
+  __shared__ SimtShared<HG> sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int dp = 32;
-  while (dp < a.d) dp *= 2;
-  const int vd = tid % dp, vgroup = tid / dp, vgroups = kSimtThreads / dp;
-  // words of a token: thread tid has word `col` of tokens row0, row0 + step, ...
-  const bool words = (a.d & 3) == 0;
-  int wsh = 0;
-  while ((4 << wsh) < a.d) ++wsh;
-  const int col = tid & ((1 << wsh) - 1), row0 = tid >> wsh, step = kSimtThreads >> wsh;
-  const bool has_col = 4 * col < a.d;
+  int lpt = 1;  // lanes of a token
+  while (16 * lpt < a.d) lpt *= 2;
+  const int tpw = 32 / lpt;  // tokens a warp reads at once
+  const int lt = lane & (lpt - 1), grp = lane / lpt, dim0 = 16 * lt;
+  const bool has_dims = dim0 < a.d;
 
   pdl_wait();
   const int64_t items = (int64_t)plan_units(a, tid == 0) * a.hkv * a.head_tiles;
   zero_empty_rows<T>(a, kSimtThreads);
 
-  // where the tokens [t0, t0 + ntok) of the item are
-  auto locate = [&](const Item& it, int t0, int buf) {
-    if (tid >= ntok) return;
-    const int t = t0 + tid;
-    int64_t r = -1;
-    if (t < it.t1) {
-      const int lb = t / a.bs;
-      const int64_t phys = a.block_tables[(int64_t)it.table_row * a.bt_stride + lb];
-      if (phys < 0 || phys >= a.num_blocks) {
-        raise_dev(a.err, BL_DEVERR_BLOCK_ID);
+  auto load = [&](const uint8_t* pool, int at, uint4 (&w)[kSimtTok]) {
+#pragma unroll
+    for (int u = 0; u < kSimtTok; ++u) {
+      const int t = at + (u * kSimtWarps + warp) * tpw + grp;
+      const int64_t r = t < kChunk ? sh.row[t] : -1;
+      w[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < 0 || !has_dims) continue;
+      const uint8_t* p = pool + r + dim0;
+      if constexpr (WIDE) {
+        w[u] = *reinterpret_cast<const uint4*>(p);
       } else {
-        const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + it.h;
-        r = (slot * a.bs + (t - lb * a.bs)) * a.d;
-        sh->ks[buf][tid] = a.k_scale[slot];
-        sh->vs[buf][tid] = a.v_scale[slot];
-      }
-    }
-    sh->row[buf][tid] = r;
-  };
-  auto fetch = [&](const uint8_t* pool, int buf, uint32_t (&w)[kSimtWords]) {
-    if (!words) return;
+        uint32_t x[4] = {0u, 0u, 0u, 0u};
+        const int n = min(16, a.d - dim0);
+        if ((a.d & 3) == 0) {
 #pragma unroll
-    for (int i = 0; i < kSimtWords; ++i) {
-      const int t = row0 + i * step;
-      w[i] = 0;
-      if (t < ntok && has_col) {
-        const int64_t r = sh->row[buf][t];
-        if (r >= 0) w[i] = *reinterpret_cast<const uint32_t*>(pool + r + 4 * col);
-      }
-    }
-  };
-  auto expand = [&](const uint8_t* pool, const float* sc, int buf, const uint32_t (&w)[kSimtWords]) {
-    if (words) {
+          for (int c = 0; c < 4; ++c)
+            if (4 * c < n) x[c] = *reinterpret_cast<const uint32_t*>(p + 4 * c);
+        } else {
 #pragma unroll
-      for (int i = 0; i < kSimtWords; ++i) {
-        const int t = row0 + i * step;
-        if (t < ntok && has_col) {
-          const float s = sh->row[buf][t] >= 0 ? sc[t] : 0.f;
-          const float2 x = e4m3x2_to_float2((uint16_t)w[i]), y = e4m3x2_to_float2((uint16_t)(w[i] >> 16));
-          *reinterpret_cast<float4*>(tile + t * ts + 4 * col) = make_float4(x.x * s, x.y * s, y.x * s, y.y * s);
+          for (int e = 0; e < 16; ++e)
+            if (e < n) x[e >> 2] |= (uint32_t)p[e] << (8 * (e & 3));
         }
+        w[u] = make_uint4(x[0], x[1], x[2], x[3]);
       }
-    } else {
-      for (int e = tid; e < ntok * dq; e += kSimtThreads) {
-        const int t = e / dq, c = e - t * dq;
-        const int64_t r = sh->row[buf][t];
-        tile[t * ts + c] = r >= 0 && c < a.d ? e4m3_to_float(pool[r + c]) * sc[t] : 0.f;
-      }
-    }
-  };
-  // acc = acc * alpha + sum over this thread's tokens of p[t][h] * V[t][vd], heads [0, N)
-  float acc[8];
-  auto add_values = [&](auto n) {
-    constexpr int N = decltype(n)::value;
-#pragma unroll
-    for (int h = 0; h < N; ++h) acc[h] *= sh->alpha[h];
-#pragma unroll 8
-    for (int t = vgroup; t < ntok; t += vgroups) {
-      const float v = tile[t * ts + vd];
-#pragma unroll
-      for (int h = 0; h < N; ++h) acc[h] = fmaf(sh->p[t][h], v, acc[h]);
     }
   };
 
@@ -1091,111 +1080,209 @@ __global__ void __launch_bounds__(kSimtThreads, 2) fp8_decode_simt_kernel(const 
       continue;
     }
     __syncthreads();  // the previous item's shared state is no longer read
-    for (int e = tid; e < it.heads * dq; e += kSimtThreads) {
-      const int h = e / dq, d = e - h * dq;
-      qs[e] = d < a.d ? to_f32<T>(reinterpret_cast<const T*>(a.q)[(int64_t)it.b * a.q_sb + (int64_t)(it.hq0 + h) * a.q_sh + d]) *
-                            a.scale_log2
-                      : 0.f;
-    }
-    float m = -INFINITY, l = 0.f;  // warp h: head h
-#pragma unroll
-    for (int k = 0; k < 8; ++k) acc[k] = 0.f;
-    // (heads that the item does not have are weighted too, up to the next power of two: with zeros)
-    if (tid < 8) sh->alpha[tid] = 0.f;
-    for (int e = tid; e < kSimtMaxTokens * 8; e += kSimtThreads) (&sh->p[0][0])[e] = 0.f;
-    uint32_t kw[kSimtWords], vw[kSimtWords];
-    locate(it, it.t0, 0);
-    __syncthreads();
-    fetch(a.k_pool, 0, kw);
-    int buf = 0;
-    for (int t0 = it.t0; t0 < it.t1; t0 += ntok, buf ^= 1) {
-      const bool more = t0 + ntok < it.t1;
-      expand(a.k_pool, sh->ks[buf], buf, kw);
-      fetch(a.v_pool, buf, vw);
-      if (more) locate(it, t0 + ntok, buf ^ 1);
-      __syncthreads();
-      for (int u = warp; u < it.heads * (ntok / 32); u += kSimtThreads / 32) {
-        const int h = u / (ntok / 32), t = (u - h * (ntok / 32)) * 32 + lane;
-        const float4* qh = reinterpret_cast<const float4*>(qs + h * dq);
-        const float4* kt = reinterpret_cast<const float4*>(tile + t * ts);
-        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-#pragma unroll 4
-        for (int d = 0; d < dq / 4; ++d) {
-          const float4 x = qh[d], y = kt[d];
-          s0 = fmaf(x.x, y.x, s0), s1 = fmaf(x.y, y.y, s1), s2 = fmaf(x.z, y.z, s2), s3 = fmaf(x.w, y.w, s3);
+    const int n = it.t1 - it.t0;
+    for (int i = tid; i < kChunk; i += kSimtThreads) {
+      int64_t r = -1;
+      float ks = 0.f, vs = 0.f;
+      if (i < n) {
+        const int t = it.t0 + i, lb = t / a.bs;
+        const int64_t phys = a.block_tables[(int64_t)it.table_row * a.bt_stride + lb];
+        if (phys < 0 || phys >= a.num_blocks) {
+          raise_dev(a.err, BL_DEVERR_BLOCK_ID);
+        } else {
+          const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + it.h;
+          r = (slot * a.bs + (t - lb * a.bs)) * a.d;
+          ks = a.k_scale[slot];
+          vs = a.v_scale[slot];
         }
-        sh->p[t][h] = sh->row[buf][t] < 0 ? -INFINITY : (s0 + s1) + (s2 + s3);
       }
-      __syncthreads();
-      if (warp < it.heads) {
-        float s[kSimtMaxTokens / 32], mx = -INFINITY;
+      sh.row[i] = r;
+      sh.ks[i] = ks;
+      sh.vs[i] = vs;
+    }
+    for (int e = tid; e < HG * 256; e += kSimtThreads) {
+      const int h = e >> 8, d = e & 255;
+      float x = 0.f;
+      if (h < it.heads && d < a.d)
+        x = to_f32<T>(reinterpret_cast<const T*>(a.q)[(int64_t)it.b * a.q_sb + (int64_t)(it.hq0 + h) * a.q_sh + d]) *
+            a.scale_log2;
+      reinterpret_cast<float*>(&sh.q[h][(d >> 2) & 3][d >> 4])[d & 3] = x;
+    }
+    __syncthreads();
+
+    float m[HG], l[HG];
+    F2 o[HG][8];
 #pragma unroll
-        for (int i = 0; i < kSimtMaxTokens / 32; ++i)
-          if (i < ntok / 32) mx = fmaxf(mx, s[i] = sh->p[lane + 32 * i][warp]);
+    for (int h = 0; h < HG; ++h) {
+      m[h] = -INFINITY;
+      l[h] = 0.f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float mn = fmaxf(m, mx), u = mn == -INFINITY ? 0.f : mn;
-        const float al = mn == m ? 1.f : fast_exp2(m - mn);
-        float ps = 0.f;
+      for (int j = 0; j < 8; ++j) o[h][j] = 0ull;
+    }
+    uint4 kc[kSimtTok], vc[kSimtTok];
+    load(a.k_pool, 0, kc);
+    load(a.v_pool, 0, vc);
+    const int step = kSimtWarps * tpw * kSimtTok;
+    for (int at = 0; at < n; at += step) {
+      float s[kSimtTok][HG];
+      float vs[kSimtTok];
+      {
+        F2 z[kSimtTok][HG], ks[kSimtTok];
 #pragma unroll
-        for (int i = 0; i < kSimtMaxTokens / 32; ++i)
-          if (i < ntok / 32) {
-            const float p = fast_exp2(s[i] - u);
-            ps += p;
-            sh->p[lane + 32 * i][warp] = p;
+        for (int u = 0; u < kSimtTok; ++u) {
+          const int t = at + (u * kSimtWarps + warp) * tpw + grp;
+          const float x = t < kChunk ? sh.ks[t] : 0.f;
+          vs[u] = t < kChunk ? sh.vs[t] : 0.f;
+          ks[u] = f2(x, x);
+#pragma unroll
+          for (int h = 0; h < HG; ++h) z[u][h] = 0ull;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          F2 q[HG][2];
+#pragma unroll
+          for (int h = 0; h < HG; ++h) {
+            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&sh.q[h][c][lt]);
+            q[h][0] = x.x, q[h][1] = x.y;
           }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
-        m = mn;
-        l = l * al + ps;
-        if (lane == 0) sh->alpha[warp] = al;
-      }
-      expand(a.v_pool, sh->vs[buf], buf, vw);  // (K's tile was last read before the barrier above)
-      __syncthreads();
-      if (more) fetch(a.k_pool, buf ^ 1, kw);
-      if (vd < a.d) {
-        if (it.heads == 1)
-          add_values(std::integral_constant<int, 1>());
-        else if (it.heads == 2)
-          add_values(std::integral_constant<int, 2>());
-        else if (it.heads <= 4)
-          add_values(std::integral_constant<int, 4>());
-        else
-          add_values(std::integral_constant<int, 8>());
-      }
-      __syncthreads();  // the tile and the weights are no longer read
-    }
-    // join the threads that share a dim, and the heads' sums
-    if (warp < it.heads && lane == 0) {
-      sh->m[warp] = m;
-      sh->l[warp] = l;
-    }
-    if (vd < a.d) {
+          for (int u = 0; u < kSimtTok; ++u) {
+            F2 x[2];
+            decode4(c == 0 ? kc[u].x : c == 1 ? kc[u].y : c == 2 ? kc[u].z : kc[u].w, ks[u], x);
 #pragma unroll
-      for (int h = 0; h < 8; ++h)
-        if (h < it.heads) tile[(vgroup * 8 + h) * a.d + vd] = acc[h];
+            for (int h = 0; h < HG; ++h) z[u][h] = fma2(x[1], q[h][1], fma2(x[0], q[h][0], z[u][h]));
+          }
+        }
+        load(a.k_pool, at + step, kc);
+#pragma unroll
+        for (int u = 0; u < kSimtTok; ++u)
+#pragma unroll
+          for (int h = 0; h < HG; ++h) {
+            const float2 x = un2(z[u][h]);
+            s[u][h] = x.x + x.y;
+          }
+      }
+      for (int off = 1; off < lpt; off <<= 1)
+#pragma unroll
+        for (int u = 0; u < kSimtTok; ++u)
+#pragma unroll
+          for (int h = 0; h < HG; ++h) s[u][h] += __shfl_xor_sync(0xffffffffu, s[u][h], off);
+      bool moved = false;
+      float top[HG];
+#pragma unroll
+      for (int h = 0; h < HG; ++h) top[h] = m[h];
+#pragma unroll
+      for (int u = 0; u < kSimtTok; ++u) {
+        const int t = at + (u * kSimtWarps + warp) * tpw + grp;
+        const bool live = t < kChunk && sh.row[t] >= 0;
+#pragma unroll
+        for (int h = 0; h < HG; ++h) {
+          if (!live) s[u][h] = -INFINITY;
+          top[h] = fmaxf(top[h], s[u][h]);
+        }
+      }
+      // the maximum moves only when a score passes it by 8 (log2 units): P <= 2^8
+#pragma unroll
+      for (int h = 0; h < HG; ++h) moved |= top[h] > m[h] + 8.f;
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int h = 0; h < HG; ++h) {
+          const float al = top[h] == m[h] ? 1.f : fast_exp2(m[h] - top[h]);
+          m[h] = top[h];
+          l[h] *= al;
+          const F2 al2 = f2(al, al);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[h][j] = mul2(o[h][j], al2);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        const float unit = m[h] == -INFINITY ? 0.f : m[h];
+#pragma unroll
+        for (int u = 0; u < kSimtTok; ++u) {
+          s[u][h] = fast_exp2(s[u][h] - unit);
+          l[h] += s[u][h];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kSimtTok; ++u) {
+        const F2 v2 = f2(vs[u], vs[u]);
+        F2 p[HG];
+#pragma unroll
+        for (int h = 0; h < HG; ++h) p[h] = f2(s[u][h], s[u][h]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          F2 x[2];
+          decode4(c == 0 ? vc[u].x : c == 1 ? vc[u].y : c == 2 ? vc[u].z : vc[u].w, v2, x);
+#pragma unroll
+          for (int h = 0; h < HG; ++h) {
+            o[h][2 * c] = fma2(p[h], x[0], o[h][2 * c]);
+            o[h][2 * c + 1] = fma2(p[h], x[1], o[h][2 * c + 1]);
+          }
+        }
+      }
+      load(a.v_pool, at + step, vc);
+    }
+
+    // ---- join the groups of the warp, then the warps ----
+    auto weight = [](float x, float top) { return x == -INFINITY ? 0.f : (x == top ? 1.f : fast_exp2(x - top)); };
+    for (int off = lpt; off < 32; off <<= 1) {
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        const float om = __shfl_xor_sync(0xffffffffu, m[h], off), ol = __shfl_xor_sync(0xffffffffu, l[h], off);
+        const float top = fmaxf(m[h], om);
+        const float w = weight(m[h], top), ow = weight(om, top);
+        m[h] = top;
+        l[h] = w * l[h] + ow * ol;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const F2 x = __shfl_xor_sync(0xffffffffu, o[h][j], off);
+          o[h][j] = fma2(f2(ow, ow), x, mul2(f2(w, w), o[h][j]));
+        }
+      }
+    }
+    if (grp == 0) {
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        if (lt == 0) sh.ml[warp][h] = make_float2(m[h], l[h]);
+        if (has_dims)
+#pragma unroll
+          for (int j = 0; j < 8; j += 2)
+            *reinterpret_cast<ulonglong2*>(&sh.o[warp][h][dim0 + 2 * j]) = make_ulonglong2(o[h][j], o[h][j + 1]);
+      }
     }
     __syncthreads();
-    for (int e = tid; e < it.heads * a.d; e += kSimtThreads) {
-      const int h = e / a.d, d = e - h * a.d, hq = it.hq0 + h;
-      float x = 0.f;
-      for (int g = 0; g < vgroups; ++g) x += tile[(g * 8 + h) * a.d + d];
-      const float L = sh->l[h], val = L == 0.f ? 0.f : x / L;  // a NaN sum stays NaN
-      if (it.nch <= 1) {
-        reinterpret_cast<T*>(a.out)[(int64_t)it.b * a.o_sb + (int64_t)hq * a.o_sh + d] = from_f32<T>(val);
-      } else if (!has_part(a, it)) {
-        if (d == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
-      } else {
-        a.ws_o[((int64_t)it.part * a.hq + hq) * a.d + d] = val;
-        if (d == 0) a.ws_lse[(int64_t)it.part * a.hq + hq] = L == 0.f ? -INFINITY : sh->m[h] + __log2f(L);
+    const bool parts = it.nch > 1;
+    if (parts && !has_part(a, it)) {
+      if (tid == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);
+      continue;
+    }
+    for (int h = 0; h < it.heads; ++h) {
+      float top = -INFINITY, sum = 0.f, w[kSimtWarps];
+#pragma unroll
+      for (int i = 0; i < kSimtWarps; ++i) top = fmaxf(top, sh.ml[i][h].x);
+#pragma unroll
+      for (int i = 0; i < kSimtWarps; ++i) {
+        w[i] = weight(sh.ml[i][h].x, top);
+        sum += w[i] * sh.ml[i][h].y;
+      }
+      // sum 0: no token (nothing seen); a NaN sum stays NaN
+      const int hq = it.hq0 + h;
+      T* dst = reinterpret_cast<T*>(a.out) + (int64_t)it.b * a.o_sb + (int64_t)hq * a.o_sh;
+      float* part = a.ws_o + ((int64_t)it.part * a.hq + hq) * a.d;
+      if (parts && tid == 0) a.ws_lse[(int64_t)it.part * a.hq + hq] = sum == 0.f ? -INFINITY : top + __log2f(sum);
+      for (int d = tid; d < a.d; d += kSimtThreads) {
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < kSimtWarps; ++i) x += w[i] * sh.o[i][h][d];
+        x = sum == 0.f ? 0.f : x / sum;
+        if (parts)
+          part[d] = x;
+        else
+          dst[d] = from_f32<T>(x);
       }
     }
   }
-}
-
-// (the join's [groups][8][d] sums fit the tile: groups * 8 <= tokens of a tile)
-size_t simt_smem(int d) {
-  return sizeof(SimtShared) + sizeof(float) * (8 * (size_t)((d + 3) / 4 * 4) + (size_t)simt_tokens(d) * simt_stride(d));
 }
 
 // ---------------------------------------------------------------------------
@@ -1336,18 +1423,24 @@ int launch_tc(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
   return BL_OK;
 }
 
-template <typename T>
-int launch_simt(const Args& k, cudaStream_t s) {
-  const size_t smem = simt_smem(k.d);
+template <typename T, int HG>
+int launch_simt_heads(const Args& k, cudaStream_t s) {
   const int64_t items = (int64_t)k.max_units * k.hkv * k.head_tiles;
-  const int64_t grid = std::min<int64_t>((int64_t)num_sms() * 2, items);
-  if (cudaFuncSetAttribute(fp8_decode_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-          cudaSuccess ||
-      launch_pdl(fp8_decode_simt_kernel<T>, dim3((unsigned)grid), dim3(kSimtThreads), smem, s, k) != cudaSuccess) {
+  const int64_t grid = std::min<int64_t>((int64_t)num_sms() * simt_ctas(HG), items);
+  const bool wide = k.d % 16 == 0;
+  if (launch_pdl(wide ? fp8_decode_simt_kernel<T, HG, true> : fp8_decode_simt_kernel<T, HG, false>, dim3((unsigned)grid),
+                 dim3(kSimtThreads), 0, s, k) != cudaSuccess) {
     set_error("fp8_decode_simt_kernel: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
     return BL_ERR_LAUNCH;
   }
   return BL_OK;
+}
+
+template <typename T>
+int launch_simt(const Args& k, cudaStream_t s) {
+  return k.tile_heads == 1   ? launch_simt_heads<T, 1>(k, s)
+         : k.tile_heads == 2 ? launch_simt_heads<T, 2>(k, s)
+                             : launch_simt_heads<T, 4>(k, s);
 }
 
 template <typename T>
@@ -1430,10 +1523,11 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
   k.hq = (int32_t)a.num_q_heads;
   k.hkv = (int32_t)kv.num_kv_heads;
   k.g = k.hq / k.hkv;
-  k.head_tiles = (k.g + 7) / 8;
+  k.tile_heads = use_tc(kv) ? 8 : std::min(k.g == 3 ? 4 : k.g, kSimtHeads);
+  k.head_tiles = (k.g + k.tile_heads - 1) / k.tile_heads;
   k.bs = (int32_t)kv.block_size;
   k.d = (int32_t)kv.head_dim;
-  k.q_vec = ((uintptr_t)a.q & 7) == 0 && a.q_stride_b % 4 == 0 && a.q_stride_h % 4 == 0;
+  k.q_vec = (k.d == 64 || k.d == 128 || k.d == 256) && ((uintptr_t)a.q & 7) == 0 && a.q_stride_b % 4 == 0 && a.q_stride_h % 4 == 0;
   k.o_vec = ((uintptr_t)a.out & 7) == 0 && a.out_stride_b % 4 == 0 && a.out_stride_h % 4 == 0;
   k.scale_log2 = a.scale * kLog2e;
   k.hdr = (int32_t*)(ws + w.hdr);
