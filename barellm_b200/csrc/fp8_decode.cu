@@ -9,16 +9,17 @@
 //                          the units, full chunks first, then partial ones by
 //                          decreasing size.  A unit's record holds all that the
 //                          attention kernel's producer needs to start on it.
-//   fp8_decode_tc_kernel   bf16 / fp16 q, head_dim and block_size multiples of 16
-//                          (built for 64, 128 and 256 dims; the copies fill the
-//                          dims up to the next of these with zeros).  Persistent CTAs claim (chunk, KV head,
-//                          8 query heads) items.  A planner warp describes the
-//                          next item (query fragments, page rows, scales) while
-//                          four consumer warps work on one, each on every fourth
-//                          step of 32 tokens, copied by TMA into a ring of its own.
+//   fp8_decode_tc_kernel   bf16 / fp16 q, head_dim a multiple of 16, block_size
+//                          one of 8.  Built for 64, 128 and 256 dims; the copies
+//                          fill the dims up to the next of these with zeros.
+//                          Persistent CTAs claim (chunk, KV head, 8 query heads)
+//                          items.  A planner warp describes the next item (query
+//                          fragments, page rows, scales) while four consumer
+//                          warps work on one, each on every fourth step of 32
+//                          tokens, copied by TMA into a ring of its own.
 //   fp8_decode_simt_kernel everything else (fp32 q, other head_dims and block
 //                          sizes, pools past the tensor map's 2^31 rows): the
-//                          same chunks, fp32 multiplies on dequantised tiles.
+//                          same chunks, fp32 multiplies in registers.
 //   fp8_decode_reduce_kernel  joins the chunks of rows that have several.
 //
 // Arithmetic of the tensor-core kernel.  Codes are converted to fp16, which
@@ -322,18 +323,20 @@ struct Cfg {
   static constexpr int kVecs = D / 16;            // float4s of sums a lane holds (two heads)
 };
 
-// What the planner warp hands to the consumers, an item at a time.
-template <int D>
+// What the planner warp hands to the consumers, an item at a time.  NP: pieces of
+// a tile that lie in one block: one of 16 tokens, or two of 8 where the block
+// size is no multiple of 16.
+template <int D, int NP>
 struct alignas(16) ItemSlot {
-  float2 f[4];                      // score factors of heads 2t and 2t + 1
-  int32_t y[kTiles];                // pool row of each tile
-  float ks[kTiles], vs[kTiles];     // its scales
+  float2 f[4];                             // score factors of heads 2t and 2t + 1
+  int32_t y[kTiles * NP];                  // pool row of each piece
+  float ks[kTiles * NP], vs[kTiles * NP];  // its scales
   Item it;
 };
 
-template <int D>
+template <int D, int NP>
 struct alignas(16) TCShared {  // the query fragments and the merge buffer behind it are read 16 bytes at a time
-  ItemSlot<D> items[2];
+  ItemSlot<D, NP> items[2];
   float2 ml[kNW][8];  // maximum and sum of each class and head
   uint64_t full[kNW][Cfg<D>::kDepth];
   uint64_t item_full[2], item_empty[2];
@@ -385,21 +388,25 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, in
 // An item on its way to the consumers: lane i holds tile i of the chunk.  begin()
 // makes the loads that the plan's record leads to, finish() those behind the
 // block id.
-template <typename T, int D>
+template <typename T, int D, int NP>
 struct Pending {
   Item it;
   bool valid;
-  int tok, lb;
-  int32_t phys, y;
-  float ks, vs;
+  int tok, lb[NP];
+  int32_t phys[NP], y[NP];
+  float ks[NP], vs[NP];
   uint2 q[Cfg<D>::kKS];  // dims 16 k + 4 t + {0..3} of head g, as stored
 
   __device__ __forceinline__ void begin(const Args& a, int64_t item, const Unit& u, int lane) {
     valid = make_item(a, item, u, it);
     tok = it.t0 + 16 * lane;
-    lb = tok / a.bs;
-    phys = 0;
-    if (tok < it.t1) phys = a.block_tables[(int64_t)it.table_row * a.bt_stride + lb];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int t = tok + p * (16 / NP);
+      lb[p] = t / a.bs;
+      phys[p] = 0;
+      if (t < it.t1) phys[p] = a.block_tables[(int64_t)it.table_row * a.bt_stride + lb[p]];
+    }
     const int g_row = lane >> 2, t4 = lane & 3;
     const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(valid ? it.b : 0) * a.q_sb +
                   (int64_t)(it.hq0 + (g_row < it.heads ? g_row : 0)) * a.q_sh + 4 * t4;
@@ -417,18 +424,25 @@ struct Pending {
   }
 
   __device__ __forceinline__ void finish(const Args& a) {
-    y = 0;
-    ks = vs = 1.f;
-    if (tok < it.t1) {
-      int64_t p = phys;
-      if (p < 0 || p >= a.num_blocks) {
-        raise_dev(a.err, BL_DEVERR_BLOCK_ID);
-        p = 0;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int t = tok + p * (16 / NP);
+      if (t < it.t1) {
+        int64_t b = phys[p];
+        if (b < 0 || b >= a.num_blocks) {
+          raise_dev(a.err, BL_DEVERR_BLOCK_ID);
+          b = 0;
+        }
+        const int64_t slot = (a.layer * a.num_blocks + b) * a.hkv + it.h;
+        ks[p] = a.k_scale[slot];
+        vs[p] = a.v_scale[slot];
+        y[p] = (int32_t)(slot * a.bs + (t - lb[p] * a.bs));
+      } else {
+        // a missing second piece repeats the first one (no effect: its codes are masked)
+        y[p] = p ? y[0] : 0;
+        ks[p] = p ? ks[0] : 1.f;
+        vs[p] = p ? vs[0] : 1.f;
       }
-      const int64_t slot = (a.layer * a.num_blocks + p) * a.hkv + it.h;
-      ks = a.k_scale[slot];
-      vs = a.v_scale[slot];
-      y = (int32_t)(slot * a.bs + (tok - lb * a.bs));
     }
   }
 
@@ -438,7 +452,7 @@ struct Pending {
   // codes of one 32-bit word.
   // Lanes of heads that the item does not have store nothing: `qs` has room for
   // min(g, 8) heads, lane by lane.
-  __device__ __forceinline__ void stage(const Args& a, int lane, ItemSlot<D>& out, uint2* qs) const {
+  __device__ __forceinline__ void stage(const Args& a, int lane, ItemSlot<D, NP>& out, uint2* qs) const {
     const int t4 = lane & 3, room = 4 * min(a.g, 8);
     float amax = 0.f;
 #pragma unroll
@@ -461,25 +475,30 @@ struct Pending {
     const float f0 = __shfl_sync(0xffffffffu, f, 8 * t4);
     const float f1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
     if (lane < 4) out.f[lane] = make_float2(f0, f1);
-    out.y[lane] = y;
-    out.ks[lane] = ks;
     // a step with one tile repeats its V scale for the missing one (no effect: its codes are masked)
-    const float before = __shfl_up_sync(0xffffffffu, vs, 1);
-    out.vs[lane] = tok < it.t1 ? vs : before;
+    const float before = __shfl_up_sync(0xffffffffu, vs[NP - 1], 1);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      out.y[lane * NP + p] = y[p];
+      out.ks[lane * NP + p] = ks[p];
+      out.vs[lane * NP + p] = tok < it.t1 ? vs[p] : before;
+    }
     if (lane == 0) out.it = it;
   }
 };
 
-template <typename T, int D>
+template <typename T, int D, int NP>
 __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
     fp8_decode_tc_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using C = Cfg<D>;
-  static_assert(sizeof(TCShared<D>) % 16 == 0 && C::kDepth * C::kSlot % 1024 == 0 && C::kKS * 4 * sizeof(uint2) % 16 == 0 &&
-                    offsetof(ItemSlot<D>, ks) % 8 == 0 && offsetof(ItemSlot<D>, vs) % 8 == 0,
+  using Shared = TCShared<D, NP>;
+  using Slot = ItemSlot<D, NP>;
+  static_assert(sizeof(Shared) % 16 == 0 && C::kDepth * C::kSlot % 1024 == 0 && C::kKS * 4 * sizeof(uint2) % 16 == 0 &&
+                    sizeof(Slot) % 16 == 0 && offsetof(Slot, ks) % 16 == 0 && offsetof(Slot, vs) % 16 == 0,
                 "vector accesses to shared memory");
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* slots = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  TCShared<D>* sh = reinterpret_cast<TCShared<D>*>(slots + kNW * C::kDepth * C::kSlot);
+  Shared* sh = reinterpret_cast<Shared*>(slots + kNW * C::kDepth * C::kSlot);
   const int room = 4 * min(a.g, 8);                              // lanes of the heads an item can have
   uint2* qs = reinterpret_cast<uint2*>(sh + 1);                  // [2][kKS][room] fragments
   float* comb = reinterpret_cast<float*>(qs + 2 * C::kKS * room);  // [kNW - 1][kVecs][8 * head pairs] float4
@@ -509,7 +528,7 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
     // when the consumers begin the item before it, late enough to be fair and a
     // whole item's time ahead of its use.)
     unsigned long long* claimed = reinterpret_cast<unsigned long long*>(a.hdr + 4);
-    Pending<T, D> p;
+    Pending<T, D, NP> p;
     int64_t item = blockIdx.x, items = 0;
     Unit first = {};
     if (a.planned) {
@@ -615,7 +634,7 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
     }
     const int slot = issued % kDepth;
     if (lane == 0) {
-      const ItemSlot<D>& is = sh->items[at_item & 1];
+      const ItemSlot<D, NP>& is = sh->items[at_item & 1];
       const int n = min(2, at_tiles - 2 * at_step);
       uint64_t* bar = &sh->full[warp][slot];
       fence_proxy_async_smem();  // the warp's reads of the slot come before the copies into it
@@ -625,11 +644,15 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         if (x < n) {
-          const int32_t y = is.y[2 * at_step + x];
 #pragma unroll
-          for (int hf = 0; hf < C::kHalves; ++hf) {
-            tma_load_2d_hint(kd + x * C::kTile + hf * C::kBox, &kmap, bar, hf * 128, y, policy);
-            tma_load_2d_hint(vd + x * C::kTile + hf * C::kBox, &vmap, bar, hf * 128, y, policy);
+          for (int p = 0; p < NP; ++p) {
+            const int32_t y = is.y[(2 * at_step + x) * NP + p];
+            const int to = x * C::kTile + p * (C::kBox / NP);
+#pragma unroll
+            for (int hf = 0; hf < C::kHalves; ++hf) {
+              tma_load_2d_hint(kd + to + hf * C::kBox, &kmap, bar, hf * 128, y, policy);
+              tma_load_2d_hint(vd + to + hf * C::kBox, &vmap, bar, hf * 128, y, policy);
+            }
           }
         }
       }
@@ -684,9 +707,17 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
       ok = issued > taken && __all_sync(0xffffffffu, wait_or_abort(&sh->full[warp][slot], (taken / kDepth) & 1, &sh->abort,
                                                                    a.err));
       if (!ok) break;
-      const float2 ks2 = *reinterpret_cast<const float2*>(&sh->items[slot_i].ks[2 * i]);
-      const float2 vs2 = *reinterpret_cast<const float2*>(&sh->items[slot_i].vs[2 * i]);
-      const float4 sc = make_float4(ks2.x, ks2.y, vs2.x, vs2.y);
+      float ksc[2 * NP], vsc[2 * NP];  // scales of the step's pieces
+      if constexpr (NP == 1) {
+        const float2 ks2 = *reinterpret_cast<const float2*>(&sh->items[slot_i].ks[2 * i]);
+        const float2 vs2 = *reinterpret_cast<const float2*>(&sh->items[slot_i].vs[2 * i]);
+        ksc[0] = ks2.x, ksc[1] = ks2.y, vsc[0] = vs2.x, vsc[1] = vs2.y;
+      } else {
+        const float4 ks4 = *reinterpret_cast<const float4*>(&sh->items[slot_i].ks[4 * i]);
+        const float4 vs4 = *reinterpret_cast<const float4*>(&sh->items[slot_i].vs[4 * i]);
+        ksc[0] = ks4.x, ksc[1] = ks4.y, ksc[2] = ks4.z, ksc[3] = ks4.w;
+        vsc[0] = vs4.x, vsc[1] = vs4.y, vsc[2] = vs4.z, vsc[3] = vs4.w;
+      }
       const uint32_t kb = smem_u32(ring + slot * C::kSlot);
       const unsigned char* vb = ring + slot * C::kSlot + 2 * C::kTile + v_off;
 
@@ -725,7 +756,9 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
           for (int e = 0; e < 4; ++e) s[x][e] = z[x][0][e] + z[x][1][e];
       }
       const int nvalid = it.t1 - (it.t0 + i * kStepTokens);  // tokens of the step that exist
-      float c00 = f0 * sc.x, c01 = f1 * sc.x, c10 = f0 * sc.y, c11 = f1 * sc.y;  // log2 units
+      float c0[2 * NP], c1[2 * NP];  // factors of heads 2t, 2t + 1 for each piece's scores, log2 units
+#pragma unroll
+      for (int p = 0; p < 2 * NP; ++p) c0[p] = f0 * ksc[p], c1[p] = f1 * ksc[p];
       if (nvalid < kStepTokens) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -733,10 +766,17 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
           if (16 * x + g_row + 8 >= nvalid) s[x][2] = s[x][3] = -INFINITY;
         }
         // (a factor that underflowed would make NaN of the mask)
-        c00 = fmaxf(c00, 1.2e-38f), c01 = fmaxf(c01, 1.2e-38f), c10 = fmaxf(c10, 1.2e-38f), c11 = fmaxf(c11, 1.2e-38f);
+#pragma unroll
+        for (int p = 0; p < 2 * NP; ++p) c0[p] = fmaxf(c0[p], 1.2e-38f), c1[p] = fmaxf(c1[p], 1.2e-38f);
       }
-      float mx0 = fmaxf(fmaxf(s[0][0], s[0][2]) * c00, fmaxf(s[1][0], s[1][2]) * c10);
-      float mx1 = fmaxf(fmaxf(s[0][1], s[0][3]) * c01, fmaxf(s[1][1], s[1][3]) * c11);
+      float mx0, mx1;
+      if constexpr (NP == 1) {
+        mx0 = fmaxf(fmaxf(s[0][0], s[0][2]) * c0[0], fmaxf(s[1][0], s[1][2]) * c0[1]);
+        mx1 = fmaxf(fmaxf(s[0][1], s[0][3]) * c1[0], fmaxf(s[1][1], s[1][3]) * c1[1]);
+      } else {
+        mx0 = fmaxf(fmaxf(s[0][0] * c0[0], s[0][2] * c0[1]), fmaxf(s[1][0] * c0[2], s[1][2] * c0[3]));
+        mx1 = fmaxf(fmaxf(s[0][1] * c1[0], s[0][3] * c1[1]), fmaxf(s[1][1] * c1[2], s[1][3] * c1[3]));
+      }
       if (__any_sync(0xffffffffu, mx0 > m0 + 8.f || mx1 > m1 + 8.f)) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
@@ -760,23 +800,26 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
       }
       const float u0 = m0 == -INFINITY ? 0.f : -m0, u1 = m1 == -INFINITY ? 0.f : -m1;
       // exponentials and row sums
-      s[0][0] = fast_exp2(fmaf(s[0][0], c00, u0)), s[0][2] = fast_exp2(fmaf(s[0][2], c00, u0));
-      s[0][1] = fast_exp2(fmaf(s[0][1], c01, u1)), s[0][3] = fast_exp2(fmaf(s[0][3], c01, u1));
-      s[1][0] = fast_exp2(fmaf(s[1][0], c10, u0)), s[1][2] = fast_exp2(fmaf(s[1][2], c10, u0));
-      s[1][1] = fast_exp2(fmaf(s[1][1], c11, u1)), s[1][3] = fast_exp2(fmaf(s[1][3], c11, u1));
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int a0 = x * NP, a1 = x * NP + NP - 1;  // pieces of the lane's two tokens
+        s[x][0] = fast_exp2(fmaf(s[x][0], c0[a0], u0)), s[x][2] = fast_exp2(fmaf(s[x][2], c0[a1], u0));
+        s[x][1] = fast_exp2(fmaf(s[x][1], c1[a0], u1)), s[x][3] = fast_exp2(fmaf(s[x][3], c1[a1], u1));
+      }
       l0 += (s[0][0] + s[0][2]) + (s[1][0] + s[1][2]);
       l1 += (s[0][1] + s[0][3]) + (s[1][1] + s[1][3]);
 
       // O^T[dim][head] += V^T[dim][token] P^T[token][head] of tile x.  A lane takes the
       // kLaneDims consecutive dims g_row * kLaneDims of tokens 2t, 2t+1, 2t+8, 2t+9 and
       // pairs two tokens' bytes, so a converted pair is one A register (row =
-      // dim, two consecutive tokens).  APART: the tile's sums are made on their
-      // own and added times `ratio`.
-      auto pv = [&](int x, float ratio, auto apart) {
+      // dim, two consecutive tokens).  ONLY: -1, or the half of the tile whose tokens
+      // are taken.  APART: the sums are made on their own and added times `ratio`.
+      auto pv = [&](int x, float ratio, auto apart, auto only) {
         constexpr bool kApart = decltype(apart)::value;
+        constexpr int kOnly = decltype(only)::value;
         // P^T (tokens x heads) -> B fragment (k = token, n = head)
-        const uint32_t pb0 = movmatrix_trans(pack2<__half>(s[x][0], s[x][1]));
-        const uint32_t pb1 = movmatrix_trans(pack2<__half>(s[x][2], s[x][3]));
+        const uint32_t pb0 = kOnly == 1 ? 0u : movmatrix_trans(pack2<__half>(s[x][0], s[x][1]));
+        const uint32_t pb1 = kOnly == 0 ? 0u : movmatrix_trans(pack2<__half>(s[x][2], s[x][3]));
         const int left = nvalid - 16 * x;
 #pragma unroll
         for (int hf = 0; hf < C::kHalves; ++hf) {
@@ -825,7 +868,8 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
       };
       // A much larger V scale becomes the reference (the sums shrink by a power
       // of two); a much smaller one is added apart.
-      const float vmax = fmaxf(sc.z, sc.w);
+      float vmax = fmaxf(vsc[0], vsc[1]);
+      if constexpr (NP == 2) vmax = fmaxf(vmax, fmaxf(vsc[2], vsc[3]));
       if (vmax > vref * 16.f) {
         const float r = vref * pow2_inverse(vmax);
         vref = vmax;
@@ -839,17 +883,28 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
               for (int e = 0; e < 4; ++e) o[hf][j][e] *= r;
         }
       }
-      const float r0 = sc.z * vinv, r1 = sc.w * vinv;
-      if (fminf(r0, r1) >= 0.015625f) {
-        if (r0 != 1.f || r1 != 1.f) {
+      float r[2 * NP], rmin = INFINITY, rmax = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[0][e] *= r0, s[1][e] *= r1;
+      for (int p = 0; p < 2 * NP; ++p) r[p] = vsc[p] * vinv, rmin = fminf(rmin, r[p]), rmax = fmaxf(rmax, r[p]);
+      using Both = std::integral_constant<int, -1>;
+      if (rmin >= 0.015625f) {
+        if (rmin != 1.f || rmax != 1.f) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[x][e] *= r[x * NP + (e >> 1) * (NP - 1)];
         }
-        pv(0, 1.f, std::false_type());
-        pv(1, 1.f, std::false_type());
+        pv(0, 1.f, std::false_type(), Both());
+        pv(1, 1.f, std::false_type(), Both());
+      } else if constexpr (NP == 1) {
+        pv(0, r[0], std::true_type(), Both());
+        pv(1, r[1], std::true_type(), Both());
       } else {
-        pv(0, r0, std::true_type());
-        pv(1, r1, std::true_type());
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          pv(x, r[2 * x], std::true_type(), std::integral_constant<int, 0>());
+          pv(x, r[2 * x + 1], std::true_type(), std::integral_constant<int, 1>());
+        }
       }
       ++taken;
       __syncwarp();
@@ -1368,27 +1423,27 @@ __global__ void __launch_bounds__(kReduceThreads) fp8_decode_reduce_kernel(const
 // host side
 // ---------------------------------------------------------------------------
 // The tensor-core kernel: 16-bit q, pool rows of whole 16-byte units (a tensor
-// map's stride), whole 16-token tiles in a block, and pool rows within the
+// map's stride), whole 8-token pieces in a block, and pool rows within the
 // tensor map's 32-bit coordinates.  Columns behind head_dim lie outside the map,
 // so that the copies fill them with zeros; they cost products but no bytes.
 bool use_tc(const bl_paged_layer& kv) {
   const double rows = (double)kv.num_layers * kv.num_blocks * kv.num_kv_heads * kv.block_size;
   return (kv.dtype == BL_BF16 || kv.dtype == BL_F16) && kv.head_dim % 16 == 0 && kv.head_dim <= 256 &&
-         kv.block_size % 16 == 0 && rows <= (double)INT32_MAX;
+         kv.block_size % 8 == 0 && rows <= (double)INT32_MAX;
 }
 
-template <typename T, int D>
+template <typename T, int D, int NP>
 int launch_tc(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
   using C = Cfg<D>;
   CUtensorMap kmap, vmap;
   const uint64_t rows = (uint64_t)kv.num_layers * kv.num_blocks * kv.num_kv_heads * kv.block_size;
   const uint64_t row_bytes = (uint64_t)kv.head_dim;
-  if (!make_tmap_rows_8bit(&kmap, kv.k_pool, row_bytes, rows, C::kRow, 16) ||
-      !make_tmap_rows_8bit(&vmap, kv.v_pool, row_bytes, rows, C::kRow, 16))
+  if (!make_tmap_rows_8bit(&kmap, kv.k_pool, row_bytes, rows, C::kRow, 16 / NP) ||
+      !make_tmap_rows_8bit(&vmap, kv.v_pool, row_bytes, rows, C::kRow, 16 / NP))
     return BL_ERR_LAUNCH;
   const auto smem_for = [](int g) {
     const size_t heads = std::min(g, 8);
-    return 1024 + (size_t)kNW * C::kDepth * C::kSlot + sizeof(TCShared<D>) + 2 * C::kKS * 4 * heads * sizeof(uint2) +
+    return 1024 + (size_t)kNW * C::kDepth * C::kSlot + sizeof(TCShared<D, NP>) + 2 * C::kKS * 4 * heads * sizeof(uint2) +
            (size_t)(kNW - 1) * C::kVecs * 8 * ((heads + 1) / 2) * sizeof(float4);
   };
   const size_t smem = smem_for(k.g);
@@ -1403,9 +1458,9 @@ int launch_tc(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
     int* slot = dev >= 0 && dev < 64 ? &occ_cache[dev][std::min(k.g, 8)] : &occ;
     if (*slot == 0) {
       int o = 0;
-      if (cudaFuncSetAttribute(fp8_decode_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      if (cudaFuncSetAttribute(fp8_decode_tc_kernel<T, D, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                (int)smem_for(8)) != cudaSuccess ||
-          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&o, fp8_decode_tc_kernel<T, D>, kThreadsTC, smem) !=
+          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&o, fp8_decode_tc_kernel<T, D, NP>, kThreadsTC, smem) !=
               cudaSuccess) {
         set_error("fp8_decode_tc_kernel: %s", cudaGetErrorString(cudaGetLastError()));
         return BL_ERR_LAUNCH;
@@ -1415,12 +1470,19 @@ int launch_tc(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
     occ = *slot;
   }
   const int64_t grid = std::min<int64_t>((int64_t)num_sms() * occ, items);
-  if (launch_pdl(fp8_decode_tc_kernel<T, D>, dim3((unsigned)grid), dim3(kThreadsTC), smem, s, k, kmap, vmap) !=
+  if (launch_pdl(fp8_decode_tc_kernel<T, D, NP>, dim3((unsigned)grid), dim3(kThreadsTC), smem, s, k, kmap, vmap) !=
       cudaSuccess) {
     set_error("fp8_decode_tc_kernel: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
     return BL_ERR_LAUNCH;
   }
   return BL_OK;
+}
+
+template <typename T, int NP>
+int launch_tc_dims(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
+  return k.d <= 64    ? launch_tc<T, 64, NP>(k, kv, s)
+         : k.d <= 128 ? launch_tc<T, 128, NP>(k, kv, s)
+                      : launch_tc<T, 256, NP>(k, kv, s);
 }
 
 template <typename T, int HG>
@@ -1448,7 +1510,7 @@ int launch_all(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
   int rc = BL_ERR_UNSUPPORTED;
   if constexpr (sizeof(T) == 2) {
     if (use_tc(kv))
-      rc = k.d <= 64 ? launch_tc<T, 64>(k, kv, s) : k.d <= 128 ? launch_tc<T, 128>(k, kv, s) : launch_tc<T, 256>(k, kv, s);
+      rc = k.bs % 16 == 0 ? launch_tc_dims<T, 1>(k, kv, s) : launch_tc_dims<T, 2>(k, kv, s);
     else
       rc = launch_simt<T>(k, s);
   } else {

@@ -103,6 +103,40 @@ def test_decode_scales_far_apart(cuda, native_lib, spread):
         check_decode(ops.paged_decode_fp8(q, *pool.args, 0, bt, i32([n], cuda), n), q, pool, table, [n], 0)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("bs,d", [(8, 64), (8, 128), (8, 256), (8, 80), (24, 128), (40, 64), (72, 128)])
+def test_decode_blocks_of_eights(cuda, native_lib, dtype, bs, d):
+    """A 16-token tile that lies in two blocks; rows that end in either of them, stale NaN codes behind."""
+    lens = [1, 7, 8, 9, 0, 15, 16, 17, 24, 25, 40, 505, 511, 513, 521, 1100]
+    pool, table, bt = filled(cuda, lens, 2, bs, d, dtype, seed=bs + d)
+    q = torch.randn(len(lens), 8, d, generator=torch.Generator().manual_seed(d)).to(dtype).to(cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = ops.paged_decode_fp8(q, *pool.args, 1, bt, i32(lens, cuda), 1100, err=err)
+    assert int(err) == 0
+    check_decode(out, q, pool, table, lens, 1)
+    for b in (3, 13):  # alone and in the batch
+        one = ops.paged_decode_fp8(q[b:b + 1], *pool.args, 1, bt[b:b + 1], i32(lens[b:b + 1], cuda), lens[b])
+        assert torch.equal(one, out[b:b + 1])
+
+
+@pytest.mark.parametrize("bs", [8, 24])
+def test_decode_scales_far_apart_within_a_tile(cuda, native_lib, bs):
+    rs = np.random.RandomState(bs)
+    n, h, d = 700, 2, 128
+    pool = Pool(cuda, 1, 100, h, bs, d)
+    table = pool.table([n])
+    bt = torch.from_numpy(table).to(cuda)
+    size = np.exp2(np.repeat(rs.uniform(-12, 12, (h, 100)), bs, axis=1)[:, :n, None])
+    k = rs.randn(1, h, n, d).astype(np.float32)
+    v = (rs.randn(h, n, d) * size).astype(np.float32)[None]
+    v[0, 0, 8 * bs:9 * bs] = 0.0
+    ops.paged_append_fp8(*pool.args, 0, bt, i32([0], cuda), torch.from_numpy(k).to(cuda), torch.from_numpy(v).to(cuda))
+    pool.download()
+    for dtype in (BF16, F16):
+        q = (3 * torch.randn(1, 8, d, generator=torch.Generator().manual_seed(1))).to(dtype).to(cuda)
+        check_decode(ops.paged_decode_fp8(q, *pool.args, 0, bt, i32([n], cuda), n), q, pool, table, [n], 0)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("factor", [0.0, 2.0 ** -40, 30.0])
 def test_decode_q_magnitudes(cuda, native_lib, dtype, factor):
