@@ -1040,33 +1040,11 @@ constexpr int kSimtTok = 4;    // tokens a lane group has in hand
 __host__ __device__ constexpr int simt_ctas(int heads) { return heads == 4 ? 2 : heads == 2 ? 3 : 4; }
 constexpr int kSimtHeads = 4;  // query heads of an item, at most
 
-// two fp32 values side by side: one instruction multiplies and adds both
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 f2(float x, float y) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ float2 un2(F2 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // the four codes of a word, times s
-__device__ __forceinline__ void decode4(uint32_t w, F2 s, F2 (&x)[2]) {
+__device__ __forceinline__ void decode4(uint32_t w, uint64_t s, uint64_t (&x)[2]) {
   const float2 lo = unpack2<__half>(e4m3lo_to_f16x2(w)), hi = unpack2<__half>(e4m3hi_to_f16x2(w));
-  x[0] = mul2(f2(lo.x, lo.y), s);
-  x[1] = mul2(f2(hi.x, hi.y), s);
+  x[0] = f2_mul(f2_pack(lo.x, lo.y), s);
+  x[1] = f2_mul(f2_pack(hi.x, hi.y), s);
 }
 
 template <int HG>
@@ -1085,7 +1063,8 @@ struct alignas(16) SimtShared {
 // own, and the groups and warps are joined once per chunk.  K codes of the next
 // step are on their way during the V half of this one, V codes during the K half.
 // What bounds it (64 requests of 1k..8k tokens, 32 / 8 heads of 128 dims, fp32 q,
-// 617 MB): SIMT_MEASURED.
+// 617 MB): issue slots and latency, 352 us, 1.75 TB/s; 2 and 1 heads
+// a KV head 2.3 and 3.9 TB/s.  (Through fp32 tiles in shared memory: 889 us.)
 // WIDE: head_dim and the pool's rows in whole 16-byte units.
 template <typename T, int HG, bool WIDE>
 __global__ void __launch_bounds__(kSimtThreads, simt_ctas(HG)) fp8_decode_simt_kernel(const Args a) {
@@ -1166,7 +1145,7 @@ __global__ void __launch_bounds__(kSimtThreads, simt_ctas(HG)) fp8_decode_simt_k
     __syncthreads();
 
     float m[HG], l[HG];
-    F2 o[HG][8];
+    uint64_t o[HG][8];
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
       m[h] = -INFINITY;
@@ -1182,19 +1161,19 @@ __global__ void __launch_bounds__(kSimtThreads, simt_ctas(HG)) fp8_decode_simt_k
       float s[kSimtTok][HG];
       float vs[kSimtTok];
       {
-        F2 z[kSimtTok][HG], ks[kSimtTok];
+        uint64_t z[kSimtTok][HG], ks[kSimtTok];
 #pragma unroll
         for (int u = 0; u < kSimtTok; ++u) {
           const int t = at + (u * kSimtWarps + warp) * tpw + grp;
           const float x = t < kChunk ? sh.ks[t] : 0.f;
           vs[u] = t < kChunk ? sh.vs[t] : 0.f;
-          ks[u] = f2(x, x);
+          ks[u] = f2_pack(x, x);
 #pragma unroll
           for (int h = 0; h < HG; ++h) z[u][h] = 0ull;
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          F2 q[HG][2];
+          uint64_t q[HG][2];
 #pragma unroll
           for (int h = 0; h < HG; ++h) {
             const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&sh.q[h][c][lt]);
@@ -1202,10 +1181,10 @@ __global__ void __launch_bounds__(kSimtThreads, simt_ctas(HG)) fp8_decode_simt_k
           }
 #pragma unroll
           for (int u = 0; u < kSimtTok; ++u) {
-            F2 x[2];
+            uint64_t x[2];
             decode4(c == 0 ? kc[u].x : c == 1 ? kc[u].y : c == 2 ? kc[u].z : kc[u].w, ks[u], x);
 #pragma unroll
-            for (int h = 0; h < HG; ++h) z[u][h] = fma2(x[1], q[h][1], fma2(x[0], q[h][0], z[u][h]));
+            for (int h = 0; h < HG; ++h) z[u][h] = f2_fma(x[1], q[h][1], f2_fma(x[0], q[h][0], z[u][h]));
           }
         }
         load(a.k_pool, at + step, kc);
@@ -1213,7 +1192,7 @@ __global__ void __launch_bounds__(kSimtThreads, simt_ctas(HG)) fp8_decode_simt_k
         for (int u = 0; u < kSimtTok; ++u)
 #pragma unroll
           for (int h = 0; h < HG; ++h) {
-            const float2 x = un2(z[u][h]);
+            const float2 x = f2_unpack(z[u][h]);
             s[u][h] = x.x + x.y;
           }
       }
@@ -1245,9 +1224,9 @@ __global__ void __launch_bounds__(kSimtThreads, simt_ctas(HG)) fp8_decode_simt_k
           const float al = top[h] == m[h] ? 1.f : fast_exp2(m[h] - top[h]);
           m[h] = top[h];
           l[h] *= al;
-          const F2 al2 = f2(al, al);
+          const uint64_t al2 = f2_pack(al, al);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) o[h][j] = mul2(o[h][j], al2);
+          for (int j = 0; j < 8; ++j) o[h][j] = f2_mul(o[h][j], al2);
         }
       }
 #pragma unroll
@@ -1261,18 +1240,18 @@ __global__ void __launch_bounds__(kSimtThreads, simt_ctas(HG)) fp8_decode_simt_k
       }
 #pragma unroll
       for (int u = 0; u < kSimtTok; ++u) {
-        const F2 v2 = f2(vs[u], vs[u]);
-        F2 p[HG];
+        const uint64_t v2 = f2_pack(vs[u], vs[u]);
+        uint64_t p[HG];
 #pragma unroll
-        for (int h = 0; h < HG; ++h) p[h] = f2(s[u][h], s[u][h]);
+        for (int h = 0; h < HG; ++h) p[h] = f2_pack(s[u][h], s[u][h]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          F2 x[2];
+          uint64_t x[2];
           decode4(c == 0 ? vc[u].x : c == 1 ? vc[u].y : c == 2 ? vc[u].z : vc[u].w, v2, x);
 #pragma unroll
           for (int h = 0; h < HG; ++h) {
-            o[h][2 * c] = fma2(p[h], x[0], o[h][2 * c]);
-            o[h][2 * c + 1] = fma2(p[h], x[1], o[h][2 * c + 1]);
+            o[h][2 * c] = f2_fma(p[h], x[0], o[h][2 * c]);
+            o[h][2 * c + 1] = f2_fma(p[h], x[1], o[h][2 * c + 1]);
           }
         }
       }
@@ -1291,8 +1270,8 @@ __global__ void __launch_bounds__(kSimtThreads, simt_ctas(HG)) fp8_decode_simt_k
         l[h] = w * l[h] + ow * ol;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const F2 x = __shfl_xor_sync(0xffffffffu, o[h][j], off);
-          o[h][j] = fma2(f2(ow, ow), x, mul2(f2(w, w), o[h][j]));
+          const uint64_t x = __shfl_xor_sync(0xffffffffu, o[h][j], off);
+          o[h][j] = f2_fma(f2_pack(ow, ow), x, f2_mul(f2_pack(w, w), o[h][j]));
         }
       }
     }

@@ -3,7 +3,7 @@
 // K and V are code * scale (fp8.cuh).  Reference counterpart: the prefill SDPA of
 // src/barellm/attention/backend.py:52-61 over a dense read of the cache.
 //
-// Two ways, chosen by shape (use_tc below):
+// Three ways, chosen by shape (use_tc below):
 //   expand + prefill_tc_kernel  16-bit q, head_dim a multiple of 8 up to 128.  The rows' pages are
 //       dequantised once into a 16-bit paged scratch (exact in bf16: a code has
 //       four significant bits), which the tcgen05 kernel of prefill_tc.cu then
@@ -16,6 +16,7 @@
 //       with the same contents and a group of 8, 4, 2 or 1.  A head_dim below
 //       128 is widened with zeros, which change neither scores nor outputs: K
 //       and V on the way, q and out through copies.
+//   fp8_prefill_mma_kernel      16-bit q, head_dim a multiple of 16 from 144 to 256.
 //   fp8_prefill_simt_kernel     any element type, head_dim <= 256, block size
 //       and group: 64 queries x 64 keys a tile in fp32, pages dequantised
 //       into shared memory.
@@ -43,6 +44,10 @@ struct Scratch {
 
 bool use_tc(int32_t dtype, int64_t d) {
   return (dtype == BL_BF16 || dtype == BL_F16) && d > 0 && d <= kTCDim && d % 8 == 0;
+}
+
+bool use_mma(int32_t dtype, int64_t d) {
+  return (dtype == BL_BF16 || dtype == BL_F16) && d > kTCDim && d <= 256 && d % 16 == 0;
 }
 
 // False when the scratch would not fit the tcgen05 kernel's 32-bit row coordinates.
@@ -253,6 +258,281 @@ int launch_widen(const WidenArgs& k, cudaStream_t s) {
   fp8_widen_kernel<T, IN><<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(k);
   BL_CHECK_LAUNCH("fp8_widen_kernel");
   return BL_OK;
+}
+
+// ---------------------------------------------------------------------------
+// head_dims above 128: mma.sync kernel
+// ---------------------------------------------------------------------------
+constexpr int kMmaRows = 128, kMmaKeys = 64;  // query rows and keys of a tile
+constexpr int kMmaDim = 256;
+constexpr int kMmaThreads = 256;  // a warp has 16 query rows
+constexpr int kMmaRow = kMmaDim * 2;  // bytes of a 16-bit row in shared memory
+
+struct MmaArgs {
+  const void* q;
+  int64_t q_sb, q_st, q_sh;
+  void* out;
+  int64_t o_sb, o_st, o_sh;
+  const int32_t* q_offsets;
+  const int32_t* seq_lens;
+  const uint8_t* k_pool;
+  const uint8_t* v_pool;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* block_tables;
+  int64_t bt_stride, bt_width;
+  const int32_t* row_ids;
+  int64_t num_blocks, layer, max_q;
+  int32_t hkv, g, bs, d;
+  int32_t q_vec, o_pair;  // q rows can be read 16 bytes at a time, out rows written two elements at a time
+  float scale_log2;
+  int32_t* err;
+};
+
+struct MmaShared {
+  uint8_t q[kMmaRows * kMmaRow];
+  uint8_t k[kMmaKeys * kMmaRow], v[kMmaKeys * kMmaRow];     // the tile, in q's type
+  uint8_t kc[kMmaKeys * kMmaDim], vc[kMmaKeys * kMmaDim];   // its codes, or the next tile's on their way
+  int64_t row[2][kMmaKeys];                                 // byte offset of a token's codes, -1: none
+  float ks[2][kMmaKeys], vs[2][kMmaKeys];
+};
+
+// byte offset of 16-byte chunk c of row r: rows are 512 bytes, and eight rows'
+// equal chunks lie in different banks
+__device__ __forceinline__ uint32_t mma_at(int r, int c) { return (uint32_t)(r * kMmaRow + ((c ^ (r & 7)) << 4)); }
+
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// S = Q K^T and O += P V on mma.sync, 128 query rows by 64 keys a tile.  The rows
+// of a tile are (token, head of the group) pairs, so that one pass over the keys
+// serves the whole group and a short chunk still fills a tile.  Codes come by
+// cp.async while the tile before is worked on and become 16-bit rows once per tile.
+// (The tcgen05 kernel's tile for 128 dims does not fit 256: its rings of 16-bit
+// keys and values would need 256 KB.)  What bounds it: the phases of a tile (widen,
+// scores, softmax, values) wait for one another, with 8 warps on an SM.  4 chunks
+// of 256..1024 tokens over 0..4k, 32 / 8 heads of 256 dims, bf16, 181 GFLOP: 1.02 ms,
+// 177 TFLOP/s (the fp32 SIMT kernel below: 11.0 ms).
+// grid: (ceil(max_q * g / kMmaRows), hkv, batch)
+template <typename T>
+__global__ void __launch_bounds__(kMmaThreads, 1) fp8_prefill_mma_kernel(const MmaArgs a) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  MmaShared* sh = reinterpret_cast<MmaShared*>(smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t b = blockIdx.z;
+  const int h = blockIdx.y;
+  int64_t qo = 0, nq = a.max_q;
+  if (a.q_offsets) {
+    qo = a.q_offsets[b];
+    nq = (int64_t)a.q_offsets[b + 1] - qo;
+  }
+  const int64_t r0 = ((int64_t)gridDim.x - 1 - blockIdx.x) * kMmaRows;  // the tiles with most keys first
+  const int64_t rows = nq * a.g;
+  if (r0 >= rows) return;
+  const int64_t len = a.seq_lens[b], prefix = len - nq;
+  const int64_t kend = prefix + (min(r0 + kMmaRows, rows) - 1) / a.g + 1;  // keys that the last row sees
+  const int64_t trow = a.row_ids ? (int64_t)a.row_ids[b] : b;
+  const int chunks = a.d / 16;  // 16-byte chunks of a token's codes
+
+  auto locate = [&](int64_t k0, int buf) {
+    if (tid >= kMmaKeys) return;
+    const int64_t t = k0 + tid;
+    int64_t r = -1;
+    float ks = 0.f, vs = 0.f;
+    if (t < kend) {
+      const int64_t lb = t / a.bs;
+      if (lb >= a.bt_width) {
+        raise_dev(a.err, BL_DEVERR_TABLE);
+      } else {
+        const int64_t phys = a.block_tables[trow * a.bt_stride + lb];
+        if (phys < 0 || phys >= a.num_blocks) {
+          raise_dev(a.err, BL_DEVERR_BLOCK_ID);
+        } else {
+          const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + h;
+          r = (slot * a.bs + (t - lb * a.bs)) * a.d;
+          ks = a.k_scale[slot];
+          vs = a.v_scale[slot];
+        }
+      }
+    }
+    sh->row[buf][tid] = r;
+    sh->ks[buf][tid] = ks;
+    sh->vs[buf][tid] = vs;
+  };
+  auto fetch = [&](int buf) {
+    for (int e = tid; e < kMmaKeys * 16; e += kMmaThreads) {
+      const int t = e >> 4, c = e & 15;
+      const int64_t r = sh->row[buf][t];
+      if (r >= 0 && c < chunks) {
+        copy16_async(smem_u32(sh->kc + t * kMmaDim + c * 16), a.k_pool + r + c * 16);
+        copy16_async(smem_u32(sh->vc + t * kMmaDim + c * 16), a.v_pool + r + c * 16);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto widen = [&](const uint8_t* codes, uint8_t* to, const float* scale, int buf) {
+    for (int e = tid; e < kMmaKeys * 16; e += kMmaThreads) {
+      const int t = e >> 4, c = e & 15;
+      union {
+        T t[16];
+        uint4 u[2];
+      } x;
+      x.u[0] = x.u[1] = make_uint4(0u, 0u, 0u, 0u);
+      if (sh->row[buf][t] >= 0 && c < chunks) {
+        const uint4 w = *reinterpret_cast<const uint4*>(codes + t * kMmaDim + c * 16);
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+        const float s = scale[t];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 lo = unpack2<__half>(e4m3lo_to_f16x2(ww[i])), hi = unpack2<__half>(e4m3hi_to_f16x2(ww[i]));
+          x.t[4 * i] = dequant_to<T>(lo.x * s), x.t[4 * i + 1] = dequant_to<T>(lo.y * s);
+          x.t[4 * i + 2] = dequant_to<T>(hi.x * s), x.t[4 * i + 3] = dequant_to<T>(hi.y * s);
+        }
+      }
+      *reinterpret_cast<uint4*>(to + mma_at(t, 2 * c)) = x.u[0];
+      *reinterpret_cast<uint4*>(to + mma_at(t, 2 * c + 1)) = x.u[1];
+    }
+  };
+
+  locate(0, 0);
+  // the tile's query rows, zeros behind the last one and behind head_dim
+  for (int e = tid; e < kMmaRows * 32; e += kMmaThreads) {
+    const int i = e >> 5, c = e & 31;
+    const int64_t r = r0 + i;
+    union {
+      T t[8];
+      uint4 u;
+    } x;
+    x.u = make_uint4(0u, 0u, 0u, 0u);
+    if (r < rows && c < 2 * chunks) {
+      const int64_t t = r / a.g;
+      const T* p = reinterpret_cast<const T*>(a.q) + b * a.q_sb + (qo + t) * a.q_st + (h * a.g + (r - t * a.g)) * a.q_sh + c * 8;
+      if (a.q_vec) {
+        x.u = *reinterpret_cast<const uint4*>(p);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x.t[j] = p[j];
+      }
+    }
+    *reinterpret_cast<uint4*>(sh->q + mma_at(i, c)) = x.u;
+  }
+  __syncthreads();
+  fetch(0);
+
+  const int g_row = lane >> 2, t4 = lane & 3;
+  // the lane's two rows; the last key each sees
+  int64_t last[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t r = r0 + warp * 16 + g_row + 8 * i;
+    last[i] = r < rows ? prefix + r / a.g : -1;
+  }
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float o[kMmaDim / 8][4];
+#pragma unroll
+  for (int j = 0; j < kMmaDim / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+
+  const uint32_t qs = smem_u32(sh->q), ks = smem_u32(sh->k), vs = smem_u32(sh->v);
+  const int q_row = warp * 16 + (lane & 15), q_half = lane >> 4;
+  const int k_row = (lane & 7) + ((lane & 16) >> 1), k_half = (lane >> 3) & 1;
+  const int v_row = lane & 15, v_half = lane >> 4;
+
+  int buf = 0;
+  for (int64_t k0 = 0; k0 < kend; k0 += kMmaKeys, buf ^= 1) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // the codes are here; the tile before is no longer read
+    widen(sh->kc, sh->k, sh->ks[buf], buf);
+    widen(sh->vc, sh->v, sh->vs[buf], buf);
+    locate(k0 + kMmaKeys, buf ^ 1);
+    __syncthreads();
+    fetch(buf ^ 1);
+
+    float s[kMmaKeys / 8][4];
+#pragma unroll
+    for (int j = 0; j < kMmaKeys / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < kMmaDim / 16; ++c) {
+      uint32_t q0, q1, q2, q3;
+      ldmatrix_x4(qs + mma_at(q_row, 2 * c + q_half), q0, q1, q2, q3);
+#pragma unroll
+      for (int j = 0; j < kMmaKeys / 8; j += 2) {
+        uint32_t b0, b1, b2, b3;
+        ldmatrix_x4(ks + mma_at(j * 8 + k_row, 2 * c + k_half), b0, b1, b2, b3);
+        mma_16816<T>(s[j][0], s[j][1], s[j][2], s[j][3], q0, q1, q2, q3, b0, b1);
+        mma_16816<T>(s[j + 1][0], s[j + 1][1], s[j + 1][2], s[j + 1][3], q0, q1, q2, q3, b2, b3);
+      }
+    }
+    // softmax in log2 units; keys that a row does not see, or that cannot be read, are out
+    float mx[2] = {m[0], m[1]};
+#pragma unroll
+    for (int j = 0; j < kMmaKeys / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = j * 8 + 2 * t4 + (e & 1), i = e >> 1;
+        s[j][e] = k0 + key <= last[i] && sh->row[buf][key] >= 0 ? s[j][e] * a.scale_log2 : -INFINITY;
+        mx[i] = fmaxf(mx[i], s[j][e]);
+      }
+    float al[2], unit[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+      al[i] = mx[i] == m[i] ? 1.f : fast_exp2(m[i] - mx[i]);
+      unit[i] = mx[i] == -INFINITY ? 0.f : mx[i];
+      m[i] = mx[i];
+      l[i] *= al[i];
+    }
+    if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+#pragma unroll
+      for (int j = 0; j < kMmaDim / 8; ++j) o[j][0] *= al[0], o[j][1] *= al[0], o[j][2] *= al[1], o[j][3] *= al[1];
+    }
+#pragma unroll
+    for (int c = 0; c < kMmaKeys / 16; ++c) {
+      uint32_t p[4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float(&y)[4] = s[2 * c + x];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[e] = fast_exp2(y[e] - unit[e >> 1]);
+          l[e >> 1] += y[e];
+        }
+        p[2 * x] = pack2<T>(y[0], y[1]);
+        p[2 * x + 1] = pack2<T>(y[2], y[3]);
+      }
+#pragma unroll
+      for (int j = 0; j < kMmaDim / 8; j += 2) {
+        uint32_t b0, b1, b2, b3;
+        ldmatrix_x4_trans(vs + mma_at(c * 16 + v_row, j + v_half), b0, b1, b2, b3);
+        mma_16816<T>(o[j][0], o[j][1], o[j][2], o[j][3], p[0], p[1], p[2], p[3], b0, b1);
+        mma_16816<T>(o[j + 1][0], o[j + 1][1], o[j + 1][2], o[j + 1][3], p[0], p[1], p[2], p[3], b2, b3);
+      }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    const int64_t r = r0 + warp * 16 + g_row + 8 * i;
+    if (r >= rows) continue;
+    const int64_t t = r / a.g;
+    T* dst = reinterpret_cast<T*>(a.out) + b * a.o_sb + (qo + t) * a.o_st + (h * a.g + (r - t * a.g)) * a.o_sh;
+    const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];  // 0: no key seen; a NaN sum stays NaN
+#pragma unroll
+    for (int j = 0; j < kMmaDim / 8; ++j) {
+      const int d = j * 8 + 2 * t4;
+      if (d >= a.d) break;
+      const float x = o[j][2 * i] * inv, y = o[j][2 * i + 1] * inv;
+      if (a.o_pair) {
+        *reinterpret_cast<uint32_t*>(dst + d) = pack2<T>(x, y);
+      } else {
+        dst[d] = from_f32<T>(x);
+        dst[d + 1] = from_f32<T>(y);
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -528,6 +808,49 @@ int launch_simt(const bl_prefill_fp8_args& a, cudaStream_t s) {
 }
 
 template <typename T>
+int launch_mma(const bl_prefill_fp8_args& a, cudaStream_t s) {
+  const bl_paged_layer& kv = a.layer.kv;
+  MmaArgs k;
+  k.q = a.q;
+  k.q_sb = a.q_stride_b, k.q_st = a.q_stride_t, k.q_sh = a.q_stride_h;
+  k.out = a.out;
+  k.o_sb = a.out_stride_b, k.o_st = a.out_stride_t, k.o_sh = a.out_stride_h;
+  k.q_offsets = a.q_offsets;
+  k.seq_lens = a.seq_lens;
+  k.k_pool = (const uint8_t*)kv.k_pool;
+  k.v_pool = (const uint8_t*)kv.v_pool;
+  k.k_scale = a.layer.k_scale;
+  k.v_scale = a.layer.v_scale;
+  k.block_tables = kv.block_tables;
+  k.bt_stride = kv.bt_stride;
+  k.bt_width = kv.bt_width;
+  k.row_ids = kv.row_ids;
+  k.num_blocks = kv.num_blocks;
+  k.layer = kv.layer;
+  k.max_q = a.max_q_len;
+  k.hkv = (int32_t)kv.num_kv_heads;
+  k.g = (int32_t)(a.num_q_heads / kv.num_kv_heads);
+  k.bs = (int32_t)kv.block_size;
+  k.d = (int32_t)kv.head_dim;
+  k.q_vec = ((uintptr_t)a.q & 15) == 0 && a.q_stride_b % 8 == 0 && a.q_stride_t % 8 == 0 && a.q_stride_h % 8 == 0;
+  k.o_pair = ((uintptr_t)a.out & 3) == 0 && a.out_stride_b % 2 == 0 && a.out_stride_t % 2 == 0 && a.out_stride_h % 2 == 0;
+  k.scale_log2 = a.scale * kLog2e;
+  k.err = a.err;
+  const int64_t tiles = (a.max_q_len * k.g + kMmaRows - 1) / kMmaRows;
+  BL_CHECK_ARG(tiles <= INT32_MAX, "bl_paged_prefill_fp8: too many queries");
+  const size_t smem = sizeof(MmaShared) + 128;
+  if (cudaFuncSetAttribute(fp8_prefill_mma_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+      cudaSuccess) {
+    set_error("fp8_prefill_mma_kernel: %s", cudaGetErrorString(cudaGetLastError()));
+    return BL_ERR_LAUNCH;
+  }
+  fp8_prefill_mma_kernel<T>
+      <<<dim3((unsigned)tiles, (unsigned)k.hkv, (unsigned)a.batch), kMmaThreads, smem, s>>>(k);
+  BL_CHECK_LAUNCH("fp8_prefill_mma_kernel");
+  return BL_OK;
+}
+
+template <typename T>
 int launch_tc(const bl_prefill_fp8_args& a, const Scratch& w, cudaStream_t s) {
   const bl_paged_layer& kv = a.layer.kv;
   char* ws = (char*)a.workspace;
@@ -678,6 +1001,7 @@ extern "C" int bl_paged_prefill_fp8(const bl_prefill_fp8_args* args, void* strea
     BL_CHECK_ARG(((uintptr_t)a.workspace & 255) == 0, "%s: workspace must be 256-byte aligned", who);
     return kv.dtype == BL_BF16 ? launch_tc<__nv_bfloat16>(a, w, s) : launch_tc<__half>(a, w, s);
   }
+  if (use_mma(kv.dtype, kv.head_dim)) return kv.dtype == BL_BF16 ? launch_mma<__nv_bfloat16>(a, s) : launch_mma<__half>(a, s);
   switch (kv.dtype) {
     case BL_F32: return launch_simt<float>(a, s);
     case BL_F16: return launch_simt<__half>(a, s);

@@ -295,7 +295,32 @@ def test_prefill(cuda, native_lib, dtype, hq, hkv, bs, d):
     out = ops.paged_prefill_fp8(q, *pool.args, 1, bt, i32(lens, cuda), max(lens), total_blocks=total, q_offsets=off,
                                 max_q_len=max(chunks), err=err)
     assert int(err) == 0
-    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32 and d <= 128 and d % 8 == 0)
+    # (16-bit shapes of these dims run on the tensor cores, with P rounded to the element type)
+    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32 and d % 8 == 0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hq,hkv,bs,d", [(8, 2, 16, 256), (6, 2, 8, 144), (3, 3, 5, 192), (10, 1, 48, 208)])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_prefill_wide_heads(cuda, native_lib, dtype, hq, hkv, bs, d, pad):
+    """Head dims above 128: rows of (token, head) pairs that end inside a tile, more queries than tokens, strided q and out."""
+    prefixes, chunks = [0, 3, 200, 64, 63, 0], [1, 40, 7, 130, 65, 300]
+    pool, table, bt, lens, _, off = prefill_case(cuda, prefixes, chunks, hq, hkv, bs, d, dtype, seed=hq + d)
+    total = sum(chunks)
+    q = torch.full((1, total, hq, d + pad), float("nan"), dtype=dtype, device=cuda)[..., :d].transpose(1, 2)
+    q.copy_(torch.randn(1, hq, total, d, generator=torch.Generator().manual_seed(d)).to(dtype))
+    whole = torch.full((1, total + 2, hq, d + pad), 9.0, dtype=dtype, device=cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = whole[:, :total, :, :d].transpose(1, 2)
+    ops.paged_prefill_fp8(q, *pool.args, 1, bt, i32(lens, cuda), max(lens), total_blocks=sum(-(-n // bs) for n in lens),
+                          q_offsets=off, max_q_len=max(chunks), out=out, err=err)
+    assert int(err) == 0
+    check_prefill(out, q, pool, table, lens, chunks, 1)
+    assert bool((whole[..., d:] == 9.0).all()) and bool((whole[:, total:] == 9.0).all())
+    # queries that see no key are zeros
+    short = [n if b != 5 else 2 for b, n in enumerate(lens)]
+    ops.paged_prefill_fp8(q, *pool.args, 1, bt, i32(short, cuda), max(lens), q_offsets=off, max_q_len=max(chunks), out=out, err=err)
+    assert int(err) == 0 and bool((out[:, :, sum(chunks[:5]):-2] == 0).all()) and not bool((out[:, :, -2:] == 0).all())
 
 
 @pytest.mark.parametrize("d", [128, 80])
@@ -320,7 +345,8 @@ def test_prefill_queries_that_see_no_key(cuda, native_lib, dtype, d):
     off = i32(np.concatenate([[0], np.cumsum(chunks)]), cuda)
     out = torch.full_like(q, 5.0)
     ops.paged_prefill_fp8(q, *pool.args, 1, bt, i32(lens, cuda), 13, q_offsets=off, max_q_len=300, out=out)
-    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32 and d <= 128 and d % 8 == 0)
+    # (16-bit shapes of these dims run on the tensor cores, with P rounded to the element type)
+    check_prefill(out, q, pool, table, lens, chunks, 1, tc=dtype is not F32 and d % 8 == 0)
     assert bool((out[0, :, :27] == 0).all()) and bool((out[0, :, 40:47] == 0).all())
 
 
