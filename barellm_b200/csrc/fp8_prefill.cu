@@ -579,7 +579,10 @@ size_t simt_smem(int d) {
 }
 
 // S = q K^T and O += P V as outer products in registers: a thread's 4 x 4 block
-// reads 8 float4 of shared memory for 64 multiplies.  Bound by the fp32 pipe.
+// reads 8 float4 of shared memory for 64 multiplies.  4 chunks of 256..1024 tokens
+// over 0..4k, 32 / 8 fp32 heads of 128 dims, 91 GFLOP: 3.7 ms, 24 TFLOP/s, a third of
+// the fp32 pipe.  Packed products (two dims an instruction) and codes fetched a
+// tile ahead by cp.async changed nothing (3.8, 3.7 ms).
 // grid: (ceil(max_q / kBQ), hq, batch).  NC = ceil(head_dim / 64).
 template <typename T, int NC>
 __global__ void __launch_bounds__(kSimtThreads) fp8_prefill_simt_kernel(const SimtArgs a) {
