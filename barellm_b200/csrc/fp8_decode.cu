@@ -208,6 +208,7 @@ struct Args {
   float* ws_o;
   int32_t max_units, has_parts;
   int32_t planned;  // 0: a small call without a plan; every CTA has at most one item
+  int32_t cluster;  // > 0 (a small call): a row's chunks are the CTAs of a cluster of this size, which joins them itself
   int32_t* err;
 };
 
@@ -243,6 +244,24 @@ __device__ __forceinline__ Unit find_unit(const Args& a, int u, int lane, int& u
   r.chunk = u - __shfl_sync(0xffffffffu, incl - n, r.row);
   r.len = __shfl_sync(0xffffffffu, (int)len, r.row);
   r.part = u;
+  r.table_row = a.row_ids ? a.row_ids[r.row] : r.row;
+  return r;
+}
+
+// The unit of this CTA in a call whose clusters are rows.
+__device__ __forceinline__ Unit cluster_unit(const Args& a, bool tell) {
+  Unit r = {};
+  const int c = blockIdx.x / a.cluster;
+  r.chunk = blockIdx.x - c * a.cluster;
+  r.row = c / (a.hkv * a.head_tiles);
+  int64_t len = a.seq_lens[r.row];
+  const int64_t cap = a.bt_width * a.bs;
+  if (len > cap) {
+    if (tell) raise_dev(a.err, BL_DEVERR_TABLE);
+    len = cap;
+  }
+  if (len > (int64_t)a.cluster * kChunk && tell) raise_dev(a.err, BL_DEVERR_WORKSPACE);  // longer than max_seq_len
+  r.len = (int)max(len, (int64_t)0);
   r.table_row = a.row_ids ? a.row_ids[r.row] : r.row;
   return r;
 }
@@ -487,8 +506,67 @@ struct Pending {
   }
 };
 
-template <typename T, int D, int NP>
-__global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float cluster_load(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+constexpr int kMaxCluster = 8;  // the portable size
+constexpr int kReduceWarps = 4;
+
+// Joins the chunks of a row that a cluster holds: o[head][D] and lse[head] of every
+// CTA, in shared memory.  Every thread of the cluster comes here; the outputs
+// are dealt to all of them.  The sums go in the order of fp8_decode_reduce_kernel,
+// so that a row's result is the same in a call of either kind.
+template <typename T, int D>
+__device__ __forceinline__ void cluster_join(const Args& a, const float* o, const float2* lse) {
+  __syncwarp();
+  cluster_sync();
+  const int c = blockIdx.x / a.cluster, rank = blockIdx.x - c * a.cluster;
+  const int per_row = a.hkv * a.head_tiles, b = c / per_row, r = c - b * per_row;
+  const int h = r / a.head_tiles, ht = r - h * a.head_tiles;
+  const int hq0 = h * a.g + ht * a.tile_heads, heads = min(a.tile_heads, a.g - ht * a.tile_heads);
+  const int64_t len = min((int64_t)a.seq_lens[b], a.bt_width * a.bs);
+  const int nch = (int)((max(len, (int64_t)0) + kChunk - 1) / kChunk);
+  if (nch > 1 && nch <= a.cluster) {
+    for (int e = rank * kThreadsTC + (int)threadIdx.x; e < heads * D; e += a.cluster * kThreadsTC) {
+      const int g = e / D, d = e - g * D;
+      if (d >= a.d) continue;
+      float l[kMaxCluster], x[kMaxCluster], M = -INFINITY, den = 0.f;
+      float num[kReduceWarps] = {};
+#pragma unroll
+      for (int i = 0; i < kMaxCluster; ++i) {
+        l[i] = -INFINITY, x[i] = 0.f;
+        if (i < nch) l[i] = cluster_load(cluster_addr(&lse[g].x, i)), x[i] = cluster_load(cluster_addr(o + e, i));
+      }
+#pragma unroll
+      for (int i = 0; i < kMaxCluster; ++i) M = fmaxf(M, l[i]);
+#pragma unroll
+      for (int i = 0; i < kMaxCluster; ++i) {
+        const float w = l[i] == -INFINITY ? 0.f : (l[i] == M ? 1.f : fast_exp2(l[i] - M));
+        num[i % kReduceWarps] += w * x[i], den += w;
+      }
+      static_assert(kReduceWarps == 4, "the order of the sums");
+      const float all = (num[0] + num[1]) + (num[2] + num[3]);
+      reinterpret_cast<T*>(a.out)[(int64_t)b * a.o_sb + (int64_t)(hq0 + g) * a.o_sh + d] =
+          from_f32<T>(den == 0.f ? 0.f : all / den);
+    }
+  }
+  cluster_sync();  // no CTA leaves while another reads its sums
+}
+
+// ROWS: a call whose clusters are rows (a.cluster > 0); at most one CTA per SM then.
+template <typename T, int D, int NP, bool ROWS>
+__global__ void __launch_bounds__(kThreadsTC, D == 128 && !ROWS ? 3 : 1)
     fp8_decode_tc_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using C = Cfg<D>;
   using Shared = TCShared<D, NP>;
@@ -550,7 +628,11 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
         if (!end) unit = n_item > 0 ? load_unit(a, item) : first;
       } else {
         end = n_item > 0;
-        if (!end) {
+        if (!end && ROWS) {
+          unit = cluster_unit(a, lane == 0);
+          item = blockIdx.x / a.cluster;
+          end = unit.chunk * kChunk >= unit.len;
+        } else if (!end) {
           const int per_unit = a.hkv * a.head_tiles;
           int units;
           unit = find_unit(a, (int)(item / per_unit), lane, units);
@@ -577,6 +659,7 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
       a.hdr[6] = 0;
       *claimed = 0;
     }
+    if constexpr (ROWS) cluster_join<T, D>(a, comb, sh->ml[kNW - 1]);
     return;
   }
 
@@ -927,6 +1010,7 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
     }
     const int h0 = 2 * t4, h1 = 2 * t4 + 1;
     const bool holds = h0 < it.heads;
+    const unsigned holders = ROWS ? __ballot_sync(0xffffffffu, holds) : 0u;
     // the previous item's sums have been read (every warp waits here, so no phase is skipped)
     ok = __all_sync(0xffffffffu, wait_or_abort(&sh->comb_free, (n_item & 1) ^ 1, &sh->abort, a.err));
     if (!ok) break;
@@ -985,10 +1069,12 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
             x[0] += w0 * y.x, x[1] += w1 * y.y, x[2] += w0 * y.z, x[3] += w1 * y.w;
           }
       }
+      // (in a cluster the joined sums go where the other warps' were: every lane has read its own)
+      if (ROWS) __syncwarp(holders);
       // sum 0: no token (nothing seen); a NaN sum stays NaN
       const float i0 = L0 == 0.f ? 0.f : 1.f / L0, i1 = L1 == 0.f ? 0.f : 1.f / L1;
       const bool parts = it.nch > 1;
-      if (parts && !has_part(a, it)) {
+      if (parts && !ROWS && !has_part(a, it)) {
         raise_dev(a.err, BL_DEVERR_WORKSPACE);
       } else {
 #pragma unroll
@@ -997,10 +1083,11 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
           const int hq = it.hq0 + (c ? h1 : h0);
           const float inv = c ? i1 : i0;
           T* dst = reinterpret_cast<T*>(a.out) + (int64_t)it.b * a.o_sb + (int64_t)hq * a.o_sh;
-          float* part = a.ws_o + ((int64_t)it.part * a.hq + hq) * a.d;
+          float* part = ROWS ? comb + (c ? h1 : h0) * D : a.ws_o + ((int64_t)it.part * a.hq + hq) * a.d;
+          float* lse = ROWS ? &sh->ml[kNW - 1][c ? h1 : h0].x : a.ws_lse + (int64_t)it.part * a.hq + hq;
           if (parts && g_row == 0)
-            a.ws_lse[(int64_t)it.part * a.hq + hq] = c ? (L1 == 0.f ? -INFINITY : M1 + __log2f(L1))
-                                                       : (L0 == 0.f ? -INFINITY : M0 + __log2f(L0));
+            *lse = c ? (L1 == 0.f ? -INFINITY : M1 + __log2f(L1))
+                     : (L0 == 0.f ? -INFINITY : M0 + __log2f(L0));
 #pragma unroll
           for (int hf = 0; hf < C::kHalves; ++hf)
 #pragma unroll
@@ -1028,6 +1115,7 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 ? 3 : 1)
   // left only where the CTA gave up).
   for (; taken < issued; ++taken)
     if (!mbar_wait(&sh->full[warp][taken % kDepth], (taken / kDepth) & 1)) raise_dev(a.err, BL_DEVERR_TIMEOUT);
+  if constexpr (ROWS) cluster_join<T, D>(a, comb, sh->ml[kNW - 1]);
 }
 
 // ---------------------------------------------------------------------------
@@ -1322,7 +1410,7 @@ __global__ void __launch_bounds__(kSimtThreads, simt_ctas(HG)) fp8_decode_simt_k
 // ---------------------------------------------------------------------------
 // reduce: rows of several chunks
 // ---------------------------------------------------------------------------
-constexpr int kReduceThreads = 128;
+constexpr int kReduceThreads = 32 * kReduceWarps;
 constexpr int kReduceTile = 512;  // chunks whose weights are in shared memory at a time
 
 // grid: (batch, hq).  Warp w sums every fourth chunk, a lane four consecutive
@@ -1411,7 +1499,7 @@ bool use_tc(const bl_paged_layer& kv) {
          kv.block_size % 8 == 0 && rows <= (double)INT32_MAX;
 }
 
-template <typename T, int D, int NP>
+template <typename T, int D, int NP, bool ROWS>
 int launch_tc(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
   using C = Cfg<D>;
   CUtensorMap kmap, vmap;
@@ -1437,9 +1525,9 @@ int launch_tc(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
     int* slot = dev >= 0 && dev < 64 ? &occ_cache[dev][std::min(k.g, 8)] : &occ;
     if (*slot == 0) {
       int o = 0;
-      if (cudaFuncSetAttribute(fp8_decode_tc_kernel<T, D, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      if (cudaFuncSetAttribute(fp8_decode_tc_kernel<T, D, NP, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                (int)smem_for(8)) != cudaSuccess ||
-          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&o, fp8_decode_tc_kernel<T, D, NP>, kThreadsTC, smem) !=
+          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&o, fp8_decode_tc_kernel<T, D, NP, ROWS>, kThreadsTC, smem) !=
               cudaSuccess) {
         set_error("fp8_decode_tc_kernel: %s", cudaGetErrorString(cudaGetLastError()));
         return BL_ERR_LAUNCH;
@@ -1449,19 +1537,31 @@ int launch_tc(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
     occ = *slot;
   }
   const int64_t grid = std::min<int64_t>((int64_t)num_sms() * occ, items);
-  if (launch_pdl(fp8_decode_tc_kernel<T, D, NP>, dim3((unsigned)grid), dim3(kThreadsTC), smem, s, k, kmap, vmap) !=
-      cudaSuccess) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(ROWS ? items : grid));
+  cfg.blockDim = dim3(kThreadsTC);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)k.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ROWS ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, fp8_decode_tc_kernel<T, D, NP, ROWS>, k, kmap, vmap) != cudaSuccess) {
     set_error("fp8_decode_tc_kernel: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
     return BL_ERR_LAUNCH;
   }
   return BL_OK;
 }
 
-template <typename T, int NP>
+template <typename T, int NP, bool ROWS>
 int launch_tc_dims(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
-  return k.d <= 64    ? launch_tc<T, 64, NP>(k, kv, s)
-         : k.d <= 128 ? launch_tc<T, 128, NP>(k, kv, s)
-                      : launch_tc<T, 256, NP>(k, kv, s);
+  return k.d <= 64    ? launch_tc<T, 64, NP, ROWS>(k, kv, s)
+         : k.d <= 128 ? launch_tc<T, 128, NP, ROWS>(k, kv, s)
+                      : launch_tc<T, 256, NP, ROWS>(k, kv, s);
 }
 
 template <typename T, int HG>
@@ -1489,13 +1589,14 @@ int launch_all(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
   int rc = BL_ERR_UNSUPPORTED;
   if constexpr (sizeof(T) == 2) {
     if (use_tc(kv))
-      rc = k.bs % 16 == 0 ? launch_tc_dims<T, 1>(k, kv, s) : launch_tc_dims<T, 2>(k, kv, s);
+      rc = k.bs % 16 == 0 ? (k.cluster ? launch_tc_dims<T, 1, true>(k, kv, s) : launch_tc_dims<T, 1, false>(k, kv, s))
+                          : (k.cluster ? launch_tc_dims<T, 2, true>(k, kv, s) : launch_tc_dims<T, 2, false>(k, kv, s));
     else
       rc = launch_simt<T>(k, s);
   } else {
     rc = launch_simt<T>(k, s);
   }
-  if (rc || !k.has_parts) return rc;
+  if (rc || !k.has_parts || k.cluster) return rc;
   if (launch_pdl(fp8_decode_reduce_kernel<T>, dim3((unsigned)k.batch, (unsigned)k.hq), dim3(kReduceThreads), 0, s, k) !=
       cudaSuccess) {
     set_error("fp8_decode_reduce_kernel: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
@@ -1584,6 +1685,10 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
   // claims that it brings would change nothing (one request of 777 tokens: 14.4 us
   // on the device without it, 20.5 us with it).
   k.planned = !(use_tc(kv) && a.batch <= 32 && (int64_t)k.max_units * k.hkv * k.head_tiles <= num_sms());
+  // Up to kMaxCluster chunks a row, they are joined within a cluster: no join kernel
+  // either (CLUSTER_MEASURED).
+  if (!k.planned && k.has_parts && (a.max_seq_len + kChunk - 1) / kChunk <= kMaxCluster)
+    k.cluster = (int32_t)((a.max_seq_len + kChunk - 1) / kChunk);
   if (k.planned && !a.plan_ready) {
     PlanArgs p;
     p.seq_lens = a.seq_lens;

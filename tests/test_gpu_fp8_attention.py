@@ -217,6 +217,32 @@ def test_decode_many_items(cuda, native_lib, lens, hkv):
     assert int(err) == 0
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hq,hkv,bs,d", [(16, 8, 16, 128), (4, 4, 16, 64), (20, 2, 8, 256), (5, 1, 16, 80)])
+@pytest.mark.parametrize("max_len", [513, 1024, 1025, 2500, 4096])
+def test_decode_small_calls_join_their_chunks(cuda, native_lib, dtype, hq, hkv, bs, d, max_len):
+    """Small calls of up to eight chunks a row: rows of one chunk, of all, of none beside one another; the same bits as
+    with a plan, and as the row alone."""
+    lens = [max_len] if hkv == 8 else [max_len, 1, 512]
+    pool, table, bt = filled(cuda, lens, hkv, bs, d, dtype, seed=d + max_len)
+    q = torch.randn(len(lens), hq, d, generator=torch.Generator().manual_seed(d)).to(dtype).to(cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = torch.full((len(lens), hq, d + 2), 9.0, dtype=dtype, device=cuda)
+    ops.paged_decode_fp8(q, *pool.args, 1, bt, i32(lens, cuda), max_len, out=out[..., :d], err=err)
+    check_decode(out[..., :d], q, pool, table, lens, 1)
+    assert bool((out[..., d:] == 9.0).all())
+    for bound in (4097, 60000):  # a cluster would be too large; a plan
+        assert torch.equal(ops.paged_decode_fp8(q, *pool.args, 1, bt, i32(lens, cuda), bound, err=err), out[..., :d])
+    for b, n in enumerate(lens):
+        assert torch.equal(ops.paged_decode_fp8(q[b:b + 1], *pool.args, 1, bt[b:b + 1], i32([n], cuda), n, err=err), out[b:b + 1, :, :d])
+    lens[-1] = 0
+    assert bool((ops.paged_decode_fp8(q, *pool.args, 1, bt, i32(lens, cuda), max_len, err=err)[-1] == 0).all())
+    assert int(err) == 0
+    # a row longer than the bound is reported
+    ops.paged_decode_fp8(q[:1], *pool.args, 1, bt[:1], i32([max_len], cuda), 512 if max_len <= 1024 else 1024, err=err)
+    assert int(err) == nat.BL_DEVERR_WORKSPACE
+
+
 def test_decode_reports_what_it_cannot_do(cuda, native_lib):
     pool, table, bt = filled(cuda, [40, 600], 2, 16, 128, BF16)
     q = torch.randn(2, 4, 128, device=cuda).to(BF16)
