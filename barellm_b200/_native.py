@@ -50,6 +50,7 @@ EXPORTED = (
     "bl_paged_append_fp8",
     "bl_paged_gather_fp8",
     "bl_paged_decode_fp8_workspace_bytes",
+    "bl_paged_decode_fp8_scratch_bytes",
     "bl_paged_decode_fp8",
     "bl_paged_prefill_fp8_workspace_bytes",
     "bl_paged_prefill_fp8",
@@ -421,6 +422,8 @@ def load() -> ctypes.CDLL:
     lib.bl_paged_gather_fp8.restype = c_int
     lib.bl_paged_decode_fp8_workspace_bytes.argtypes = [c_int64] * 4
     lib.bl_paged_decode_fp8_workspace_bytes.restype = c_size_t
+    lib.bl_paged_decode_fp8_scratch_bytes.argtypes = [c_void_p]  # a packed DecodeFp8Args, or a reference to one
+    lib.bl_paged_decode_fp8_scratch_bytes.restype = c_size_t
     lib.bl_paged_decode_fp8.argtypes = [c_void_p, c_void_p]  # a packed DecodeFp8Args, or a reference to one
     lib.bl_paged_decode_fp8.restype = c_int
     lib.bl_paged_prefill_fp8_workspace_bytes.argtypes = [c_int32] + [c_int64] * 8

@@ -1605,6 +1605,32 @@ int launch_all(const Args& k, const bl_paged_layer& kv, cudaStream_t s) {
   return BL_OK;
 }
 
+// How a call runs, by its sizes.
+struct Way {
+  int tile_heads, head_tiles;
+  int cluster;   // chunks of a row, joined within a cluster; 0: by the join kernel
+  bool planned;
+  bool scratch;  // uses the workspace
+};
+
+Way way_of(const bl_decode_fp8_args& a) {
+  const bl_paged_layer& kv = a.layer.kv;
+  const int64_t g = a.num_q_heads / kv.num_kv_heads, chunks = (a.max_seq_len + kChunk - 1) / kChunk;
+  const bool tc = use_tc(kv);
+  Way w;
+  w.tile_heads = tc ? 8 : (int)std::min<int64_t>(g == 3 ? 4 : g, kSimtHeads);
+  w.head_tiles = (int)((g + w.tile_heads - 1) / w.tile_heads);
+  // A call whose items all fit the GPU at once needs no plan: the order and the
+  // claims that it brings would change nothing (one request of 777 tokens: 14.4 us
+  // on the device without it, 20.5 us with it).
+  w.planned = !(tc && a.batch <= 32 && a.batch * chunks * kv.num_kv_heads * w.head_tiles <= num_sms());
+  // Up to kMaxCluster chunks a row, they are joined within a cluster: no join kernel
+  // and no workspace either (the same request, calls in a row: 18.0 to 11.4 us).
+  w.cluster = !w.planned && chunks > 1 && chunks <= kMaxCluster ? (int)chunks : 0;
+  w.scratch = w.planned || (chunks > 1 && !w.cluster);
+  return w;
+}
+
 }  // namespace
 }  // namespace bl
 
@@ -1614,6 +1640,14 @@ extern "C" size_t bl_paged_decode_fp8_workspace_bytes(int64_t batch, int64_t num
                                                       int64_t max_seq_len) {
   if (batch <= 0 || num_q_heads <= 0 || head_dim <= 0 || max_seq_len <= 0) return 0;
   return ws_layout(batch, num_q_heads, head_dim, max_seq_len).total;
+}
+
+extern "C" size_t bl_paged_decode_fp8_scratch_bytes(const bl_decode_fp8_args* args) {
+  if (!args || check_fp8_layer(args->layer, "bl_paged_decode_fp8_scratch_bytes")) return 0;
+  const bl_decode_fp8_args& a = *args;
+  const bl_paged_layer& kv = a.layer.kv;
+  if (a.batch <= 0 || a.num_q_heads <= 0 || a.num_q_heads % kv.num_kv_heads || a.max_seq_len <= 0) return 0;
+  return way_of(a).scratch ? ws_layout(a.batch, a.num_q_heads, kv.head_dim, a.max_seq_len).total : 0;
 }
 
 extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream) {
@@ -1633,13 +1667,15 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
   BL_CHECK_ARG(((uintptr_t)a.q % es) == 0 && ((uintptr_t)a.out % es) == 0,
                "%s: q/out must be aligned to their element type", who);
   const WsLayout w = ws_layout(a.batch, a.num_q_heads, kv.head_dim, a.max_seq_len);
-  if (!a.workspace || a.workspace_bytes < w.total) {
-    set_error("%s: workspace too small (%zu < %zu bytes)", who, a.workspace ? a.workspace_bytes : (size_t)0, w.total);
-    return BL_ERR_CAPACITY;
-  }
-  BL_CHECK_ARG(((uintptr_t)a.workspace & 255) == 0, "%s: workspace must be 256-byte aligned", who);
   BL_CHECK_ARG(w.max_units <= INT32_MAX, "%s: too many split-K units", who);
-  char* ws = (char*)a.workspace;
+  const Way way = way_of(a);
+  if (way.scratch || a.workspace || a.workspace_bytes) {
+    if (!a.workspace || a.workspace_bytes < w.total) {
+      set_error("%s: workspace too small (%zu < %zu bytes)", who, a.workspace ? a.workspace_bytes : (size_t)0, w.total);
+      return BL_ERR_CAPACITY;
+    }
+    BL_CHECK_ARG(((uintptr_t)a.workspace & 255) == 0, "%s: workspace must be 256-byte aligned", who);
+  }
   cudaStream_t s = (cudaStream_t)stream;
 
   Args k;
@@ -1665,30 +1701,27 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
   k.hq = (int32_t)a.num_q_heads;
   k.hkv = (int32_t)kv.num_kv_heads;
   k.g = k.hq / k.hkv;
-  k.tile_heads = use_tc(kv) ? 8 : std::min(k.g == 3 ? 4 : k.g, kSimtHeads);
-  k.head_tiles = (k.g + k.tile_heads - 1) / k.tile_heads;
+  k.tile_heads = way.tile_heads;
+  k.head_tiles = way.head_tiles;
+  k.planned = way.planned;
+  k.cluster = way.cluster;
   k.bs = (int32_t)kv.block_size;
   k.d = (int32_t)kv.head_dim;
   k.q_vec = (k.d == 64 || k.d == 128 || k.d == 256) && ((uintptr_t)a.q & 7) == 0 && a.q_stride_b % 4 == 0 && a.q_stride_h % 4 == 0;
   k.o_vec = ((uintptr_t)a.out & 7) == 0 && a.out_stride_b % 4 == 0 && a.out_stride_h % 4 == 0;
   k.scale_log2 = a.scale * kLog2e;
-  k.hdr = (int32_t*)(ws + w.hdr);
-  k.row_base = (const int32_t*)(ws + w.row_base);
-  k.units = (const Unit*)(ws + w.units);
-  k.ws_lse = (float*)(ws + w.lse);
-  k.ws_o = (float*)(ws + w.o);
+  char* ws = (char*)a.workspace;
+  if (way.scratch) {
+    k.hdr = (int32_t*)(ws + w.hdr);
+    k.row_base = (const int32_t*)(ws + w.row_base);
+    k.units = (const Unit*)(ws + w.units);
+    k.ws_lse = (float*)(ws + w.lse);
+    k.ws_o = (float*)(ws + w.o);
+  }
   k.max_units = (int32_t)w.max_units;
   k.has_parts = a.max_seq_len > kChunk;
   k.err = a.err;
 
-  // A call whose items all fit the GPU at once needs no plan: the order and the
-  // claims that it brings would change nothing (one request of 777 tokens: 14.4 us
-  // on the device without it, 20.5 us with it).
-  k.planned = !(use_tc(kv) && a.batch <= 32 && (int64_t)k.max_units * k.hkv * k.head_tiles <= num_sms());
-  // Up to kMaxCluster chunks a row, they are joined within a cluster: no join kernel
-  // either (CLUSTER_MEASURED).
-  if (!k.planned && k.has_parts && (a.max_seq_len + kChunk - 1) / kChunk <= kMaxCluster)
-    k.cluster = (int32_t)((a.max_seq_len + kChunk - 1) / kChunk);
   if (k.planned && !a.plan_ready) {
     PlanArgs p;
     p.seq_lens = a.seq_lens;

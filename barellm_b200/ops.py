@@ -862,8 +862,8 @@ def paged_gather_fp8(
     _check(max_len > 0, "KV cache is empty")
     shape = (batch, pool[2], max_len, pool[4])
     if out is None:
-        k_out = torch.empty(shape, dtype=dtype, device=key_cache.device)
-        v_out = torch.empty(shape, dtype=dtype, device=key_cache.device)
+        k_out = key_scale.new_empty(shape, dtype=dtype)
+        v_out = torch.empty_like(k_out)
         st = k_out.stride()
     else:
         k_out, v_out = out
@@ -906,7 +906,7 @@ def paged_decode_fp8(
     The 8-bit form of :func:`paged_decode`.  ``seq_lens`` are post-append
     lengths; a row of length 0 gets zeros.  ``max_seq_len`` is a host-side
     upper bound on them.  ``ws``: at least :func:`decode_fp8_workspace_bytes`;
-    by default every call takes its own from torch's allocator.  With
+    by default a call that needs one takes its own from torch's allocator.  With
     ``plan_ready`` the (required) ``ws`` still holds the plan of an earlier call
     with the same ``seq_lens``, ``row_ids`` (their contents too), table width,
     pool shape, ``max_seq_len`` and q shape, as a step's later layers have it.
@@ -928,7 +928,7 @@ def paged_decode_fp8(
     _vector_i32(seq_lens, dev, batch, "seq_lens")
     _check(max_seq_len > 0, "KV cache is empty")
     if out is None:
-        out = torch.empty(qs, dtype=dtype, device=q.device)
+        out = torch.empty_like(q) if q.dim() == 3 and q.is_contiguous() else q.new_empty(qs)
         ost = (hq * d, d)
     else:
         os_, ost = out.shape, out.stride()
@@ -937,11 +937,20 @@ def paged_decode_fp8(
         _check(tuple(os_) == tuple(qs) and (ost[2] == 1 or d == 1) and out.dtype is dtype and out.get_device() == dev,
                "decode output must be [B, Hq, D] like q, D contiguous")
     _check(ws is not None or not plan_ready, "plan_ready needs the workspace that holds the plan")
-    ws = _scratch(ws, decode_fp8_workspace_bytes(batch, hq, d, max_seq_len), q)
-    a = nat.pack_decode_fp8_args(*fields, q.data_ptr(), qst[0], qst[1], out.data_ptr(), ost[0], ost[1], seq_lens.data_ptr(),
-                                 batch, hq, _softmax_scale(scale, d), 1 if plan_ready else 0, ws.data_ptr(), ws.nbytes,
-                                 max_seq_len, _err_word(err, dev))
-    _call(nat.load().bl_paged_decode_fp8, a, dev)
+    lib = nat.load()
+    fields += (q.data_ptr(), qst[0], qst[1], out.data_ptr(), ost[0], ost[1], seq_lens.data_ptr(), batch, hq,
+               _softmax_scale(scale, d), 1 if plan_ready else 0)
+    word = _err_word(err, dev)
+    if ws is None:
+        a = nat.pack_decode_fp8_args(*fields, 0, 0, max_seq_len, word)
+        nbytes = lib.bl_paged_decode_fp8_scratch_bytes(a)
+        ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    else:
+        _check(ws.get_device() == dev and ws.is_contiguous(), f"ws must be a contiguous tensor on cuda:{dev}")
+        nbytes = ws.nbytes
+    if ws is not None:
+        a = nat.pack_decode_fp8_args(*fields, ws.data_ptr(), nbytes, max_seq_len, word)
+    _call(lib.bl_paged_decode_fp8, a, dev)
     return out
 
 

@@ -461,7 +461,7 @@ typedef struct bl_decode_fp8_args {
   int64_t num_q_heads;
   float scale;
   int32_t plan_ready;
-  void* workspace; /* device scratch, >= bl_paged_decode_fp8_workspace_bytes, 256-byte aligned */
+  void* workspace; /* device scratch, >= bl_paged_decode_fp8_workspace_bytes, 256-byte aligned; or NULL, see below */
   size_t workspace_bytes;
   int64_t max_seq_len; /* host upper bound on seq_lens[] */
   int32_t* err;
@@ -469,6 +469,10 @@ typedef struct bl_decode_fp8_args {
 
 BL_API size_t bl_paged_decode_fp8_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t head_dim,
                                                   int64_t max_seq_len);
+/* What a call with these arguments (pointers and workspace aside) needs: 0, or  */
+/* bl_paged_decode_fp8_workspace_bytes.  Small calls need none: they also     */
+/* take a NULL workspace of 0 bytes.                                          */
+BL_API size_t bl_paged_decode_fp8_scratch_bytes(const bl_decode_fp8_args* args);
 BL_API int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream);
 
 /* Chunked-prefill attention over the 8-bit pages (bl_paged_prefill): query i */

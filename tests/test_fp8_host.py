@@ -176,3 +176,21 @@ def test_cpu_tensors_are_refused():
     kc = torch.zeros((1, 2, 1, 16, 64), dtype=torch.float8_e4m3fn)
     with pytest.raises(RuntimeError, match="CUDA devices only"):
         ops.copy_blocks(kc, kc, [0], [1])
+
+
+def test_small_decode_calls_need_no_scratch(native_lib):
+    """(64 blocks of 2 KV heads: what fits 148 SMs at once and has at most 8 chunks a row)"""
+    def need(dtype=nat.BL_BF16, **kw):
+        a = entry_points(fake_layer(dtype=dtype))["bl_paged_decode_fp8"]
+        a.workspace, a.workspace_bytes = None, 0
+        for k, v in kw.items():
+            setattr(a, k, v)
+        n = native_lib.bl_paged_decode_fp8_scratch_bytes(ctypes.byref(a))
+        if n:
+            assert n == native_lib.bl_paged_decode_fp8_workspace_bytes(a.batch, a.num_q_heads, a.layer.kv.head_dim, a.max_seq_len)
+            assert native_lib.bl_paged_decode_fp8(ctypes.byref(a), None) == nat.BL_ERR_CAPACITY
+        return n
+    assert need(max_seq_len=16) == need(max_seq_len=4096) == need(max_seq_len=512, batch=8) == 0
+    assert need(max_seq_len=4097) and need(max_seq_len=512, batch=33) and need(max_seq_len=4096, batch=32)
+    assert need(dtype=nat.BL_F32, max_seq_len=16) and need(max_seq_len=0) == need(num_q_heads=3) == 0
+    assert native_lib.bl_paged_decode_fp8_scratch_bytes(None) == 0
