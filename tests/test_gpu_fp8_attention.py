@@ -243,6 +243,35 @@ def test_decode_small_calls_join_their_chunks(cuda, native_lib, dtype, hq, hkv, 
     assert int(err) == nat.BL_DEVERR_WORKSPACE
 
 
+@pytest.mark.parametrize("batch", [1, 33, 700])
+@pytest.mark.parametrize("hq,hkv,bs,d", [(16, 8, 16, 128), (4, 4, 8, 64), (20, 2, 16, 256)])
+def test_decode_rows_of_one_chunk(cuda, native_lib, batch, hq, hkv, bs, d):
+    """Rows of 0..512 tokens, fewer and more of them than CTAs: no join, the same bits as in a call that has one."""
+    lens = [(b * 97) % 514 if b % 5 else 0 for b in range(1, batch + 1)]
+    lens = [min(n, 512) for n in lens]
+    lens[0] = 512
+    pool, table, bt = filled(cuda, lens, hkv, bs, d, BF16, seed=batch + d, layers=1, layer=0)
+    q = torch.randn(batch, hq, d, generator=torch.Generator().manual_seed(d)).to(BF16).to(cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = torch.full((batch, hq, d), 9.0, dtype=BF16, device=cuda)
+    ops.paged_decode_fp8(q, *pool.args, 0, bt, i32(lens, cuda), 512, out=out, err=err)
+    assert int(err) == 0
+    pick = list(range(0, batch, 1 + batch // 40))
+    check_decode(out[pick], q[pick], pool, table[pick], [lens[i] for i in pick], 0)
+    assert torch.equal(ops.paged_decode_fp8(q, *pool.args, 0, bt, i32(lens, cuda), 513, err=err), out)
+    rows = i32(range(batch - 1, -1, -1), cuda)
+    turned = ops.paged_decode_fp8(q.flip(0), *pool.args, 0, bt, i32(lens[::-1], cuda), 512, row_ids=rows, err=err)
+    assert torch.equal(turned.flip(0), out) and int(err) == 0
+    ops.paged_decode_fp8(q, *pool.args, 0, bt, i32([0] * batch, cuda), 512, out=out, err=err)
+    assert bool((out == 0).all()) and int(err) == 0
+    # a row longer than the bound is reported (its table would hold it), the others are not touched by it
+    if bs == 16:
+        wide = torch.cat([bt, bt[:, :1]], dim=1)
+        more = ops.paged_decode_fp8(q, *pool.args, 0, wide, i32([513] + lens[1:], cuda), 512, err=err)
+        assert int(err) == nat.BL_DEVERR_WORKSPACE
+        assert torch.equal(more[1:], turned.flip(0)[1:])
+
+
 def test_decode_reports_what_it_cannot_do(cuda, native_lib):
     pool, table, bt = filled(cuda, [40, 600], 2, 16, 128, BF16)
     q = torch.randn(2, 4, 128, device=cuda).to(BF16)
