@@ -72,6 +72,22 @@ template <> __device__ __forceinline__ __half dequant_to<__half>(float v) {
 }
 
 // Validates an 8-bit layer: the shared checks plus the scale tables.
+// code * scale of two codes, packed; as dequant_to
+template <typename T> __device__ __forceinline__ uint32_t dequant2(float2 x, float s) {
+  return pack2<T>(x.x * s, x.y * s);
+}
+template <> __device__ __forceinline__ uint32_t dequant2<__half>(float2 x, float s) {
+  // (fminf and fmaxf drop a NaN, which a code or its product may be)
+  const float lo = x.x * s, hi = x.y * s;
+  const float l = fminf(fmaxf(lo, -65504.f), 65504.f), h = fminf(fmaxf(hi, -65504.f), 65504.f);
+  return pack2<__half>(lo != lo ? lo : l, hi != hi ? hi : h);
+}
+// eight codes times scale, as 16-bit values
+template <typename T> __device__ __forceinline__ uint4 dequant8(uint2 c, float s) {
+  return make_uint4(dequant2<T>(unpack2<__half>(e4m3lo_to_f16x2(c.x)), s), dequant2<T>(unpack2<__half>(e4m3hi_to_f16x2(c.x)), s),
+                    dequant2<T>(unpack2<__half>(e4m3lo_to_f16x2(c.y)), s), dequant2<T>(unpack2<__half>(e4m3hi_to_f16x2(c.y)), s));
+}
+
 inline int check_fp8_layer(const bl_fp8_layer& l, const char* who) {
   const int rc = check_paged_layer(l.kv, who);
   if (rc) return rc;

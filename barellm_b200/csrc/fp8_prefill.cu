@@ -93,7 +93,7 @@ struct ExpandArgs {
   const int32_t* q_offsets;
   int64_t max_q, o_sb, o_st, o_sh;
   void* out;
-  int32_t hkv, bs, d, dup, hq;
+  int32_t hkv, bs, bs_shift, d, dup, hq;  // bs_shift: log2 of the block size, or -1
   int32_t* err;
 };
 
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(const Expand
     const int64_t j = j0 + p, t = j * kPage + tok;
     ok[p] = false;
     if (j >= a.width || t >= len) continue;
-    const int64_t lb = t / a.bs;
+    const int64_t lb = a.bs_shift >= 0 ? t >> a.bs_shift : t / a.bs;
     if (lb >= a.bt_width) {
       raise_dev(a.err, BL_DEVERR_TABLE);
       continue;
@@ -189,27 +189,15 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(const Expand
     const int64_t j = j0 + p;
     if (j >= a.width || base + j >= a.pages || j * kPage >= len) continue;
     // a token whose block cannot be read, and the slots behind the length, become zeros
-    union {
-      T t[8];
-      uint4 u;
-    } ko, vo;
-    ko.u = vo.u = make_uint4(0, 0, 0, 0);
+    uint4 ko = make_uint4(0, 0, 0, 0), vo = ko;
     if (ok[p]) {
-      const uint32_t kw[2] = {kc[p].x, kc[p].y}, vw[2] = {vc[p].x, vc[p].y};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float2 a0 = e4m3x2_to_float2((uint16_t)kw[i]), a1 = e4m3x2_to_float2((uint16_t)(kw[i] >> 16));
-        const float2 b0 = e4m3x2_to_float2((uint16_t)vw[i]), b1 = e4m3x2_to_float2((uint16_t)(vw[i] >> 16));
-        ko.t[4 * i] = dequant_to<T>(a0.x * ks[p]), ko.t[4 * i + 1] = dequant_to<T>(a0.y * ks[p]);
-        ko.t[4 * i + 2] = dequant_to<T>(a1.x * ks[p]), ko.t[4 * i + 3] = dequant_to<T>(a1.y * ks[p]);
-        vo.t[4 * i] = dequant_to<T>(b0.x * vs[p]), vo.t[4 * i + 1] = dequant_to<T>(b0.y * vs[p]);
-        vo.t[4 * i + 2] = dequant_to<T>(b1.x * vs[p]), vo.t[4 * i + 3] = dequant_to<T>(b1.y * vs[p]);
-      }
+      ko = dequant8<T>(kc[p], ks[p]);
+      vo = dequant8<T>(vc[p], vs[p]);
     }
     for (int r = 0; r < a.dup; ++r) {
       const int64_t dst = ((((base + j) * a.hkv + h) * a.dup + r) * kPage + tok) * kTCDim + v * 8;
-      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.k_out) + dst) = ko.u;
-      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.v_out) + dst) = vo.u;
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.k_out) + dst) = ko;
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.v_out) + dst) = vo;
     }
   }
 }
@@ -374,24 +362,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1) fp8_prefill_mma_kernel(const M
   auto widen = [&](const uint8_t* codes, uint8_t* to, const float* scale, int buf) {
     for (int e = tid; e < kMmaKeys * 16; e += kMmaThreads) {
       const int t = e >> 4, c = e & 15;
-      union {
-        T t[16];
-        uint4 u[2];
-      } x;
-      x.u[0] = x.u[1] = make_uint4(0u, 0u, 0u, 0u);
+      uint4 x[2];
+      x[0] = x[1] = make_uint4(0u, 0u, 0u, 0u);
       if (sh->row[buf][t] >= 0 && c < chunks) {
         const uint4 w = *reinterpret_cast<const uint4*>(codes + t * kMmaDim + c * 16);
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-        const float s = scale[t];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 lo = unpack2<__half>(e4m3lo_to_f16x2(ww[i])), hi = unpack2<__half>(e4m3hi_to_f16x2(ww[i]));
-          x.t[4 * i] = dequant_to<T>(lo.x * s), x.t[4 * i + 1] = dequant_to<T>(lo.y * s);
-          x.t[4 * i + 2] = dequant_to<T>(hi.x * s), x.t[4 * i + 3] = dequant_to<T>(hi.y * s);
-        }
+        x[0] = dequant8<T>(make_uint2(w.x, w.y), scale[t]);
+        x[1] = dequant8<T>(make_uint2(w.z, w.w), scale[t]);
       }
-      *reinterpret_cast<uint4*>(to + mma_at(t, 2 * c)) = x.u[0];
-      *reinterpret_cast<uint4*>(to + mma_at(t, 2 * c + 1)) = x.u[1];
+      *reinterpret_cast<uint4*>(to + mma_at(t, 2 * c)) = x[0];
+      *reinterpret_cast<uint4*>(to + mma_at(t, 2 * c + 1)) = x[1];
     }
   };
 
@@ -906,6 +885,9 @@ int launch_tc(const bl_prefill_fp8_args& a, const Scratch& w, cudaStream_t s) {
   e.o_sb = o_sb, e.o_st = o_st, e.o_sh = o_sh;
   e.hkv = (int32_t)kv.num_kv_heads;
   e.bs = (int32_t)kv.block_size;
+  e.bs_shift = -1;
+  for (int i = 0; i <= 16; ++i)
+    if (kv.block_size == 1 << i) e.bs_shift = i;
   e.d = (int32_t)kv.head_dim;
   e.dup = (int32_t)w.dup;
   e.hq = (int32_t)a.num_q_heads;

@@ -60,6 +60,29 @@ def test_append_equals_oracle(cuda, native_lib, dtype, hkv, bs, d):
     pool.assert_equal()
 
 
+@pytest.mark.parametrize("batch", [2, 31, 33, 64, 1100])
+@pytest.mark.parametrize("bs,first", [(16, 0), (16, 37), (1, 2), (5, 0), (64, 5)])
+def test_append_rows_of_very_different_lengths(cuda, native_lib, batch, bs, first):
+    """A few long chunks among short and empty ones, the first token of the packed axis not row 0's, tokens of no row behind."""
+    rs = np.random.RandomState(batch + bs)
+    new = [int(n) for n in rs.choice([0, 0, 1, 2, 7], batch)]
+    new[0], new[batch // 2], new[-1] = 130, 0, 75
+    starts = [int(x) for x in rs.randint(0, 2 * bs + 2, batch)]
+    pool = Pool(cuda, 1, sum(-(-(s + n) // bs) for s, n in zip(starts, new)) + 3, 2, bs, 8)
+    table = pool.table([s + n for s, n in zip(starts, new)])
+    bt = torch.from_numpy(table).to(cuda)
+    k, v = (torch.from_numpy(rs.randn(1, 2, first + sum(new) + 3, 8).astype(np.float32)).to(cuda) for _ in range(2))
+    off = first + np.concatenate([[0], np.cumsum(new)])
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    ops.paged_append_fp8(*pool.args, 0, bt, i32(starts, cuda), k, v, new_offsets=i32(off, cuda), max_new_tokens=max(new), err=err)
+    kn, vn = k[0].double().cpu().numpy(), v[0].double().cpu().numpy()
+    pick = [b for b in range(batch) if new[b]]
+    oracle_append(pool, 0, table[pick], [starts[b] for b in pick], [kn[:, off[b]:off[b + 1]] for b in pick],
+                  [vn[:, off[b]:off[b + 1]] for b in pick])
+    assert int(err) == 0
+    pool.assert_equal()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_append_token_by_token_raises_scales(cuda, native_lib, dtype):
     """Magnitudes that grow and shrink inside a block: old codes are rounded to each raised scale, in order."""
