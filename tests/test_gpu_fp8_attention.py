@@ -378,6 +378,36 @@ def test_prefill_wide_heads(cuda, native_lib, dtype, hq, hkv, bs, d, pad):
     assert int(err) == 0 and bool((out[:, :, sum(chunks[:5]):-2] == 0).all()) and not bool((out[:, :, -2:] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_prefill_wide_heads_rectangular(cuda, native_lib, dtype):
+    """[B, Hq, T, D] queries, rows by row_ids, a row whose table ends early, a captured call, another stream."""
+    lens, t, hq, hkv, d = [40, 300, 70], 37, 8, 2, 256
+    pool, table, bt = filled(cuda, lens, hkv, 16, d, dtype)
+    q = torch.randn(3, hq, t, d, generator=torch.Generator().manual_seed(0)).to(dtype).to(cuda)
+    rows = i32([2, 0, 1], cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    seq = i32([lens[2], lens[0], lens[1]], cuda)
+    args = dict(row_ids=rows, err=err)
+    out = ops.paged_prefill_fp8(q, *pool.args, 1, bt, seq, 300, **args)
+    for i, b in enumerate((2, 0, 1)):
+        check_prefill(out[i:i + 1], q[i:i + 1], pool, table[b:b + 1], [lens[b]], [t], 1)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        again = ops.paged_prefill_fp8(q, *pool.args, 1, bt, seq, 300, **args)
+    again.fill_(5.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, out) and int(err) == 0
+    ops.paged_prefill_fp8(q, *pool.args, 1, bt[:, :10].contiguous(), seq, 300, **args)
+    assert int(err) == nat.BL_DEVERR_TABLE
+    err.zero_()
+    bad = bt.clone()
+    bad[1, 3] = 10 ** 6
+    wrong = ops.paged_prefill_fp8(q, *pool.args, 1, bad, seq, 300, **args)
+    assert int(err) == nat.BL_DEVERR_BLOCK_ID and torch.equal(wrong[:2], out[:2])
+
+
 @pytest.mark.parametrize("d", [128, 80])
 def test_prefill_leaves_tokens_of_no_row(cuda, native_lib, d):
     """A packed q with room behind its last row: those outputs stay as they were; narrow, strided q and out."""
