@@ -12,10 +12,14 @@
 namespace bl {
 namespace {
 
-constexpr int kPairsPerLaunch = 1000;  // 8000 bytes of kernel parameters
+// Pairs in a launch's parameters: 1000 (8000 bytes), or 32 where there are no more,
+// since the driver copies all of a kernel's parameters on every launch (8 pairs,
+// calls in a row: 8.7 against 9.5 us).
+constexpr int kPairsPerLaunch = 1000, kFewPairs = 32;
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;  // 16-byte vectors a thread has in flight
 
+template <int N>
 struct CopyArgs {
   char* k_pool;
   char* v_pool;
@@ -23,13 +27,13 @@ struct CopyArgs {
   float* v_scale;
   int64_t num_blocks, slab;  // slab: bytes of one block's K (or V) in one layer
   int32_t hkv, parts;        // parts: CTAs per slab
-  int32_t src[kPairsPerLaunch];
-  int32_t dst[kPairsPerLaunch];
+  int32_t src[N];
+  int32_t dst[N];
 };
 
 // grid: (pairs * parts, 2, layers)
-template <typename V>
-__global__ void __launch_bounds__(kThreads) copy_blocks_kernel(const __grid_constant__ CopyArgs a) {
+template <typename V, int N>
+__global__ void __launch_bounds__(kThreads) copy_blocks_kernel(const __grid_constant__ CopyArgs<N> a) {
   const int pair = blockIdx.x / a.parts, part = blockIdx.x - pair * a.parts;
   const bool is_v = blockIdx.y;
   const int64_t layer = blockIdx.z;
@@ -88,6 +92,35 @@ int check_pairs(const bl_copy_blocks_args& a) {
   return BL_OK;
 }
 
+template <int N>
+int launch_copies(const bl_copy_blocks_args& a, cudaStream_t s) {
+  CopyArgs<N> k;
+  k.k_pool = (char*)a.k_pool;
+  k.v_pool = (char*)a.v_pool;
+  k.k_scale = a.k_scale;
+  k.v_scale = a.v_scale;
+  k.num_blocks = a.num_blocks;
+  k.slab = a.num_kv_heads * a.block_size * a.head_dim * a.elem_bytes;
+  k.hkv = (int32_t)a.num_kv_heads;
+  const bool vec = k.slab % 16 == 0 && ((uintptr_t)a.k_pool & 15) == 0 && ((uintptr_t)a.v_pool & 15) == 0;
+  const int64_t nvec = vec ? k.slab / 16 : k.slab;
+  k.parts = (int32_t)std::min<int64_t>(64, (nvec + kThreads * kUnroll - 1) / (kThreads * kUnroll));
+  for (int64_t at = 0; at < a.count; at += N) {
+    const int n = (int)std::min<int64_t>(N, a.count - at);
+    for (int i = 0; i < n; ++i) {
+      k.src[i] = (int32_t)a.src[at + i];
+      k.dst[i] = (int32_t)a.dst[at + i];
+    }
+    dim3 grid((unsigned)(n * k.parts), 2, (unsigned)a.num_layers);
+    if (vec)
+      copy_blocks_kernel<uint4, N><<<grid, kThreads, 0, s>>>(k);
+    else
+      copy_blocks_kernel<uint8_t, N><<<grid, kThreads, 0, s>>>(k);
+    BL_CHECK_LAUNCH("copy_blocks_kernel");
+  }
+  return BL_OK;
+}
+
 }  // namespace
 }  // namespace bl
 
@@ -108,29 +141,6 @@ extern "C" int bl_copy_blocks(const bl_copy_blocks_args* args, void* stream) {
   BL_CHECK_ARG(a.src && a.dst, "bl_copy_blocks: null block ids");
   const int rc = check_pairs(a);
   if (rc) return rc;
-  CopyArgs k;
-  k.k_pool = (char*)a.k_pool;
-  k.v_pool = (char*)a.v_pool;
-  k.k_scale = a.k_scale;
-  k.v_scale = a.v_scale;
-  k.num_blocks = a.num_blocks;
-  k.slab = a.num_kv_heads * a.block_size * a.head_dim * a.elem_bytes;
-  k.hkv = (int32_t)a.num_kv_heads;
-  const bool vec = k.slab % 16 == 0 && ((uintptr_t)a.k_pool & 15) == 0 && ((uintptr_t)a.v_pool & 15) == 0;
-  const int64_t nvec = vec ? k.slab / 16 : k.slab;
-  k.parts = (int32_t)std::min<int64_t>(64, (nvec + kThreads * kUnroll - 1) / (kThreads * kUnroll));
-  for (int64_t at = 0; at < a.count; at += kPairsPerLaunch) {
-    const int n = (int)std::min<int64_t>(kPairsPerLaunch, a.count - at);
-    for (int i = 0; i < n; ++i) {
-      k.src[i] = (int32_t)a.src[at + i];
-      k.dst[i] = (int32_t)a.dst[at + i];
-    }
-    dim3 grid((unsigned)(n * k.parts), 2, (unsigned)a.num_layers);
-    if (vec)
-      copy_blocks_kernel<uint4><<<grid, kThreads, 0, (cudaStream_t)stream>>>(k);
-    else
-      copy_blocks_kernel<uint8_t><<<grid, kThreads, 0, (cudaStream_t)stream>>>(k);
-    BL_CHECK_LAUNCH("copy_blocks_kernel");
-  }
-  return BL_OK;
+  return a.count <= kFewPairs ? launch_copies<kFewPairs>(a, (cudaStream_t)stream)
+                              : launch_copies<kPairsPerLaunch>(a, (cudaStream_t)stream);
 }

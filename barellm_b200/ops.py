@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+from array import array
 
 import numpy as np
 import torch
@@ -1032,14 +1033,26 @@ def paged_prefill_fp8(
     return out
 
 
-def _block_ids(ids, name: str) -> np.ndarray:
-    """Host block ids as int64 (the library checks their range)."""
+_INTS = frozenset((int,))
+
+
+def _block_ids(ids, name: str):
+    """(owner, address, number) of host block ids as int64 (the library checks their range)."""
+    if (type(ids) is list or type(ids) is tuple) and _INTS.issuperset(map(type, ids)):
+        try:
+            a = array("q", ids)
+        except OverflowError:
+            raise ValueError(f"{name} must be a sequence of block ids") from None
+        return a, *a.buffer_info()
     a = np.asarray(ids)
+    if isinstance(ids, (list, tuple)):
+        _check(bool not in map(type, ids), f"{name} must be a sequence of block ids")
     if a.dtype != np.int64:
         _check(a.dtype.kind in "iu" or a.size == 0, f"{name} must be a sequence of block ids")
         a = a.astype(np.int64)
     _check(a.ndim == 1, f"{name} must be a sequence of block ids")
-    return np.ascontiguousarray(a)
+    a = np.ascontiguousarray(a)
+    return a, a.ctypes.data, len(a)
 
 
 def copy_blocks(
@@ -1073,13 +1086,13 @@ def copy_blocks(
             _check(t.shape == shape[:3] and t.dtype is _F32 and t.get_device() == dev and t.is_contiguous(),
                    f"{name} must be a contiguous float32 [L, P, H] tensor on the pool's device")
         kp, vp = key_scale.data_ptr(), value_scale.data_ptr()
-    sa, da = _block_ids(src, "src"), _block_ids(dst, "dst")
-    n = len(sa)
-    _check(n == len(da), "src and dst must have the same length")
+    src_ids, src_at, n = _block_ids(src, "src")  # (the owners live until the call is over)
+    dst_ids, dst_at, m = _block_ids(dst, "dst")
+    _check(n == m, "src and dst must have the same length")
     if n == 0:
         return
     a = nat.pack_copy_blocks_args(key_cache.data_ptr(), value_cache.data_ptr(), kp, vp, *shape, key_cache.element_size(),
-                                  sa.ctypes.data, da.ctypes.data, n)
+                                  src_at, dst_at, n)
     _call(nat.load().bl_copy_blocks, a, dev)
 
 

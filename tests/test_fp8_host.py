@@ -194,3 +194,18 @@ def test_small_decode_calls_need_no_scratch(native_lib):
     assert need(max_seq_len=4097) and need(max_seq_len=512, batch=33) and need(max_seq_len=4096, batch=32)
     assert need(dtype=nat.BL_F32, max_seq_len=16) and need(max_seq_len=0) == need(num_q_heads=3) == 0
     assert native_lib.bl_paged_decode_fp8_scratch_bytes(None) == 0
+
+
+@pytest.mark.parametrize("ids", [[3, 1, 2], (3, 1, 2), np.array([3, 1, 2], dtype=np.int32), np.array([3, 0, 1, 0, 2, 0])[::2],
+                                 np.array([3, 1, 2], dtype=np.uint8), range(3, 0, -1)])
+def test_block_ids_of_any_host_sequence(ids):
+    owner, at, n = ops._block_ids(ids, "src")
+    got = list((ctypes.c_int64 * n).from_address(at))
+    assert got == [int(i) for i in ids]
+    assert ops._block_ids([], "src")[2] == ops._block_ids(np.zeros(0), "src")[2] == 0
+
+
+@pytest.mark.parametrize("ids", [[1.5], [True, 2], [1, 2.0], [[1, 2]], ["a"], (None,), [2 ** 70], np.array([1.0]), np.array([[1, 2]])])
+def test_what_is_no_block_id_is_refused(ids):
+    with pytest.raises(ValueError, match="dst must be a sequence of block ids"):
+        ops._block_ids(ids, "dst")
