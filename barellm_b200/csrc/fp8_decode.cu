@@ -123,7 +123,7 @@ __device__ __forceinline__ int cta_exclusive(int v, int* s, int& total) {
 }
 
 __global__ void __launch_bounds__(kPlanThreads) fp8_decode_plan_kernel(const PlanArgs a) {
-  pdl_trigger();  // the attention kernel may launch; it waits for this grid to complete
+  pdl_trigger();  // the attention kernel may launch; it waits for this grid (and for those before it) to complete
   __shared__ int s_sum[kPlanThreads / 32];
   __shared__ int s_count[kChunkTiles], s_next[kChunkTiles];  // partial chunks by size in tiles, minus one
   const int tid = threadIdx.x;
@@ -143,12 +143,16 @@ __global__ void __launch_bounds__(kPlanThreads) fp8_decode_plan_kernel(const Pla
   for (int b0 = 0; b0 < a.batch; b0 += blockDim.x) {
     const int b = b0 + tid;
     const int len = b < a.batch ? length(b) : 0;
-    if (b < a.batch && a.seq_lens[b] > a.cap) raise_dev(a.err, BL_DEVERR_TABLE);
     const int nfull = len / kChunk, nall = (int)(((int64_t)len + kChunk - 1) / kChunk);
     int tot_all, tot_full;
     const int my_all = all + cta_exclusive(nall, s_sum, tot_all);
     const int my_full = full + cta_exclusive(nfull, s_sum, tot_full);
+    // Nothing is written before the kernel ahead has completed: the workspace may be
+    // memory that it still reads (an append's tokens, freed since; the plan of the
+    // call before).
+    if (b0 == 0) pdl_wait();
     if (b < a.batch) {
+      if (a.seq_lens[b] > a.cap) raise_dev(a.err, BL_DEVERR_TABLE);
       a.row_base[b] = my_all;
       const int table_row = a.row_ids ? a.row_ids[b] : b;
       for (int c = 0; c < nfull; ++c) put(my_full + c, b, c, len, my_all, table_row);
@@ -179,8 +183,6 @@ __global__ void __launch_bounds__(kPlanThreads) fp8_decode_plan_kernel(const Pla
     if (rest > 0)
       put(atomicAdd(&s_next[(rest + 15) / 16 - 1], 1), b, nfull, len, a.row_base[b], a.row_ids ? a.row_ids[b] : b);
   }
-  // complete only after the kernel before it has (the step's append)
-  pdl_wait();
 }
 
 struct Args {

@@ -574,3 +574,48 @@ def test_graphs_streams_and_concurrent_calls(cuda, native_lib):
         for s, g in zip(steps, got):
             for x, y in zip(run(s), g):
                 assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_a_workspace_may_be_what_the_kernel_before_read(cuda, native_lib, n):
+    """In stream order an append's tokens are free for the next call's scratch: the plan is written only then."""
+    batch, hkv, d = 300, 8, 128
+    lens = [n + (b * 7) % 90 for b in range(batch)]
+    pool, table, bt = filled(cuda, [x + n for x in lens], hkv, 16, d, BF16, layers=1, layer=0)
+    q = torch.randn(batch, 2 * hkv, d, device=cuda).to(BF16)
+    seq, start = i32([x + n for x in lens], cuda), i32(lens, cuda)
+    off = i32([b * n for b in range(batch + 1)], cuda)
+    bytes_kv = batch * n * hkv * d * 2
+    need = ops.decode_fp8_workspace_bytes(batch, 2 * hkv, d, 512)
+    last = (bytes_kv - 20 * n * hkv * d * 2) // 256 * 256  # the scratch begins at the tokens that are appended last
+    buf = torch.zeros(last + max(need, bytes_kv - last), dtype=torch.uint8, device=cuda)
+    k = buf[:bytes_kv].view(BF16).view(1, batch * n, hkv, d).transpose(1, 2)
+    g = torch.Generator(device=cuda).manual_seed(n)
+    tokens = torch.randn(k.shape, generator=g, device=cuda).to(BF16)
+    clean = [c.clone() for c in pool.args]
+    ops.paged_append_fp8(*clean, 0, bt, start, tokens, tokens, new_offsets=off, max_new_tokens=n)
+    want = ops.paged_decode_fp8(q, *clean, 0, bt, seq, 512)
+    for _ in range(20):
+        k.copy_(tokens)
+        got = [c.clone() for c in pool.args]
+        ops.paged_append_fp8(*got, 0, bt, start, k, k, new_offsets=off, max_new_tokens=n)
+        out = ops.paged_decode_fp8(q, *got, 0, bt, seq, 512, ws=buf[last:])
+        for a, b in zip(got, clean):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("max_len", [512, 1300])
+def test_calls_in_a_row_share_a_workspace(cuda, native_lib, max_len):
+    """Plans of different batches written over one another, call after call."""
+    lens = [(b * 53) % max_len + 1 for b in range(120)]
+    pool, table, bt = filled(cuda, lens, 4, 16, 128, BF16, layers=1, layer=0)
+    q = torch.randn(120, 8, 128, device=cuda).to(BF16)
+    seq, err = i32(lens, cuda), torch.zeros(1, dtype=torch.int32, device=cuda)
+    want = ops.paged_decode_fp8(q, *pool.args, 0, bt, seq, max_len)
+    ws = torch.empty(ops.decode_fp8_workspace_bytes(120, 8, 128, max_len), dtype=torch.uint8, device=cuda)
+    outs = []
+    for i in range(60):
+        n = 120 - (i % 3) * 25
+        outs.append((n, ops.paged_decode_fp8(q[:n], *pool.args, 0, bt[:n], seq[:n], max_len, ws=ws, err=err)))
+    assert all(torch.equal(o, want[:n]) for n, o in outs) and int(err) == 0
