@@ -149,6 +149,9 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const PlanArg
     int tot_all, tot_full;
     const int ex_all = block_excl_scan(nch, warp_tot, tot_all);
     const int ex_full = block_excl_scan(nfull, warp_tot, tot_full);
+    // written only when the kernel ahead has completed: the workspace may be memory
+    // that it still reads (an append's tokens, freed since)
+    if (base == 0) pdl_wait();
     if (b < a.batch) {
       a.row_base[b] = carry_all + ex_all;
       const int p0 = carry_full + ex_full;
@@ -189,8 +192,6 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const PlanArg
       if (p < a.max_units) a.exec[p] = make_int2(b, nfull);
     }
   }
-  // complete only after the previous kernel (the step's K/V append) has
-  pdl_wait();
 }
 
 // ---------------------------------------------------------------------------
