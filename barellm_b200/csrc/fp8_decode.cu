@@ -124,6 +124,10 @@ __device__ __forceinline__ int cta_exclusive(int v, int* s, int& total) {
 
 __global__ void __launch_bounds__(kPlanThreads) fp8_decode_plan_kernel(const PlanArgs a) {
   pdl_trigger();  // the attention kernel may launch; it waits for this grid (and for those before it) to complete
+  // Nothing is read or written before the kernel ahead has completed: it may be what
+  // writes the lengths or the row ids, and the workspace may be memory that it still
+  // reads (an append's tokens, freed since; the plan of the call before).
+  pdl_wait();
   __shared__ int s_sum[kPlanThreads / 32];
   __shared__ int s_count[kChunkTiles], s_next[kChunkTiles];  // partial chunks by size in tiles, minus one
   const int tid = threadIdx.x;
@@ -147,10 +151,6 @@ __global__ void __launch_bounds__(kPlanThreads) fp8_decode_plan_kernel(const Pla
     int tot_all, tot_full;
     const int my_all = all + cta_exclusive(nall, s_sum, tot_all);
     const int my_full = full + cta_exclusive(nfull, s_sum, tot_full);
-    // Nothing is written before the kernel ahead has completed: the workspace may be
-    // memory that it still reads (an append's tokens, freed since; the plan of the
-    // call before).
-    if (b0 == 0) pdl_wait();
     if (b < a.batch) {
       if (a.seq_lens[b] > a.cap) raise_dev(a.err, BL_DEVERR_TABLE);
       a.row_base[b] = my_all;
