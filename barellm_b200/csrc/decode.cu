@@ -131,6 +131,10 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const PlanArg
   // the attention kernel may launch now; it waits for this grid (and, through
   // the pdl_wait below, for the append before it) before reading the plan
   pdl_trigger();
+  // nothing is read or written before the kernel ahead has completed: it may be what
+  // writes the lengths, and the workspace may be memory that it still reads (an
+  // append's tokens, freed since)
+  pdl_wait();
   __shared__ int warp_tot[32];
   __shared__ int hist[kChunkTokens + 1];    // partial-chunk sizes (blocks), 1..chunk_blocks-1
   __shared__ int bucket[kChunkTokens + 1];
@@ -149,9 +153,6 @@ __global__ void __launch_bounds__(kPlanThreads) decode_plan_kernel(const PlanArg
     int tot_all, tot_full;
     const int ex_all = block_excl_scan(nch, warp_tot, tot_all);
     const int ex_full = block_excl_scan(nfull, warp_tot, tot_full);
-    // written only when the kernel ahead has completed: the workspace may be memory
-    // that it still reads (an append's tokens, freed since)
-    if (base == 0) pdl_wait();
     if (b < a.batch) {
       a.row_base[b] = carry_all + ex_all;
       const int p0 = carry_full + ex_full;

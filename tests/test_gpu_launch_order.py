@@ -42,7 +42,7 @@ class LateWriter:
 
 @pytest.mark.parametrize("before", [0, 1900])
 @pytest.mark.parametrize("captured", [False, True])
-@pytest.mark.parametrize("kind", ["fp8", "fp8_f32"])
+@pytest.mark.parametrize("kind", ["fp8", "fp8_f32", "bf16"])
 def test_lengths_written_by_the_kernel_just_ahead(cuda, native_lib, kind, captured, before):
     hkv, hq, d, most = 2, 8, 128, 1920
     dtype = F32 if kind == "fp8_f32" else BF16
@@ -50,8 +50,14 @@ def test_lengths_written_by_the_kernel_just_ahead(cuda, native_lib, kind, captur
     pool, table, bt = filled(cuda, table_lens, hkv, 16, d, dtype, layers=1, layer=0)
     q = torch.randn(40, hq, d, generator=torch.Generator().manual_seed(3)).to(dtype).to(cuda)
     err = torch.zeros(1, dtype=torch.int32, device=cuda)
-    ws = torch.zeros(ops.decode_fp8_workspace_bytes(40, hq, d, most), dtype=torch.uint8, device=cuda)
-    call = lambda seq, rows: ops.paged_decode_fp8(q, *pool.args, 0, bt, seq, most, row_ids=rows, ws=ws, err=err)
+    if kind == "bf16":
+        g = torch.Generator(device=cuda).manual_seed(4)
+        cache = [torch.randn(pool.dev[0].shape, generator=g, device=cuda).to(BF16) for _ in range(2)]
+        ws = torch.zeros(ops.decode_workspace_bytes(40, hq, d, 16, most), dtype=torch.uint8, device=cuda)
+        call = lambda seq, rows: ops.paged_decode(q, *cache, 0, bt, seq, most, row_ids=rows, ws=ws, err=err)
+    else:
+        ws = torch.zeros(ops.decode_fp8_workspace_bytes(40, hq, d, most), dtype=torch.uint8, device=cuda)
+        call = lambda seq, rows: ops.paged_decode_fp8(q, *pool.args, 0, bt, seq, most, row_ids=rows, ws=ws, err=err)
     want = call(i32(LENS, cuda), i32(ROWS, cuda)).clone()
     late = LateWriter(cuda, LENS + ROWS)
     seq, rows = late.values[:40], late.values[40:]
