@@ -498,12 +498,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) fp8_prefill_mma_kernel(const M
     if (r >= rows) continue;
     const int64_t t = r / a.g;
     T* dst = reinterpret_cast<T*>(a.out) + b * a.o_sb + (qo + t) * a.o_st + (h * a.g + (r - t * a.g)) * a.o_sh;
-    const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];  // 0: no key seen; a NaN sum stays NaN
+    // 0: no key seen, so zeros whatever the keys of the tile hold; a NaN sum stays NaN
+    const bool none = l[i] == 0.f;
+    const float inv = none ? 0.f : 1.f / l[i];
 #pragma unroll
     for (int j = 0; j < kMmaDim / 8; ++j) {
       const int d = j * 8 + 2 * t4;
       if (d >= a.d) break;
-      const float x = o[j][2 * i] * inv, y = o[j][2 * i + 1] * inv;
+      const float x = none ? 0.f : o[j][2 * i] * inv, y = none ? 0.f : o[j][2 * i + 1] * inv;
       if (a.o_pair) {
         *reinterpret_cast<uint32_t*>(dst + d) = pack2<T>(x, y);
       } else {

@@ -117,7 +117,9 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Sh
   return false;
 }
 
-template <bool BF16>
+// EXPANDED: the pools are the expansion of an 8-bit cache (fp8_prefill.cu), whose rows
+// may have queries that see no key.
+template <bool BF16, bool EXPANDED>
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_tc_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
@@ -489,6 +491,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) {
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : 0.f;
+        // a query that sees no key: zeros, whatever the keys of its tile hold (0 * NaN is NaN)
+        const uint32_t keep = EXPANDED && l == 0.f ? 0u : 0xffffffffu;
         if (a.o_vec16) {
           // Every S MMA finished before the last P V of either tile (they were
           // issued earlier by the same thread), so Q's shared memory is free:
@@ -505,10 +509,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int k = 0; k < 4; ++k) {
               const int ch = c * 4 + k;
               uint4 w;
-              w.x = pack2<T>(o[8 * k + 0] * inv, o[8 * k + 1] * inv);
-              w.y = pack2<T>(o[8 * k + 2] * inv, o[8 * k + 3] * inv);
-              w.z = pack2<T>(o[8 * k + 4] * inv, o[8 * k + 5] * inv);
-              w.w = pack2<T>(o[8 * k + 6] * inv, o[8 * k + 7] * inv);
+              w.x = pack2<T>(o[8 * k + 0] * inv, o[8 * k + 1] * inv) & keep;
+              w.y = pack2<T>(o[8 * k + 2] * inv, o[8 * k + 3] * inv) & keep;
+              w.z = pack2<T>(o[8 * k + 4] * inv, o[8 * k + 5] * inv) & keep;
+              w.w = pack2<T>(o[8 * k + 6] * inv, o[8 * k + 7] * inv) & keep;
               *reinterpret_cast<uint4*>(stage + lane * 256 + ((ch ^ (lane & 7)) << 4)) = w;
             }
           }
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (valid) {
 #pragma unroll
               for (int j = 0; j < 16; ++j)
-                reinterpret_cast<uint32_t*>(orow + c * 32)[j] = pack2<T>(o[2 * j] * inv, o[2 * j + 1] * inv);
+                reinterpret_cast<uint32_t*>(orow + c * 32)[j] = pack2<T>(o[2 * j] * inv, o[2 * j + 1] * inv) & keep;
             }
           }
         }
@@ -555,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 size_t smem_bytes() { return 1024 + kSmemData + sizeof(Shared); }
 
-template <bool BF16>
+template <bool BF16, bool EXPANDED>
 int launch(const bl_prefill_args& a, const int32_t* row_order, cudaStream_t s) {
   // the attribute belongs to one device's copy of the kernel: set once per device
   static std::atomic<bool> attr_done[64];
@@ -563,7 +567,7 @@ int launch(const bl_prefill_args& a, const int32_t* row_order, cudaStream_t s) {
   cudaGetDevice(&dev);
   const bool known = dev >= 0 && dev < 64 && attr_done[dev].load();
   if (!known) {
-    if (cudaFuncSetAttribute(prefill_tc_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(prefill_tc_kernel<BF16, EXPANDED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)smem_bytes()) != cudaSuccess) {
       set_error("prefill: cudaFuncSetAttribute failed");
       return BL_ERR_LAUNCH;
@@ -606,18 +610,19 @@ int launch(const bl_prefill_args& a, const int32_t* row_order, cudaStream_t s) {
   k.err = a.err;
   const int64_t tiles = (a.max_q_len + k.bq - 1) / k.bq;
   dim3 grid((unsigned)tiles, (unsigned)a.kv.num_kv_heads, (unsigned)a.batch);
-  if (row_order) {
+  if constexpr (EXPANDED) {
     // the kernel before it on the stream is the expansion: this launch is prepared
     // while that one runs
-    if (launch_pdl(prefill_tc_kernel<BF16>, grid, dim3(kThreads), smem_bytes(), s, k, kmap, vmap) != cudaSuccess) {
+    if (launch_pdl(prefill_tc_kernel<BF16, EXPANDED>, grid, dim3(kThreads), smem_bytes(), s, k, kmap, vmap) != cudaSuccess) {
       set_error("prefill_tc_kernel: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
       return BL_ERR_LAUNCH;
     }
     return BL_OK;
+  } else {
+    prefill_tc_kernel<BF16, EXPANDED><<<grid, kThreads, smem_bytes(), s>>>(k, kmap, vmap);
+    BL_CHECK_LAUNCH("prefill_tc_kernel");
+    return BL_OK;
   }
-  prefill_tc_kernel<BF16><<<grid, kThreads, smem_bytes(), s>>>(k, kmap, vmap);
-  BL_CHECK_LAUNCH("prefill_tc_kernel");
-  return BL_OK;
 }
 
 }  // namespace
@@ -639,8 +644,8 @@ int prefill_tc_launch(const bl_prefill_args& a, cudaStream_t s, const int32_t* r
                    a.q_stride_t % 2 == 0 && a.q_stride_h % 2 == 0 && a.out_stride_b % 2 == 0 &&
                    a.out_stride_t % 2 == 0 && a.out_stride_h % 2 == 0,
                "bl_paged_prefill: q/out must be 4-byte aligned with even strides");
-  if (a.kv.dtype == BL_BF16) return launch<true>(a, row_order, s);
-  return launch<false>(a, row_order, s);
+  if (a.kv.dtype == BL_BF16) return row_order ? launch<true, true>(a, row_order, s) : launch<true, false>(a, nullptr, s);
+  return row_order ? launch<false, true>(a, row_order, s) : launch<false, false>(a, nullptr, s);
 }
 
 }  // namespace bl

@@ -619,3 +619,20 @@ def test_calls_in_a_row_share_a_workspace(cuda, native_lib, max_len):
         n = 120 - (i % 3) * 25
         outs.append((n, ops.paged_decode_fp8(q[:n], *pool.args, 0, bt[:n], seq[:n], max_len, ws=ws, err=err)))
     assert all(torch.equal(o, want[:n]) for n, o in outs) and int(err) == 0
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 128), (F16, 64), (BF16, 256), (F16, 144), (BF16, 12), (F32, 128)])
+@pytest.mark.parametrize("pad", [0, 2])
+def test_prefill_queries_that_see_no_key_beside_nan(cuda, native_lib, dtype, d, pad):
+    """They are zeros even where the keys that later queries of their tile see hold NaN."""
+    chunks, lens = [40, 300], [13, 150]
+    pool, table, bt = filled(cuda, lens, 2, 16, d, dtype)
+    q = torch.randn(1, sum(chunks), 8, d, device=cuda).to(dtype).transpose(1, 2)
+    off = i32([0, 40, 340], cuda)
+    whole = torch.full((1, sum(chunks), 8, d + pad), 5.0, dtype=dtype, device=cuda)
+    out = whole[..., :d].transpose(1, 2)
+    for which in pool.dev:  # K, then V too: the rows' first tokens, of one head
+        which.view(torch.uint8)[1, bt[:, 0].long(), 1, 2, :] = 0x7F
+        ops.paged_prefill_fp8(q, *pool.args, 1, bt, i32(lens, cuda), 150, q_offsets=off, max_q_len=300, out=out)
+        assert bool((out[0, :, :27] == 0).all()) and bool((out[0, :, 40:190] == 0).all())
+        assert bool(out[0, 4:, 39].isnan().all()) and not bool(out[0, :4].isnan().any())
