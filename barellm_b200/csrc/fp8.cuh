@@ -71,16 +71,19 @@ template <> __device__ __forceinline__ __half dequant_to<__half>(float v) {
   return __float2half_rn(v != v ? v : fminf(fmaxf(v, -65504.f), 65504.f));
 }
 
-// Validates an 8-bit layer: the shared checks plus the scale tables.
-// code * scale of two codes, packed; as dequant_to
+// Fp16 operands of the matrix instructions.  bf16 holds every code times every scale
+// exactly, fp16 does not: 448 * 2^8 is past its range, 2^-9 * 2^-16 below its last bit.
+// So for fp16 the values of a row's KV head are taken in units of a power of two, u,
+// such that its largest scale becomes 2^7 of them (codes up to 57344): exact for
+// the blocks whose scale is within 2^22 of the largest, and to 2^-25 u, less than
+// 2^-40 of the largest code's value, for the others.  The products take u back in fp32.
+__device__ __forceinline__ float half_unit(float largest_scale) {
+  const uint32_t e = __float_as_uint(largest_scale) >> 23;  // (0: no block; 255: no scale that an append leaves)
+  return e > 7 && e < 255 ? __uint_as_float((e - 7) << 23) : 1.f;
+}
+// code * scale of two codes, packed
 template <typename T> __device__ __forceinline__ uint32_t dequant2(float2 x, float s) {
   return pack2<T>(x.x * s, x.y * s);
-}
-template <> __device__ __forceinline__ uint32_t dequant2<__half>(float2 x, float s) {
-  // (fminf and fmaxf drop a NaN, which a code or its product may be)
-  const float lo = x.x * s, hi = x.y * s;
-  const float l = fminf(fmaxf(lo, -65504.f), 65504.f), h = fminf(fmaxf(hi, -65504.f), 65504.f);
-  return pack2<__half>(lo != lo ? lo : l, hi != hi ? hi : h);
 }
 // eight codes times scale, as 16-bit values
 template <typename T> __device__ __forceinline__ uint4 dequant8(uint2 c, float s) {
@@ -88,6 +91,7 @@ template <typename T> __device__ __forceinline__ uint4 dequant8(uint2 c, float s
                     dequant2<T>(unpack2<__half>(e4m3lo_to_f16x2(c.y)), s), dequant2<T>(unpack2<__half>(e4m3hi_to_f16x2(c.y)), s));
 }
 
+// Validates an 8-bit layer: the shared checks plus the scale tables.
 inline int check_fp8_layer(const bl_fp8_layer& l, const char* who) {
   const int rc = check_paged_layer(l.kv, who);
   if (rc) return rc;

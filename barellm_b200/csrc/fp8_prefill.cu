@@ -5,12 +5,13 @@
 //
 // Three ways, chosen by shape (use_tc below):
 //   expand + prefill_tc_kernel  16-bit q, head_dim a multiple of 8 up to 128.  The rows' pages are
-//       dequantised once into a 16-bit paged scratch (exact in bf16: a code has
-//       four significant bits), which the tcgen05 kernel of prefill_tc.cu then
-//       reads.  The expansion moves 1 + 2 bytes per cached element once; a
-//       CTA of the attention kernel reads the 2-byte form, and every 128 query
-//       tokens times group re-read it (mostly from L2), so dequantising in that
-//       kernel would repeat the conversion for every query tile.  Block sizes
+//       dequantised once into a 16-bit paged scratch (bf16: exact, a code has
+//       four significant bits; fp16: in units of each row and KV head, half_unit in
+//       fp8.cuh), which the tcgen05 kernel of prefill_tc.cu then reads.  The
+//       expansion moves 1 + 2 bytes per cached element once; a CTA of the
+//       attention kernel reads the 2-byte form, and every 128 query tokens times
+//       group re-read it (mostly from L2), so dequantising in that kernel would
+//       repeat the conversion for every query tile.  Block sizes
 //       other than 16 become 16-token pages on the way, and a query group
 //       that the kernel is not built for (3, 5, 16, ...) becomes several KV heads
 //       with the same contents and a group of 8, 4, 2 or 1.  A head_dim below
@@ -20,8 +21,13 @@
 //   fp8_prefill_simt_kernel     any element type, head_dim <= 256, block size
 //       and group: 64 queries x 64 keys a tile in fp32, pages dequantised
 //       into shared memory.
+// The two on the tensor cores round P to the element type, whose product with V
+// the matrix instructions take: half a step (2^-8 in bf16, 2^-11 in fp16) of each
+// weight in the numerator; the weights' sum, the maxima and the outputs' sums are fp32.
+// A key that a query does not see has weight 0, and 0 * NaN is NaN: a NaN among the
+// V of a chunk may reach the chunk's queries before it (never those that see nothing).
 #include <cstring>
-#include <mutex>
+#include <type_traits>
 
 #include "fp8.cuh"
 #include "prefill_tc.cuh"
@@ -39,7 +45,7 @@ inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 // head repeated `dup` times; q and out widened to 128 dims where head_dim is less.
 struct Scratch {
   int64_t width, pages, heads, dup;
-  size_t table, order, k, v, q, out, total;
+  size_t table, order, units, k, v, q, out, total;
 };
 
 bool use_tc(int32_t dtype, int64_t d) {
@@ -51,7 +57,7 @@ bool use_mma(int32_t dtype, int64_t d) {
 }
 
 // False when the scratch would not fit the tcgen05 kernel's 32-bit row coordinates.
-bool plan_scratch(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t bs, int64_t total_q, int64_t max_seq_len,
+bool plan_scratch(int32_t dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t bs, int64_t total_q, int64_t max_seq_len,
                   int64_t total_blocks, Scratch* w) {
   const int64_t g = hq / hkv;
   int64_t gt = 8;
@@ -64,7 +70,8 @@ bool plan_scratch(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t bs,
   w->pages = (int64_t)std::min(bound, (double)batch * (double)w->width);
   if ((double)w->pages * w->heads * kPage > (double)(INT32_MAX - 64) || w->heads > 65535) return false;
   const size_t table_bytes = align256((size_t)batch * w->width * sizeof(int32_t));
-  const size_t off = table_bytes + align256((size_t)batch * sizeof(int32_t));
+  w->units = table_bytes + align256((size_t)batch * sizeof(int32_t));
+  const size_t off = w->units + (dtype == BL_F16 ? align256((size_t)batch * w->heads * 2 * sizeof(float)) : 0);
   const size_t half = align256((size_t)w->pages * w->heads * kPage * kTCDim * 2);
   w->table = 0;
   w->order = table_bytes;
@@ -86,6 +93,8 @@ struct ExpandArgs {
   void* v_out;
   int32_t* table;  // [batch][width]
   int32_t* order;  // [batch] rows, the longest first
+  float* k_unit;   // fp16: [batch, hkv * dup]
+  float* v_unit;
   int64_t num_blocks, layer, width, pages, bt_stride, bt_width;
   const int32_t* block_tables;
   const int32_t* row_ids;
@@ -94,18 +103,77 @@ struct ExpandArgs {
   int64_t max_q, o_sb, o_st, o_sh;
   void* out;
   int32_t hkv, bs, bs_shift, d, dup, hq;  // bs_shift: log2 of the block size, or -1
+  int32_t own_units;                      // fp16: every CTA finds its row's units itself
   int32_t* err;
 };
+
+constexpr int kExpandThreads = 256;  // one page of one head: 16 tokens x 16 eight-code vectors
+
+// fp16: the units of a row's KV head (half_unit), from the scales of the row's blocks.
+// Bound by two dependent loads a block, 256 blocks at a time.  Every warp leaves its
+// maxima in `s` (before a __syncthreads); units_of joins them.
+struct UnitShared {
+  float k[kExpandThreads / 32], v[kExpandThreads / 32];
+};
+template <typename A>
+__device__ __forceinline__ void find_units(const A& a, int64_t row, int64_t len, int h, UnitShared& s) {
+  const int64_t blocks = len > 0 ? min((len + a.bs - 1) / a.bs, a.bt_width) : 0;
+  float km = 0.f, vm = 0.f;
+#pragma unroll 2
+  for (int64_t j = threadIdx.x; j < blocks; j += kExpandThreads) {
+    const int64_t phys = a.block_tables[row * a.bt_stride + j];
+    if (phys < 0 || phys >= a.num_blocks) continue;  // (reported where the block's tokens are read)
+    const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + h;
+    km = fmaxf(km, a.k_scale[slot]);
+    vm = fmaxf(vm, a.v_scale[slot]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, o));
+    vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+  }
+  if ((threadIdx.x & 31) == 0) s.k[threadIdx.x >> 5] = km, s.v[threadIdx.x >> 5] = vm;
+}
+__device__ __forceinline__ float2 units_of(const UnitShared& s) {
+  float km = s.k[0], vm = s.v[0];
+#pragma unroll
+  for (int w = 1; w < kExpandThreads / 32; ++w) km = fmaxf(km, s.k[w]), vm = fmaxf(vm, s.v[w]);
+  return make_float2(half_unit(km), half_unit(vm));
+}
+__device__ __forceinline__ void store_units(const ExpandArgs& a, int64_t b, int h, float2 unit) {
+  for (int r = threadIdx.x; r < a.dup; r += kExpandThreads) {
+    a.k_unit[(b * a.hkv + h) * a.dup + r] = unit.x;
+    a.v_unit[(b * a.hkv + h) * a.dup + r] = unit.y;
+  }
+}
+
+// The units ahead of the expansion, whose first loads are on their way meanwhile.
+// Rows of few blocks need no such kernel: every CTA of the expansion finds them by
+// itself (ExpandArgs::own_units).
+// grid: (hkv, batch)
+__global__ void __launch_bounds__(kExpandThreads) fp8_units_kernel(const ExpandArgs a) {
+  pdl_trigger();  // the expansion may start; it waits for this grid before it needs a unit
+  const int64_t b = blockIdx.y;
+  __shared__ UnitShared s;
+  find_units(a, a.row_ids ? (int64_t)a.row_ids[b] : b, a.seq_lens[b], blockIdx.x, s);
+  __syncthreads();
+  store_units(a, b, blockIdx.x, units_of(s));
+}
 
 // Bound by HBM: 1 byte read and 2 written per element (8 rows, 41.8k tokens, 8 KV
 // heads, head_dim 128: 257 MB in 45..50 us, 5.1..5.7 TB/s).  Four pages a CTA, so
 // that 8 loads a thread are in flight while the CTA counts the pages before its row.
 constexpr int kExpandPages = 4;  // pages of a CTA
-constexpr int kExpandThreads = 256;  // one page of one head: 16 tokens x 16 eight-code vectors
+// fp16 rows of at most so many blocks: every CTA finds the units by itself, which saves a
+// launch (8 rows of 300 tokens, calls in a row: 25.4 against 28.4 us; of 1000: 40.0 and
+// 40.4).  Rows of more are read by too many CTAs (of 4000: 118.6 against 116.1 us; of
+// 32k: 917 and 789).
+constexpr int64_t kOwnUnitBlocks = 128;
 
 // grid: (ceil(width / kExpandPages), hkv, batch)
 template <typename T>
-__global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(const ExpandArgs a) {
+__global__ void __launch_bounds__(kExpandThreads, 4) fp8_expand_kernel(const ExpandArgs a) {
+  constexpr bool kUnits = std::is_same<T, __half>::value;
   const int tid = threadIdx.x, h = blockIdx.y;
   const int64_t b = blockIdx.z;
   const int64_t len = max((int64_t)a.seq_lens[b], (int64_t)0);
@@ -136,7 +204,10 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(const Expand
     if (tid == 0) a.order[s_rank] = (int32_t)b;
   }
   const int64_t j0 = (int64_t)blockIdx.x * kExpandPages;
-  if (j0 * kPage >= len) return;
+  if (j0 * kPage >= len) {
+    if (kUnits) pdl_wait();  // (this grid is complete only when the units are; a no-op without their kernel)
+    return;
+  }
 
   const int64_t row = a.row_ids ? (int64_t)a.row_ids[b] : b;
   const int tok = tid >> 4, v = tid & 15;
@@ -175,6 +246,8 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(const Expand
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o);
   if ((tid & 31) == 0) s_sum[tid >> 5] = base;
+  __shared__ UnitShared s_unit;
+  if (kUnits && a.own_units) find_units(a, row, len, h, s_unit);
   __syncthreads();
   base = 0;
 #pragma unroll
@@ -183,6 +256,20 @@ __global__ void __launch_bounds__(kExpandThreads) fp8_expand_kernel(const Expand
     const bool fits = base + j0 + tid < a.pages;
     a.table[b * a.width + j0 + tid] = fits ? (int32_t)(base + j0 + tid) : -1;
     if (!fits) raise_dev(a.err, BL_DEVERR_WORKSPACE);
+  }
+  if (kUnits) {
+    pdl_wait();  // the units are written
+    const int64_t at = (b * a.hkv + h) * a.dup;
+    float2 unit;
+    if (a.own_units) {
+      unit = units_of(s_unit);
+      if (blockIdx.x == 0) store_units(a, b, h, unit);
+    } else {
+      unit = make_float2(a.k_unit[at], a.v_unit[at]);
+    }
+    const float k_inv = pow2_inverse(unit.x), v_inv = pow2_inverse(unit.y);
+#pragma unroll
+    for (int p = 0; p < kExpandPages; ++p) ks[p] *= k_inv, vs[p] *= v_inv;
   }
 #pragma unroll
   for (int p = 0; p < kExpandPages; ++p) {
@@ -282,7 +369,8 @@ struct MmaShared {
   uint8_t k[kMmaKeys * kMmaRow], v[kMmaKeys * kMmaRow];     // the tile, in q's type
   uint8_t kc[kMmaKeys * kMmaDim], vc[kMmaKeys * kMmaDim];   // its codes, or the next tile's on their way
   int64_t row[2][kMmaKeys];                                 // byte offset of a token's codes, -1: none
-  float ks[2][kMmaKeys], vs[2][kMmaKeys];
+  float ks[2][kMmaKeys], vs[2][kMmaKeys];                   // in the units below
+  UnitShared unit;
 };
 
 // byte offset of 16-byte chunk c of row r: rows are 512 bytes, and eight rows'
@@ -323,6 +411,18 @@ __global__ void __launch_bounds__(kMmaThreads, 1) fp8_prefill_mma_kernel(const M
   const int64_t trow = a.row_ids ? (int64_t)a.row_ids[b] : b;
   const int chunks = a.d / 16;  // 16-byte chunks of a token's codes
 
+  // fp16: the units of the keys that the tile sees (half_unit)
+  float k_unit = 1.f, v_unit = 1.f, k_inv = 1.f, v_inv = 1.f;
+  if constexpr (std::is_same<T, __half>::value) {
+    static_assert(kMmaThreads == kExpandThreads, "find_units");
+    find_units(a, trow, kend, h, sh->unit);
+    __syncthreads();
+    const float2 unit = units_of(sh->unit);
+    k_unit = unit.x, v_unit = unit.y;
+    k_inv = pow2_inverse(k_unit), v_inv = pow2_inverse(v_unit);
+  }
+  const float scale_log2 = a.scale_log2 * k_unit;
+
   auto locate = [&](int64_t k0, int buf) {
     if (tid >= kMmaKeys) return;
     const int64_t t = k0 + tid;
@@ -339,8 +439,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) fp8_prefill_mma_kernel(const M
         } else {
           const int64_t slot = (a.layer * a.num_blocks + phys) * a.hkv + h;
           r = (slot * a.bs + (t - lb * a.bs)) * a.d;
-          ks = a.k_scale[slot];
-          vs = a.v_scale[slot];
+          ks = a.k_scale[slot] * k_inv;
+          vs = a.v_scale[slot] * v_inv;
         }
       }
     }
@@ -449,7 +549,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) fp8_prefill_mma_kernel(const M
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = j * 8 + 2 * t4 + (e & 1), i = e >> 1;
-        s[j][e] = k0 + key <= last[i] && sh->row[buf][key] >= 0 ? s[j][e] * a.scale_log2 : -INFINITY;
+        s[j][e] = k0 + key <= last[i] && sh->row[buf][key] >= 0 ? s[j][e] * scale_log2 : -INFINITY;
         mx[i] = fmaxf(mx[i], s[j][e]);
       }
     float al[2], unit[2];
@@ -500,7 +600,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) fp8_prefill_mma_kernel(const M
     T* dst = reinterpret_cast<T*>(a.out) + b * a.o_sb + (qo + t) * a.o_st + (h * a.g + (r - t * a.g)) * a.o_sh;
     // 0: no key seen, so zeros whatever the keys of the tile hold; a NaN sum stays NaN
     const bool none = l[i] == 0.f;
-    const float inv = none ? 0.f : 1.f / l[i];
+    const float inv = none ? 0.f : 1.f / l[i] * v_unit;
 #pragma unroll
     for (int j = 0; j < kMmaDim / 8; ++j) {
       const int d = j * 8 + 2 * t4;
@@ -872,6 +972,8 @@ int launch_tc(const bl_prefill_fp8_args& a, const Scratch& w, cudaStream_t s) {
   e.v_out = ws + w.v;
   e.table = (int32_t*)(ws + w.table);
   e.order = (int32_t*)(ws + w.order);
+  e.k_unit = (float*)(ws + w.units);
+  e.v_unit = e.k_unit + a.batch * w.heads;
   e.num_blocks = kv.num_blocks;
   e.layer = kv.layer;
   e.width = w.width;
@@ -895,8 +997,18 @@ int launch_tc(const bl_prefill_fp8_args& a, const Scratch& w, cudaStream_t s) {
   e.hq = (int32_t)a.num_q_heads;
   e.err = a.err;
   dim3 grid((unsigned)((w.width + kExpandPages - 1) / kExpandPages), (unsigned)e.hkv, (unsigned)a.batch);
-  fp8_expand_kernel<T><<<grid, kExpandThreads, 0, s>>>(e);
-  BL_CHECK_LAUNCH("fp8_expand_kernel");
+  e.own_units = std::min(kv.bt_width, (a.max_seq_len + kv.block_size - 1) / kv.block_size) <= kOwnUnitBlocks;
+  if (std::is_same<T, __half>::value && !e.own_units) {
+    fp8_units_kernel<<<dim3((unsigned)e.hkv, (unsigned)a.batch), kExpandThreads, 0, s>>>(e);
+    BL_CHECK_LAUNCH("fp8_units_kernel");
+    if (launch_pdl(fp8_expand_kernel<T>, grid, dim3(kExpandThreads), 0, s, e) != cudaSuccess) {
+      set_error("fp8_expand_kernel: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
+      return BL_ERR_LAUNCH;
+    }
+  } else {
+    fp8_expand_kernel<T><<<grid, kExpandThreads, 0, s>>>(e);
+    BL_CHECK_LAUNCH("fp8_expand_kernel");
+  }
 
   bl_prefill_args p;
   memset(&p, 0, sizeof(p));
@@ -924,7 +1036,8 @@ int launch_tc(const bl_prefill_fp8_args& a, const Scratch& w, cudaStream_t s) {
   p.max_q_len = a.max_q_len;
   p.scale = a.scale;
   p.err = a.err;
-  const int rc = prefill_tc_launch(p, s, e.order);
+  const Expansion expansion = {e.order, e.k_unit, e.v_unit};
+  const int rc = prefill_tc_launch(p, s, &expansion);
   if (rc || !wide) return rc;
   x.narrow = a.out;
   x.wide = out;
@@ -952,7 +1065,7 @@ extern "C" size_t bl_paged_prefill_fp8_workspace_bytes(int32_t dtype, int64_t ba
       max_seq_len <= 0 || total_blocks <= 0 || !use_tc(dtype, head_dim))
     return 0;
   Scratch w;
-  return plan_scratch(batch, num_q_heads, num_kv_heads, head_dim, block_size, total_q_len, max_seq_len, total_blocks, &w)
+  return plan_scratch(dtype, batch, num_q_heads, num_kv_heads, head_dim, block_size, total_q_len, max_seq_len, total_blocks, &w)
              ? w.total
              : 0;
 }
@@ -979,7 +1092,7 @@ extern "C" int bl_paged_prefill_fp8(const bl_prefill_fp8_args* args, void* strea
   cudaStream_t s = (cudaStream_t)stream;
   Scratch w;
   if (use_tc(kv.dtype, kv.head_dim) && tc_alignment(a) &&
-      plan_scratch(a.batch, a.num_q_heads, kv.num_kv_heads, kv.head_dim, kv.block_size, a.total_q_len, a.max_seq_len,
+      plan_scratch(kv.dtype, a.batch, a.num_q_heads, kv.num_kv_heads, kv.head_dim, kv.block_size, a.total_q_len, a.max_seq_len,
                    a.total_blocks, &w)) {
     if (!a.workspace || a.workspace_bytes < w.total) {
       set_error("%s: workspace too small (%zu < %zu bytes)", who, a.workspace ? a.workspace_bytes : (size_t)0, w.total);

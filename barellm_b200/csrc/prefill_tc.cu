@@ -100,6 +100,8 @@ struct Args {
   int64_t num_blocks, layer_row0, max_q;
   float scale_log2;
   int32_t* err;
+  const float* k_unit;  // [batch, hkv]: K and V are these times what the pools hold (powers of two); EXPANDED fp16 only
+  const float* v_unit;
 };
 
 struct Shared {
@@ -118,7 +120,8 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Sh
 }
 
 // EXPANDED: the pools are the expansion of an 8-bit cache (fp8_prefill.cu), whose rows
-// may have queries that see no key.
+// may have queries that see no key, and which in fp16 comes in units of each row
+// and KV head.
 template <bool BF16, bool EXPANDED>
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_tc_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -415,6 +418,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_proxy_async_smem();
     mbar_arrive(&sh->q_full);
 
+    constexpr bool kUnits = EXPANDED && !BF16;
+    float unit_scale = 0.f;
+    if constexpr (kUnits) {
+      // (a factor that underflowed would make NaN of the mask)
+      const float f = fmaxf(a.scale_log2 * a.k_unit[b * a.hkv + h], 1.2e-38f);
+      // The maximum of equal, positive values: through it the factor is kept in a register of
+      // the warp, not of every thread, which has none to spare (chunks over 1.5k..6k
+      // tokens: 204.9 against 207.5 us).
+      unit_scale = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(f)));
+    }
+    auto scale_log2 = [&] { return kUnits ? unit_scale : a.scale_log2; };
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
     for (int t = 0; t < ntiles; ++t) {
@@ -443,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int j = 8; j < kKT; ++j) mp[j & 7] = fmaxf(mp[j & 7], v[j]);
       const float mt = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])),
-                             fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7]))) * a.scale_log2;
+                             fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7]))) * scale_log2();
       const float m_new = fmaxf(m_used, mt);
       const bool need = (t > 0) && (m_new > m_used + kRescaleThreshold);
       const float alpha = need ? fast_exp2(m_used - m_new) : 1.f;
@@ -457,8 +471,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t pk[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const float p0 = fast_exp2(fmaf(v[c * 32 + 2 * j], a.scale_log2, -ms));
-          const float p1 = fast_exp2(fmaf(v[c * 32 + 2 * j + 1], a.scale_log2, -ms));
+          const float p0 = fast_exp2(fmaf(v[c * 32 + 2 * j], scale_log2(), -ms));
+          const float p1 = fast_exp2(fmaf(v[c * 32 + 2 * j + 1], scale_log2(), -ms));
           rp[j & 3] += p0 + p1;
           pk[j] = pack2<T>(p0, p1);
         }
@@ -490,7 +504,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, wait_or_abort(&sh->pv_done[x], 0, sh, a.err));
       if (ok) {
         tc_fence_after();
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        float inv = l > 0.f ? 1.f / l : 0.f;
+        if (kUnits) inv *= a.v_unit[b * a.hkv + h];
         // a query that sees no key: zeros, whatever the keys of its tile hold (0 * NaN is NaN)
         const uint32_t keep = EXPANDED && l == 0.f ? 0u : 0xffffffffu;
         if (a.o_vec16) {
@@ -560,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 size_t smem_bytes() { return 1024 + kSmemData + sizeof(Shared); }
 
 template <bool BF16, bool EXPANDED>
-int launch(const bl_prefill_args& a, const int32_t* row_order, cudaStream_t s) {
+int launch(const bl_prefill_args& a, cudaStream_t s, const Expansion* x) {
   // the attribute belongs to one device's copy of the kernel: set once per device
   static std::atomic<bool> attr_done[64];
   int dev = 0;
@@ -589,7 +604,9 @@ int launch(const bl_prefill_args& a, const int32_t* row_order, cudaStream_t s) {
   k.bt_stride = a.kv.bt_stride;
   k.bt_width = (int32_t)std::min<int64_t>(a.kv.bt_width, INT32_MAX);
   k.row_ids = a.kv.row_ids;
-  k.row_order = row_order;
+  k.row_order = x ? x->row_order : nullptr;
+  k.k_unit = x ? x->k_unit : nullptr;
+  k.v_unit = x ? x->v_unit : nullptr;
   k.hkv = (int32_t)a.kv.num_kv_heads;
   k.g = (int32_t)(a.num_q_heads / a.kv.num_kv_heads);
   k.bq = kRows / k.g;
@@ -635,7 +652,7 @@ bool prefill_tc_supported(int32_t dtype, int64_t head_dim, int64_t block_size, i
   return g == 1 || g == 2 || g == 4 || g == 8;
 }
 
-int prefill_tc_launch(const bl_prefill_args& a, cudaStream_t s, const int32_t* row_order) {
+int prefill_tc_launch(const bl_prefill_args& a, cudaStream_t s, const Expansion* x) {
   const uint64_t rows = (uint64_t)a.kv.num_layers * a.kv.num_blocks * a.kv.num_kv_heads * kBS;
   BL_CHECK_ARG(rows + kBS <= (uint64_t)INT32_MAX, "bl_paged_prefill: pool has more than 2^31 rows");
   BL_CHECK_ARG(((uintptr_t)a.kv.k_pool & 15) == 0 && ((uintptr_t)a.kv.v_pool & 15) == 0,
@@ -644,8 +661,8 @@ int prefill_tc_launch(const bl_prefill_args& a, cudaStream_t s, const int32_t* r
                    a.q_stride_t % 2 == 0 && a.q_stride_h % 2 == 0 && a.out_stride_b % 2 == 0 &&
                    a.out_stride_t % 2 == 0 && a.out_stride_h % 2 == 0,
                "bl_paged_prefill: q/out must be 4-byte aligned with even strides");
-  if (a.kv.dtype == BL_BF16) return row_order ? launch<true, true>(a, row_order, s) : launch<true, false>(a, nullptr, s);
-  return row_order ? launch<false, true>(a, row_order, s) : launch<false, false>(a, nullptr, s);
+  if (a.kv.dtype == BL_BF16) return x ? launch<true, true>(a, s, x) : launch<true, false>(a, s, nullptr);
+  return x ? launch<false, true>(a, s, x) : launch<false, false>(a, s, nullptr);
 }
 
 }  // namespace bl

@@ -484,6 +484,11 @@ BL_API int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream);
 /* axis; else batch * max_q_len).  They size the workspace (0 bytes where    */
 /* the call needs none).  Tokens of a packed q that no row has are left as   */
 /* they were in out.                                                         */
+/* K and V are code * scale whatever the range of kv.dtype: fp16 calls keep   */
+/* an element to 2^-32 of the largest scale among the row's blocks, bf16     */
+/* ones exactly.  16-bit calls with head_dim % 8 == 0 (% 16 above 128) round  */
+/* the softmax weights to kv.dtype.  A NaN among the V of a row's new tokens  */
+/* may reach the row's queries before it.                                    */
 typedef struct bl_prefill_fp8_args {
   bl_fp8_layer layer;
   const void* q;

@@ -636,3 +636,100 @@ def test_prefill_queries_that_see_no_key_beside_nan(cuda, native_lib, dtype, d, 
         ops.paged_prefill_fp8(q, *pool.args, 1, bt, i32(lens, cuda), 150, q_offsets=off, max_q_len=300, out=out)
         assert bool((out[0, :, :27] == 0).all()) and bool((out[0, :, 40:190] == 0).all())
         assert bool(out[0, 4:, 39].isnan().all()) and not bool(out[0, :4].isnan().any())
+
+
+def far_bound(want, spread, reach, flat, q, k, v, dtype, eps, k_scales, v_scales, scale):
+    """attention_bound, and what fp16 operands add where scales lie far apart (fp8.cuh,
+    half_unit).  A K or V element is kept to 2^-25 of its unit, 2^-7 of the largest
+    scale: a score moves by 2^-25 unit sum |q| scale (a weight by twice its expm1, as
+    there), an output by 2^-25 unit.  A weight below 2^-14 of the largest is kept to 2^-25 of
+    that, and the weights' sum is at least the largest: 2^-25 sum |v| over the keys."""
+    err = attention_bound(want, spread, reach, flat, q, dtype, eps, k.shape[1])
+    if dtype is F16:
+        g = q.shape[0] // k.shape[0]
+        unit = lambda s: np.repeat(s.max(axis=0), g)[:, None, None] * 2.0 ** -7
+        move = 2.0 ** -25 * unit(k_scales) * np.abs(q).sum(axis=2, keepdims=True) * scale
+        err = err + 2 * np.expm1(2 * move) * spread + 2.0 ** -25 * unit(v_scales)
+    if dtype is not F32:
+        err = err + 2.0 ** -25 * np.repeat(np.abs(v).sum(axis=1), q.shape[0] // v.shape[0], axis=0)[:, None]
+    return err
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("hq,hkv,bs,d", [(8, 2, 16, 128), (6, 2, 16, 128), (4, 2, 32, 64), (8, 2, 16, 256), (4, 2, 8, 144), (4, 2, 16, 36),
+                                          (8, 2, 4, 128), (10, 2, 5, 64)])  # (the last two: rows of more than 128 blocks)
+@pytest.mark.parametrize("k_exp,q_exp,v_exp,v_spread,scale", [(17, -17, 16, 0.0, None), (-22, 12, 0, 0.0, 64.0), (0, 0, -4, 12.0, None),
+                                                              (-60, 12, 3, 4.0, 2.0 ** 44)], ids=["large", "small", "apart", "tiny"])
+def test_prefill_values_far_from_one(cuda, native_lib, dtype, hq, hkv, bs, d, k_exp, q_exp, v_exp, v_spread, scale):
+    """A pool filled from fp32: K and V past fp16's range, below its normal numbers, and V whose blocks lie far apart."""
+    rs = np.random.RandomState(100 + d + k_exp)
+    n, c = 700, 90
+    pool = Pool(cuda, 1, -(-n // bs) + 3, hkv, bs, d)
+    table = pool.table([n])
+    bt = torch.from_numpy(table).to(cuda)
+    size = np.exp2(np.repeat(rs.uniform(-v_spread, v_spread, (hkv, n // 16 + 1)), 16, axis=1)[:, :n, None])
+    k = (rs.randn(1, hkv, n, d) * 2.0 ** k_exp).astype(np.float32)
+    v = (rs.randn(1, hkv, n, d) * size * 2.0 ** v_exp).astype(np.float32)
+    ops.paged_append_fp8(*pool.args, 0, bt, i32([0], cuda), torch.from_numpy(k).to(cuda), torch.from_numpy(v).to(cuda))
+    pool.download()
+    q = (torch.randn(1, hq, c, d, generator=torch.Generator().manual_seed(1)) * 2.0 ** q_exp).to(dtype).to(cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = ops.paged_prefill_fp8(q, *pool.args, 0, bt, i32([n], cuda), n, scale=scale, err=err)
+    assert int(err) == 0
+    kd, vd = (f8.read(x, s, 0, table[0], n) for x, s in zip(pool.codes, pool.scales))
+    qn = q.double().cpu().numpy()[0]
+    want, spread, reach, flat = f8.attention(qn, kd, vd, scale)
+    eps = torch.finfo(dtype).eps / 2 if dtype is not F32 and d % 8 == 0 else 0.0
+    used, scale_d = table[0][table[0] >= 0], scale or 1 / np.sqrt(d)
+    bound = far_bound(want, spread, reach, flat, qn, kd, vd, dtype, eps, *(s[0][used] for s in pool.scales), scale_d)
+    assert_within(out.double().cpu().numpy()[0], want, bound)
+    # the decode of the last token stays within the same bound
+    got = ops.paged_decode_fp8(q[:, :, -1].contiguous(), *pool.args, 0, bt, i32([n], cuda), n, scale=scale)
+    bound = far_bound(*(x[:, -1:] for x in (want, spread, reach, flat, qn)), kd, vd, dtype, 2.0 ** -11 if dtype is not F32 else 0.0,
+                      *(s[0][used] for s in pool.scales), scale_d)
+    assert_within(got.double().cpu().numpy()[0][:, None], want[:, -1:], bound)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hq,hkv,bs,d", [(8, 2, 16, 128), (6, 2, 4, 128), (8, 2, 16, 256)])
+@pytest.mark.parametrize("exps", [[17, 0, -18, 2], [17, 0, -13, 2]])  # (-18: q holds infinities in fp16)
+def test_prefill_rows_and_heads_of_different_magnitudes(cuda, native_lib, dtype, hq, hkv, bs, d, exps):
+    """Each row's KV heads have units of their own; empty rows, queries that see nothing, rows by row_ids, a captured call."""
+    rs = np.random.RandomState(d + bs)
+    lens, chunks = [600, 0, 33, 520], [40, 3, 50, 17]
+    pool = Pool(cuda, 1, sum(-(-n // bs) for n in lens) + 3, hkv, bs, d)
+    table = pool.table(lens)
+    bt = torch.from_numpy(table).to(cuda)
+    tokens = [[rs.randn(hkv, n, d) * 2.0 ** (e + np.array([0, -9]))[:, None, None] for n, e in zip(lens, exps)] for _ in range(2)]
+    off = i32(np.concatenate([[0], np.cumsum(lens)]), cuda)
+    k, v = (torch.from_numpy(np.concatenate(x, axis=1).astype(np.float32)).to(cuda).unsqueeze(0) for x in tokens)
+    ops.paged_append_fp8(*pool.args, 0, bt, i32([0] * 4, cuda), k, v * 0.25, new_offsets=off, max_new_tokens=max(lens))
+    pool.download()
+    order = [2, 0, 3, 1]  # of the queries' rows in the table
+    g = torch.Generator().manual_seed(7)
+    qs = [torch.randn(hq, chunks[r], d, generator=g) * 2.0 ** -exps[r] for r in order]
+    q = torch.cat(qs, dim=1).to(dtype).to(cuda).unsqueeze(0)
+    q_off = i32(np.concatenate([[0], np.cumsum([chunks[r] for r in order])]), cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    call = lambda: ops.paged_prefill_fp8(q, *pool.args, 0, bt, i32_lens, 600, q_offsets=q_off, max_q_len=50, row_ids=rows, err=err)
+    i32_lens, rows = i32([lens[r] for r in order], cuda), i32(order, cuda)
+    out = call()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        again = call()
+    again.fill_(5.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again.view(torch.int16), out.view(torch.int16)) and int(err) == 0
+    at, got = 0, out.double().cpu().numpy()[0]
+    for r in order:
+        kd, vd = (f8.read(x, s, 0, table[r], lens[r]) for x, s in zip(pool.codes, pool.scales))
+        qn = q[0, :, at:at + chunks[r]].double().cpu().numpy()
+        want, spread, reach, flat = f8.attention(qn, kd, vd)
+        used = table[r][:-(-lens[r] // bs)]
+        scales = [s[0][used] if len(used) else np.ones((1, hkv)) for s in pool.scales]
+        bound = far_bound(want, spread, reach, flat, qn, kd, vd, dtype, torch.finfo(dtype).eps / 2, *scales, 1 / np.sqrt(d))
+        bound[:, :max(0, chunks[r] - lens[r])] = 0.0  # no key: zeros (the terms above may be inf * 0)
+        assert_within(got[:, at:at + chunks[r]], want, bound)
+        at += chunks[r]
