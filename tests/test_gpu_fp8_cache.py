@@ -271,3 +271,34 @@ def test_offsets_past_32_bits(cuda, native_lib):
                            ops.paged_decode_fp8(q, *small.args, 0, sbt, i32([n], cuda), n))
         assert torch.equal(ops.paged_prefill_fp8(q2, kc, vc, ks, vs, 1, table, i32([n], cuda), n),
                            ops.paged_prefill_fp8(q2, *small.args, 0, sbt, i32([n], cuda), n))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("step", [0.7, 1.0, 3.5])
+def test_stored_values_stay_near_the_appended_ones(cuda, native_lib, dtype, step):
+    """Blocks whose scale is raised with almost every token, against the values that were appended.
+
+    The first rounding is off by at most 2^-4 |x| or 2^-10 of the scale of then; every raise
+    rounds to at most 2^-10 of the new scale, at least twice the one before: together
+    2^-4 |x| + 2^-9 of the block's scale.  A block that is filled at once is off by half a step."""
+    rs = np.random.RandomState(int(10 * step))
+    bs, n, d = 16, 48, 64
+    pool = Pool(cuda, 1, 7, 2, bs, d)
+    table = pool.table([n, n])
+    bt = torch.from_numpy(table).to(cuda)
+    x = rounded(rs.randn(2, n, d) * 2.0 ** (step * (np.arange(n) % bs - 15) + 2)[None, :, None] * np.exp(rs.randn(2, n, d)), dtype)
+    for t in range(n):
+        new = x[:, t:t + 1].astype(np.float32)
+        gpu_append(pool, 0, bt, [t], [new], [new], dtype, row_ids=i32([0], cuda))
+    whole = x.astype(np.float32)
+    gpu_append(pool, 0, bt, [0], [whole], [whole], dtype, row_ids=i32([1], cuda))
+    pool.download()
+    for codes, scales in zip(pool.codes, pool.scales):
+        for row, raised in ((0, True), (1, False)):
+            got = f8.read(codes, scales, 0, table[row], n)
+            s = np.repeat(scales[0][table[row]].T.astype(np.float64), bs, axis=1)[..., None]
+            half = np.maximum(2.0 ** -4 * np.abs(x), 2.0 ** -10 * s)
+            bound = 2.0 ** -4 * np.abs(x) + 2.0 ** -9 * s if raised else half
+            assert (np.abs(got - x) <= bound).all()
+            assert not raised or (np.abs(got - x) > half).any()  # (roundings on the way do add up)
+        np.testing.assert_array_equal(scales[0][table[0]], scales[0][table[1]])  # the scale does not depend on the steps
