@@ -214,6 +214,8 @@ class Qwen3(nn.Module):
         for i, blk in enumerate(self.layers):
             h = blk(h, cos, sin, None if kv_cache is None else kv_cache.layer(i))
         if logits_index is not None:
+            if logits_index.numel() == 0:  # (a chunk inside a long prompt: no row ends here)
+                return h.new_empty((h.shape[0], 0, self.embed.shape[0]))
             h = h[:, logits_index]
         return torch.matmul(self.norm(h), self.embed.T)
 

@@ -216,3 +216,20 @@ def test_qwen06b_whole_configuration_bf16_teacher_forced(cuda, native_lib):
     print(f"\nwhole configuration: {len(prompts)} prompts x {n_new} steps = {len(prompts) * n_new} steps, "
           f"{len(diffs)} differ; oracle top-2 margin there, in bf16 rounding steps: count = {hist}")
     assert not bad, f"argmax differs away from a near-tie (prompt, step, oracle top-2 margin): {bad}"
+
+
+@pytest.mark.parametrize("dtype,kv_dtype", [(torch.float32, None), (torch.bfloat16, None), (torch.bfloat16, torch.float8_e4m3fn)])
+def test_prompts_longer_than_a_prefill_chunk(cuda, native_lib, dtype, kv_dtype):
+    """Chunks that end no prompt: they only fill the cache."""
+    shape = Qwen3Shape(vocab_size=512, hidden_size=256, intermediate_size=512, head_dim=64, num_layers=3, num_heads=4, num_kv_heads=2)
+    model = random_qwen3(shape, dtype=dtype, device=cuda, seed=0)
+    prompts = prompts_for(3, 150, 200, shape.vocab_size, seed=1) + [[7] * 5]
+    blocks = PagedEngine.blocks_needed([len(p) for p in prompts], 8, 16) + 4
+    outs = []
+    for graph in (False, True):
+        engine = PagedEngine(model, num_blocks=blocks, prefill_tokens=32, kv_dtype=kv_dtype)
+        outs.append(engine.generate(prompts, max_new_tokens=8, use_graph=graph))
+        assert engine.pool.num_free == blocks
+    assert outs[0] == outs[1] and all(len(o) == 8 for o in outs[0])
+    if dtype is torch.float32:
+        assert outs[0] == generate_contiguous(model, prompts, 8)[0]
