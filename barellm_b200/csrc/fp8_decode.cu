@@ -33,11 +33,13 @@
 // sums of its own where it is far smaller.
 //
 // What bounds it (64 requests of 1k..32k tokens, 32 / 8 heads, head_dim 128, bf16:
-// 2.12 GB): HBM.  Plan, attention and join together 354 us, 5.98 TB/s, the
-// attention kernel alone 339 us, 6.25 TB/s (a copy on this card: 6.56).  Under a
+// 2.12 GB): HBM, while the chip is cool: plan, attention and join together 353 us, 5.99 TB/s,
+// the attention kernel alone 339 us, 6.25 TB/s (a copy on this card: 6.56).  Under a
 // load that goes on for 100 ms the card reaches its power cap and the SM
 // clock falls to 1.6 GHz; the conversions and products then take longer than
-// the copies (380..410 us; without them 343 us).  Measured and not kept: one
+// the copies (calls in a loop: 388..406 us, 5.2..5.45 TB/s; without them 343 us).  The
+// three CTAs per SM leave 128 registers, of which the 128-dim kernel spills 56
+// bytes (68 at block sizes of 8).  Measured and not kept: one
 // producer warp for the CTA (375 us without any arithmetic), rings of 4 steps a
 // warp or 2 CTAs per SM with larger rings (more than 96 KB in flight per SM is
 // slower), 4 CTAs of 96 registers (425 us), static rounds in place of claims (373 us).

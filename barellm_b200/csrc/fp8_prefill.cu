@@ -8,10 +8,12 @@
 //       dequantised once into a 16-bit paged scratch (bf16: exact, a code has
 //       four significant bits; fp16: in units of each row and KV head, half_unit in
 //       fp8.cuh), which the tcgen05 kernel of prefill_tc.cu then reads.  The
-//       expansion moves 1 + 2 bytes per cached element once; a CTA of the
-//       attention kernel reads the 2-byte form, and every 128 query tokens times
-//       group re-read it (mostly from L2), so dequantising in that kernel would
-//       repeat the conversion for every query tile.  Block sizes
+//       expansion moves 1 + 2 bytes per cached element (1 + 2 n where a KV head
+//       becomes n, below); a CTA of the attention kernel reads the 2-byte form,
+//       and every 128 query tokens times group re-read it (mostly from L2), so
+//       dequantising in that kernel would repeat the conversion for every query
+//       tile.  (Few queries over a long prefix pay for that: 8 rows of 4 queries over 8k
+//       tokens take 204 us, ten times their codes' bytes.)  Block sizes
 //       other than 16 become 16-token pages on the way, and a query group
 //       that the kernel is not built for (3, 5, 16, ...) becomes several KV heads
 //       with the same contents and a group of 8, 4, 2 or 1.  A head_dim below
@@ -56,7 +58,8 @@ bool use_mma(int32_t dtype, int64_t d) {
   return (dtype == BL_BF16 || dtype == BL_F16) && d > kTCDim && d <= 256 && d % 16 == 0;
 }
 
-// False when the scratch would not fit the tcgen05 kernel's 32-bit row coordinates.
+// False when the scratch would not fit the tcgen05 kernel's 32-bit row coordinates
+// (the call then takes the SIMT kernel).
 bool plan_scratch(int32_t dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t bs, int64_t total_q, int64_t max_seq_len,
                   int64_t total_blocks, Scratch* w) {
   const int64_t g = hq / hkv;
