@@ -7,8 +7,7 @@
 // Kernels
 //   fp8_decode_plan_kernel one CTA.  Splits rows into 512-token chunks and lists
 //                          the units, full chunks first, then partial ones by
-//                          decreasing size.  A unit's record holds all that the
-//                          attention kernel's producer needs to start on it.
+//                          decreasing size.
 //   fp8_decode_tc_kernel   bf16 / fp16 q, head_dim a multiple of 16, block_size
 //                          one of 8.  Built for 64, 128 and 256 dims; the copies
 //                          fill the dims up to the next of these with zeros.
@@ -63,7 +62,6 @@ inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 // One chunk of a row, as the plan records it.
 struct alignas(16) Unit {
   int32_t row, chunk, len, part;  // len: the row's length, at most what its table covers; part: slot of its partial
-  int32_t table_row, pad[3];
 };
 
 struct WsLayout {
@@ -93,7 +91,6 @@ constexpr int kPlanThreads = 1024;  // at most; a batch of fewer rows takes fewe
 
 struct PlanArgs {
   const int32_t* seq_lens;
-  const int32_t* row_ids;
   int32_t batch, max_units;
   int64_t cap;        // tokens a table row covers
   int32_t* hdr;       // [0] units, [1] magic, [2] batch, [3] max_units, [4..5] items claimed, [6] CTAs done
@@ -135,11 +132,9 @@ __global__ void __launch_bounds__(kPlanThreads) fp8_decode_plan_kernel(const Pla
   const int tid = threadIdx.x;
   if (tid < kChunkTiles) s_count[tid] = 0;
   __syncthreads();
-  auto put = [&](int pos, int row, int chunk, int len, int base, int table_row) {
+  auto put = [&](int pos, int row, int chunk, int len, int base) {
     if ((uint32_t)pos >= (uint32_t)a.max_units) return;  // (rows far past max_seq_len may wrap the sums)
-    int4* u = reinterpret_cast<int4*>(a.units + pos);
-    u[0] = make_int4(row, chunk, len, base + chunk);
-    u[1] = make_int4(table_row, 0, 0, 0);
+    *reinterpret_cast<int4*>(a.units + pos) = make_int4(row, chunk, len, base + chunk);
   };
   auto length = [&](int b) {
     const int64_t len = a.seq_lens[b];
@@ -156,8 +151,7 @@ __global__ void __launch_bounds__(kPlanThreads) fp8_decode_plan_kernel(const Pla
     if (b < a.batch) {
       if (a.seq_lens[b] > a.cap) raise_dev(a.err, BL_DEVERR_TABLE);
       a.row_base[b] = my_all;
-      const int table_row = a.row_ids ? a.row_ids[b] : b;
-      for (int c = 0; c < nfull; ++c) put(my_full + c, b, c, len, my_all, table_row);
+      for (int c = 0; c < nfull; ++c) put(my_full + c, b, c, len, my_all);
       if (nall > nfull) atomicAdd(&s_count[(len - nfull * kChunk + 15) / 16 - 1], 1);
     }
     all += tot_all;
@@ -183,7 +177,7 @@ __global__ void __launch_bounds__(kPlanThreads) fp8_decode_plan_kernel(const Pla
   for (int b = tid; b < a.batch; b += blockDim.x) {
     const int len = length(b), nfull = len / kChunk, rest = len - nfull * kChunk;
     if (rest > 0)
-      put(atomicAdd(&s_next[(rest + 15) / 16 - 1], 1), b, nfull, len, a.row_base[b], a.row_ids ? a.row_ids[b] : b);
+      put(atomicAdd(&s_next[(rest + 15) / 16 - 1], 1), b, nfull, len, a.row_base[b]);
   }
 }
 
@@ -248,7 +242,6 @@ __device__ __forceinline__ Unit find_unit(const Args& a, int u, int lane, int& u
   r.chunk = u - __shfl_sync(0xffffffffu, incl - n, r.row);
   r.len = __shfl_sync(0xffffffffu, (int)len, r.row);
   r.part = u;
-  r.table_row = a.row_ids ? a.row_ids[r.row] : r.row;
   return r;
 }
 
@@ -266,15 +259,13 @@ __device__ __forceinline__ Unit cluster_unit(const Args& a, bool tell) {
   }
   if (len > (int64_t)a.cluster * kChunk && tell) raise_dev(a.err, BL_DEVERR_WORKSPACE);  // longer than max_seq_len
   r.len = (int)max(len, (int64_t)0);
-  r.table_row = a.row_ids ? a.row_ids[r.row] : r.row;
   return r;
 }
 
 __device__ __forceinline__ Unit load_unit(const Args& a, int64_t item) {
-  const int4* p = reinterpret_cast<const int4*>(a.units + item / (a.hkv * a.head_tiles));
-  const int4 x = p[0], y = p[1];
+  const int4 x = *reinterpret_cast<const int4*>(a.units + item / (a.hkv * a.head_tiles));
   Unit u;
-  u.row = x.x, u.chunk = x.y, u.len = x.z, u.part = x.w, u.table_row = y.x;
+  u.row = x.x, u.chunk = x.y, u.len = x.z, u.part = x.w;
   return u;
 }
 
@@ -286,12 +277,13 @@ __device__ __forceinline__ bool make_item(const Args& a, int64_t item, const Uni
   it.hq0 = it.h * a.g + ht * a.tile_heads;
   it.heads = min(a.tile_heads, a.g - ht * a.tile_heads);
   it.b = u.row;
-  it.table_row = u.table_row;
   it.part = u.part;
   it.t0 = u.chunk * kChunk;
   it.t1 = min(it.t0 + kChunk, u.len);
   it.nch = (u.len + kChunk - 1) / kChunk;
-  const bool ok = u.row >= 0 && u.row < a.batch && u.chunk >= 0 && it.t0 < u.len && u.len <= a.bt_width * a.bs;
+  const bool ok = u.row >= 0 && u.row < a.batch && (uint32_t)u.chunk <= (uint32_t)(INT32_MAX - kChunk) / kChunk &&
+                  it.t0 < u.len && u.len <= a.bt_width * a.bs;
+  it.table_row = ok && a.row_ids ? a.row_ids[u.row] : u.row;
   if (!ok) it.t0 = it.t1 = it.heads = 0;  // no steps, no outputs
   return ok;
 }
@@ -627,8 +619,9 @@ __global__ void __launch_bounds__(kThreadsTC, D == 128 && !ROWS ? 3 : 1)
           unsigned long long c = 0;
           if (lane == 0) c = atomicAdd(claimed, 1ull);
           item = (int64_t)__shfl_sync(0xffffffffu, c, 0) + gridDim.x;
+          if (item < 0 && lane == 0) raise_dev(a.err, BL_DEVERR_WORKSPACE);  // (no plan's counter)
         }
-        end = item >= items;
+        end = item < 0 || item >= items;
         if (!end) unit = n_item > 0 ? load_unit(a, item) : first;
       } else {
         end = n_item > 0;
@@ -1729,7 +1722,6 @@ extern "C" int bl_paged_decode_fp8(const bl_decode_fp8_args* args, void* stream)
   if (k.planned && !a.plan_ready) {
     PlanArgs p;
     p.seq_lens = a.seq_lens;
-    p.row_ids = kv.row_ids;
     p.batch = k.batch;
     p.max_units = k.max_units;
     p.cap = k.bt_width * kv.block_size;

@@ -733,3 +733,43 @@ def test_prefill_rows_and_heads_of_different_magnitudes(cuda, native_lib, dtype,
         bound[:, :max(0, chunks[r] - lens[r])] = 0.0  # no key: zeros (the terms above may be inf * 0)
         assert_within(got[:, at:at + chunks[r]], want, bound)
         at += chunks[r]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("use_rows", [False, True])
+def test_decode_skips_records_that_are_no_plan(cuda, native_lib, dtype, use_rows):
+    """A workspace whose header is a plan's and whose records are not: the kernel checks each before it
+    follows it (rows, chunks whose tokens overflow, lengths), flags it, and leaves its output."""
+    batch, n = 40, 700
+    pool, table, bt = filled(cuda, [n] * batch, 2, 16, 128, dtype)
+    q, seq = torch.randn(batch, 4, 128, device=cuda).to(dtype), i32([n] * batch, cuda)
+    rows = i32([(7 * b + 3) % batch for b in range(batch)], cuda) if use_rows else None
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    ws = torch.zeros(ops.decode_fp8_workspace_bytes(batch, 4, 128, n), dtype=torch.uint8, device=cuda)
+    call = lambda out, ready: ops.paged_decode_fp8(q, *pool.args, 1, bt, seq, n, row_ids=rows, ws=ws, plan_ready=ready, out=out, err=err)
+    want = call(None, False).clone()
+    good = ws.clone()
+    words = ws.view(torch.int32)
+    units = words[(256 + 256) // 4:][:4 * 80].view(80, 4)  # row, chunk, len, part
+    assert words[0] == 80 and units[:, 2].tolist() == [n] * 80 and sorted(units[:, 0].tolist()) == sorted(2 * list(range(batch)))
+    for field, value in ((0, 10 ** 6), (0, -1), (1, 2 ** 22), (1, 2 ** 23), (1, 2 ** 31 - 1), (1, -1), (1, 2), (2, 2 ** 30), (2, 0),
+                         (2, -5)):
+        for record in (0, 79):
+            ws.copy_(good)
+            hit = int(units[record, 0])
+            units[record, field] = value
+            out = torch.full_like(want, 9.0)
+            err.zero_()
+            call(out, True)
+            assert int(err) & nat.BL_DEVERR_WORKSPACE, (field, value)
+            others = [b for b in range(batch) if b != hit]
+            assert torch.equal(out[others], want[others]), (field, value)
+    if dtype is BF16:  # the counter of claims (the other kernel has none)
+        err.zero_()
+        ws.copy_(good)
+        words[4:6] = -10 ** 6
+        call(torch.empty_like(want), True)
+        assert int(err) & nat.BL_DEVERR_WORKSPACE
+    err.zero_()
+    ws.copy_(good)
+    assert torch.equal(call(None, True), want) and int(err) == 0
