@@ -245,7 +245,7 @@ __device__ __forceinline__ bool unit_in_range(const TCArgs& a, int2 bc, int& len
   if (bc.x < 0 || bc.x >= a.batch || bc.y < 0) return false;
   len = a.seq_lens[bc.x];
   nbt = min((len + kBS - 1) / kBS, a.bt_width);
-  return bc.y * a.chunk_blocks < nbt;
+  return (int64_t)bc.y * a.chunk_blocks < nbt;
 }
 
 template <typename T>

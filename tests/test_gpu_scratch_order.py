@@ -38,3 +38,37 @@ def test_a_workspace_may_be_what_the_append_read(cuda, native_lib, n):
         out = ops.paged_decode(q, *got, 0, bt, seq, 512, ws=buf[last:])
         assert all(torch.equal(a, b) for a, b in zip(got, clean))
         assert torch.equal(out, want)
+
+
+def test_records_that_are_no_plan_are_skipped(cuda, native_lib):
+    """A workspace whose header is a plan's and whose records are not: rows and chunks outside the batch, also
+    chunks whose first block overflows 32 bits, are flagged and skipped; the other rows keep their results."""
+    from barellm_b200 import _native as nat
+
+    batch, n, hkv, hq = 20, 700, 2, 8
+    g = torch.Generator(device=cuda).manual_seed(0)
+    pools = [torch.randn(1, batch * 44, hkv, 16, 128, generator=g, device=cuda).to(BF16) for _ in range(2)]
+    bt = torch.randperm(batch * 44, generator=g, device=cuda).to(torch.int32).view(batch, 44)
+    q = torch.randn(batch, hq, 128, generator=g, device=cuda).to(BF16)
+    seq = torch.full((batch,), n, dtype=torch.int32, device=cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    ws = torch.zeros(ops.decode_workspace_bytes(batch, hq, 128, 16, n), dtype=torch.uint8, device=cuda)
+    call = lambda out, ready: ops.paged_decode(q, *pools, 0, bt, seq, n, ws=ws, plan_ready=ready, out=out, err=err)
+    want = call(torch.empty_like(q), False).clone()
+    good, words = ws.clone(), ws.view(torch.int32)
+    units = words[512 // 4:][:2 * 2 * batch].view(2 * batch, 2)  # row, chunk
+    assert words[0] == 2 * batch and sorted(units[:, 0].tolist()) == sorted(2 * list(range(batch)))
+    for field, value in ((0, batch), (0, -1), (0, 2 ** 31 - 1), (1, -1), (1, 2), (1, 2 ** 26), (1, 2 ** 27), (1, 2 ** 31 - 1)):
+        for record in (0, 2 * batch - 1):
+            ws.copy_(good)
+            hit = int(units[record, 0])
+            units[record, field] = value
+            out = torch.full_like(want, 9.0)
+            err.zero_()
+            call(out, True)
+            assert int(err) & nat.BL_DEVERR_WORKSPACE, (field, value)
+            others = [b for b in range(batch) if b != hit]
+            assert torch.equal(out[others], want[others]), (field, value)
+    ws.copy_(good)
+    err.zero_()
+    assert torch.equal(call(torch.empty_like(q), True), want) and int(err) == 0
