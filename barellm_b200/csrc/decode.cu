@@ -80,7 +80,7 @@ WsLayout ws_layout(int64_t batch, int64_t hq, int64_t d, int64_t bs, int64_t max
 // ---------------------------------------------------------------------------
 // plan
 // ---------------------------------------------------------------------------
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024;  // at most; a batch of fewer rows takes fewer warps, which meet sooner
 
 __device__ __forceinline__ int block_excl_scan(int v, int* warp_tot, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -93,7 +93,7 @@ __device__ __forceinline__ int block_excl_scan(int v, int* warp_tot, int& total)
   if (lane == 31) warp_tot[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    int t = warp_tot[lane];
+    int t = lane < (int)(blockDim.x >> 5) ? warp_tot[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       int y = __shfl_up_sync(0xffffffffu, t, o);
@@ -924,7 +924,8 @@ extern "C" int bl_paged_decode_plan(const bl_decode_args* args, void* stream) {
   p.row_base = (int32_t*)(ws + w.row_base);
   p.exec = (int2*)(ws + w.exec);
   p.err = a.err;
-  if (launch_pdl(decode_plan_kernel, dim3(1), dim3(kPlanThreads), 0, (cudaStream_t)stream, p) != cudaSuccess) {
+  const int threads = (int)std::min<int64_t>(kPlanThreads, (a.batch + 31) / 32 * 32);
+  if (launch_pdl(decode_plan_kernel, dim3(1), dim3(threads), 0, (cudaStream_t)stream, p) != cudaSuccess) {
     set_error("decode_plan_kernel: launch failed: %s", cudaGetErrorString(cudaGetLastError()));
     return BL_ERR_LAUNCH;
   }
