@@ -113,3 +113,32 @@ def test_lengths_that_grow_on_the_device(cuda, native_lib, captured):
         want = ops.paged_decode_fp8(q, *pool.args, 0, bt, i32([x + n for x in lens], cuda), 720)
         assert torch.equal(got, want)
     assert int(err) == 0
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("most", [500, 1920, 6000])
+def test_lengths_written_just_ahead_of_a_small_call(cuda, native_lib, most, captured):
+    """Calls without a plan: rows of one chunk, rows joined within clusters, rows joined by a kernel."""
+    lens, order = [min(n, most) for n in (300, 1500, 1, 777)], [2, 0, 3, 1]
+    pool, table, bt = filled(cuda, [1920] * 4, 2, 16, 128, BF16, layers=1, layer=0)
+    q = torch.randn(4, 8, 128, generator=torch.Generator().manual_seed(3)).to(BF16).to(cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    call = lambda seq, rows: ops.paged_decode_fp8(q, *pool.args, 0, bt, seq, most, row_ids=rows, err=err)
+    want = call(i32(lens, cuda), i32(order, cuda)).clone()
+    late = LateWriter(cuda, lens + order)
+    seq, rows = late.values[:4], late.values[4:]
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            late.write()
+            out = call(seq, rows)
+    for _ in range(5):
+        late.pools[0].view(torch.uint8).zero_()
+        if captured:
+            graph.replay()
+        else:
+            late.write()
+            out = call(seq, rows)
+        assert torch.equal(out, want)
+    assert int(err) == 0
